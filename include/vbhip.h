@@ -365,6 +365,79 @@ int vb_rms_norm(const float* x, const float* w, float* y, int64_t rows, int64_t 
  * vibeblade/gpu.py:192-198). */
 int vb_softmax(const float* x, float* y, int64_t rows, int64_t n, void* stream);
 
+/* ---- the seam between two blocks -------------------------------------------
+ * Element types of activations below: 0 = fp32, 1 = fp16, 2 = bf16.
+ *
+ * For each of `rows` rows of `dim` values:
+ *   p = branch / sqrt(mean(branch^2) + eps) * post_w   (branch without post_w)
+ *   y = x + scale * gate * p                           (gate NULL: 1)
+ *   n = y / sqrt(mean(y^2) + eps) * pre_w              (NULL: n is not written)
+ * that is a block's output, normalised, gated and scaled into the residual
+ * stream, and the next block's normalised input (the engine's RMSNorm and
+ * residual steps between blocks, cpp/src/fast_model.cpp:61-71, :837-840,
+ * :966-975, as one pass).  Arithmetic is fp32 and y is not rounded before n
+ * is computed from it; y (of x's type) and n are rounded once.  Row r of a
+ * tensor starts at element r * its stride (branch_ld, x_ld of 0 or more, y_ld,
+ * n_ld at least dim, where rows > 1).  Element i of the gate of row r is
+ * gate[r * gate_row + i * gate_col], gate_col 0 or 1.  post_w, pre_w: dim
+ * fp32.  y may be x (same stride); no other overlap.  Any alignment of whole
+ * elements. */
+int vb_block_norm(const void* branch, int32_t branch_type, int64_t branch_ld, const float* post_w, const void* gate,
+                  int32_t gate_type, int64_t gate_row, int64_t gate_col, float scale, const void* x, int32_t x_type,
+                  int64_t x_ld, void* y, int64_t y_ld, const float* pre_w, void* n, int32_t n_type, int64_t n_ld,
+                  int64_t rows, int64_t dim, float eps, void* stream);
+
+/* ---- log probabilities ------------------------------------------------------
+ * logits: `rows` rows of `vocab` values (row stride ld, element type as
+ * above); z = logits / temperature (in [1e-30, 1e30]).
+ *   logprobs[r, j] = log softmax(z_r)[tokens[r, j]], j < n_tokens; an id
+ *       outside [0, vocab) gives 0 (a padded position);
+ *   entropy[r] = - sum p log p (optional, may be NULL);
+ *   top_ids / top_logprobs[r, j], j < top <= 64: the largest logits in
+ *       descending order, equal ones by the lower id.
+ * tokens: rows x n_tokens ids of token_bytes (4 or 8), contiguous; all
+ * outputs contiguous, fp32 (ids int32).  A row whose logits are all -inf has
+ * log probabilities -inf and entropy 0; a -inf logit is not named among the
+ * alternatives (id -1, log probability -inf); a row with a NaN or +inf has
+ * NaN for its log probabilities and entropy.  workspace: at least
+ * vb_token_logprobs_workspace(rows, vocab, top) bytes (0: none), 16-byte
+ * aligned, free again when the call's work is done. */
+int64_t vb_token_logprobs_workspace(int64_t rows, int64_t vocab, int32_t top);
+int vb_token_logprobs(const void* logits, int32_t type, int64_t ld, int64_t rows, int64_t vocab, float temperature,
+                      const void* tokens, int32_t token_bytes, int32_t n_tokens, float* logprobs, float* entropy,
+                      int32_t top, int32_t* top_ids, float* top_logprobs, void* workspace, size_t workspace_bytes,
+                      void* stream);
+
+/* ---- 4-bit weights with group scales -----------------------------------------
+ * W[n, k] = (q[n, k] - z[n, g]) * s[n, g], g = k / group: codes q of 4 bits,
+ * fp16 scales s and, optionally, zero points z of 0..15 (8 without them) per
+ * `group` consecutive weights of a row (32, 64 or any multiple of 128; the
+ * last group of a row may be short).  Not a GGUF type: the weights of files
+ * that keep codes, scales and zero points apart.
+ *
+ * A program packs them once (vb_group4_pack) into vb_group4_bytes(...) bytes
+ * of device memory (16-byte aligned) in the layout that the products read,
+ * and may then drop the parts.  packed: rows x ceil(k / 2) bytes, code 2i of a
+ * row in the low half of its byte i; scales: rows x ceil(k / group) fp16;
+ * zeros: the same shape, one byte each (NULL: symmetric). */
+int64_t vb_group4_bytes(int64_t rows, int64_t k, int32_t group, int32_t has_zeros);
+int vb_group4_pack(const uint8_t* packed, const void* scales, const uint8_t* zeros, void* w, int64_t rows, int64_t k,
+                   int32_t group, void* stream);
+/* The parts of a weight matrix src (rows x k, row stride ld, element type as
+ * above).  Symmetric (zeros NULL): s = fp16(max |w| / 7).  With zeros: over
+ * the group's range stretched to hold 0, s = fp16((hi - lo) / 15), z =
+ * round(-lo / s).  q = round(w / s) + z, clamped to 0..15. */
+int vb_group4_quantize(const void* src, int32_t type, int64_t ld, int64_t rows, int64_t k, int32_t group,
+                       uint8_t* packed, void* scales, uint8_t* zeros, void* stream);
+/* out[n * k + i] = W[n, i] of packed weights w, fp32 (exact). */
+int vb_group4_dequant_rows(const void* w, float* out, int64_t rows, int64_t k, int32_t group, int32_t has_zeros,
+                           void* stream);
+/* y[t * rows + n] = sum_i W[n, i] x[t, i] for the m activation rows of x (row
+ * stride x_ld, element type as above), fp32.  Sums are fp32 and fp32
+ * activations keep 22 bits or more of their largest neighbour among 128. */
+int vb_group4_gemv(const void* w, int64_t rows, int64_t k, int32_t group, int32_t has_zeros, const void* x,
+                   int32_t x_type, int64_t x_ld, int64_t m, float* y, void* stream);
+
 /* ---- GGUF ingestion --------------------------------------------------------
  * A .gguf file mapped read-only and parsed (header, metadata, tensor table).
  * Replaces GGUFFile (cpp/include/gguf.h:29-60, cpp/src/gguf.cpp) and the

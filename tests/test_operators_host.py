@@ -1,0 +1,147 @@
+"""Refusals and host-side rules of block_norm, token_logprobs and the 4-bit
+group products.  CPU only: every call here is turned down before a launch, or
+touches no device at all."""
+import ctypes
+
+import pytest
+import torch
+
+from vibeblade_amd import _lib
+from vibeblade_amd.group4 import GroupQTensor, group_gemv
+from vibeblade_amd.tensor import block_norm, token_logprobs
+
+OK, INVAL = 0, -1
+PTR = 0x1000  # never dereferenced: the calls below are refused or empty
+
+
+@pytest.fixture(scope="module")
+def lib():
+    return _lib.load()
+
+
+def norm_args(**kw):
+    a = dict(branch=PTR, branch_type=0, branch_ld=8, post_w=PTR, gate=None, gate_type=0, gate_row=0, gate_col=0,
+             scale=1.0, x=PTR, x_type=0, x_ld=8, y=PTR, y_ld=8, pre_w=PTR, n=PTR, n_type=0, n_ld=8, rows=2, dim=8,
+             eps=1e-5, stream=None)
+    assert set(kw) <= set(a)
+    a.update(kw)
+    return list(a.values())
+
+
+@pytest.mark.parametrize("bad", [dict(branch_type=3), dict(x_type=-1), dict(n_type=7), dict(gate=PTR, gate_type=9),
+                                 dict(rows=-1), dict(dim=0), dict(dim=1 << 31), dict(eps=-1.0), dict(eps=float("nan")),
+                                 dict(branch=None), dict(x=None), dict(y=None), dict(n=None), dict(y_ld=7), dict(n_ld=7),
+                                 dict(x_ld=-8), dict(branch_ld=-1), dict(gate=PTR, gate_col=2),
+                                 dict(gate=PTR, gate_row=-1)])
+def test_block_norm_refuses(lib, bad):
+    assert lib.vb_block_norm(*norm_args(**bad)) == INVAL
+    assert b"vb_block_norm" in lib.vb_last_error()
+
+
+def test_block_norm_without_rows_does_nothing(lib):
+    assert lib.vb_block_norm(*norm_args(rows=0, branch=None, x=None, y=None, n=None)) == OK
+
+
+def lp_args(**kw):
+    a = dict(logits=PTR, type=0, ld=100, rows=2, vocab=100, temperature=1.0, tokens=PTR, token_bytes=8, n_tokens=1,
+             logprobs=PTR, entropy=PTR, top=3, top_ids=PTR, top_logprobs=PTR, workspace=PTR, workspace_bytes=1 << 30,
+             stream=None)
+    assert set(kw) <= set(a)
+    a.update(kw)
+    return list(a.values())
+
+
+@pytest.mark.parametrize("bad", [dict(type=3), dict(rows=-1), dict(vocab=0), dict(vocab=1 << 31), dict(ld=-1),
+                                 dict(temperature=0.0), dict(temperature=-1.0), dict(temperature=float("nan")),
+                                 dict(temperature=float("inf")), dict(temperature=1e-40), dict(n_tokens=-1),
+                                 dict(token_bytes=2), dict(tokens=None), dict(logprobs=None), dict(top=-1), dict(top=65),
+                                 dict(top_ids=None), dict(top_logprobs=None), dict(logits=None)])
+def test_token_logprobs_refuses(lib, bad):
+    assert lib.vb_token_logprobs(*lp_args(**bad)) == INVAL
+    assert b"vb_token_logprobs" in lib.vb_last_error()
+
+
+def test_token_logprobs_workspace(lib):
+    for bad in ((-1, 10, 1), (1, 0, 1), (1, 1 << 31, 1), (1, 10, 65), (1, 10, -1)):
+        assert lib.vb_token_logprobs_workspace(*bad) == -1
+    for rows, vocab, top in ((0, 10, 0), (1, 1, 1), (1, 128256, 20), (1500, 151669, 0), (1 << 20, 200000, 64)):
+        need = lib.vb_token_logprobs_workspace(rows, vocab, top)
+        assert need >= 0
+        if need:
+            assert lib.vb_token_logprobs(*lp_args(rows=rows, vocab=vocab, ld=vocab, top=top,
+                                                  workspace_bytes=need - 1)) == INVAL
+            assert lib.vb_token_logprobs(*lp_args(rows=rows, vocab=vocab, ld=vocab, top=top, workspace=PTR + 8,
+                                                  workspace_bytes=need)) == INVAL
+    assert lib.vb_token_logprobs(*lp_args(rows=0, logits=None, tokens=None, logprobs=None)) == OK
+
+
+@pytest.mark.parametrize("group", [0, -32, 16, 48, 96, 100, 192])
+def test_group4_has_no_layout_for_other_groups(lib, group):
+    assert lib.vb_group4_bytes(16, 256, group, 0) == -1
+    assert lib.vb_group4_pack(PTR, PTR, None, PTR, 16, 256, group, None) == INVAL
+
+
+def test_group4_bytes(lib):
+    # whole blocks of 16 rows x 128: codes 1024, then per group of 16 rows 32 bytes of scales and 8 of zero points
+    assert lib.vb_group4_bytes(16, 128, 128, 0) == 1024 + 32
+    assert lib.vb_group4_bytes(16, 128, 32, 1) == 1024 + 4 * 40
+    assert lib.vb_group4_bytes(17, 129, 64, 1) == 4 * (1024 + 2 * 40)
+    assert lib.vb_group4_bytes(1, 1, 1024, 0) == 1024 + 32
+    assert lib.vb_group4_bytes(128256, 16384, 128, 1) == 8016 * 128 * (1024 + 40)
+    for bad in ((0, 128), (16, 0), (-1, 128), (1 << 31, 128), (16, 1 << 31)):
+        assert lib.vb_group4_bytes(*bad, 128, 0) == -1
+
+
+@pytest.mark.parametrize("call", [
+    lambda lib: lib.vb_group4_pack(None, PTR, None, PTR, 16, 128, 128, None),
+    lambda lib: lib.vb_group4_pack(PTR, None, None, PTR, 16, 128, 128, None),
+    lambda lib: lib.vb_group4_pack(PTR, PTR, None, PTR + 8, 16, 128, 128, None),
+    lambda lib: lib.vb_group4_quantize(PTR, 3, 128, 16, 128, 128, PTR, PTR, None, None),
+    lambda lib: lib.vb_group4_quantize(PTR, 0, -1, 16, 128, 128, PTR, PTR, None, None),
+    lambda lib: lib.vb_group4_quantize(None, 0, 128, 16, 128, 128, PTR, PTR, None, None),
+    lambda lib: lib.vb_group4_dequant_rows(PTR, None, 16, 128, 128, 0, None),
+    lambda lib: lib.vb_group4_dequant_rows(PTR + 4, PTR, 16, 128, 128, 0, None),
+    lambda lib: lib.vb_group4_gemv(PTR, 16, 128, 128, 0, PTR, 3, 128, 1, PTR, None),
+    lambda lib: lib.vb_group4_gemv(PTR, 16, 128, 128, 0, PTR, 0, 128, -1, PTR, None),
+    lambda lib: lib.vb_group4_gemv(PTR, 16, 128, 128, 0, PTR, 0, -1, 2, PTR, None),
+    lambda lib: lib.vb_group4_gemv(PTR, 16, 0, 128, 0, PTR, 0, 128, 1, PTR, None),
+    lambda lib: lib.vb_group4_gemv(PTR, 16, 128, 48, 0, PTR, 0, 128, 1, PTR, None),
+    lambda lib: lib.vb_group4_gemv(None, 16, 128, 128, 0, PTR, 0, 128, 1, PTR, None),
+    lambda lib: lib.vb_group4_gemv(PTR + 8, 16, 128, 128, 0, PTR, 0, 128, 1, PTR, None),
+])
+def test_group4_refuses(lib, call):
+    assert call(lib) == INVAL
+
+
+def test_group4_gemv_of_no_tokens_does_nothing(lib):
+    assert lib.vb_group4_gemv(PTR, 16, 128, 128, 0, None, 0, 128, 0, None, None) == OK
+
+
+def test_python_calls_take_gpu_tensors_only():
+    x = torch.zeros(2, 8)
+    with pytest.raises(ValueError, match="cuda"):
+        block_norm(x, x)
+    with pytest.raises(ValueError, match="cuda"):
+        token_logprobs(x, torch.zeros(2, dtype=torch.int64))
+    with pytest.raises(ValueError, match="cuda"):
+        GroupQTensor.from_packed(torch.zeros((2, 4), dtype=torch.uint8), torch.zeros((2, 1), dtype=torch.float16), k=8)
+    with pytest.raises(ValueError, match="cuda"):
+        GroupQTensor(torch.zeros(1056, dtype=torch.uint8), 16, 128, 128, False)
+    with pytest.raises(ValueError, match="cuda"):
+        group_gemv(None, x)
+
+
+def test_ctypes_signatures_have_the_header_s_argument_count():
+    import os
+    import re
+    text = open(os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "include", "vbhip.h")).read()
+    text = re.sub(r"/\*.*?\*/", "", text, flags=re.S)
+    for name in ("vb_block_norm", "vb_token_logprobs", "vb_token_logprobs_workspace", "vb_group4_bytes",
+                 "vb_group4_pack", "vb_group4_quantize", "vb_group4_dequant_rows", "vb_group4_gemv"):
+        args = re.search(name + r"\(([^)]*)\)", text).group(1).split(",")
+        sig = _lib.SIGNATURES[name][1]
+        assert len(args) == len(sig), name
+        for a, c in zip(args, sig):
+            want = ctypes.c_void_p if "*" in a else ctypes.c_float if "float" in a else \
+                ctypes.c_size_t if "size_t" in a else ctypes.c_int64 if "int64_t" in a else ctypes.c_int32
+            assert c is want, (name, a)

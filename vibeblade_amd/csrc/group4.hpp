@@ -1,0 +1,44 @@
+// 4-bit weights with one scale (and zero point) per group of a row, as they
+// lie in HBM.
+//
+// Rows are taken 16 at a time and k 128 at a time: a block of 16 x 128 codes
+// is 1 KB, in the order in which the lanes of a wave feed them to
+// v_mfma_f32_16x16x32_f16.  Lane l holds row l % 16 and, in its dword t
+// (t = 0..3, one per 32 of k), the codes of k = 32 t + 8 (l / 16) + 0..7:
+// code 2p at bit 4p and code 2p + 1 at bit 4p + 16, so that a mask gives two
+// neighbours in the halves of a register.  A wave reads a block with one
+// 16-byte load per lane, and block after block along k as one linear stream.
+//
+// Planes, each [row tile][128-step][...]:
+//   codes   1024 bytes
+//   scales  G x 16 rows fp16 (G = 4, 2, 1 groups per 128 for groups of 32, 64
+//           and 128 or more; a longer group repeats its scale)
+//   zeros   G x 16 rows, 4 bits each (row r at bit 4 r of 8 bytes); no plane
+//           for symmetric weights (zero point 8)
+// Rows and k past the tensor have scale 0 and code 0.
+#pragma once
+
+#include <cstdint>
+
+namespace vb {
+
+struct Group4Layout {
+    int64_t tiles, steps, per;  // row tiles, 128-steps, groups per step
+    int64_t scales, zeros, total;  // byte offsets of the planes (codes at 0), bytes in all
+};
+
+// false for shapes and groups that there is no layout for
+inline bool group4_layout(int64_t rows, int64_t k, int32_t group, bool has_zeros, Group4Layout* out) {
+    if (rows <= 0 || k <= 0 || rows > 0x7fffffff || k > 0x7fffff00 || group <= 0) return false;
+    if (group != 32 && group != 64 && group % 128 != 0) return false;
+    out->tiles = (rows + 15) / 16;
+    out->steps = (k + 127) / 128;
+    out->per = group >= 128 ? 1 : 128 / group;
+    const int64_t blocks = out->tiles * out->steps;
+    out->scales = blocks * 1024;
+    out->zeros = out->scales + blocks * out->per * 32;
+    out->total = out->zeros + (has_zeros ? blocks * out->per * 8 : 0);
+    return true;
+}
+
+}  // namespace vb

@@ -5,7 +5,7 @@ executor and callers use: ``is_gpu``, ``drelu``, ``silu``, ``rms_norm``,
 ``softmax`` and ``matmul`` run as libvbhip kernels on the GPU.  ``matmul``
 also takes a ``QTensor`` for ``b`` (GGUF orientation: rows = outputs), which
 is the dequant-fused quantized path (GEMV per row, or the MFMA GEMM for Q4_K
-with two or more rows).  There is no numpy fallback.
+with two or more rows), or a ``GroupQTensor``.  There is no numpy fallback.
 """
 from __future__ import annotations
 
@@ -13,6 +13,7 @@ import numpy as np
 import torch
 
 from . import ggml
+from .group4 import GroupQTensor, group_gemv
 from .tensor import QTensor, as_qtensor, gemv, gemm, activation, _dev, _stream
 from . import _lib
 
@@ -75,8 +76,10 @@ class HipBackend:
 
     def matmul(self, a: np.ndarray, b) -> np.ndarray:
         """C = A x B (vibeblade/gpu.py:148-168).  a: (M, K) fp32.  b: (K, N)
-        fp32, or a ``QTensor`` with N rows of K (GGUF orientation)."""
+        fp32, or a ``QTensor`` / ``GroupQTensor`` with N rows of K (GGUF orientation)."""
         a2 = np.atleast_2d(np.asarray(a, dtype=np.float32))
+        if isinstance(b, GroupQTensor):
+            return group_gemv(b, _to_dev(a2, b.device)).cpu().numpy()
         w = b if isinstance(b, QTensor) else as_qtensor(np.ascontiguousarray(np.asarray(b, dtype=np.float32).T),
                                                         device=self._device)
         if a2.shape[1] != w.k:

@@ -359,3 +359,154 @@ def activation(x: torch.Tensor, kind: int) -> torch.Tensor:
     out = torch.empty_like(x)
     _lib.call("vb_activation", x.data_ptr(), out.data_ptr(), x.numel(), kind, _stream())
     return out
+
+
+# element types of activations (block_norm, token_logprobs, group_gemv)
+_ELEM = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+
+
+def _elem(t: torch.Tensor, what: str) -> int:
+    code = _ELEM.get(t.dtype)
+    if code is None:
+        raise ValueError(f"{what} must be float32, float16 or bfloat16, got {t.dtype}")
+    return code
+
+
+def _gpu_tensor(t, what: str) -> torch.device:
+    if not isinstance(t, torch.Tensor) or t.device.type != "cuda":
+        raise ValueError(f"{what} must be a cuda tensor (vibeblade_amd has no CPU path)")
+    return t.device
+
+
+def _rows_of(t: torch.Tensor, dim: int) -> torch.Tensor:
+    """t as (rows, dim) with unit stride along the row: a view where there is one."""
+    if t.dim() != 2:
+        t = t.reshape(-1, dim)
+    return t if t.stride(1) == 1 or dim == 1 else t.contiguous()
+
+
+def _launch(dev: torch.device, fn: str, *args) -> None:
+    """fn(*args, stream) on the current stream of the device that the tensors are on."""
+    if dev.index == torch.cuda.current_device():
+        _lib.init(dev.index)
+        _lib.call(fn, *args, torch.cuda.current_stream(dev).cuda_stream)
+        return
+    with torch.cuda.device(dev):
+        _lib.init(dev.index)
+        _lib.call(fn, *args, torch.cuda.current_stream(dev).cuda_stream)
+
+
+def _norm_weight(w, dim: int, dev, what: str) -> torch.Tensor | None:
+    if w is None:
+        return None
+    if not (isinstance(w, torch.Tensor) and w.dtype == torch.float32 and w.device == dev and w.is_contiguous()):
+        w = _as_f32_dev(w, dev)
+    if w.numel() != dim:
+        raise ValueError(f"block_norm: {what} has {w.numel()} elements, expected {dim}")
+    return w
+
+
+def block_norm(x: torch.Tensor, branch: torch.Tensor, post_w=None, gate: torch.Tensor | None = None,
+               scale: float = 1.0, pre_w=None, eps: float = 1e-5, normed_dtype: torch.dtype | None = None,
+               out: torch.Tensor | None = None):
+    """The seam between two blocks, in one launch (vb_block_norm): the output ``branch`` of a block joins the
+    residual stream ``x`` and the stream is normalised for the next block.  Returns ``(y, n)``:
+
+        p = rms_norm(branch, post_w, eps)   (branch itself without post_w)
+        y = x + scale * gate * p            (x's type; ``out``, which may be x, or a new tensor)
+        n = rms_norm(y, pre_w, eps)         (``normed_dtype``, x's type by default; None without pre_w)
+
+    x and branch: (..., dim) of one shape, float32 / float16 / bfloat16 each, rows of any stride.  ``gate``
+    broadcasts against x ((dim,), (..., 1), (..., dim)).  n goes straight into ``gemm`` / ``group_gemv``
+    (float16 halves what they read)."""
+    dev = _gpu_tensor(x, "block_norm: x")
+    if x.dim() == 0 or x.shape[-1] == 0:
+        raise ValueError(f"block_norm: x must be (..., dim) with dim > 0, got {tuple(x.shape)}")
+    if _gpu_tensor(branch, "block_norm: branch") != dev or branch.shape != x.shape:
+        raise ValueError(f"block_norm: branch must be {tuple(x.shape)} on {dev}, got {tuple(branch.shape)} on "
+                         f"{branch.device}")
+    dim = x.shape[-1]
+    x_type, b_type = _elem(x, "block_norm: x"), _elem(branch, "block_norm: branch")
+    xr, br = _rows_of(x, dim), _rows_of(branch, dim)
+    rows = xr.shape[0]
+    post, pre = _norm_weight(post_w, dim, dev, "post_w"), _norm_weight(pre_w, dim, dev, "pre_w")
+    g_ptr, g_type, g_row, g_col = None, 0, 0, 0
+    if gate is not None:
+        if _gpu_tensor(gate, "block_norm: gate") != dev:
+            raise ValueError(f"block_norm: gate is on {gate.device}, x on {dev}")
+        g_type = _elem(gate, "block_norm: gate")
+        try:
+            g = gate.expand(x.shape)
+        except RuntimeError:
+            raise ValueError(f"block_norm: gate {tuple(gate.shape)} does not broadcast to {tuple(x.shape)}") from None
+        if g.dim() != 2:
+            g = g.reshape(-1, dim)
+        if g.stride(1) not in (0, 1):
+            g = g.contiguous()
+        g_ptr, g_row, g_col = g.data_ptr(), g.stride(0), g.stride(1)
+    if out is None:
+        out = torch.empty(x.shape, dtype=x.dtype, device=dev)
+    elif not isinstance(out, torch.Tensor) or out.dtype != x.dtype or out.device != dev or out.shape != x.shape:
+        raise ValueError(f"block_norm: out must be {tuple(x.shape)} {x.dtype} on {dev}")
+    try:
+        yr = out if out.dim() == 2 else out.view(-1, dim)
+    except RuntimeError:
+        yr = None
+    if yr is None or (yr.stride(1) != 1 and dim != 1):
+        raise ValueError("block_norm: out must be rows of unit stride")
+    n = nr = None
+    if pre is not None:
+        n = torch.empty(x.shape, dtype=normed_dtype or x.dtype, device=dev)
+        nr = n.view(-1, dim)
+    _launch(dev, "vb_block_norm", br.data_ptr(), b_type, br.stride(0), None if post is None else post.data_ptr(),
+            g_ptr, g_type, g_row, g_col, float(scale), xr.data_ptr(), x_type, xr.stride(0), yr.data_ptr(),
+            yr.stride(0), None if pre is None else pre.data_ptr(), None if nr is None else nr.data_ptr(),
+            0 if nr is None else _elem(n, "block_norm: normed_dtype"), 0 if nr is None else nr.stride(0), rows, dim,
+            float(eps))
+    return out, n
+
+
+TOP_MAX = 64  # alternatives per row of token_logprobs
+
+
+def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor | None, top: int = 0, temperature: float = 1.0):
+    """Log probabilities of given tokens under softmax(logits / temperature), with each row's entropy and its
+    ``top`` (at most 64) most likely alternatives (vb_token_logprobs).  Returns
+    ``(logprobs, entropy, top_ids, top_logprobs)``, float32 (ids int32), of the shapes of ``tokens``, (rows,),
+    (rows, top) and (rows, top).
+
+    logits: (rows, vocab) float32 / float16 / bfloat16 with rows of any stride, as ``gemv`` / ``gemm`` leave them
+    (one row may be (vocab,)).  tokens: (rows,) or (rows, t) ids, int32 or int64; an id outside the vocabulary (a
+    padded position) gives 0; None asks for none.  Alternatives are ordered by logit, equal ones by the lower id;
+    logits of -inf are not named (id -1, log probability -inf), and a row of nothing else has log probabilities
+    -inf and entropy 0.  A row with a NaN or +inf has NaN log probabilities."""
+    dev = _gpu_tensor(logits, "token_logprobs: logits")
+    z = logits.reshape(1, -1) if logits.dim() == 1 else logits
+    if z.dim() != 2 or z.shape[1] == 0:
+        raise ValueError(f"token_logprobs: logits must be (rows, vocab) with vocab > 0, got {tuple(logits.shape)}")
+    kind = _elem(z, "token_logprobs: logits")
+    rows, vocab = z.shape
+    z = _rows_of(z, vocab)
+    top = int(top)
+    if not 0 <= top <= min(TOP_MAX, vocab):
+        raise ValueError(f"token_logprobs: top={top} is out of range (at most {min(TOP_MAX, vocab)})")
+    if tokens is None:
+        tokens = torch.empty((rows, 0), dtype=torch.int32, device=dev)
+    if _gpu_tensor(tokens, "token_logprobs: tokens") != dev:
+        raise ValueError(f"token_logprobs: tokens are on {tokens.device}, logits on {dev}")
+    if tokens.dtype not in (torch.int32, torch.int64):
+        raise ValueError(f"token_logprobs: tokens must be int32 or int64, got {tokens.dtype}")
+    if tokens.dim() not in (1, 2) or tokens.shape[0] != rows:
+        raise ValueError(f"token_logprobs: tokens must be ({rows},) or ({rows}, t), got {tuple(tokens.shape)}")
+    tokens = tokens.contiguous()
+    each = tokens.shape[1] if tokens.dim() == 2 else 1
+    lp = torch.empty(tokens.shape, dtype=torch.float32, device=dev)
+    entropy = torch.empty(rows, dtype=torch.float32, device=dev)
+    ids = torch.empty((rows, top), dtype=torch.int32, device=dev)
+    best = torch.empty((rows, top), dtype=torch.float32, device=dev)
+    nbytes = _lib.load().vb_token_logprobs_workspace(rows, vocab, top)
+    ws = _workspace(nbytes, dev) if nbytes > 0 else None
+    _launch(dev, "vb_token_logprobs", z.data_ptr(), kind, z.stride(0), rows, vocab, float(temperature),
+            tokens.data_ptr(), tokens.element_size(), each, lp.data_ptr(), entropy.data_ptr(), top, ids.data_ptr(),
+            best.data_ptr(), None if ws is None else ws.data_ptr(), max(nbytes, 0))
+    return lp, entropy, ids, best
