@@ -4,10 +4,9 @@
 //
 //   W[n, k] = (q[n, k] - z[n, g]) * s[n, g],   g = k / group,  z = 8 without zeros
 //   y[t, n] = sum_k W[n, k] x[t, k]
-//
-// One wave per row.
 #include "elem_types.hpp"
 #include "group4.hpp"
+#include "vb_internal.hpp"
 #include "../../include/vbhip.h"
 
 namespace vb {
@@ -112,15 +111,330 @@ __global__ void __launch_bounds__(256) g4_quantize_kernel(const void* src, int32
     }
 }
 
-__global__ void __launch_bounds__(256) g4_gemv_kernel(G4Weights g, const void* x, int32_t type, int64_t ld, int m,
-                                                      float* y) {
-    for (int64_t row = first_item() >> 6; row < g.rows; row += item_stride() >> 6)
-        for (int t = 0; t < m; t++) {
-            float s = 0.f;
-            for (int64_t i = threadIdx.x & 63; i < g.k; i += 64) s += g4_value(g, row, i) * elem_ld(x, t * ld + i, type);
-            s = wave_sum_dpp(s);
-            if ((threadIdx.x & 63) == 0) y[t * g.rows + row] = s;
+// ---- products ---------------------------------------------------------------
+//
+// A wave takes a row tile (16 rows) and every KS-th of its 128-steps: one
+// 16-byte load per lane brings a step's codes in the order of the A operand of
+// v_mfma_f32_16x16x32_f16 (group4.hpp).  Two codes become two halves by one
+// mask: in the low bits of the mantissa of 1024 (codes at bits 0-3) or at bit 4
+// of that of 64 (codes at bits 4-7) they are 1024 + q and 64 + q, and a packed
+// subtraction leaves q - z exactly.  The scale stays out of the operand: a
+// group's products are summed in fp32 and then scaled, so nothing is rounded
+// but the sums.
+//
+// The B operand's 16 columns are the tokens.  fp16 activations are taken as
+// they are; fp32 ones as two halves hi + lo in two columns (22 bits), bf16 ones
+// as one (all 8 bits), each block of 128 brought to [2^14, 2^15) by a power of
+// two that the group's sum is multiplied back by.  Columns past the tokens
+// repeat the last one and are dropped.
+typedef _Float16 half2_t __attribute__((ext_vector_type(2)));
+typedef _Float16 half8_t __attribute__((ext_vector_type(8)));
+typedef float float4_t __attribute__((ext_vector_type(4)));
+
+constexpr int G4_WAVES = 8;
+constexpr int G4_THREADS = 64 * G4_WAVES;
+
+struct G4Args {
+    const uint8_t* w;
+    Group4Layout l;
+    const void* x;
+    float* y;
+    int64_t x_ld, rows, k;
+    int32_t m;          // tokens of this launch
+    int32_t ks;         // waves that share a row tile
+    int32_t groups;     // sets of G4_WAVES / ks row tiles
+    int32_t chunk;      // 128-steps of x in LDS at a time
+    bool whole;         // all of x fits: staged once
+};
+
+template <int XT>
+struct XUnit {
+    uint32_t u[XT == ELEM_F32 ? 8 : 4];
+};
+
+template <int XT>
+__device__ __forceinline__ XUnit<XT> x_load(const G4Args& a, int token, int64_t k0) {
+    XUnit<XT> r;
+    if constexpr (XT == ELEM_F32) {
+        typedef uint32_t v4 __attribute__((ext_vector_type(4), aligned(4)));
+        const float* p = static_cast<const float*>(a.x) + token * a.x_ld + k0;
+        if (k0 + 8 <= a.k) {
+            const v4 lo = *reinterpret_cast<const v4*>(p), hi = *reinterpret_cast<const v4*>(p + 4);
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                r.u[i] = lo[i];
+                r.u[4 + i] = hi[i];
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; i++) r.u[i] = k0 + i < a.k ? __float_as_uint(p[i]) : 0u;
         }
+    } else {
+        typedef uint32_t v4 __attribute__((ext_vector_type(4), aligned(2)));
+        const uint16_t* p = static_cast<const uint16_t*>(a.x) + token * a.x_ld + k0;
+        if (k0 + 8 <= a.k) {
+            const v4 v = *reinterpret_cast<const v4*>(p);
+#pragma unroll
+            for (int i = 0; i < 4; i++) r.u[i] = v[i];
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const uint32_t lo = k0 + 2 * i < a.k ? p[2 * i] : 0u, hi = k0 + 2 * i + 1 < a.k ? p[2 * i + 1] : 0u;
+                r.u[i] = lo | hi << 16;
+            }
+        }
+    }
+    return r;
+}
+
+// The largest of 16 lanes' values (a DPP row), in each of them.
+__device__ __forceinline__ float row_max(float v) {
+    v = fmaxf(v, dpp_f<0xB1>(v));
+    v = fmaxf(v, dpp_f<0x4E>(v));
+    v = fmaxf(v, dpp_f<0x141>(v));
+    return fmaxf(v, dpp_f<0x140>(v));
+}
+
+__device__ __forceinline__ uint32_t pack_half2(float a, float b) {
+    const half2_t h = {static_cast<_Float16>(a), static_cast<_Float16>(b)};
+    return __builtin_bit_cast(uint32_t, h);
+}
+
+// A unit's columns into LDS.  xs: [step][t][c][col] of 8 halves; inv: [step][token].
+template <int XT>
+__device__ __forceinline__ void x_store(const XUnit<XT>& r, uint4* xs, float* inv, int cols, int m, int token, int kc) {
+    uint4* at = xs + static_cast<int64_t>(kc) * cols + (XT == ELEM_F32 ? 2 * token : token);
+    if constexpr (XT == ELEM_F16) {
+        *at = make_uint4(r.u[0], r.u[1], r.u[2], r.u[3]);
+    } else {
+        float v[8];
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            if constexpr (XT == ELEM_F32) v[i] = __uint_as_float(r.u[i]);
+            else v[i] = __uint_as_float(i & 1 ? r.u[i >> 1] & 0xffff0000u : r.u[i >> 1] << 16);
+        }
+        // the largest magnitude of the 128 by its bits (NaN and infinity are the largest)
+        uint32_t big = 0;
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            const uint32_t b = __float_as_uint(v[i]) & 0x7fffffffu;
+            big = b > big ? b : big;
+        }
+        const uint32_t top = static_cast<uint32_t>(row_max(static_cast<float>(big >> 23)));  // its exponent
+        // 2^(14 - exponent), within the normal numbers with its reciprocal; 1 for a block without bounds
+        uint32_t f = top == 255 ? 127 : 268 - top;
+        f = f > 253 ? 253 : f;
+        const float scale = __uint_as_float(f << 23);
+        float hi[8];
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            v[i] *= scale;
+            hi[i] = static_cast<float>(static_cast<_Float16>(v[i]));
+        }
+        *at = make_uint4(pack_half2(hi[0], hi[1]), pack_half2(hi[2], hi[3]), pack_half2(hi[4], hi[5]),
+                         pack_half2(hi[6], hi[7]));
+        if constexpr (XT == ELEM_F32) {
+#pragma unroll
+            for (int i = 0; i < 8; i++) v[i] = top == 255 ? 0.f : v[i] - hi[i];
+            at[1] = make_uint4(pack_half2(v[0], v[1]), pack_half2(v[2], v[3]), pack_half2(v[4], v[5]),
+                               pack_half2(v[6], v[7]));
+        }
+        if ((kc & 15) == 0) inv[(kc >> 4) * m + token] = __uint_as_float((254 - f) << 23);
+    }
+}
+
+// The wave's LDS accesses are done, then everyone's; its loads from memory stay in flight.
+__device__ __forceinline__ void lds_barrier() {
+    __builtin_amdgcn_sched_barrier(0);
+    __builtin_amdgcn_s_waitcnt(0xC07F);
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+}
+
+template <int PER, bool ZEROS>
+struct WStep {
+    u32x4 q;
+    uint2 s[PER];
+    uint32_t z[ZEROS ? PER : 1];
+};
+
+template <int PER, bool ZEROS, int XT, int NT>
+__global__ void __launch_bounds__(G4_THREADS) g4_gemv_kernel(G4Args a) {
+    constexpr int DEPTH = 4;
+    constexpr int PARTS = XT == ELEM_F32 ? 2 : 1;
+    extern __shared__ uint4 lds[];
+    const int tid = static_cast<int>(threadIdx.x), lane = tid & 63, n = lane & 15, c = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int cols = PARTS * a.m, ks = a.ks, sub = wave % ks, local = wave / ks, per_group = G4_WAVES / ks;
+    const int steps = static_cast<int>(a.l.steps), tiles = static_cast<int>(a.l.tiles);
+    float4_t* red = reinterpret_cast<float4_t*>(lds);  // [wave][nt][lane]
+    float* inv = reinterpret_cast<float*>(lds + G4_WAVES * NT * 64);
+    uint4* xs = lds + G4_WAVES * NT * 64 + (XT == ELEM_F16 ? 0 : (a.chunk * a.m + 3) / 4);
+    const uint32_t* codes = reinterpret_cast<const uint32_t*>(a.w);
+    const uint8_t* scales = a.w + a.l.scales;
+    const uint8_t* zeros = a.w + a.l.zeros;
+
+    int col[NT];
+#pragma unroll
+    for (int t = 0; t < NT; t++) col[t] = t * 16 + n < cols ? t * 16 + n : cols - 1;
+
+    const int pieces = a.chunk * 16;  // of a token in a chunk
+    auto stage_all = [&](int first) {  // steps first .. first + chunk of x
+        for (int u = tid; u < pieces * a.m; u += G4_THREADS) {
+            const int token = u / pieces, kc = u % pieces;
+            x_store<XT>(x_load<XT>(a, token, (static_cast<int64_t>(first) * 16 + kc) * 8), xs, inv, cols, a.m, token, kc);
+        }
+    };
+
+    for (int grp = static_cast<int>(blockIdx.x); grp < a.groups; grp += static_cast<int>(gridDim.x)) {
+        const int tile_ = grp * per_group + local;
+        const bool live = tile_ < tiles;
+        const int64_t base = static_cast<int64_t>(live ? tile_ : tiles - 1) * steps;
+        auto load = [&](int step, WStep<PER, ZEROS>& r) __attribute__((always_inline)) {
+            const int64_t b = base + (step < steps ? step : steps - 1);
+            r.q = *reinterpret_cast<const u32x4*>(codes + b * 256 + lane * 4);
+#pragma unroll
+            for (int g = 0; g < PER; g++) {
+                r.s[g] = *reinterpret_cast<const uint2*>(scales + (b * PER + g) * 32 + c * 8);
+                if (ZEROS) r.z[g] = *reinterpret_cast<const uint32_t*>(zeros + (b * PER + g) * 8 + (n >> 3) * 4);
+            }
+        };
+        float4_t acc[NT];
+#pragma unroll
+        for (int t = 0; t < NT; t++) acc[t] = float4_t{0.f, 0.f, 0.f, 0.f};
+        WStep<PER, ZEROS> ring[DEPTH];
+        auto multiply = [&](const WStep<PER, ZEROS>& r, int at) __attribute__((always_inline)) {  // step `at` of the chunk
+            const uint4* xb = xs + static_cast<int64_t>(at) * 16 * cols + c * cols;
+            float4_t p[NT];
+            float f[NT];
+            if (XT != ELEM_F16) {
+#pragma unroll
+                for (int t = 0; t < NT; t++) f[t] = inv[at * a.m + col[t] / PARTS];
+            }
+#pragma unroll
+            for (int t = 0; t < 4; t++) {
+                const int g = t * PER / 4;
+                uint32_t z = 8;
+                if (ZEROS) z = (r.z[g] >> ((n & 7) * 4)) & 15;
+                const half2_t z0 = __builtin_bit_cast(half2_t, z * 0x00010001u + 0xE400E400u);  // -(1024 + z)
+                const half2_t z1 = __builtin_bit_cast(half2_t, z * 0x00100010u + 0xD400D400u);  // -(64 + z)
+                const uint32_t q = r.q[t], qh = q >> 8;
+                const half2_t h0 = __builtin_bit_cast(half2_t, (q & 0x000f000fu) | 0x64006400u) + z0;
+                const half2_t h1 = __builtin_bit_cast(half2_t, (q & 0x00f000f0u) | 0x54005400u) + z1;
+                const half2_t h2 = __builtin_bit_cast(half2_t, (qh & 0x000f000fu) | 0x64006400u) + z0;
+                const half2_t h3 = __builtin_bit_cast(half2_t, (qh & 0x00f000f0u) | 0x54005400u) + z1;
+                const half8_t wv = {h0[0], h0[1], h1[0], h1[1], h2[0], h2[1], h3[0], h3[1]};
+#pragma unroll
+                for (int u = 0; u < NT; u++) {
+                    const half8_t xv = __builtin_bit_cast(half8_t, xb[t * 4 * cols + col[u]]);
+                    const float4_t zero = {0.f, 0.f, 0.f, 0.f};
+                    p[u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(wv, xv, t % (4 / PER) == 0 ? zero : p[u], 0, 0, 0);
+                }
+                if ((t + 1) % (4 / PER) == 0) {
+                    const float s0 = f16lo(r.s[g].x), s1 = f16hi(r.s[g].x), s2 = f16lo(r.s[g].y), s3 = f16hi(r.s[g].y);
+#pragma unroll
+                    for (int u = 0; u < NT; u++) {
+                        // (s f) p: f p by itself may leave fp32's range where W x does not
+                        const float fu = XT == ELEM_F16 ? 1.f : f[u];
+                        acc[u][0] += s0 * fu * p[u][0];
+                        acc[u][1] += s1 * fu * p[u][1];
+                        acc[u][2] += s2 * fu * p[u][2];
+                        acc[u][3] += s3 * fu * p[u][3];
+                    }
+                }
+            }
+        };
+
+        const bool first_of_all = grp == static_cast<int>(blockIdx.x);
+#pragma unroll
+        for (int d = 0; d < DEPTH; d++) load(sub + d * ks, ring[d]);
+        for (int first = 0; first < steps; first += a.chunk) {
+            if (!a.whole || first_of_all) {
+                if (!(first == 0 && first_of_all)) lds_barrier();  // the chunk before is read
+                stage_all(first);
+                lds_barrier();
+            }
+            // the wave's steps sub, sub + ks, ... within the chunk (whose length is a multiple of DEPTH * ks)
+            const int end = first + a.chunk < steps ? first + a.chunk : steps;
+            for (int s = first + sub; s < end; s += DEPTH * ks) {
+#pragma unroll
+                for (int d = 0; d < DEPTH; d++) {
+                    const int step = s + d * ks;
+                    if (step < end) multiply(ring[d], step - first);
+                    load(step + DEPTH * ks, ring[d]);
+                }
+            }
+        }
+
+        // y: the waves of a tile, and the two halves of fp32 activations, added in order
+#pragma unroll
+        for (int t = 0; t < NT; t++) red[(wave * NT + t) * 64 + lane] = acc[t];
+        lds_barrier();
+        const float* rf = reinterpret_cast<const float*>(red);
+        for (int o = tid; o < per_group * 16 * a.m; o += G4_THREADS) {
+            const int r = o & 15, tt = (o >> 4) % per_group, token = (o >> 4) / per_group;
+            const int64_t row = (static_cast<int64_t>(grp) * per_group + tt) * 16 + r;
+            float sum = 0.f;
+#pragma unroll
+            for (int h = 0; h < PARTS; h++) {
+                const int cc = PARTS * token + h;
+                for (int v = 0; v < ks; v++)
+                    sum += rf[(((tt * ks + v) * NT + (cc >> 4)) * 64 + (r >> 2) * 16 + (cc & 15)) * 4 + (r & 3)];
+            }
+            if (row < a.rows) a.y[static_cast<int64_t>(token) * a.rows + row] = sum;
+        }
+        lds_barrier();  // red is free
+    }
+}
+
+template <int PER, bool ZEROS, int XT>
+void g4_launch(const G4Args& a, int nt, uint32_t grid, uint32_t lds, hipStream_t st) {
+    if (nt == 1) g4_gemv_kernel<PER, ZEROS, XT, 1><<<grid, G4_THREADS, lds, st>>>(a);
+    else if (nt == 2) g4_gemv_kernel<PER, ZEROS, XT, 2><<<grid, G4_THREADS, lds, st>>>(a);
+    else if constexpr (XT == ELEM_F16) g4_gemv_kernel<PER, ZEROS, XT, 4><<<grid, G4_THREADS, lds, st>>>(a);
+}
+
+template <int PER, bool ZEROS>
+void g4_launch_x(const G4Args& a, int xt, int nt, uint32_t grid, uint32_t lds, hipStream_t st) {
+    if (xt == ELEM_F32) g4_launch<PER, ZEROS, ELEM_F32>(a, nt, grid, lds, st);
+    else if (xt == ELEM_F16) g4_launch<PER, ZEROS, ELEM_F16>(a, nt, grid, lds, st);
+    else g4_launch<PER, ZEROS, ELEM_BF16>(a, nt, grid, lds, st);
+}
+
+constexpr int G4_DEPTH = 4;
+constexpr int64_t G4_LDS = 120 << 10;  // of x in LDS, at most
+
+int g4_run(G4Args a, int x_type, bool has_zeros, hipStream_t st) {
+    const int parts = x_type == ELEM_F32 ? 2 : 1, cols = parts * a.m, nt = cols <= 16 ? 1 : cols <= 32 ? 2 : 4;
+    const int64_t want = 16 * num_cus();  // waves
+    a.ks = 1;
+    while (a.ks < G4_WAVES && a.l.tiles * a.ks < want && a.ks < a.l.steps) a.ks *= 2;
+    // the 128-steps of x that LDS takes (4 at the least: 64 columns are 16 KB a step)
+    const int64_t step_bytes = 256 * cols + (x_type == ELEM_F16 ? 0 : 4 * a.m);
+    int64_t chunk = G4_LDS / step_bytes;
+    a.whole = chunk >= a.l.steps;
+    while (!a.whole && a.ks > 1 && chunk < G4_DEPTH * a.ks) a.ks /= 2;
+    chunk = a.whole ? a.l.steps : chunk / (G4_DEPTH * a.ks) * (G4_DEPTH * a.ks);
+    a.chunk = static_cast<int32_t>(chunk);
+    const int per_group = G4_WAVES / a.ks;
+    a.groups = static_cast<int32_t>((a.l.tiles + per_group - 1) / per_group);
+    const uint32_t lds = static_cast<uint32_t>(G4_WAVES * nt * 1024 + (x_type == ELEM_F16 ? 0 : (chunk * a.m + 3) / 4 * 16) +
+                                               chunk * 256 * cols);
+    const int64_t most = 4 * num_cus();
+    const uint32_t grid = static_cast<uint32_t>(a.groups < most ? a.groups : most);
+    const int per = static_cast<int>(a.l.per);
+    if (has_zeros) {
+        if (per == 1) g4_launch_x<1, true>(a, x_type, nt, grid, lds, st);
+        else if (per == 2) g4_launch_x<2, true>(a, x_type, nt, grid, lds, st);
+        else g4_launch_x<4, true>(a, x_type, nt, grid, lds, st);
+    } else {
+        if (per == 1) g4_launch_x<1, false>(a, x_type, nt, grid, lds, st);
+        else if (per == 2) g4_launch_x<2, false>(a, x_type, nt, grid, lds, st);
+        else g4_launch_x<4, false>(a, x_type, nt, grid, lds, st);
+    }
+    return check_launch("vb_group4_gemv");
 }
 
 // The layout of a call's weights, or an error.
@@ -203,8 +517,15 @@ int vb_group4_gemv(const void* w, int64_t rows, int64_t k, int32_t group, int32_
         set_error("vb_group4_gemv: null pointer, or w not 16-byte aligned");
         return E_INVAL;
     }
-    g4_gemv_kernel<<<item_blocks(rows * 64), 256, 0, as_stream(stream)>>>(g, x, x_type, x_ld, static_cast<int>(m), y);
-    return check_launch("vb_group4_gemv");
+    // tokens a launch takes: 32 columns of scaled activations, 64 of fp16 ones (the registers of four column tiles)
+    const int64_t slab = x_type == ELEM_F32 ? 16 : x_type == ELEM_F16 ? 64 : 32;
+    for (int64_t t = 0; t < m; t += slab) {
+        const void* xt = static_cast<const uint8_t*>(x) + t * x_ld * elem_bytes(x_type);
+        const G4Args a{g.w, g.l, xt, y + t * rows, x_ld, rows, k, static_cast<int32_t>(m - t < slab ? m - t : slab),
+                       0, 0, 0, false};
+        if (const int rc = g4_run(a, x_type, g.has_zeros, as_stream(stream)); rc != OK) return rc;
+    }
+    return OK;
 }
 
 }  // extern "C"
