@@ -23,14 +23,17 @@ __device__ __forceinline__ int64_t block_of(const G4Weights& g, int64_t row, int
     return (row >> 4) * g.l.steps + (k >> 7);
 }
 
+// Row r's scale of group g among the 16 x per of a block.
+__device__ __forceinline__ int scale_at(int r, int g, int per) { return ((r >> 2) * per + g) * 4 + (r & 3); }
+
 __device__ __forceinline__ float g4_value(const G4Weights& g, int64_t row, int64_t k) {
     const int64_t b = block_of(g, row, k);
     const int r = static_cast<int>(row & 15), kk = static_cast<int>(k & 127), j = kk & 7;
     const uint32_t word = reinterpret_cast<const uint32_t*>(g.w)[b * 256 + (((kk >> 3) & 3) * 16 + r) * 4 + (kk >> 5)];
     const int q = (word >> ((j >> 1) * 4 + (j & 1) * 16)) & 15;
-    const int64_t gi = b * g.l.per + (kk * g.l.per >> 7);
-    const float s = static_cast<float>(reinterpret_cast<const _Float16*>(g.w + g.l.scales)[gi * 16 + r]);
-    const int z = g.has_zeros ? (g.w[g.l.zeros + gi * 8 + (r >> 1)] >> ((r & 1) * 4)) & 15 : 8;
+    const int per = static_cast<int>(g.l.per), gi = kk * per >> 7, zi = r * per + gi;
+    const float s = static_cast<float>(reinterpret_cast<const _Float16*>(g.w + g.l.scales)[b * per * 16 + scale_at(r, gi, per)]);
+    const int z = g.has_zeros ? (g.w[g.l.zeros + b * per * 8 + (zi >> 1)] >> ((zi & 1) * 4)) & 15 : 8;
     return static_cast<float>(q - z) * s;
 }
 
@@ -40,7 +43,7 @@ __device__ __forceinline__ int64_t first_item() { return static_cast<int64_t>(bl
 __device__ __forceinline__ int64_t item_stride() { return static_cast<int64_t>(gridDim.x) * 256; }
 uint32_t item_blocks(int64_t n) { return static_cast<uint32_t>(n > (1 << 28) ? 1 << 20 : (n + 255) / 256); }
 
-// One thread per dword of codes, then per group of 16 scales (and zeros).
+// One thread per dword of codes, then per block's scales and zero points.
 __global__ void __launch_bounds__(256) g4_pack_codes_kernel(const uint8_t* packed, uint32_t* out, Group4Layout l,
                                                             int64_t rows, int64_t k) {
     for (int64_t i = first_item(); i < l.tiles * l.steps * 256; i += item_stride()) {
@@ -58,20 +61,23 @@ __global__ void __launch_bounds__(256) g4_pack_codes_kernel(const uint8_t* packe
 }
 
 __global__ void __launch_bounds__(256) g4_pack_groups_kernel(const _Float16* scales, const uint8_t* zeros, uint8_t* out,
-                                                             Group4Layout l, int64_t rows, int64_t k, int32_t group,
-                                                             int64_t groups) {
-    for (int64_t i = first_item(); i < l.tiles * l.steps * l.per; i += item_stride()) {
-        const int64_t b = i / l.per, tile = b / l.steps;
-        const int64_t gi = (b % l.steps * 128 + i % l.per * (128 / l.per)) / group;
-        uint64_t zs = 0;
-        for (int r = 0; r < 16; r++) {
-            const int64_t row = tile * 16 + r;
-            const bool in = row < rows && gi < groups;
-            reinterpret_cast<_Float16*>(out + l.scales)[i * 16 + r] =
-                in ? scales[row * groups + gi] : static_cast<_Float16>(0.f);
-            if (zeros && in) zs |= static_cast<uint64_t>(zeros[row * groups + gi] & 15) << (4 * r);
+                                                             Group4Layout l, int64_t rows, int32_t group, int64_t groups) {
+    const int per = static_cast<int>(l.per);
+    for (int64_t b = first_item(); b < l.tiles * l.steps; b += item_stride()) {
+        const int64_t tile = b / l.steps, k0 = b % l.steps * 128;
+        _Float16* so = reinterpret_cast<_Float16*>(out + l.scales) + b * per * 16;
+        uint8_t* zo = out + l.zeros + b * per * 8;
+        for (int i = 0; i < 16 * per; i += 2) {  // a byte of zero points: rows or groups next to each other
+            uint32_t zs = 0;
+            for (int h = 0; h < 2; h++) {
+                const int r = (i + h) / per, g = (i + h) % per;
+                const int64_t row = tile * 16 + r, gi = (k0 + g * (128 / per)) / group;
+                const bool in = row < rows && gi < groups;
+                so[scale_at(r, g, per)] = in ? scales[row * groups + gi] : static_cast<_Float16>(0.f);
+                if (zeros && in) zs |= (zeros[row * groups + gi] & 15u) << (4 * h);
+            }
+            if (zeros) zo[i >> 1] = static_cast<uint8_t>(zs);
         }
-        if (zeros) reinterpret_cast<uint64_t*>(out + l.zeros)[i] = zs;
     }
 }
 
@@ -187,6 +193,57 @@ __device__ __forceinline__ XUnit<XT> x_load(const G4Args& a, int token, int64_t 
     return r;
 }
 
+// The same without a branch around a load: a piece that reaches past k (k >= 8)
+// takes the row's last eight values and moves its own to the front.
+template <int XT>
+__device__ __forceinline__ XUnit<XT> x_load_whole(const G4Args& a, int token, int64_t k0) {
+    XUnit<XT> r;
+    k0 = k0 + 8 <= a.k ? k0 : a.k - 8;
+    if constexpr (XT == ELEM_F32) {
+        typedef uint32_t v4 __attribute__((ext_vector_type(4), aligned(4)));
+        const v4* p = reinterpret_cast<const v4*>(static_cast<const float*>(a.x) + token * a.x_ld + k0);
+        const v4 lo = p[0], hi = p[1];
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            r.u[i] = lo[i];
+            r.u[4 + i] = hi[i];
+        }
+    } else {
+        typedef uint32_t v4 __attribute__((ext_vector_type(4), aligned(2)));
+        const v4 v = *reinterpret_cast<const v4*>(static_cast<const uint16_t*>(a.x) + token * a.x_ld + k0);
+#pragma unroll
+        for (int i = 0; i < 4; i++) r.u[i] = v[i];
+    }
+    return r;
+}
+
+template <int XT>
+__device__ __forceinline__ void x_shift(XUnit<XT>& r, int by) {  // values `by`.. of the eight to the front, zeros behind
+    if constexpr (XT == ELEM_F32) {
+#pragma unroll
+        for (int b = 4; b >= 1; b >>= 1) {
+            if (!(by & b)) continue;
+#pragma unroll
+            for (int i = 0; i < 8; i++) r.u[i] = i + b < 8 ? r.u[i + b] : 0u;
+        }
+        if (by & 8) {
+#pragma unroll
+            for (int i = 0; i < 8; i++) r.u[i] = 0u;
+        }
+    } else {
+#pragma unroll
+        for (int b = 4; b >= 1; b >>= 1) {
+            if (!(by & (2 * b))) continue;
+#pragma unroll
+            for (int i = 0; i < 4; i++) r.u[i] = i + b < 4 ? r.u[i + b] : 0u;
+        }
+        if (by & 1) {
+#pragma unroll
+            for (int i = 0; i < 4; i++) r.u[i] = r.u[i] >> 16 | (i < 3 ? r.u[i + 1] << 16 : 0u);
+        }
+    }
+}
+
 // The largest of 16 lanes' values (a DPP row), in each of them.
 __device__ __forceinline__ float row_max(float v) {
     v = fmaxf(v, dpp_f<0xB1>(v));
@@ -253,16 +310,22 @@ __device__ __forceinline__ void lds_barrier() {
     __builtin_amdgcn_sched_barrier(0);
 }
 
+typedef _Float16 half4_t __attribute__((ext_vector_type(4)));
+
+// What a wave loads of one block.
 template <int PER, bool ZEROS>
 struct WStep {
     u32x4 q;
-    uint2 s[PER];
-    uint32_t z[ZEROS ? PER : 1];
+    half4_t s[PER];
+    uint32_t z;  // zero points of 8 / PER rows, the lane's among them
 };
 
+template <int PER>
+constexpr int g4_depth() { return PER == 1 ? 8 : 4; }  // blocks in flight per wave
+
 template <int PER, bool ZEROS, int XT, int NT>
-__global__ void __launch_bounds__(G4_THREADS) g4_gemv_kernel(G4Args a) {
-    constexpr int DEPTH = 4;
+__global__ void __launch_bounds__(G4_THREADS, NT == 4 ? 2 : 4) g4_gemv_kernel(G4Args a) {
+    constexpr int DEPTH = g4_depth<PER>();
     constexpr int PARTS = XT == ELEM_F32 ? 2 : 1;
     extern __shared__ uint4 lds[];
     const int tid = static_cast<int>(threadIdx.x), lane = tid & 63, n = lane & 15, c = lane >> 4;
@@ -270,104 +333,171 @@ __global__ void __launch_bounds__(G4_THREADS) g4_gemv_kernel(G4Args a) {
     const int cols = PARTS * a.m, ks = a.ks, sub = wave % ks, local = wave / ks, per_group = G4_WAVES / ks;
     const int steps = static_cast<int>(a.l.steps), tiles = static_cast<int>(a.l.tiles);
     float4_t* red = reinterpret_cast<float4_t*>(lds);  // [wave][nt][lane]
-    float* inv = reinterpret_cast<float*>(lds + G4_WAVES * NT * 64);
-    uint4* xs = lds + G4_WAVES * NT * 64 + (XT == ELEM_F16 ? 0 : (a.chunk * a.m + 3) / 4);
-    const uint32_t* codes = reinterpret_cast<const uint32_t*>(a.w);
-    const uint8_t* scales = a.w + a.l.scales;
-    const uint8_t* zeros = a.w + a.l.zeros;
+    float* inv = reinterpret_cast<float*>(lds + (ks > 1 ? G4_WAVES * NT * 64 : 0));
+    uint4* xs = reinterpret_cast<uint4*>(inv) + (XT == ELEM_F16 ? 0 : (a.chunk * a.m + 3) / 4);
 
     int col[NT];
 #pragma unroll
     for (int t = 0; t < NT; t++) col[t] = t * 16 + n < cols ? t * 16 + n : cols - 1;
 
-    const int pieces = a.chunk * 16;  // of a token in a chunk
-    auto stage_all = [&](int first) {  // steps first .. first + chunk of x
-        for (int u = tid; u < pieces * a.m; u += G4_THREADS) {
+    const int pieces = a.chunk * 16, units = pieces * a.m;  // of a token, of all tokens in a chunk
+    auto stage = [&](int first, int from) {                 // pieces from .. of steps first .. first + chunk of x
+#pragma unroll 1
+        for (int u = from + tid; u < units; u += G4_THREADS) {
             const int token = u / pieces, kc = u % pieces;
             x_store<XT>(x_load<XT>(a, token, (static_cast<int64_t>(first) * 16 + kc) * 8), xs, inv, cols, a.m, token, kc);
         }
     };
-
-    for (int grp = static_cast<int>(blockIdx.x); grp < a.groups; grp += static_cast<int>(gridDim.x)) {
-        const int tile_ = grp * per_group + local;
-        const bool live = tile_ < tiles;
-        const int64_t base = static_cast<int64_t>(live ? tile_ : tiles - 1) * steps;
-        auto load = [&](int step, WStep<PER, ZEROS>& r) __attribute__((always_inline)) {
-            const int64_t b = base + (step < steps ? step : steps - 1);
-            r.q = *reinterpret_cast<const u32x4*>(codes + b * 256 + lane * 4);
+    // Loads of the ring: a step or tile past the last is outside of its
+    // buffer and reads nothing.  (A branch around a load would make the
+    // compiler wait for all loads in flight.)
+    auto load = [&](int tile, int step, WStep<PER, ZEROS>& r) __attribute__((always_inline)) {
+        const bool in = tile < tiles;
+        const int64_t b = in ? static_cast<int64_t>(tile) * steps : 0;
+        const uint32_t size = in ? static_cast<uint32_t>(steps) : 0u;
+        const __amdgpu_buffer_rsrc_t rq = make_rsrc(a.w + b * 1024, size * 1024);
+        const __amdgpu_buffer_rsrc_t rs = make_rsrc(a.w + a.l.scales + b * (32 * PER), size * (32 * PER));
+        r.q = buf_ld128(rq, static_cast<uint32_t>(step) * 1024 + lane * 16, 0);
+        const uint32_t so = (static_cast<uint32_t>(step) * 4 + c) * (8 * PER);
+        if constexpr (PER == 1) {
+            typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+            r.s[0] = __builtin_bit_cast(half4_t, __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(rs, static_cast<int>(so), 0, 0)));
+        } else {
 #pragma unroll
-            for (int g = 0; g < PER; g++) {
-                r.s[g] = *reinterpret_cast<const uint2*>(scales + (b * PER + g) * 32 + c * 8);
-                if (ZEROS) r.z[g] = *reinterpret_cast<const uint32_t*>(zeros + (b * PER + g) * 8 + (n >> 3) * 4);
+            for (int g = 0; g < PER; g += 2) {
+                const half8_t v = __builtin_bit_cast(half8_t, buf_ld128(rs, so + 8 * g, 0));
+                r.s[g] = half4_t{v[0], v[1], v[2], v[3]};
+                r.s[g + 1] = half4_t{v[4], v[5], v[6], v[7]};
             }
-        };
-        float4_t acc[NT];
+        }
+        if constexpr (ZEROS) {
+            const __amdgpu_buffer_rsrc_t rz = make_rsrc(a.w + a.l.zeros + b * (8 * PER), size * (8 * PER));
+            r.z = __builtin_amdgcn_raw_buffer_load_b32(rz, static_cast<int>(step * (8 * PER) + n * PER / 8 * 4), 0, 0);
+        }
+        __builtin_amdgcn_sched_barrier(0);  // slot after slot, as they are waited for
+    };
+    float4_t acc[NT];
+    auto multiply = [&](const WStep<PER, ZEROS>& r, int at) __attribute__((always_inline)) {  // step `at` of the chunk
+        const uint4* xb = xs + (at * 16 + c) * cols;
+        float4_t p[NT], sum[NT];
+        half8_t xv[4][NT];
 #pragma unroll
-        for (int t = 0; t < NT; t++) acc[t] = float4_t{0.f, 0.f, 0.f, 0.f};
-        WStep<PER, ZEROS> ring[DEPTH];
-        auto multiply = [&](const WStep<PER, ZEROS>& r, int at) __attribute__((always_inline)) {  // step `at` of the chunk
-            const uint4* xb = xs + static_cast<int64_t>(at) * 16 * cols + c * cols;
-            float4_t p[NT];
-            float f[NT];
-            if (XT != ELEM_F16) {
+        for (int t = 0; t < 4; t++)
 #pragma unroll
-                for (int t = 0; t < NT; t++) f[t] = inv[at * a.m + col[t] / PARTS];
-            }
+            for (int u = 0; u < NT; u++) xv[t][u] = __builtin_bit_cast(half8_t, xb[t * 4 * cols + col[u]]);
 #pragma unroll
-            for (int t = 0; t < 4; t++) {
-                const int g = t * PER / 4;
-                uint32_t z = 8;
-                if (ZEROS) z = (r.z[g] >> ((n & 7) * 4)) & 15;
-                const half2_t z0 = __builtin_bit_cast(half2_t, z * 0x00010001u + 0xE400E400u);  // -(1024 + z)
-                const half2_t z1 = __builtin_bit_cast(half2_t, z * 0x00100010u + 0xD400D400u);  // -(64 + z)
-                const uint32_t q = r.q[t], qh = q >> 8;
-                const half2_t h0 = __builtin_bit_cast(half2_t, (q & 0x000f000fu) | 0x64006400u) + z0;
-                const half2_t h1 = __builtin_bit_cast(half2_t, (q & 0x00f000f0u) | 0x54005400u) + z1;
-                const half2_t h2 = __builtin_bit_cast(half2_t, (qh & 0x000f000fu) | 0x64006400u) + z0;
-                const half2_t h3 = __builtin_bit_cast(half2_t, (qh & 0x00f000f0u) | 0x54005400u) + z1;
-                const half8_t wv = {h0[0], h0[1], h1[0], h1[1], h2[0], h2[1], h3[0], h3[1]};
+        for (int t = 0; t < 4; t++) {
+            const int g = t * PER / 4;
+            uint32_t z = 8;
+            if (ZEROS) z = (r.z >> (n * PER % 8 * 4 + 4 * g)) & 15;
+            const half2_t z0 = __builtin_bit_cast(half2_t, z * 0x00010001u + 0xE400E400u);  // -(1024 + z)
+            const half2_t z1 = __builtin_bit_cast(half2_t, z * 0x00100010u + 0xD400D400u);  // -(64 + z)
+            const uint32_t q = r.q[t], qh = q >> 8;
+            const half2_t h0 = __builtin_bit_cast(half2_t, (q & 0x000f000fu) | 0x64006400u) + z0;
+            const half2_t h1 = __builtin_bit_cast(half2_t, (q & 0x00f000f0u) | 0x54005400u) + z1;
+            const half2_t h2 = __builtin_bit_cast(half2_t, (qh & 0x000f000fu) | 0x64006400u) + z0;
+            const half2_t h3 = __builtin_bit_cast(half2_t, (qh & 0x00f000f0u) | 0x54005400u) + z1;
+            const half8_t wv = {h0[0], h0[1], h1[0], h1[1], h2[0], h2[1], h3[0], h3[1]};
 #pragma unroll
-                for (int u = 0; u < NT; u++) {
-                    const half8_t xv = __builtin_bit_cast(half8_t, xb[t * 4 * cols + col[u]]);
-                    const float4_t zero = {0.f, 0.f, 0.f, 0.f};
-                    p[u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(wv, xv, t % (4 / PER) == 0 ? zero : p[u], 0, 0, 0);
-                }
+            for (int u = 0; u < NT; u++) {
+                const float4_t zero = {0.f, 0.f, 0.f, 0.f};
+                p[u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(wv, xv[t][u], t % (4 / PER) == 0 ? zero : p[u], 0, 0, 0);
                 if ((t + 1) % (4 / PER) == 0) {
-                    const float s0 = f16lo(r.s[g].x), s1 = f16hi(r.s[g].x), s2 = f16lo(r.s[g].y), s3 = f16hi(r.s[g].y);
+                    // fp16 x adds to acc; the others to the block's sum, which then takes the block's power of two
+                    float4_t& to = XT == ELEM_F16 ? acc[u] : sum[u];
 #pragma unroll
-                    for (int u = 0; u < NT; u++) {
-                        // (s f) p: f p by itself may leave fp32's range where W x does not
-                        const float fu = XT == ELEM_F16 ? 1.f : f[u];
-                        acc[u][0] += s0 * fu * p[u][0];
-                        acc[u][1] += s1 * fu * p[u][1];
-                        acc[u][2] += s2 * fu * p[u][2];
-                        acc[u][3] += s3 * fu * p[u][3];
+                    for (int i = 0; i < 4; i++) {
+                        const float s = static_cast<float>(r.s[g][i]);
+                        to[i] = XT != ELEM_F16 && g == 0 ? s * p[u][i] : __builtin_fmaf(s, p[u][i], to[i]);
                     }
                 }
             }
-        };
-
-        const bool first_of_all = grp == static_cast<int>(blockIdx.x);
+        }
+        if (XT != ELEM_F16) {
 #pragma unroll
-        for (int d = 0; d < DEPTH; d++) load(sub + d * ks, ring[d]);
-        for (int first = 0; first < steps; first += a.chunk) {
-            if (!a.whole || first_of_all) {
-                if (!(first == 0 && first_of_all)) lds_barrier();  // the chunk before is read
-                stage_all(first);
-                lds_barrier();
-            }
-            // the wave's steps sub, sub + ks, ... within the chunk (whose length is a multiple of DEPTH * ks)
-            const int end = first + a.chunk < steps ? first + a.chunk : steps;
-            for (int s = first + sub; s < end; s += DEPTH * ks) {
+            for (int u = 0; u < NT; u++) {
+                const float f = inv[at * a.m + col[u] / PARTS];
 #pragma unroll
-                for (int d = 0; d < DEPTH; d++) {
-                    const int step = s + d * ks;
-                    if (step < end) multiply(ring[d], step - first);
-                    load(step + DEPTH * ks, ring[d]);
-                }
+                for (int i = 0; i < 4; i++) acc[u][i] = __builtin_fmaf(f, sum[u][i], acc[u][i]);
             }
         }
+    };
 
+    // The wave's steps of a tile: sub, sub + ks, ..., in rounds of DEPTH; the
+    // last rounds load the next tile's first ones.
+    const int rounds = (steps + ks * DEPTH - 1) / (ks * DEPTH);
+    const int hop = static_cast<int>(gridDim.x) * per_group;
+    int tile = static_cast<int>(blockIdx.x) * per_group + local;
+    WStep<PER, ZEROS> ring[DEPTH];
+    // x first, as loads come back in order: pieces past HELD per thread, then
+    // HELD of them on the way together with the ring's first round.
+    constexpr int HELD = 4;
+    XUnit<XT> held[HELD];
+    const bool hold = a.k >= 8;
+    stage(0, hold ? HELD * G4_THREADS : 0);
+    if (hold) {
+#pragma unroll
+        for (int i = 0; i < HELD; i++) {
+            const int u = i * G4_THREADS + tid, v = u < units ? u : units - 1;
+            held[i] = x_load_whole<XT>(a, v / pieces, static_cast<int64_t>(v % pieces) * 8);
+        }
+    }
+#pragma unroll
+    for (int d = 0; d < DEPTH; d++) load(tile, sub + d * ks, ring[d]);
+    if (hold) {
+#pragma unroll
+        for (int i = 0; i < HELD; i++) {
+            const int u = i * G4_THREADS + tid;
+            if (u >= units) continue;
+            const int token = u / pieces, kc = u % pieces;
+            if (kc * 8 + 8 > a.k) x_shift<XT>(held[i], static_cast<int>(kc * 8 >= a.k ? 8 : kc * 8 + 8 - a.k));
+            x_store<XT>(held[i], xs, inv, cols, a.m, token, kc);
+        }
+    }
+    lds_barrier();
+    bool staged = true;  // the chunk in LDS is the next one to be used
+    for (int grp = static_cast<int>(blockIdx.x); grp < a.groups; grp += static_cast<int>(gridDim.x), tile += hop) {
+#pragma unroll
+        for (int t = 0; t < NT; t++) acc[t] = float4_t{0.f, 0.f, 0.f, 0.f};
+        int first = 0;  // of the chunk (whose length is whole rounds)
+        for (int i = 0; i < rounds; i++) {
+            const int s = i * ks * DEPTH + sub;
+            if (s - sub == first + a.chunk) first += a.chunk;
+            if (!a.whole && s - sub == first) {
+                if (!staged) {
+                    lds_barrier();  // the chunk before is read
+                    stage(first, 0);
+                    lds_barrier();
+                }
+                staged = false;
+            }
+            const bool last = i + 1 == rounds;
+            const int next = last ? tile + hop : tile, from = last ? sub : s + DEPTH * ks;
+#pragma unroll
+            for (int d = 0; d < DEPTH; d++) {
+                if (tile < tiles && s + d * ks < steps) multiply(ring[d], s + d * ks - first);
+                load(next, from + d * ks, ring[d]);
+            }
+        }
+        if (ks == 1) {
+            // the wave's tile is done: its lanes hold rows 4 c + 0..3 of column n
+#pragma unroll
+            for (int t = 0; t < NT; t++) {
+                if (PARTS == 2) {
+#pragma unroll
+                    for (int i = 0; i < 4; i++) acc[t][i] += dpp_f<0xB1>(acc[t][i]);
+                }
+                const int cc = t * 16 + n;
+                const int64_t row = static_cast<int64_t>(tile) * 16 + 4 * c;
+                if (tile < tiles && cc < cols && cc % PARTS == 0) {
+                    float* y = a.y + static_cast<int64_t>(cc / PARTS) * a.rows + row;
+#pragma unroll
+                    for (int i = 0; i < 4; i++)
+                        if (row + i < a.rows) y[i] = acc[t][i];
+                }
+            }
+            continue;
+        }
         // y: the waves of a tile, and the two halves of fp32 activations, added in order
 #pragma unroll
         for (int t = 0; t < NT; t++) red[(wave * NT + t) * 64 + lane] = acc[t];
@@ -403,26 +533,27 @@ void g4_launch_x(const G4Args& a, int xt, int nt, uint32_t grid, uint32_t lds, h
     else g4_launch<PER, ZEROS, ELEM_BF16>(a, nt, grid, lds, st);
 }
 
-constexpr int G4_DEPTH = 4;
 constexpr int64_t G4_LDS = 120 << 10;  // of x in LDS, at most
 
 int g4_run(G4Args a, int x_type, bool has_zeros, hipStream_t st) {
     const int parts = x_type == ELEM_F32 ? 2 : 1, cols = parts * a.m, nt = cols <= 16 ? 1 : cols <= 32 ? 2 : 4;
-    const int64_t want = 16 * num_cus();  // waves
+    const int depth = a.l.per == 1 ? g4_depth<1>() : g4_depth<4>();
+    const int64_t slots = 16 * num_cus();  // waves that are resident at once
     a.ks = 1;
-    while (a.ks < G4_WAVES && a.l.tiles * a.ks < want && a.ks < a.l.steps) a.ks *= 2;
-    // the 128-steps of x that LDS takes (4 at the least: 64 columns are 16 KB a step)
+    while (a.ks < G4_WAVES && a.l.tiles * a.ks * 2 <= slots && a.ks < a.l.steps) a.ks *= 2;
+    // the 128-steps of x that LDS takes, whole rounds of the ring (64 columns are 16 KB a step)
     const int64_t step_bytes = 256 * cols + (x_type == ELEM_F16 ? 0 : 4 * a.m);
     int64_t chunk = G4_LDS / step_bytes;
     a.whole = chunk >= a.l.steps;
-    while (!a.whole && a.ks > 1 && chunk < G4_DEPTH * a.ks) a.ks /= 2;
-    chunk = a.whole ? a.l.steps : chunk / (G4_DEPTH * a.ks) * (G4_DEPTH * a.ks);
+    while (!a.whole && a.ks > 1 && chunk < depth * a.ks) a.ks /= 2;
+    chunk = a.whole ? a.l.steps : chunk / (depth * a.ks) * (depth * a.ks);
+    if (chunk == 0) chunk = depth;
     a.chunk = static_cast<int32_t>(chunk);
     const int per_group = G4_WAVES / a.ks;
     a.groups = static_cast<int32_t>((a.l.tiles + per_group - 1) / per_group);
-    const uint32_t lds = static_cast<uint32_t>(G4_WAVES * nt * 1024 + (x_type == ELEM_F16 ? 0 : (chunk * a.m + 3) / 4 * 16) +
-                                               chunk * 256 * cols);
-    const int64_t most = 4 * num_cus();
+    const uint32_t lds = static_cast<uint32_t>((a.ks > 1 ? G4_WAVES * nt * 1024 : 0) +
+                                               (x_type == ELEM_F16 ? 0 : (chunk * a.m + 3) / 4 * 16) + chunk * 256 * cols);
+    const int64_t most = (lds > (80 << 10) ? 1 : 2) * num_cus();
     const uint32_t grid = static_cast<uint32_t>(a.groups < most ? a.groups : most);
     const int per = static_cast<int>(a.l.per);
     if (has_zeros) {
@@ -471,8 +602,8 @@ int vb_group4_pack(const uint8_t* packed, const void* scales, const uint8_t* zer
     g4_pack_codes_kernel<<<item_blocks(l.tiles * l.steps * 256), 256, 0, st>>>(packed, static_cast<uint32_t*>(w), l,
                                                                                   rows, k);
     if (const int rc = check_launch("vb_group4_pack"); rc != OK) return rc;
-    g4_pack_groups_kernel<<<item_blocks(l.tiles * l.steps * l.per), 256, 0, st>>>(
-        static_cast<const _Float16*>(scales), zeros, static_cast<uint8_t*>(w), l, rows, k, group, (k + group - 1) / group);
+    g4_pack_groups_kernel<<<item_blocks(l.tiles * l.steps), 256, 0, st>>>(
+        static_cast<const _Float16*>(scales), zeros, static_cast<uint8_t*>(w), l, rows, group, (k + group - 1) / group);
     return check_launch("vb_group4_pack");
 }
 

@@ -11,10 +11,12 @@
 //
 // Planes, each [row tile][128-step][...]:
 //   codes   1024 bytes
-//   scales  G x 16 rows fp16 (G = 4, 2, 1 groups per 128 for groups of 32, 64
-//           and 128 or more; a longer group repeats its scale)
-//   zeros   G x 16 rows, 4 bits each (row r at bit 4 r of 8 bytes); no plane
-//           for symmetric weights (zero point 8)
+//   scales  4 x G x 4 fp16 (G = 4, 2, 1 groups per 128 for groups of 32, 64
+//           and 128 or more; a longer group repeats its scale): the scales
+//           that lane l multiplies its four outputs (rows 4 (l / 16) + 0..3)
+//           by lie together
+//   zeros   16 x G values of 4 bits, row by row; no plane for symmetric
+//           weights (zero point 8)
 // Rows and k past the tensor have scale 0 and code 0.
 #pragma once
 
@@ -29,7 +31,7 @@ struct Group4Layout {
 
 // false for shapes and groups that there is no layout for
 inline bool group4_layout(int64_t rows, int64_t k, int32_t group, bool has_zeros, Group4Layout* out) {
-    if (rows <= 0 || k <= 0 || rows > 0x7fffffff || k > 0x7fffff00 || group <= 0) return false;
+    if (rows <= 0 || k <= 0 || rows > 0x7fffffff || k > 1 << 28 || group <= 0) return false;  // a row tile below 4 GB
     if (group != 32 && group != 64 && group % 128 != 0) return false;
     out->tiles = (rows + 15) / 16;
     out->steps = (k + 127) / 128;
