@@ -28,13 +28,13 @@ __device__ __forceinline__ int scale_at(int r, int g, int per) { return ((r >> 2
 
 __device__ __forceinline__ float g4_value(const G4Weights& g, int64_t row, int64_t k) {
     const int64_t b = block_of(g, row, k);
-    const int r = static_cast<int>(row & 15), kk = static_cast<int>(k & 127), j = kk & 7;
+    const int r = static_cast<int>(row & 15), kk = static_cast<int>(k & 127);
     const uint32_t word = reinterpret_cast<const uint32_t*>(g.w)[b * 256 + (((kk >> 3) & 3) * 16 + r) * 4 + (kk >> 5)];
-    const int q = (word >> ((j >> 1) * 4 + (j & 1) * 16)) & 15;
-    const int per = static_cast<int>(g.l.per), gi = kk * per >> 7, zi = r * per + gi;
-    const float s = static_cast<float>(reinterpret_cast<const _Float16*>(g.w + g.l.scales)[b * per * 16 + scale_at(r, gi, per)]);
-    const int z = g.has_zeros ? (g.w[g.l.zeros + b * per * 8 + (zi >> 1)] >> ((zi & 1) * 4)) & 15 : 8;
-    return static_cast<float>(q - z) * s;
+    const int q = (word >> (kk & 7) * 4) & 15;
+    const int per = static_cast<int>(g.l.per), at = scale_at(r, kk * per >> 7, per);
+    const float s = static_cast<float>(reinterpret_cast<const _Float16*>(g.w + g.l.scales)[b * per * 16 + at]);
+    const int z = g.has_zeros ? (g.w[g.l.zeros + b * per * 8 + (at >> 1)] >> ((at & 1) * 4)) & 15 : 0;
+    return static_cast<float>((q ^ 8) - (z ^ 8)) * s;
 }
 
 // Work items of 256-thread workgroups, as many per thread as it takes: a
@@ -54,7 +54,7 @@ __global__ void __launch_bounds__(256) g4_pack_codes_kernel(const uint8_t* packe
         if (row < rows)
             for (int j = 0; j < 8 && k0 + j < k; j++) {
                 const uint32_t byte = packed[row * ((k + 1) >> 1) + ((k0 + j) >> 1)];
-                word |= ((j & 1 ? byte >> 4 : byte) & 15u) << ((j >> 1) * 4 + (j & 1) * 16);
+                word |= (((j & 1 ? byte >> 4 : byte) & 15u) ^ 8u) << (4 * j);
             }
         out[i] = word;
     }
@@ -67,14 +67,14 @@ __global__ void __launch_bounds__(256) g4_pack_groups_kernel(const _Float16* sca
         const int64_t tile = b / l.steps, k0 = b % l.steps * 128;
         _Float16* so = reinterpret_cast<_Float16*>(out + l.scales) + b * per * 16;
         uint8_t* zo = out + l.zeros + b * per * 8;
-        for (int i = 0; i < 16 * per; i += 2) {  // a byte of zero points: rows or groups next to each other
+        for (int i = 0; i < 16 * per; i += 2) {  // two rows of a group: a byte of zero points
             uint32_t zs = 0;
             for (int h = 0; h < 2; h++) {
-                const int r = (i + h) / per, g = (i + h) % per;
+                const int r = i / (4 * per) * 4 + (i & 3) + h, g = i / 4 % per;
                 const int64_t row = tile * 16 + r, gi = (k0 + g * (128 / per)) / group;
                 const bool in = row < rows && gi < groups;
-                so[scale_at(r, g, per)] = in ? scales[row * groups + gi] : static_cast<_Float16>(0.f);
-                if (zeros && in) zs |= (zeros[row * groups + gi] & 15u) << (4 * h);
+                so[i + h] = in ? scales[row * groups + gi] : static_cast<_Float16>(0.f);
+                if (zeros && in) zs |= ((zeros[row * groups + gi] & 15u) ^ 8u) << (4 * h);
             }
             if (zeros) zo[i >> 1] = static_cast<uint8_t>(zs);
         }
@@ -119,23 +119,33 @@ __global__ void __launch_bounds__(256) g4_quantize_kernel(const void* src, int32
 
 // ---- products ---------------------------------------------------------------
 //
-// A wave takes a row tile (16 rows) and every KS-th of its 128-steps: one
+// A wave takes a row tile (16 rows) and every ks-th of its 128-steps: one
 // 16-byte load per lane brings a step's codes in the order of the A operand of
-// v_mfma_f32_16x16x32_f16 (group4.hpp).  Two codes become two halves by one
-// mask: in the low bits of the mantissa of 1024 (codes at bits 0-3) or at bit 4
-// of that of 64 (codes at bits 4-7) they are 1024 + q and 64 + q, and a packed
-// subtraction leaves q - z exactly.  The scale stays out of the operand: a
-// group's products are summed in fp32 and then scaled, so nothing is rounded
-// but the sums.
+// v_mfma_i32_16x16x64_i8 (group4.hpp).  The operand needs no more than a shift
+// and two masks per eight codes: a nibble in the high half of a byte, as int8,
+// is 16 (q - 8).  Fp16 operands would take five times the instructions, and
+// instructions are what bounds a wave here: at the memory's rate a CU has about
+// 100 issue slots for a step's 1 KB.
 //
-// The B operand's 16 columns are the tokens.  fp16 activations are taken as
-// they are; fp32 ones as two halves hi + lo in two columns (22 bits), bf16 ones
-// as one (all 8 bits), each block of 128 brought to [2^14, 2^15) by a power of
-// two that the group's sum is multiplied back by.  Columns past the tokens
-// repeat the last one and are dropped.
-typedef _Float16 half2_t __attribute__((ext_vector_type(2)));
+// The B operand's 16 columns are the activations as integers: each block of 128
+// of a token, brought by a power of two to |X| < 2^30 (fp32 x) or 2^22 (16-bit
+// x) and rounded, is split into 4 or 3 signed digits to the base 256, one
+// column each.  fp32 values keep all their bits down to 2^-6 of the block's
+// largest, bf16 and fp16 ones down to 2^-14 and 2^-11; what is lost below is at
+// most 2^-31 (2^-23) of the largest.  Sums over a group are exact:
+//
+//   sum (q - z) X = sum (q - 8) X - (z - 8) sum X
+//
+// with sum X found once as x is staged.  Then, in fp32, a group's sum is
+// multiplied by its scale and the block's power of two and added up; the digits
+// of a token meet at the end.  A block with a NaN or an infinity has the power
+// NaN, which stays in its token.  Columns past the tokens repeat the last one
+// and are dropped.
+typedef _Float16 half4_t __attribute__((ext_vector_type(4)));
 typedef _Float16 half8_t __attribute__((ext_vector_type(8)));
 typedef float float4_t __attribute__((ext_vector_type(4)));
+typedef int int4_t __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 
 constexpr int G4_WAVES = 8;
 constexpr int G4_THREADS = 64 * G4_WAVES;
@@ -146,158 +156,147 @@ struct G4Args {
     const void* x;
     float* y;
     int64_t x_ld, rows, k;
-    int32_t m;          // tokens of this launch
-    int32_t ks;         // waves that share a row tile
-    int32_t groups;     // sets of G4_WAVES / ks row tiles
-    int32_t chunk;      // 128-steps of x in LDS at a time
-    bool whole;         // all of x fits: staged once
+    int32_t x_type;
+    int32_t m;       // tokens of this launch
+    int32_t ks;      // waves that share a row tile
+    int32_t groups;  // sets of G4_WAVES / ks row tiles
+    int32_t chunk;   // 128-steps of x in LDS at a time
+    bool whole;      // all of x fits: staged once
 };
 
-template <int XT>
+// Eight activations as loaded: fp32 (8 dwords) or 16-bit (4).
+template <int PARTS>
 struct XUnit {
-    uint32_t u[XT == ELEM_F32 ? 8 : 4];
+    uint32_t u[PARTS == 4 ? 8 : 4];
 };
 
-template <int XT>
-__device__ __forceinline__ XUnit<XT> x_load(const G4Args& a, int token, int64_t k0) {
-    XUnit<XT> r;
-    if constexpr (XT == ELEM_F32) {
-        typedef uint32_t v4 __attribute__((ext_vector_type(4), aligned(4)));
-        const float* p = static_cast<const float*>(a.x) + token * a.x_ld + k0;
-        if (k0 + 8 <= a.k) {
-            const v4 lo = *reinterpret_cast<const v4*>(p), hi = *reinterpret_cast<const v4*>(p + 4);
+// Values k0 .. k0 + 7 of a token, zeros past k.  WHOLE: without a branch around
+// a load (k >= 8): a piece that reaches past k takes the row's last eight values,
+// and x_shift moves its own to the front.
+template <int PARTS, bool WHOLE>
+__device__ __forceinline__ XUnit<PARTS> x_load(const G4Args& a, int token, int64_t k0) {
+    constexpr int N = PARTS == 4 ? 8 : 4, SIZE = PARTS == 4 ? 4 : 2;
+    typedef uint32_t v4 __attribute__((ext_vector_type(4), aligned(2)));
+    XUnit<PARTS> r;
+    if (WHOLE || k0 + 8 <= a.k) {
+        const int64_t from = k0 + 8 <= a.k ? k0 : a.k - 8;
+        const v4* p = reinterpret_cast<const v4*>(static_cast<const uint8_t*>(a.x) + (token * a.x_ld + from) * SIZE);
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
-                r.u[i] = lo[i];
-                r.u[4 + i] = hi[i];
-            }
-        } else {
+        for (int i = 0; i < N; i += 4) {
+            const v4 v = p[i / 4];
 #pragma unroll
-            for (int i = 0; i < 8; i++) r.u[i] = k0 + i < a.k ? __float_as_uint(p[i]) : 0u;
+            for (int j = 0; j < 4; j++) r.u[i + j] = v[j];
         }
+    } else if constexpr (PARTS == 4) {
+        const uint32_t* p = static_cast<const uint32_t*>(a.x) + token * a.x_ld + k0;
+#pragma unroll
+        for (int i = 0; i < 8; i++) r.u[i] = k0 + i < a.k ? p[i] : 0u;
     } else {
-        typedef uint32_t v4 __attribute__((ext_vector_type(4), aligned(2)));
         const uint16_t* p = static_cast<const uint16_t*>(a.x) + token * a.x_ld + k0;
-        if (k0 + 8 <= a.k) {
-            const v4 v = *reinterpret_cast<const v4*>(p);
-#pragma unroll
-            for (int i = 0; i < 4; i++) r.u[i] = v[i];
-        } else {
-#pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const uint32_t lo = k0 + 2 * i < a.k ? p[2 * i] : 0u, hi = k0 + 2 * i + 1 < a.k ? p[2 * i + 1] : 0u;
-                r.u[i] = lo | hi << 16;
-            }
-        }
-    }
-    return r;
-}
-
-// The same without a branch around a load: a piece that reaches past k (k >= 8)
-// takes the row's last eight values and moves its own to the front.
-template <int XT>
-__device__ __forceinline__ XUnit<XT> x_load_whole(const G4Args& a, int token, int64_t k0) {
-    XUnit<XT> r;
-    k0 = k0 + 8 <= a.k ? k0 : a.k - 8;
-    if constexpr (XT == ELEM_F32) {
-        typedef uint32_t v4 __attribute__((ext_vector_type(4), aligned(4)));
-        const v4* p = reinterpret_cast<const v4*>(static_cast<const float*>(a.x) + token * a.x_ld + k0);
-        const v4 lo = p[0], hi = p[1];
 #pragma unroll
         for (int i = 0; i < 4; i++) {
-            r.u[i] = lo[i];
-            r.u[4 + i] = hi[i];
+            const uint32_t lo = k0 + 2 * i < a.k ? p[2 * i] : 0u, hi = k0 + 2 * i + 1 < a.k ? p[2 * i + 1] : 0u;
+            r.u[i] = lo | hi << 16;
         }
-    } else {
-        typedef uint32_t v4 __attribute__((ext_vector_type(4), aligned(2)));
-        const v4 v = *reinterpret_cast<const v4*>(static_cast<const uint16_t*>(a.x) + token * a.x_ld + k0);
-#pragma unroll
-        for (int i = 0; i < 4; i++) r.u[i] = v[i];
     }
     return r;
 }
 
-template <int XT>
-__device__ __forceinline__ void x_shift(XUnit<XT>& r, int by) {  // values `by`.. of the eight to the front, zeros behind
-    if constexpr (XT == ELEM_F32) {
+template <int PARTS>
+__device__ __forceinline__ void x_shift(XUnit<PARTS>& r, int by) {  // values `by`.. (0 to 8) to the front, zeros behind
+    constexpr int N = PARTS == 4 ? 8 : 4;
+    const int words = PARTS == 4 ? by : by >> 1;
 #pragma unroll
-        for (int b = 4; b >= 1; b >>= 1) {
-            if (!(by & b)) continue;
+    for (int b = N; b >= 1; b >>= 1) {
+        if (!(words & b)) continue;
 #pragma unroll
-            for (int i = 0; i < 8; i++) r.u[i] = i + b < 8 ? r.u[i + b] : 0u;
-        }
-        if (by & 8) {
+        for (int i = 0; i < N; i++) r.u[i] = i + b < N ? r.u[i + b] : 0u;
+    }
+    if (PARTS == 3 && (by & 1)) {
 #pragma unroll
-            for (int i = 0; i < 8; i++) r.u[i] = 0u;
-        }
-    } else {
-#pragma unroll
-        for (int b = 4; b >= 1; b >>= 1) {
-            if (!(by & (2 * b))) continue;
-#pragma unroll
-            for (int i = 0; i < 4; i++) r.u[i] = i + b < 4 ? r.u[i + b] : 0u;
-        }
-        if (by & 1) {
-#pragma unroll
-            for (int i = 0; i < 4; i++) r.u[i] = r.u[i] >> 16 | (i < 3 ? r.u[i + 1] << 16 : 0u);
-        }
+        for (int i = 0; i < N; i++) r.u[i] = r.u[i] >> 16 | (i + 1 < N ? r.u[i + 1] << 16 : 0u);
     }
 }
 
-// The largest of 16 lanes' values (a DPP row), in each of them.
-__device__ __forceinline__ float row_max(float v) {
-    v = fmaxf(v, dpp_f<0xB1>(v));
-    v = fmaxf(v, dpp_f<0x4E>(v));
-    v = fmaxf(v, dpp_f<0x141>(v));
-    return fmaxf(v, dpp_f<0x140>(v));
+template <int CTRL>
+__device__ __forceinline__ int dpp_i(int v) {
+    return __builtin_amdgcn_update_dpp(0, v, CTRL, 0xF, 0xF, false);
 }
 
-__device__ __forceinline__ uint32_t pack_half2(float a, float b) {
-    const half2_t h = {static_cast<_Float16>(a), static_cast<_Float16>(b)};
-    return __builtin_bit_cast(uint32_t, h);
-}
+// x in LDS.
+//   digits  [step][half][c][col] of 16 bytes: the B operand's bytes of k = 64 half + 8 c + 0..7 and + 32
+//   power   [step][token] the block's power of two (with the weights' 1/16 and the top digit's 256^(PARTS-1))
+//   sums    [step][group][col] -16 sum X
+struct XLds {
+    uint8_t* digits;
+    float* power;
+    int* sums;
+};
 
-// A unit's columns into LDS.  xs: [step][t][c][col] of 8 halves; inv: [step][token].
-template <int XT>
-__device__ __forceinline__ void x_store(const XUnit<XT>& r, uint4* xs, float* inv, int cols, int m, int token, int kc) {
-    uint4* at = xs + static_cast<int64_t>(kc) * cols + (XT == ELEM_F32 ? 2 * token : token);
-    if constexpr (XT == ELEM_F16) {
-        *at = make_uint4(r.u[0], r.u[1], r.u[2], r.u[3]);
+// One piece (eight values; piece kc of the chunk, 16 to a block in 16 neighbouring lanes) of a token.
+template <int PARTS, int PER, bool ZEROS>
+__device__ __forceinline__ void x_store(const XUnit<PARTS>& r, const XLds& x, int type, int cols, int m, int token, int kc) {
+    float v[8];
+    if constexpr (PARTS == 4) {
+#pragma unroll
+        for (int i = 0; i < 8; i++) v[i] = __uint_as_float(r.u[i]);
+    } else if (type == ELEM_F16) {
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            v[2 * i] = f16lo(r.u[i]);
+            v[2 * i + 1] = f16hi(r.u[i]);
+        }
     } else {
-        float v[8];
 #pragma unroll
-        for (int i = 0; i < 8; i++) {
-            if constexpr (XT == ELEM_F32) v[i] = __uint_as_float(r.u[i]);
-            else v[i] = __uint_as_float(i & 1 ? r.u[i >> 1] & 0xffff0000u : r.u[i >> 1] << 16);
+        for (int i = 0; i < 4; i++) {
+            v[2 * i] = __uint_as_float(r.u[i] << 16);
+            v[2 * i + 1] = __uint_as_float(r.u[i] & 0xffff0000u);
         }
-        // the largest magnitude of the 128 by its bits (NaN and infinity are the largest)
-        uint32_t big = 0;
-#pragma unroll
-        for (int i = 0; i < 8; i++) {
-            const uint32_t b = __float_as_uint(v[i]) & 0x7fffffffu;
-            big = b > big ? b : big;
-        }
-        const uint32_t top = static_cast<uint32_t>(row_max(static_cast<float>(big >> 23)));  // its exponent
-        // 2^(14 - exponent), within the normal numbers with its reciprocal; 1 for a block without bounds
-        uint32_t f = top == 255 ? 127 : 268 - top;
-        f = f > 253 ? 253 : f;
-        const float scale = __uint_as_float(f << 23);
-        float hi[8];
-#pragma unroll
-        for (int i = 0; i < 8; i++) {
-            v[i] *= scale;
-            hi[i] = static_cast<float>(static_cast<_Float16>(v[i]));
-        }
-        *at = make_uint4(pack_half2(hi[0], hi[1]), pack_half2(hi[2], hi[3]), pack_half2(hi[4], hi[5]),
-                         pack_half2(hi[6], hi[7]));
-        if constexpr (XT == ELEM_F32) {
-#pragma unroll
-            for (int i = 0; i < 8; i++) v[i] = top == 255 ? 0.f : v[i] - hi[i];
-            at[1] = make_uint4(pack_half2(v[0], v[1]), pack_half2(v[2], v[3]), pack_half2(v[4], v[5]),
-                               pack_half2(v[6], v[7]));
-        }
-        if ((kc & 15) == 0) inv[(kc >> 4) * m + token] = __uint_as_float((254 - f) << 23);
     }
+    // the block's largest magnitude, as bits: NaN and infinity are the largest
+    int big = 0;
+#pragma unroll
+    for (int i = 0; i < 8; i++) big = max(big, static_cast<int>(__float_as_uint(v[i]) & 0x7fffffffu));
+    big = max(big, dpp_i<0xB1>(big));
+    big = max(big, dpp_i<0x4E>(big));
+    big = max(big, dpp_i<0x141>(big));
+    big = max(big, dpp_i<0x140>(big));
+    const int e = max(big >> 23, 1) - 127;  // |v| < 2^(e + 1)
+    constexpr int BITS = PARTS == 4 ? 29 : 21;
+    constexpr uint32_t BIAS = PARTS == 4 ? 0x80808080u : 0x00808080u;
+    // byte h of X + BIAS is digit h, offset by 128
+    uint32_t d[8];
+#pragma unroll
+    for (int i = 0; i < 8; i++)
+        d[i] = (static_cast<uint32_t>(static_cast<int>(__builtin_rintf(__builtin_ldexpf(v[i], BITS - e)))) + BIAS) ^ BIAS;
+    uint32_t* at = reinterpret_cast<uint32_t*>(x.digits) +
+                   (static_cast<int64_t>((kc >> 4) * 8 + ((kc >> 3) & 1) * 4 + (kc & 3)) * cols + PARTS * token) * 4 + ((kc >> 2) & 1) * 2;
+    // bytes h of four values: pairs by v_perm, then pairs of pairs
+    const auto gather = [](uint32_t a, uint32_t b, uint32_t c, uint32_t f, uint32_t* out) {
+        const uint32_t ab01 = __builtin_amdgcn_perm(b, a, 0x05010400u), ab23 = __builtin_amdgcn_perm(b, a, 0x07030602u);
+        const uint32_t cf01 = __builtin_amdgcn_perm(f, c, 0x05010400u), cf23 = __builtin_amdgcn_perm(f, c, 0x07030602u);
+        out[0] = __builtin_amdgcn_perm(cf01, ab01, 0x05040100u);
+        out[1] = __builtin_amdgcn_perm(cf01, ab01, 0x07060302u);
+        out[2] = __builtin_amdgcn_perm(cf23, ab23, 0x05040100u);
+        out[3] = __builtin_amdgcn_perm(cf23, ab23, 0x07060302u);
+    };
+    uint32_t even[4], odd[4];  // the codes of even and odd k come out of the weights apart
+    gather(d[0], d[2], d[4], d[6], even);
+    gather(d[1], d[3], d[5], d[7], odd);
+#pragma unroll
+    for (int h = 0; h < PARTS; h++) {
+        *reinterpret_cast<u32x2*>(at + 4 * h) = u32x2{even[h], odd[h]};
+        if constexpr (ZEROS) {
+            int s = sdot4(even[h], 0x01010101u, sdot4(odd[h], 0x01010101u, 0));
+            s += dpp_i<0xB1>(s);
+            s += dpp_i<0x4E>(s);
+            if (PER <= 2) s += dpp_i<0x141>(s);
+            if (PER == 1) s += dpp_i<0x140>(s);
+            if ((kc & (16 / PER - 1)) == 0) x.sums[((kc >> 4) * PER + (kc & 15) * PER / 16) * cols + PARTS * token + h] = -16 * s;
+        }
+    }
+    if ((kc & 15) == 0)
+        x.power[(kc >> 4) * m + token] = big >= 0x7f800000 ? NAN : __builtin_ldexpf(1.f, e - BITS - 4 + 8 * (PARTS - 1));
 }
 
 // The wave's LDS accesses are done, then everyone's; its loads from memory stay in flight.
@@ -310,42 +309,45 @@ __device__ __forceinline__ void lds_barrier() {
     __builtin_amdgcn_sched_barrier(0);
 }
 
-typedef _Float16 half4_t __attribute__((ext_vector_type(4)));
-
 // What a wave loads of one block.
 template <int PER, bool ZEROS>
 struct WStep {
     u32x4 q;
     half4_t s[PER];
-    uint32_t z;  // zero points of 8 / PER rows, the lane's among them
+    uint32_t z[PER == 4 ? 2 : 1];
 };
 
 template <int PER>
 constexpr int g4_depth() { return PER == 1 ? 8 : 4; }  // blocks in flight per wave
 
-template <int PER, bool ZEROS, int XT, int NT>
-__global__ void __launch_bounds__(G4_THREADS, NT == 4 ? 2 : 4) g4_gemv_kernel(G4Args a) {
+template <int PER, bool ZEROS, int PARTS, int NT>
+__global__ void __launch_bounds__(G4_THREADS, NT >= 3 ? 2 : 4) g4_gemv_kernel(G4Args a) {
     constexpr int DEPTH = g4_depth<PER>();
-    constexpr int PARTS = XT == ELEM_F32 ? 2 : 1;
     extern __shared__ uint4 lds[];
     const int tid = static_cast<int>(threadIdx.x), lane = tid & 63, n = lane & 15, c = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int cols = PARTS * a.m, ks = a.ks, sub = wave % ks, local = wave / ks, per_group = G4_WAVES / ks;
+    const int m = a.m, cols = PARTS * m, ks = a.ks, sub = wave % ks, local = wave / ks, per_group = G4_WAVES / ks;
     const int steps = static_cast<int>(a.l.steps), tiles = static_cast<int>(a.l.tiles);
     float4_t* red = reinterpret_cast<float4_t*>(lds);  // [wave][nt][lane]
-    float* inv = reinterpret_cast<float*>(lds + (ks > 1 ? G4_WAVES * NT * 64 : 0));
-    uint4* xs = reinterpret_cast<uint4*>(inv) + (XT == ELEM_F16 ? 0 : (a.chunk * a.m + 3) / 4);
+    XLds x;
+    x.digits = reinterpret_cast<uint8_t*>(lds + G4_WAVES * NT * 64);
+    x.power = reinterpret_cast<float*>(x.digits + a.chunk * 128 * cols);
+    x.sums = reinterpret_cast<int*>(x.power + a.chunk * m);
 
-    int col[NT];
+    int col[NT], token[NT];
 #pragma unroll
-    for (int t = 0; t < NT; t++) col[t] = t * 16 + n < cols ? t * 16 + n : cols - 1;
+    for (int t = 0; t < NT; t++) {
+        col[t] = t * 16 + n < cols ? t * 16 + n : cols - 1;
+        token[t] = col[t] / PARTS;
+    }
 
-    const int pieces = a.chunk * 16, units = pieces * a.m;  // of a token, of all tokens in a chunk
-    auto stage = [&](int first, int from) {                 // pieces from .. of steps first .. first + chunk of x
+    const int pieces = a.chunk * 16, units = pieces * m;  // of a token, of all tokens in a chunk
+    auto stage = [&](int first, int from) {               // pieces from .. of steps first .. first + chunk of x
 #pragma unroll 1
         for (int u = from + tid; u < units; u += G4_THREADS) {
-            const int token = u / pieces, kc = u % pieces;
-            x_store<XT>(x_load<XT>(a, token, (static_cast<int64_t>(first) * 16 + kc) * 8), xs, inv, cols, a.m, token, kc);
+            const int t = u / pieces, kc = u % pieces;
+            x_store<PARTS, PER, ZEROS>(x_load<PARTS, false>(a, t, (static_cast<int64_t>(first) * 16 + kc) * 8), x, a.x_type,
+                                       cols, m, t, kc);
         }
     };
     // Loads of the ring: a step or tile past the last is outside of its
@@ -354,13 +356,11 @@ __global__ void __launch_bounds__(G4_THREADS, NT == 4 ? 2 : 4) g4_gemv_kernel(G4
     auto load = [&](int tile, int step, WStep<PER, ZEROS>& r) __attribute__((always_inline)) {
         const bool in = tile < tiles;
         const int64_t b = in ? static_cast<int64_t>(tile) * steps : 0;
-        const uint32_t size = in ? static_cast<uint32_t>(steps) : 0u;
-        const __amdgpu_buffer_rsrc_t rq = make_rsrc(a.w + b * 1024, size * 1024);
+        const uint32_t size = in ? static_cast<uint32_t>(steps) : 0u, at = static_cast<uint32_t>(step);
+        r.q = buf_ld128(make_rsrc(a.w + b * 1024, size * 1024), at * 1024 + lane * 16, 0);
         const __amdgpu_buffer_rsrc_t rs = make_rsrc(a.w + a.l.scales + b * (32 * PER), size * (32 * PER));
-        r.q = buf_ld128(rq, static_cast<uint32_t>(step) * 1024 + lane * 16, 0);
-        const uint32_t so = (static_cast<uint32_t>(step) * 4 + c) * (8 * PER);
+        const uint32_t so = (at * 4 + c) * (8 * PER);
         if constexpr (PER == 1) {
-            typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
             r.s[0] = __builtin_bit_cast(half4_t, __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(rs, static_cast<int>(so), 0, 0)));
         } else {
 #pragma unroll
@@ -372,74 +372,96 @@ __global__ void __launch_bounds__(G4_THREADS, NT == 4 ? 2 : 4) g4_gemv_kernel(G4
         }
         if constexpr (ZEROS) {
             const __amdgpu_buffer_rsrc_t rz = make_rsrc(a.w + a.l.zeros + b * (8 * PER), size * (8 * PER));
-            r.z = __builtin_amdgcn_raw_buffer_load_b32(rz, static_cast<int>(step * (8 * PER) + n * PER / 8 * 4), 0, 0);
+            const int zo = static_cast<int>(at * (8 * PER) + c * PER / 2 * 4);
+            if constexpr (PER == 4) {
+                const u32x2 v = __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(rz, zo, 0, 0));
+                r.z[0] = v[0];
+                r.z[1] = v[1];
+            } else {
+                r.z[0] = __builtin_amdgcn_raw_buffer_load_b32(rz, zo, 0, 0);
+            }
         }
         __builtin_amdgcn_sched_barrier(0);  // slot after slot, as they are waited for
     };
     float4_t acc[NT];
     auto multiply = [&](const WStep<PER, ZEROS>& r, int at) __attribute__((always_inline)) {  // step `at` of the chunk
-        const uint4* xb = xs + (at * 16 + c) * cols;
-        float4_t p[NT], sum[NT];
-        half8_t xv[4][NT];
+        const uint4* xb = reinterpret_cast<const uint4*>(x.digits) + (at * 8 + c) * cols;
+        int4_t xv[2][NT];
 #pragma unroll
-        for (int t = 0; t < 4; t++)
+        for (int h = 0; h < 2; h++)
 #pragma unroll
-            for (int u = 0; u < NT; u++) xv[t][u] = __builtin_bit_cast(half8_t, xb[t * 4 * cols + col[u]]);
+            for (int u = 0; u < NT; u++) xv[h][u] = __builtin_bit_cast(int4_t, xb[h * 4 * cols + col[u]]);
+        float f[NT];
+        int sx[NT][PER];
 #pragma unroll
-        for (int t = 0; t < 4; t++) {
-            const int g = t * PER / 4;
-            uint32_t z = 8;
-            if (ZEROS) z = (r.z >> (n * PER % 8 * 4 + 4 * g)) & 15;
-            const half2_t z0 = __builtin_bit_cast(half2_t, z * 0x00010001u + 0xE400E400u);  // -(1024 + z)
-            const half2_t z1 = __builtin_bit_cast(half2_t, z * 0x00100010u + 0xD400D400u);  // -(64 + z)
-            const uint32_t q = r.q[t], qh = q >> 8;
-            const half2_t h0 = __builtin_bit_cast(half2_t, (q & 0x000f000fu) | 0x64006400u) + z0;
-            const half2_t h1 = __builtin_bit_cast(half2_t, (q & 0x00f000f0u) | 0x54005400u) + z1;
-            const half2_t h2 = __builtin_bit_cast(half2_t, (qh & 0x000f000fu) | 0x64006400u) + z0;
-            const half2_t h3 = __builtin_bit_cast(half2_t, (qh & 0x00f000f0u) | 0x54005400u) + z1;
-            const half8_t wv = {h0[0], h0[1], h1[0], h1[1], h2[0], h2[1], h3[0], h3[1]};
+        for (int u = 0; u < NT; u++) {
+            f[u] = x.power[at * m + token[u]];
+            if (ZEROS) {
 #pragma unroll
-            for (int u = 0; u < NT; u++) {
-                const float4_t zero = {0.f, 0.f, 0.f, 0.f};
-                p[u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(wv, xv[t][u], t % (4 / PER) == 0 ? zero : p[u], 0, 0, 0);
-                if ((t + 1) % (4 / PER) == 0) {
-                    // fp16 x adds to acc; the others to the block's sum, which then takes the block's power of two
-                    float4_t& to = XT == ELEM_F16 ? acc[u] : sum[u];
+                for (int g = 0; g < PER; g++) sx[u][g] = x.sums[(at * PER + g) * cols + col[u]];
+            }
+        }
+        int4_t p[NT];
+        float4_t sum[NT];
+        const auto group_done = [&](int g) __attribute__((always_inline)) {
+            const uint32_t zw = !ZEROS ? 0u : PER == 1 ? r.z[0] >> (c & 1) * 16 : r.z[g >> 1];
 #pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        const float s = static_cast<float>(r.s[g][i]);
-                        to[i] = XT != ELEM_F16 && g == 0 ? s * p[u][i] : __builtin_fmaf(s, p[u][i], to[i]);
-                    }
+            for (int u = 0; u < NT; u++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    int q = p[u][i];
+                    if (ZEROS) q += __mul24(static_cast<int>(__builtin_amdgcn_sbfe(zw, (PER == 1 ? 0 : (g & 1) * 16) + 4 * i, 4)), sx[u][g]);
+                    const float s = static_cast<float>(r.s[g][i]), v = static_cast<float>(q);
+                    sum[u][i] = g == 0 ? s * v : __builtin_fmaf(s, v, sum[u][i]);
                 }
+        };
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            constexpr uint32_t HIGH = 0xf0f0f0f0u;
+            const uint32_t q0 = r.q[2 * h], q1 = r.q[2 * h + 1];
+            const int4_t wv = {static_cast<int>(q0 << 4 & HIGH), static_cast<int>(q0 & HIGH), static_cast<int>(q1 << 4 & HIGH),
+                               static_cast<int>(q1 & HIGH)};
+            const int4_t zero = {0, 0, 0, 0};
+            if constexpr (PER == 4) {
+                const auto pair = [](int lo, int hi) { return static_cast<long>(static_cast<uint64_t>(static_cast<uint32_t>(hi)) << 32 | static_cast<uint32_t>(lo)); };
+#pragma unroll
+                for (int t = 0; t < 2; t++) {
+#pragma unroll
+                    for (int u = 0; u < NT; u++)
+                        p[u] = __builtin_amdgcn_mfma_i32_16x16x32_i8(pair(wv[2 * t], wv[2 * t + 1]), pair(xv[h][u][2 * t], xv[h][u][2 * t + 1]), zero, 0, 0, 0);
+                    group_done(2 * h + t);
+                }
+            } else {
+#pragma unroll
+                for (int u = 0; u < NT; u++)
+                    p[u] = __builtin_amdgcn_mfma_i32_16x16x64_i8(wv, xv[h][u], PER == 2 || h == 0 ? zero : p[u], 0, 0, 0);
+                if (PER == 2 || h == 1) group_done(PER == 2 ? h : 0);
             }
         }
-        if (XT != ELEM_F16) {
+        // (s p) f: f p by itself may leave fp32's range where W x does not
 #pragma unroll
-            for (int u = 0; u < NT; u++) {
-                const float f = inv[at * a.m + col[u] / PARTS];
+        for (int u = 0; u < NT; u++)
 #pragma unroll
-                for (int i = 0; i < 4; i++) acc[u][i] = __builtin_fmaf(f, sum[u][i], acc[u][i]);
-            }
-        }
+            for (int i = 0; i < 4; i++) acc[u][i] = __builtin_fmaf(f[u], sum[u][i], acc[u][i]);
     };
 
     // The wave's steps of a tile: sub, sub + ks, ..., in rounds of DEPTH; the
-    // last rounds load the next tile's first ones.
+    // last round loads the next tile's first ones.
     const int rounds = (steps + ks * DEPTH - 1) / (ks * DEPTH);
     const int hop = static_cast<int>(gridDim.x) * per_group;
     int tile = static_cast<int>(blockIdx.x) * per_group + local;
     WStep<PER, ZEROS> ring[DEPTH];
     // x first, as loads come back in order: pieces past HELD per thread, then
     // HELD of them on the way together with the ring's first round.
-    constexpr int HELD = 4;
-    XUnit<XT> held[HELD];
+    constexpr int HELD = 2;
+    XUnit<PARTS> held[HELD];
     const bool hold = a.k >= 8;
     stage(0, hold ? HELD * G4_THREADS : 0);
     if (hold) {
 #pragma unroll
         for (int i = 0; i < HELD; i++) {
             const int u = i * G4_THREADS + tid, v = u < units ? u : units - 1;
-            held[i] = x_load_whole<XT>(a, v / pieces, static_cast<int64_t>(v % pieces) * 8);
+            held[i] = x_load<PARTS, true>(a, v / pieces, static_cast<int64_t>(v % pieces) * 8);
         }
     }
 #pragma unroll
@@ -449,9 +471,9 @@ __global__ void __launch_bounds__(G4_THREADS, NT == 4 ? 2 : 4) g4_gemv_kernel(G4
         for (int i = 0; i < HELD; i++) {
             const int u = i * G4_THREADS + tid;
             if (u >= units) continue;
-            const int token = u / pieces, kc = u % pieces;
-            if (kc * 8 + 8 > a.k) x_shift<XT>(held[i], static_cast<int>(kc * 8 >= a.k ? 8 : kc * 8 + 8 - a.k));
-            x_store<XT>(held[i], xs, inv, cols, a.m, token, kc);
+            const int t = u / pieces, kc = u % pieces;
+            if (kc * 8 + 8 > a.k) x_shift<PARTS>(held[i], static_cast<int>(kc * 8 >= a.k ? 8 : kc * 8 + 8 - a.k));
+            x_store<PARTS, PER, ZEROS>(held[i], x, a.x_type, cols, m, t, kc);
         }
     }
     lds_barrier();
@@ -479,92 +501,74 @@ __global__ void __launch_bounds__(G4_THREADS, NT == 4 ? 2 : 4) g4_gemv_kernel(G4
                 load(next, from + d * ks, ring[d]);
             }
         }
-        if (ks == 1) {
-            // the wave's tile is done: its lanes hold rows 4 c + 0..3 of column n
-#pragma unroll
-            for (int t = 0; t < NT; t++) {
-                if (PARTS == 2) {
-#pragma unroll
-                    for (int i = 0; i < 4; i++) acc[t][i] += dpp_f<0xB1>(acc[t][i]);
-                }
-                const int cc = t * 16 + n;
-                const int64_t row = static_cast<int64_t>(tile) * 16 + 4 * c;
-                if (tile < tiles && cc < cols && cc % PARTS == 0) {
-                    float* y = a.y + static_cast<int64_t>(cc / PARTS) * a.rows + row;
-#pragma unroll
-                    for (int i = 0; i < 4; i++)
-                        if (row + i < a.rows) y[i] = acc[t][i];
-                }
-            }
-            continue;
-        }
-        // y: the waves of a tile, and the two halves of fp32 activations, added in order
+        // y: a token's digits of a tile's waves, added in order.  A wave that has
+        // a tile by itself reads what it wrote.
+        const float digit[4] = {PARTS == 4 ? 0x1p-24f : 0x1p-16f, PARTS == 4 ? 0x1p-16f : 0x1p-8f, PARTS == 4 ? 0x1p-8f : 1.f, 1.f};
 #pragma unroll
         for (int t = 0; t < NT; t++) red[(wave * NT + t) * 64 + lane] = acc[t];
-        lds_barrier();
+        if (ks > 1) lds_barrier();
         const float* rf = reinterpret_cast<const float*>(red);
-        for (int o = tid; o < per_group * 16 * a.m; o += G4_THREADS) {
-            const int r = o & 15, tt = (o >> 4) % per_group, token = (o >> 4) / per_group;
+        const int outs = (ks > 1 ? per_group : 1) * 16 * m;
+        for (int o = ks > 1 ? tid : lane; o < outs; o += ks > 1 ? G4_THREADS : 64) {
+            const int r = o & 15, tt = ks > 1 ? (o >> 4) % per_group : local, t = ks > 1 ? (o >> 4) / per_group : o >> 4;
             const int64_t row = (static_cast<int64_t>(grp) * per_group + tt) * 16 + r;
-            float sum = 0.f;
+            float total = 0.f;
 #pragma unroll
             for (int h = 0; h < PARTS; h++) {
-                const int cc = PARTS * token + h;
+                const int cc = PARTS * t + h;
+                float sum = 0.f;
                 for (int v = 0; v < ks; v++)
                     sum += rf[(((tt * ks + v) * NT + (cc >> 4)) * 64 + (r >> 2) * 16 + (cc & 15)) * 4 + (r & 3)];
+                total = __builtin_fmaf(digit[h], sum, total);
             }
-            if (row < a.rows) a.y[static_cast<int64_t>(token) * a.rows + row] = sum;
+            if (row < a.rows) a.y[static_cast<int64_t>(t) * a.rows + row] = total;
         }
-        lds_barrier();  // red is free
+        if (ks > 1) lds_barrier();  // red is free
     }
 }
 
-template <int PER, bool ZEROS, int XT>
+template <int PER, bool ZEROS, int PARTS>
 void g4_launch(const G4Args& a, int nt, uint32_t grid, uint32_t lds, hipStream_t st) {
-    if (nt == 1) g4_gemv_kernel<PER, ZEROS, XT, 1><<<grid, G4_THREADS, lds, st>>>(a);
-    else if (nt == 2) g4_gemv_kernel<PER, ZEROS, XT, 2><<<grid, G4_THREADS, lds, st>>>(a);
-    else if constexpr (XT == ELEM_F16) g4_gemv_kernel<PER, ZEROS, XT, 4><<<grid, G4_THREADS, lds, st>>>(a);
-}
-
-template <int PER, bool ZEROS>
-void g4_launch_x(const G4Args& a, int xt, int nt, uint32_t grid, uint32_t lds, hipStream_t st) {
-    if (xt == ELEM_F32) g4_launch<PER, ZEROS, ELEM_F32>(a, nt, grid, lds, st);
-    else if (xt == ELEM_F16) g4_launch<PER, ZEROS, ELEM_F16>(a, nt, grid, lds, st);
-    else g4_launch<PER, ZEROS, ELEM_BF16>(a, nt, grid, lds, st);
+    if (nt == 1) g4_gemv_kernel<PER, ZEROS, PARTS, 1><<<grid, G4_THREADS, lds, st>>>(a);
+    else if (nt == 2) g4_gemv_kernel<PER, ZEROS, PARTS, 2><<<grid, G4_THREADS, lds, st>>>(a);
+    else if (nt == 3) g4_gemv_kernel<PER, ZEROS, PARTS, 3><<<grid, G4_THREADS, lds, st>>>(a);
+    else g4_gemv_kernel<PER, ZEROS, PARTS, 4><<<grid, G4_THREADS, lds, st>>>(a);
 }
 
 constexpr int64_t G4_LDS = 120 << 10;  // of x in LDS, at most
+constexpr int G4_COLS = 64;            // columns of a launch, at most
 
-int g4_run(G4Args a, int x_type, bool has_zeros, hipStream_t st) {
-    const int parts = x_type == ELEM_F32 ? 2 : 1, cols = parts * a.m, nt = cols <= 16 ? 1 : cols <= 32 ? 2 : 4;
-    const int depth = a.l.per == 1 ? g4_depth<1>() : g4_depth<4>();
-    const int64_t slots = 16 * num_cus();  // waves that are resident at once
+int g4_run(G4Args a, bool has_zeros, hipStream_t st) {
+    const int parts = a.x_type == ELEM_F32 ? 4 : 3, cols = parts * a.m, nt = (cols + 15) / 16;
+    const int per = static_cast<int>(a.l.per), depth = per == 1 ? g4_depth<1>() : g4_depth<4>();
+    const int64_t slots = (nt >= 3 ? 8 : 16) * num_cus();  // waves that are resident at once
     a.ks = 1;
     while (a.ks < G4_WAVES && a.l.tiles * a.ks * 2 <= slots && a.ks < a.l.steps) a.ks *= 2;
-    // the 128-steps of x that LDS takes, whole rounds of the ring (64 columns are 16 KB a step)
-    const int64_t step_bytes = 256 * cols + (x_type == ELEM_F16 ? 0 : 4 * a.m);
+    // the 128-steps of x that LDS takes, whole rounds of the ring
+    const int64_t step_bytes = 128 * cols + 4 * a.m + (has_zeros ? 4 * per * cols : 0);
     int64_t chunk = G4_LDS / step_bytes;
     a.whole = chunk >= a.l.steps;
     while (!a.whole && a.ks > 1 && chunk < depth * a.ks) a.ks /= 2;
     chunk = a.whole ? a.l.steps : chunk / (depth * a.ks) * (depth * a.ks);
-    if (chunk == 0) chunk = depth;
     a.chunk = static_cast<int32_t>(chunk);
     const int per_group = G4_WAVES / a.ks;
     a.groups = static_cast<int32_t>((a.l.tiles + per_group - 1) / per_group);
-    const uint32_t lds = static_cast<uint32_t>((a.ks > 1 ? G4_WAVES * nt * 1024 : 0) +
-                                               (x_type == ELEM_F16 ? 0 : (chunk * a.m + 3) / 4 * 16) + chunk * 256 * cols);
-    const int64_t most = (lds > (80 << 10) ? 1 : 2) * num_cus();
+    const uint32_t lds = static_cast<uint32_t>(G4_WAVES * nt * 1024 + chunk * step_bytes);
+    const int64_t most = (lds > (80 << 10) || nt >= 3 ? 1 : 2) * num_cus();
     const uint32_t grid = static_cast<uint32_t>(a.groups < most ? a.groups : most);
-    const int per = static_cast<int>(a.l.per);
-    if (has_zeros) {
-        if (per == 1) g4_launch_x<1, true>(a, x_type, nt, grid, lds, st);
-        else if (per == 2) g4_launch_x<2, true>(a, x_type, nt, grid, lds, st);
-        else g4_launch_x<4, true>(a, x_type, nt, grid, lds, st);
-    } else {
-        if (per == 1) g4_launch_x<1, false>(a, x_type, nt, grid, lds, st);
-        else if (per == 2) g4_launch_x<2, false>(a, x_type, nt, grid, lds, st);
-        else g4_launch_x<4, false>(a, x_type, nt, grid, lds, st);
+    const bool f32 = parts == 4;
+#define G4_CASE(PER, Z)                                      \
+    if (per == PER && has_zeros == Z) {                      \
+        if (f32) g4_launch<PER, Z, 4>(a, nt, grid, lds, st); \
+        else g4_launch<PER, Z, 3>(a, nt, grid, lds, st);     \
     }
+    G4_CASE(1, false)
+    G4_CASE(1, true)
+    G4_CASE(2, false)
+    G4_CASE(2, true)
+    G4_CASE(4, false)
+    G4_CASE(4, true)
+#undef G4_CASE
     return check_launch("vb_group4_gemv");
 }
 
@@ -648,13 +652,12 @@ int vb_group4_gemv(const void* w, int64_t rows, int64_t k, int32_t group, int32_
         set_error("vb_group4_gemv: null pointer, or w not 16-byte aligned");
         return E_INVAL;
     }
-    // tokens a launch takes: 32 columns of scaled activations, 64 of fp16 ones (the registers of four column tiles)
-    const int64_t slab = x_type == ELEM_F32 ? 16 : x_type == ELEM_F16 ? 64 : 32;
+    const int64_t slab = G4_COLS / (x_type == ELEM_F32 ? 4 : 3);  // tokens of a launch
     for (int64_t t = 0; t < m; t += slab) {
         const void* xt = static_cast<const uint8_t*>(x) + t * x_ld * elem_bytes(x_type);
-        const G4Args a{g.w, g.l, xt, y + t * rows, x_ld, rows, k, static_cast<int32_t>(m - t < slab ? m - t : slab),
+        const G4Args a{g.w, g.l, xt, y + t * rows, x_ld, rows, k, x_type, static_cast<int32_t>(m - t < slab ? m - t : slab),
                        0, 0, 0, false};
-        if (const int rc = g4_run(a, x_type, g.has_zeros, as_stream(stream)); rc != OK) return rc;
+        if (const int rc = g4_run(a, g.has_zeros, as_stream(stream)); rc != OK) return rc;
     }
     return OK;
 }

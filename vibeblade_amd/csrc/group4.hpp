@@ -2,11 +2,10 @@
 // lie in HBM.
 //
 // Rows are taken 16 at a time and k 128 at a time: a block of 16 x 128 codes
-// is 1 KB, in the order in which the lanes of a wave feed them to
-// v_mfma_f32_16x16x32_f16.  Lane l holds row l % 16 and, in its dword t
-// (t = 0..3, one per 32 of k), the codes of k = 32 t + 8 (l / 16) + 0..7:
-// code 2p at bit 4p and code 2p + 1 at bit 4p + 16, so that a mask gives two
-// neighbours in the halves of a register.  A wave reads a block with one
+// is 1 KB, in the order in which the lanes of a wave feed them to the matrix
+// cores.  Lane l holds row l % 16 and, in its dword t (t = 0..3, one per 32 of
+// k), the codes of k = 32 t + 8 (l / 16) + 0..7, code i at bit 4 i, with its
+// top bit flipped (q - 8 in two's complement).  A wave reads a block with one
 // 16-byte load per lane, and block after block along k as one linear stream.
 //
 // Planes, each [row tile][128-step][...]:
@@ -15,9 +14,9 @@
 //           and 128 or more; a longer group repeats its scale): the scales
 //           that lane l multiplies its four outputs (rows 4 (l / 16) + 0..3)
 //           by lie together
-//   zeros   16 x G values of 4 bits, row by row; no plane for symmetric
-//           weights (zero point 8)
-// Rows and k past the tensor have scale 0 and code 0.
+//   zeros   in the order of the scales, 4 bits each, as the codes (z - 8); no
+//           plane for symmetric weights (zero point 8)
+// Rows and k past the tensor have scale 0 and the code of 0.
 #pragma once
 
 #include <cstdint>
