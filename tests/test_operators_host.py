@@ -82,12 +82,12 @@ def test_group4_has_no_layout_for_other_groups(lib, group):
 
 
 def test_group4_bytes(lib):
-    # whole blocks of 16 rows x 128: codes 1024, then per group of 16 rows 32 bytes of scales and 8 of zero points
-    assert lib.vb_group4_bytes(16, 128, 128, 0) == 1024 + 32
-    assert lib.vb_group4_bytes(16, 128, 32, 1) == 1024 + 4 * 40
-    assert lib.vb_group4_bytes(17, 129, 64, 1) == 4 * (1024 + 2 * 40)
-    assert lib.vb_group4_bytes(1, 1, 1024, 0) == 1024 + 32
-    assert lib.vb_group4_bytes(128256, 16384, 128, 1) == 8016 * 128 * (1024 + 40)
+    # whole blocks of 16 rows x 256: codes 2048, then per group of 16 rows 32 bytes of scales and 8 of zero points
+    assert lib.vb_group4_bytes(16, 256, 128, 0) == 2048 + 2 * 32
+    assert lib.vb_group4_bytes(16, 128, 32, 1) == 2048 + 8 * 40
+    assert lib.vb_group4_bytes(17, 257, 64, 1) == 4 * (2048 + 4 * 40)
+    assert lib.vb_group4_bytes(1, 1, 1024, 0) == 2048 + 2 * 32
+    assert lib.vb_group4_bytes(128256, 16384, 128, 1) == 8016 * 64 * (2048 + 2 * 40)
     for bad in ((0, 128), (16, 0), (-1, 128), (1 << 31, 128), (16, 1 << 31)):
         assert lib.vb_group4_bytes(*bad, 128, 0) == -1
 
@@ -126,7 +126,7 @@ def test_python_calls_take_gpu_tensors_only():
     with pytest.raises(ValueError, match="cuda"):
         GroupQTensor.from_packed(torch.zeros((2, 4), dtype=torch.uint8), torch.zeros((2, 1), dtype=torch.float16), k=8)
     with pytest.raises(ValueError, match="cuda"):
-        GroupQTensor(torch.zeros(1056, dtype=torch.uint8), 16, 128, 128, False)
+        GroupQTensor(torch.zeros(2112, dtype=torch.uint8), 16, 128, 128, False)
     with pytest.raises(ValueError, match="cuda"):
         group_gemv(None, x)
 

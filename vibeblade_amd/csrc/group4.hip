@@ -19,21 +19,16 @@ struct G4Weights {
     bool has_zeros;
 };
 
-__device__ __forceinline__ int64_t block_of(const G4Weights& g, int64_t row, int64_t k) {
-    return (row >> 4) * g.l.steps + (k >> 7);
-}
-
-// Row r's scale of group g among the 16 x per of a block.
-__device__ __forceinline__ int scale_at(int r, int g, int per) { return ((r >> 2) * per + g) * 4 + (r & 3); }
+// Row r's scale of group g (of 2 per) among the 32 x per of a block.
+__device__ __forceinline__ int scale_at(int r, int g, int per) { return ((r >> 2) * 2 * per + g) * 4 + (r & 3); }
 
 __device__ __forceinline__ float g4_value(const G4Weights& g, int64_t row, int64_t k) {
-    const int64_t b = block_of(g, row, k);
-    const int r = static_cast<int>(row & 15), kk = static_cast<int>(k & 127);
-    const uint32_t word = reinterpret_cast<const uint32_t*>(g.w)[b * 256 + (((kk >> 3) & 3) * 16 + r) * 4 + (kk >> 5)];
-    const int q = (word >> (kk & 7) * 4) & 15;
-    const int per = static_cast<int>(g.l.per), at = scale_at(r, kk * per >> 7, per);
-    const float s = static_cast<float>(reinterpret_cast<const _Float16*>(g.w + g.l.scales)[b * per * 16 + at]);
-    const int z = g.has_zeros ? (g.w[g.l.zeros + b * per * 8 + (at >> 1)] >> ((at & 1) * 4)) & 15 : 0;
+    const uint8_t* b = g.w + ((row >> 4) * g.l.blocks + k / GROUP4_K) * g.l.bytes;
+    const int r = static_cast<int>(row & 15), kk = static_cast<int>(k & (GROUP4_K - 1));
+    const uint32_t word = reinterpret_cast<const uint32_t*>(b)[(kk >> 7) * 256 + (((kk >> 3) & 3) * 16 + r) * 4 + ((kk >> 5) & 3)];
+    const int q = (word >> (kk & 7) * 4) & 15, at = scale_at(r, kk * g.l.per >> 7, g.l.per);
+    const float s = static_cast<float>(reinterpret_cast<const _Float16*>(b + g.l.scales)[at]);
+    const int z = g.has_zeros ? (b[g.l.zeros + (at >> 1)] >> ((at & 1) * 4)) & 15 : 0;
     return static_cast<float>((q ^ 8) - (z ^ 8)) * s;
 }
 
@@ -44,33 +39,34 @@ __device__ __forceinline__ int64_t item_stride() { return static_cast<int64_t>(g
 uint32_t item_blocks(int64_t n) { return static_cast<uint32_t>(n > (1 << 28) ? 1 << 20 : (n + 255) / 256); }
 
 // One thread per dword of codes, then per block's scales and zero points.
-__global__ void __launch_bounds__(256) g4_pack_codes_kernel(const uint8_t* packed, uint32_t* out, Group4Layout l,
+__global__ void __launch_bounds__(256) g4_pack_codes_kernel(const uint8_t* packed, uint8_t* out, Group4Layout l,
                                                             int64_t rows, int64_t k) {
-    for (int64_t i = first_item(); i < l.tiles * l.steps * 256; i += item_stride()) {
-        const int64_t b = i >> 8;
-        const int lane = static_cast<int>(i >> 2) & 63, t = static_cast<int>(i) & 3;
-        const int64_t row = b / l.steps * 16 + (lane & 15), k0 = b % l.steps * 128 + t * 32 + (lane >> 4) * 8;
+    for (int64_t i = first_item(); i < l.tiles * l.blocks * 512; i += item_stride()) {
+        const int64_t b = i >> 9;
+        const int step = static_cast<int>(i >> 8) & 1, lane = static_cast<int>(i >> 2) & 63, t = static_cast<int>(i) & 3;
+        const int64_t row = b / l.blocks * 16 + (lane & 15);
+        const int64_t k0 = b % l.blocks * GROUP4_K + step * 128 + t * 32 + (lane >> 4) * 8;
         uint32_t word = 0;
         if (row < rows)
             for (int j = 0; j < 8 && k0 + j < k; j++) {
                 const uint32_t byte = packed[row * ((k + 1) >> 1) + ((k0 + j) >> 1)];
                 word |= (((j & 1 ? byte >> 4 : byte) & 15u) ^ 8u) << (4 * j);
             }
-        out[i] = word;
+        reinterpret_cast<uint32_t*>(out + b * l.bytes)[i & 511] = word;
     }
 }
 
 __global__ void __launch_bounds__(256) g4_pack_groups_kernel(const _Float16* scales, const uint8_t* zeros, uint8_t* out,
                                                              Group4Layout l, int64_t rows, int32_t group, int64_t groups) {
-    const int per = static_cast<int>(l.per);
-    for (int64_t b = first_item(); b < l.tiles * l.steps; b += item_stride()) {
-        const int64_t tile = b / l.steps, k0 = b % l.steps * 128;
-        _Float16* so = reinterpret_cast<_Float16*>(out + l.scales) + b * per * 16;
-        uint8_t* zo = out + l.zeros + b * per * 8;
-        for (int i = 0; i < 16 * per; i += 2) {  // two rows of a group: a byte of zero points
+    const int per = l.per;
+    for (int64_t b = first_item(); b < l.tiles * l.blocks; b += item_stride()) {
+        const int64_t tile = b / l.blocks, k0 = b % l.blocks * GROUP4_K;
+        _Float16* so = reinterpret_cast<_Float16*>(out + b * l.bytes + l.scales);
+        uint8_t* zo = out + b * l.bytes + l.zeros;
+        for (int i = 0; i < 32 * per; i += 2) {  // two rows of a group: a byte of zero points
             uint32_t zs = 0;
             for (int h = 0; h < 2; h++) {
-                const int r = i / (4 * per) * 4 + (i & 3) + h, g = i / 4 % per;
+                const int r = i / (8 * per) * 4 + (i & 3) + h, g = i / 4 % (2 * per);
                 const int64_t row = tile * 16 + r, gi = (k0 + g * (128 / per)) / group;
                 const bool in = row < rows && gi < groups;
                 so[i + h] = in ? scales[row * groups + gi] : static_cast<_Float16>(0.f);
@@ -119,8 +115,8 @@ __global__ void __launch_bounds__(256) g4_quantize_kernel(const void* src, int32
 
 // ---- products ---------------------------------------------------------------
 //
-// A wave takes a row tile (16 rows) and every ks-th of its 128-steps: one
-// 16-byte load per lane brings a step's codes in the order of the A operand of
+// A wave takes a row tile (16 rows) and every ks-th of its blocks of 256 k: one
+// 16-byte load per lane brings half a block's codes in the order of the A operand of
 // v_mfma_i32_16x16x64_i8 (group4.hpp).  The operand needs no more than a shift
 // and two masks per eight codes: a nibble in the high half of a byte, as int8,
 // is 16 (q - 8).  Fp16 operands would take five times the instructions, and
@@ -160,7 +156,7 @@ struct G4Args {
     int32_t m;       // tokens of this launch
     int32_t ks;      // waves that share a row tile
     int32_t groups;  // sets of G4_WAVES / ks row tiles
-    int32_t chunk;   // 128-steps of x in LDS at a time
+    int32_t chunk;   // blocks of x in LDS at a time
     bool whole;      // all of x fits: staged once
 };
 
@@ -311,14 +307,14 @@ __device__ __forceinline__ void lds_barrier() {
 
 // What a wave loads of one block.
 template <int PER, bool ZEROS>
-struct WStep {
-    u32x4 q;
-    half4_t s[PER];
-    uint32_t z[PER == 4 ? 2 : 1];
+struct WBlock {
+    u32x4 q[2];
+    half8_t s[PER];  // group g's four at 4 (g & 1) of s[g >> 1]
+    uint32_t z[PER];  // group g's four at bit 16 (g & 1) of z[g >> 1]
 };
 
 template <int PER>
-constexpr int g4_depth() { return PER == 1 ? 8 : 4; }  // blocks in flight per wave
+constexpr int g4_depth() { return PER == 4 ? 2 : 4; }  // blocks in flight per wave
 
 template <int PER, bool ZEROS, int PARTS, int NT>
 __global__ void __launch_bounds__(G4_THREADS, NT >= 3 ? 2 : 4) g4_gemv_kernel(G4Args a) {
@@ -327,12 +323,12 @@ __global__ void __launch_bounds__(G4_THREADS, NT >= 3 ? 2 : 4) g4_gemv_kernel(G4
     const int tid = static_cast<int>(threadIdx.x), lane = tid & 63, n = lane & 15, c = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int m = a.m, cols = PARTS * m, ks = a.ks, sub = wave % ks, local = wave / ks, per_group = G4_WAVES / ks;
-    const int steps = static_cast<int>(a.l.steps), tiles = static_cast<int>(a.l.tiles);
+    const int blocks = static_cast<int>(a.l.blocks), tiles = static_cast<int>(a.l.tiles);
     float4_t* red = reinterpret_cast<float4_t*>(lds);  // [wave][nt][lane]
     XLds x;
     x.digits = reinterpret_cast<uint8_t*>(lds + G4_WAVES * NT * 64);
-    x.power = reinterpret_cast<float*>(x.digits + a.chunk * 128 * cols);
-    x.sums = reinterpret_cast<int*>(x.power + a.chunk * m);
+    x.power = reinterpret_cast<float*>(x.digits + a.chunk * 256 * cols);
+    x.sums = reinterpret_cast<int*>(x.power + a.chunk * 2 * m);
 
     int col[NT], token[NT];
 #pragma unroll
@@ -341,50 +337,49 @@ __global__ void __launch_bounds__(G4_THREADS, NT >= 3 ? 2 : 4) g4_gemv_kernel(G4
         token[t] = col[t] / PARTS;
     }
 
-    const int pieces = a.chunk * 16, units = pieces * m;  // of a token, of all tokens in a chunk
-    auto stage = [&](int first, int from) {               // pieces from .. of steps first .. first + chunk of x
+    const int pieces = a.chunk * 32, units = pieces * m;  // of a token, of all tokens in a chunk
+    auto stage = [&](int first, int from) {               // pieces from .. of blocks first .. first + chunk of x
 #pragma unroll 1
         for (int u = from + tid; u < units; u += G4_THREADS) {
             const int t = u / pieces, kc = u % pieces;
-            x_store<PARTS, PER, ZEROS>(x_load<PARTS, false>(a, t, (static_cast<int64_t>(first) * 16 + kc) * 8), x, a.x_type,
+            x_store<PARTS, PER, ZEROS>(x_load<PARTS, false>(a, t, (static_cast<int64_t>(first) * 32 + kc) * 8), x, a.x_type,
                                        cols, m, t, kc);
         }
     };
-    // Loads of the ring: a step or tile past the last is outside of its
+    // Loads of the ring: a block or tile past the last is outside of its
     // buffer and reads nothing.  (A branch around a load would make the
     // compiler wait for all loads in flight.)
-    auto load = [&](int tile, int step, WStep<PER, ZEROS>& r) __attribute__((always_inline)) {
+    const uint32_t bytes = static_cast<uint32_t>(a.l.bytes), vo = static_cast<uint32_t>(lane) * 16;
+    auto load = [&](int tile, int block, WBlock<PER, ZEROS>& r) __attribute__((always_inline)) {
         const bool in = tile < tiles;
-        const int64_t b = in ? static_cast<int64_t>(tile) * steps : 0;
-        const uint32_t size = in ? static_cast<uint32_t>(steps) : 0u, at = static_cast<uint32_t>(step);
-        r.q = buf_ld128(make_rsrc(a.w + b * 1024, size * 1024), at * 1024 + lane * 16, 0);
-        const __amdgpu_buffer_rsrc_t rs = make_rsrc(a.w + a.l.scales + b * (32 * PER), size * (32 * PER));
-        const uint32_t so = (at * 4 + c) * (8 * PER);
-        if constexpr (PER == 1) {
-            r.s[0] = __builtin_bit_cast(half4_t, __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(rs, static_cast<int>(so), 0, 0)));
-        } else {
+        const __amdgpu_buffer_rsrc_t w = make_rsrc(a.w + (in ? static_cast<int64_t>(tile) * blocks * bytes : 0),
+                                                   in ? static_cast<uint32_t>(blocks) * bytes : 0u);
+        const uint32_t at = static_cast<uint32_t>(block) * bytes;
+        const auto ld = [&](uint32_t o) __attribute__((always_inline)) {
+            return __builtin_amdgcn_raw_buffer_load_b128(w, static_cast<int>(at + o), 0, 2);
+        };
+        r.q[0] = ld(vo);
+        r.q[1] = ld(1024 + vo);
 #pragma unroll
-            for (int g = 0; g < PER; g += 2) {
-                const half8_t v = __builtin_bit_cast(half8_t, buf_ld128(rs, so + 8 * g, 0));
-                r.s[g] = half4_t{v[0], v[1], v[2], v[3]};
-                r.s[g + 1] = half4_t{v[4], v[5], v[6], v[7]};
-            }
-        }
+        for (int g = 0; g < PER; g++) r.s[g] = __builtin_bit_cast(half8_t, ld(2048 + c * (16 * PER) + 16 * g));
         if constexpr (ZEROS) {
-            const __amdgpu_buffer_rsrc_t rz = make_rsrc(a.w + a.l.zeros + b * (8 * PER), size * (8 * PER));
-            const int zo = static_cast<int>(at * (8 * PER) + c * PER / 2 * 4);
+            const uint32_t zo = 2048 + 64 * PER + c * (4 * PER);
             if constexpr (PER == 4) {
-                const u32x2 v = __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(rz, zo, 0, 0));
+                const u32x4 v = ld(zo);
+#pragma unroll
+                for (int g = 0; g < 4; g++) r.z[g] = v[g];
+            } else if constexpr (PER == 2) {
+                const u32x2 v = __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(w, static_cast<int>(at + zo), 0, 2));
                 r.z[0] = v[0];
                 r.z[1] = v[1];
             } else {
-                r.z[0] = __builtin_amdgcn_raw_buffer_load_b32(rz, zo, 0, 0);
+                r.z[0] = __builtin_amdgcn_raw_buffer_load_b32(w, static_cast<int>(at + zo), 0, 2);
             }
         }
         __builtin_amdgcn_sched_barrier(0);  // slot after slot, as they are waited for
     };
     float4_t acc[NT];
-    auto multiply = [&](const WStep<PER, ZEROS>& r, int at) __attribute__((always_inline)) {  // step `at` of the chunk
+    auto multiply = [&](const WBlock<PER, ZEROS>& r, int half, int at) __attribute__((always_inline)) {  // step `at` of the chunk
         const uint4* xb = reinterpret_cast<const uint4*>(x.digits) + (at * 8 + c) * cols;
         int4_t xv[2][NT];
 #pragma unroll
@@ -404,21 +399,21 @@ __global__ void __launch_bounds__(G4_THREADS, NT >= 3 ? 2 : 4) g4_gemv_kernel(G4
         int4_t p[NT];
         float4_t sum[NT];
         const auto group_done = [&](int g) __attribute__((always_inline)) {
-            const uint32_t zw = !ZEROS ? 0u : PER == 1 ? r.z[0] >> (c & 1) * 16 : r.z[g >> 1];
+            const int gb = half * PER + g;  // of the block
 #pragma unroll
             for (int u = 0; u < NT; u++)
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
                     int q = p[u][i];
-                    if (ZEROS) q += __mul24(static_cast<int>(__builtin_amdgcn_sbfe(zw, (PER == 1 ? 0 : (g & 1) * 16) + 4 * i, 4)), sx[u][g]);
-                    const float s = static_cast<float>(r.s[g][i]), v = static_cast<float>(q);
+                    if (ZEROS) q += __mul24(static_cast<int>(__builtin_amdgcn_sbfe(r.z[gb >> 1], (gb & 1) * 16 + 4 * i, 4)), sx[u][g]);
+                    const float s = static_cast<float>(r.s[gb >> 1][(gb & 1) * 4 + i]), v = static_cast<float>(q);
                     sum[u][i] = g == 0 ? s * v : __builtin_fmaf(s, v, sum[u][i]);
                 }
         };
 #pragma unroll
         for (int h = 0; h < 2; h++) {
             constexpr uint32_t HIGH = 0xf0f0f0f0u;
-            const uint32_t q0 = r.q[2 * h], q1 = r.q[2 * h + 1];
+            const uint32_t q0 = r.q[half][2 * h], q1 = r.q[half][2 * h + 1];
             const int4_t wv = {static_cast<int>(q0 << 4 & HIGH), static_cast<int>(q0 & HIGH), static_cast<int>(q1 << 4 & HIGH),
                                static_cast<int>(q1 & HIGH)};
             const int4_t zero = {0, 0, 0, 0};
@@ -445,12 +440,12 @@ __global__ void __launch_bounds__(G4_THREADS, NT >= 3 ? 2 : 4) g4_gemv_kernel(G4
             for (int i = 0; i < 4; i++) acc[u][i] = __builtin_fmaf(f[u], sum[u][i], acc[u][i]);
     };
 
-    // The wave's steps of a tile: sub, sub + ks, ..., in rounds of DEPTH; the
+    // The wave's blocks of a tile: sub, sub + ks, ..., in rounds of DEPTH; the
     // last round loads the next tile's first ones.
-    const int rounds = (steps + ks * DEPTH - 1) / (ks * DEPTH);
+    const int rounds = (blocks + ks * DEPTH - 1) / (ks * DEPTH);
     const int hop = static_cast<int>(gridDim.x) * per_group;
     int tile = static_cast<int>(blockIdx.x) * per_group + local;
-    WStep<PER, ZEROS> ring[DEPTH];
+    WBlock<PER, ZEROS> ring[DEPTH];
     // x first, as loads come back in order: pieces past HELD per thread, then
     // HELD of them on the way together with the ring's first round.
     constexpr int HELD = 2;
@@ -497,7 +492,10 @@ __global__ void __launch_bounds__(G4_THREADS, NT >= 3 ? 2 : 4) g4_gemv_kernel(G4
             const int next = last ? tile + hop : tile, from = last ? sub : s + DEPTH * ks;
 #pragma unroll
             for (int d = 0; d < DEPTH; d++) {
-                if (tile < tiles && s + d * ks < steps) multiply(ring[d], s + d * ks - first);
+                if (tile < tiles && s + d * ks < blocks) {
+                    multiply(ring[d], 0, 2 * (s + d * ks - first));
+                    multiply(ring[d], 1, 2 * (s + d * ks - first) + 1);
+                }
                 load(next, from + d * ks, ring[d]);
             }
         }
@@ -540,20 +538,20 @@ constexpr int G4_COLS = 64;            // columns of a launch, at most
 
 int g4_run(G4Args a, bool has_zeros, hipStream_t st) {
     const int parts = a.x_type == ELEM_F32 ? 4 : 3, cols = parts * a.m, nt = (cols + 15) / 16;
-    const int per = static_cast<int>(a.l.per), depth = per == 1 ? g4_depth<1>() : g4_depth<4>();
+    const int per = a.l.per, depth = per == 4 ? g4_depth<4>() : g4_depth<1>();
     const int64_t slots = (nt >= 3 ? 8 : 16) * num_cus();  // waves that are resident at once
     a.ks = 1;
-    while (a.ks < G4_WAVES && a.l.tiles * a.ks * 2 <= slots && a.ks < a.l.steps) a.ks *= 2;
-    // the 128-steps of x that LDS takes, whole rounds of the ring
-    const int64_t step_bytes = 128 * cols + 4 * a.m + (has_zeros ? 4 * per * cols : 0);
-    int64_t chunk = G4_LDS / step_bytes;
-    a.whole = chunk >= a.l.steps;
+    while (a.ks < G4_WAVES && a.l.tiles * a.ks * 2 <= slots && a.ks < a.l.blocks) a.ks *= 2;
+    // the blocks of x that LDS takes, whole rounds of the ring
+    const int64_t block_bytes = 256 * cols + 8 * a.m + (has_zeros ? 8 * per * cols : 0);
+    int64_t chunk = G4_LDS / block_bytes;
+    a.whole = chunk >= a.l.blocks;
     while (!a.whole && a.ks > 1 && chunk < depth * a.ks) a.ks /= 2;
-    chunk = a.whole ? a.l.steps : chunk / (depth * a.ks) * (depth * a.ks);
+    chunk = a.whole ? a.l.blocks : chunk / (depth * a.ks) * (depth * a.ks);
     a.chunk = static_cast<int32_t>(chunk);
     const int per_group = G4_WAVES / a.ks;
     a.groups = static_cast<int32_t>((a.l.tiles + per_group - 1) / per_group);
-    const uint32_t lds = static_cast<uint32_t>(G4_WAVES * nt * 1024 + chunk * step_bytes);
+    const uint32_t lds = static_cast<uint32_t>(G4_WAVES * nt * 1024 + chunk * block_bytes);
     const int64_t most = (lds > (80 << 10) || nt >= 3 ? 1 : 2) * num_cus();
     const uint32_t grid = static_cast<uint32_t>(a.groups < most ? a.groups : most);
     const bool f32 = parts == 4;
@@ -603,10 +601,10 @@ int vb_group4_pack(const uint8_t* packed, const void* scales, const uint8_t* zer
         return E_INVAL;
     }
     hipStream_t st = as_stream(stream);
-    g4_pack_codes_kernel<<<item_blocks(l.tiles * l.steps * 256), 256, 0, st>>>(packed, static_cast<uint32_t*>(w), l,
+    g4_pack_codes_kernel<<<item_blocks(l.tiles * l.blocks * 512), 256, 0, st>>>(packed, static_cast<uint8_t*>(w), l,
                                                                                   rows, k);
     if (const int rc = check_launch("vb_group4_pack"); rc != OK) return rc;
-    g4_pack_groups_kernel<<<item_blocks(l.tiles * l.steps), 256, 0, st>>>(
+    g4_pack_groups_kernel<<<item_blocks(l.tiles * l.blocks), 256, 0, st>>>(
         static_cast<const _Float16*>(scales), zeros, static_cast<uint8_t*>(w), l, rows, group, (k + group - 1) / group);
     return check_launch("vb_group4_pack");
 }
