@@ -433,10 +433,16 @@ int vb_group4_quantize(const void* src, int32_t type, int64_t ld, int64_t rows, 
 int vb_group4_dequant_rows(const void* w, float* out, int64_t rows, int64_t k, int32_t group, int32_t has_zeros,
                            void* stream);
 /* y[t * rows + n] = sum_i W[n, i] x[t, i] for the m activation rows of x (row
- * stride x_ld, element type as above), fp32.  Sums are fp32 and fp32
- * activations keep 22 bits or more of their largest neighbour among 128. */
+ * stride x_ld, element type as above), fp32.  Per token and 128 consecutive k,
+ * activations are taken as integers of 30 bits (fp32) or 22 bits (fp16, bf16)
+ * below a power of two that holds the largest of them, the products with the
+ * codes are summed exactly in a group, and groups in fp32.  A token with a NaN
+ * or an infinity gives NaN.  workspace: at least vb_group4_workspace(...) bytes
+ * (0: none), 16-byte aligned, free again when the call's work is done. */
+int64_t vb_group4_workspace(int64_t m, int64_t rows, int64_t k, int32_t group, int32_t has_zeros, int32_t x_type);
 int vb_group4_gemv(const void* w, int64_t rows, int64_t k, int32_t group, int32_t has_zeros, const void* x,
-                   int32_t x_type, int64_t x_ld, int64_t m, float* y, void* stream);
+                   int32_t x_type, int64_t x_ld, int64_t m, float* y, void* workspace, size_t workspace_bytes,
+                   void* stream);
 
 /* ---- GGUF ingestion --------------------------------------------------------
  * A .gguf file mapped read-only and parsed (header, metadata, tensor table).

@@ -101,20 +101,32 @@ def test_group4_bytes(lib):
     lambda lib: lib.vb_group4_quantize(None, 0, 128, 16, 128, 128, PTR, PTR, None, None),
     lambda lib: lib.vb_group4_dequant_rows(PTR, None, 16, 128, 128, 0, None),
     lambda lib: lib.vb_group4_dequant_rows(PTR + 4, PTR, 16, 128, 128, 0, None),
-    lambda lib: lib.vb_group4_gemv(PTR, 16, 128, 128, 0, PTR, 3, 128, 1, PTR, None),
-    lambda lib: lib.vb_group4_gemv(PTR, 16, 128, 128, 0, PTR, 0, 128, -1, PTR, None),
-    lambda lib: lib.vb_group4_gemv(PTR, 16, 128, 128, 0, PTR, 0, -1, 2, PTR, None),
-    lambda lib: lib.vb_group4_gemv(PTR, 16, 0, 128, 0, PTR, 0, 128, 1, PTR, None),
-    lambda lib: lib.vb_group4_gemv(PTR, 16, 128, 48, 0, PTR, 0, 128, 1, PTR, None),
-    lambda lib: lib.vb_group4_gemv(None, 16, 128, 128, 0, PTR, 0, 128, 1, PTR, None),
-    lambda lib: lib.vb_group4_gemv(PTR + 8, 16, 128, 128, 0, PTR, 0, 128, 1, PTR, None),
+    lambda lib: lib.vb_group4_gemv(PTR, 16, 128, 128, 0, PTR, 3, 128, 1, PTR, PTR, 1 << 30, None),
+    lambda lib: lib.vb_group4_gemv(PTR, 16, 128, 128, 0, PTR, 0, 128, -1, PTR, PTR, 1 << 30, None),
+    lambda lib: lib.vb_group4_gemv(PTR, 16, 128, 128, 0, PTR, 0, -1, 2, PTR, PTR, 1 << 30, None),
+    lambda lib: lib.vb_group4_gemv(PTR, 16, 0, 128, 0, PTR, 0, 128, 1, PTR, PTR, 1 << 30, None),
+    lambda lib: lib.vb_group4_gemv(PTR, 16, 128, 48, 0, PTR, 0, 128, 1, PTR, PTR, 1 << 30, None),
+    lambda lib: lib.vb_group4_gemv(None, 16, 128, 128, 0, PTR, 0, 128, 1, PTR, PTR, 1 << 30, None),
+    lambda lib: lib.vb_group4_gemv(PTR + 8, 16, 128, 128, 0, PTR, 0, 128, 1, PTR, PTR, 1 << 30, None),
 ])
 def test_group4_refuses(lib, call):
     assert call(lib) == INVAL
 
 
+def test_group4_workspace(lib):
+    for bad in ((-1, 16, 128, 128, 0, 0), (1, 0, 128, 128, 0, 0), (1, 16, 128, 48, 0, 0), (1, 16, 128, 128, 0, 3)):
+        assert lib.vb_group4_workspace(*bad) == -1
+    assert lib.vb_group4_workspace(0, 16, 128, 128, 0, 0) == 0
+    for m, rows, k, group, zeros, kind in ((8, 4096, 14336, 64, 1, 1), (70, 100, 4096, 32, 1, 0), (1, 64, 1 << 20, 32, 1, 0)):
+        need = lib.vb_group4_workspace(m, rows, k, group, zeros, kind)
+        assert need > 0 and need % 16 == 0
+        for ws, nbytes in ((PTR, need - 1), (None, need), (PTR + 8, need)):
+            assert lib.vb_group4_gemv(PTR, rows, k, group, zeros, PTR, kind, k, m, PTR, ws, nbytes, None) == INVAL
+            assert b"workspace" in lib.vb_last_error()
+
+
 def test_group4_gemv_of_no_tokens_does_nothing(lib):
-    assert lib.vb_group4_gemv(PTR, 16, 128, 128, 0, None, 0, 128, 0, None, None) == OK
+    assert lib.vb_group4_gemv(PTR, 16, 128, 128, 0, None, 0, 128, 0, None, None, 0, None) == OK
 
 
 def test_python_calls_take_gpu_tensors_only():
@@ -137,7 +149,7 @@ def test_ctypes_signatures_have_the_header_s_argument_count():
     text = open(os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "include", "vbhip.h")).read()
     text = re.sub(r"/\*.*?\*/", "", text, flags=re.S)
     for name in ("vb_block_norm", "vb_token_logprobs", "vb_token_logprobs_workspace", "vb_group4_bytes",
-                 "vb_group4_pack", "vb_group4_quantize", "vb_group4_dequant_rows", "vb_group4_gemv"):
+                 "vb_group4_pack", "vb_group4_quantize", "vb_group4_dequant_rows", "vb_group4_workspace", "vb_group4_gemv"):
         args = re.search(name + r"\(([^)]*)\)", text).group(1).split(",")
         sig = _lib.SIGNATURES[name][1]
         assert len(args) == len(sig), name

@@ -74,7 +74,8 @@ SIGNATURES = {
     "vb_group4_pack": (ctypes.c_int, [_vp, _vp, _vp, _vp, _i64, _i64, _i32, _vp]),
     "vb_group4_quantize": (ctypes.c_int, [_vp, _i32, _i64, _i64, _i64, _i32, _vp, _vp, _vp, _vp]),
     "vb_group4_dequant_rows": (ctypes.c_int, [_vp, _vp, _i64, _i64, _i32, _i32, _vp]),
-    "vb_group4_gemv": (ctypes.c_int, [_vp, _i64, _i64, _i32, _i32, _vp, _i32, _i64, _i64, _vp, _vp]),
+    "vb_group4_workspace": (_i64, [_i64, _i64, _i64, _i32, _i32, _i32]),
+    "vb_group4_gemv": (ctypes.c_int, [_vp, _i64, _i64, _i32, _i32, _vp, _i32, _i64, _i64, _vp, _vp, _sz, _vp]),
     "vb_gguf_open": (ctypes.c_int, [ctypes.c_char_p, ctypes.POINTER(_vp)]),
     "vb_gguf_close": (ctypes.c_int, [_vp]),
     "vb_gguf_info": (ctypes.c_int, [_vp, ctypes.POINTER(ctypes.c_uint32), ctypes.POINTER(ctypes.c_uint64),

@@ -4,6 +4,8 @@
 //
 //   W[n, k] = (q[n, k] - z[n, g]) * s[n, g],   g = k / group,  z = 8 without zeros
 //   y[t, n] = sum_k W[n, k] x[t, k]
+#include <type_traits>
+
 #include "elem_types.hpp"
 #include "group4.hpp"
 #include "vb_internal.hpp"
@@ -143,21 +145,21 @@ typedef float float4_t __attribute__((ext_vector_type(4)));
 typedef int int4_t __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 
-constexpr int G4_WAVES = 8;
-constexpr int G4_THREADS = 64 * G4_WAVES;
+constexpr int G4_WAVES = 8;  // of a workgroup, at most
 
 struct G4Args {
     const uint8_t* w;
     Group4Layout l;
     const void* x;
+    uint8_t* image;  // x as digits, chunk after chunk, laid out for LDS (null: the workgroups make it)
+    float* partial;  // [chunk][token][row]: sums of a chunk, where there are several
     float* y;
     int64_t x_ld, rows, k;
-    int32_t x_type;
-    int32_t m;       // tokens of this launch
-    int32_t ks;      // waves that share a row tile
-    int32_t groups;  // sets of G4_WAVES / ks row tiles
-    int32_t chunk;   // blocks of x in LDS at a time
-    bool whole;      // all of x fits: staged once
+    int32_t x_type, parts;  // digits of a value
+    int32_t m;              // tokens of this launch
+    int32_t ks;             // waves of a workgroup that share a row tile
+    int32_t kz, chunk;      // chunks of k, each a workgroup's of its own, and their blocks
+    int32_t groups;         // sets of waves / ks row tiles, one a workgroup's turn
 };
 
 // Eight activations as loaded: fp32 (8 dwords) or 16-bit (4).
@@ -219,19 +221,38 @@ __device__ __forceinline__ int dpp_i(int v) {
     return __builtin_amdgcn_update_dpp(0, v, CTRL, 0xF, 0xF, false);
 }
 
-// x in LDS.
+// x of a chunk as a workgroup reads it.
 //   digits  [step][half][c][col] of 16 bytes: the B operand's bytes of k = 64 half + 8 c + 0..7 and + 32
 //   power   [step][token] the block's power of two (with the weights' 1/16 and the top digit's 256^(PARTS-1))
 //   sums    [step][group][col] -16 sum X
-struct XLds {
+struct XImage {
     uint8_t* digits;
     float* power;
     int* sums;
 };
 
+// Bytes of a block's 256 k: digits, power and sums.
+__host__ __device__ constexpr int64_t digit_bytes(int64_t cols) { return 256 * cols; }
+__host__ __device__ constexpr int64_t table_bytes(int64_t cols, int64_t m, int64_t per, bool zeros) {
+    return 8 * m + (zeros ? 8 * per * cols : 0);
+}
+
+// Bytes of a chunk in LDS and in the image.
+__host__ __device__ constexpr int64_t chunk_bytes(int64_t blocks, int64_t cols, int64_t m, int64_t per, bool zeros) {
+    return (blocks * (digit_bytes(cols) + table_bytes(cols, m, per, zeros)) + 15) / 16 * 16;
+}
+
+__device__ __forceinline__ XImage x_image(uint8_t* at, int blocks, int cols, int m) {
+    XImage x;
+    x.digits = at;
+    x.power = reinterpret_cast<float*>(at + digit_bytes(cols) * blocks);
+    x.sums = reinterpret_cast<int*>(x.power + 2 * blocks * m);
+    return x;
+}
+
 // One piece (eight values; piece kc of the chunk, 16 to a block in 16 neighbouring lanes) of a token.
 template <int PARTS, int PER, bool ZEROS>
-__device__ __forceinline__ void x_store(const XUnit<PARTS>& r, const XLds& x, int type, int cols, int m, int token, int kc) {
+__device__ __forceinline__ void x_store(const XUnit<PARTS>& r, const XImage& x, int type, int cols, int m, int token, int kc) {
     float v[8];
     if constexpr (PARTS == 4) {
 #pragma unroll
@@ -313,46 +334,61 @@ struct WBlock {
     uint32_t z[PER];  // group g's four at bit 16 (g & 1) of z[g >> 1]
 };
 
-template <int PER>
-constexpr int g4_depth() { return PER == 4 ? 2 : 4; }  // blocks in flight per wave
+// x of a launch as digits into the workspace, one thread per piece.
+template <int PER, bool ZEROS, int PARTS>
+__global__ void __launch_bounds__(256) g4_image_kernel(G4Args a) {
+    const int cols = PARTS * a.m, t = static_cast<int>(blockIdx.y);
+    const int64_t at = first_item();
+    if (at >= a.l.blocks * 32) return;
+    const int64_t z = at / (a.chunk * 32);
+    const int64_t left = a.l.blocks - z * a.chunk;
+    const int blocks = static_cast<int>(left < a.chunk ? left : a.chunk);
+    const XImage x = x_image(a.image + z * chunk_bytes(a.chunk, cols, a.m, PER, ZEROS), blocks, cols, a.m);
+    x_store<PARTS, PER, ZEROS>(x_load<PARTS, false>(a, t, at * 8), x, a.x_type, cols, a.m, t,
+                               static_cast<int>(at - z * a.chunk * 32));
+}
 
-template <int PER, bool ZEROS, int PARTS, int NT>
-__global__ void __launch_bounds__(G4_THREADS, NT >= 3 ? 2 : 4) g4_gemv_kernel(G4Args a) {
-    constexpr int DEPTH = g4_depth<PER>();
+// Where a workgroup has its activations from: its own arithmetic, or the image.
+enum { G4_SELF, G4_COPY };
+
+constexpr int G4_DEPTH = 2;  // blocks in flight per wave
+
+// Kernels that take the registers of 8 waves a CU, not 16.
+__host__ __device__ constexpr bool g4_wide(int nt, int per, bool zeros) { return nt > 1 || (per == 4 && zeros); }
+
+// PARTS 0: a.parts (no code but the staging depends on it).
+template <int PER, bool ZEROS, int PARTS, int NT, int MODE>
+__global__ void __launch_bounds__(64 * G4_WAVES, g4_wide(NT, PER, ZEROS) ? 2 : 4) g4_gemv_kernel(G4Args a) {
+    constexpr int DEPTH = G4_DEPTH;
     extern __shared__ uint4 lds[];
     const int tid = static_cast<int>(threadIdx.x), lane = tid & 63, n = lane & 15, c = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int m = a.m, cols = PARTS * m, ks = a.ks, sub = wave % ks, local = wave / ks, per_group = G4_WAVES / ks;
-    const int blocks = static_cast<int>(a.l.blocks), tiles = static_cast<int>(a.l.tiles);
+    const int waves = static_cast<int>(blockDim.x) >> 6, threads = static_cast<int>(blockDim.x);
+    const int parts = PARTS ? PARTS : a.parts, m = a.m, cols = parts * m;
+    const int ks = a.ks, sub = wave % ks, local = wave / ks, per_group = waves / ks;
+    const int kz = MODE == G4_SELF ? 1 : a.kz, z = static_cast<int>(blockIdx.x) % kz;
+    const int turn = static_cast<int>(blockIdx.x) / kz, turns = static_cast<int>(gridDim.x) / kz;
+    const int64_t row_blocks = a.l.blocks, first = static_cast<int64_t>(z) * a.chunk;
+    const int tiles = static_cast<int>(a.l.tiles);
+    const int blocks = static_cast<int>(row_blocks - first < a.chunk ? row_blocks - first : a.chunk);
     float4_t* red = reinterpret_cast<float4_t*>(lds);  // [wave][nt][lane]
-    XLds x;
-    x.digits = reinterpret_cast<uint8_t*>(lds + G4_WAVES * NT * 64);
-    x.power = reinterpret_cast<float*>(x.digits + a.chunk * 256 * cols);
-    x.sums = reinterpret_cast<int*>(x.power + a.chunk * 2 * m);
+    uint8_t* const mine = reinterpret_cast<uint8_t*>(lds + waves * NT * 64);
+    const XImage x = x_image(mine, blocks, cols, m);
 
     int col[NT], token[NT];
 #pragma unroll
     for (int t = 0; t < NT; t++) {
         col[t] = t * 16 + n < cols ? t * 16 + n : cols - 1;
-        token[t] = col[t] / PARTS;
+        token[t] = col[t] / parts;
     }
 
-    const int pieces = a.chunk * 32, units = pieces * m;  // of a token, of all tokens in a chunk
-    auto stage = [&](int first, int from) {               // pieces from .. of blocks first .. first + chunk of x
-#pragma unroll 1
-        for (int u = from + tid; u < units; u += G4_THREADS) {
-            const int t = u / pieces, kc = u % pieces;
-            x_store<PARTS, PER, ZEROS>(x_load<PARTS, false>(a, t, (static_cast<int64_t>(first) * 32 + kc) * 8), x, a.x_type,
-                                       cols, m, t, kc);
-        }
-    };
     // Loads of the ring: a block or tile past the last is outside of its
     // buffer and reads nothing.  (A branch around a load would make the
     // compiler wait for all loads in flight.)
     const uint32_t bytes = static_cast<uint32_t>(a.l.bytes), vo = static_cast<uint32_t>(lane) * 16;
     auto load = [&](int tile, int block, WBlock<PER, ZEROS>& r) __attribute__((always_inline)) {
         const bool in = tile < tiles;
-        const __amdgpu_buffer_rsrc_t w = make_rsrc(a.w + (in ? static_cast<int64_t>(tile) * blocks * bytes : 0),
+        const __amdgpu_buffer_rsrc_t w = make_rsrc(a.w + (in ? (static_cast<int64_t>(tile) * row_blocks + first) * bytes : 0),
                                                    in ? static_cast<uint32_t>(blocks) * bytes : 0u);
         const uint32_t at = static_cast<uint32_t>(block) * bytes;
         const auto ld = [&](uint32_t o) __attribute__((always_inline)) {
@@ -379,195 +415,305 @@ __global__ void __launch_bounds__(G4_THREADS, NT >= 3 ? 2 : 4) g4_gemv_kernel(G4
         __builtin_amdgcn_sched_barrier(0);  // slot after slot, as they are waited for
     };
     float4_t acc[NT];
-    auto multiply = [&](const WBlock<PER, ZEROS>& r, int half, int at) __attribute__((always_inline)) {  // step `at` of the chunk
-        const uint4* xb = reinterpret_cast<const uint4*>(x.digits) + (at * 8 + c) * cols;
-        int4_t xv[2][NT];
+    // H halves of a block from half `from` on.
+    auto multiply = [&](auto halves, const WBlock<PER, ZEROS>& r, int from, int at) __attribute__((always_inline)) {
+        constexpr int H = decltype(halves)::value;
+        const int4_t zero = {0, 0, 0, 0};
+        // With few columns all operands are requested first, then all products,
+        // then the sums: a wave has little else to fill these latencies with.
+        constexpr bool EARLY = NT == 1 || (NT == 2 && PER == 1);
+        int4_t xe[H][2][EARLY ? NT : 1];
+        float fe[H][EARLY ? NT : 1];
+        int se[H][EARLY ? NT : 1][PER];
+        const auto x_of = [&](int e, int h, int u) __attribute__((always_inline)) {
+            return __builtin_bit_cast(int4_t, reinterpret_cast<const uint4*>(x.digits)[((2 * at + from + e) * 8 + 4 * h + c) * cols + col[u]]);
+        };
+        const auto f_of = [&](int e, int u) __attribute__((always_inline)) { return x.power[(2 * at + from + e) * m + token[u]]; };
+        const auto s_of = [&](int e, int u, int g) __attribute__((always_inline)) {
+            return ZEROS ? x.sums[((2 * at + from + e) * PER + g) * cols + col[u]] : 0;
+        };
+        if constexpr (EARLY) {
 #pragma unroll
-        for (int h = 0; h < 2; h++)
+            for (int e = 0; e < H; e++)
 #pragma unroll
-            for (int u = 0; u < NT; u++) xv[h][u] = __builtin_bit_cast(int4_t, xb[h * 4 * cols + col[u]]);
-        float f[NT];
-        int sx[NT][PER];
+                for (int u = 0; u < NT; u++) {
+                    xe[e][0][u] = x_of(e, 0, u);
+                    xe[e][1][u] = x_of(e, 1, u);
+                    fe[e][u] = f_of(e, u);
+#pragma unroll
+                    for (int g = 0; g < PER; g++) se[e][u][g] = s_of(e, u, g);
+                }
+        }
+        int4_t wv[H][2];
+#pragma unroll
+        for (int e = 0; e < H; e++)
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                constexpr uint32_t HIGH = 0xf0f0f0f0u;
+                const uint32_t q0 = r.q[from + e][2 * h], q1 = r.q[from + e][2 * h + 1];
+                wv[e][h] = int4_t{static_cast<int>(q0 << 4 & HIGH), static_cast<int>(q0 & HIGH),
+                                  static_cast<int>(q1 << 4 & HIGH), static_cast<int>(q1 & HIGH)};
+            }
 #pragma unroll
         for (int u = 0; u < NT; u++) {
-            f[u] = x.power[at * m + token[u]];
-            if (ZEROS) {
+            int4_t p[H][PER];
 #pragma unroll
-                for (int g = 0; g < PER; g++) sx[u][g] = x.sums[(at * PER + g) * cols + col[u]];
-            }
-        }
-        int4_t p[NT];
-        float4_t sum[NT];
-        const auto group_done = [&](int g) __attribute__((always_inline)) {
-            const int gb = half * PER + g;  // of the block
+            for (int e = 0; e < H; e++)
 #pragma unroll
-            for (int u = 0; u < NT; u++)
+                for (int h = 0; h < 2; h++) {
+                    const int4_t xv = EARLY ? xe[e][h][EARLY ? u : 0] : x_of(e, h, u);
+                    if constexpr (PER == 4) {
+                        const auto pair = [](int lo, int hi) {
+                            return static_cast<long>(static_cast<uint64_t>(static_cast<uint32_t>(hi)) << 32 | static_cast<uint32_t>(lo));
+                        };
 #pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    int q = p[u][i];
-                    if (ZEROS) q += __mul24(static_cast<int>(__builtin_amdgcn_sbfe(r.z[gb >> 1], (gb & 1) * 16 + 4 * i, 4)), sx[u][g]);
-                    const float s = static_cast<float>(r.s[gb >> 1][(gb & 1) * 4 + i]), v = static_cast<float>(q);
-                    sum[u][i] = g == 0 ? s * v : __builtin_fmaf(s, v, sum[u][i]);
+                        for (int t = 0; t < 2; t++)
+                            p[e][2 * h + t] = __builtin_amdgcn_mfma_i32_16x16x32_i8(pair(wv[e][h][2 * t], wv[e][h][2 * t + 1]),
+                                                                                   pair(xv[2 * t], xv[2 * t + 1]), zero, 0, 0, 0);
+                    } else {
+                        int4_t& to = p[e][PER == 1 ? 0 : h];
+                        to = __builtin_amdgcn_mfma_i32_16x16x64_i8(wv[e][h], xv, PER == 1 && h == 1 ? to : zero, 0, 0, 0);
+                    }
                 }
-        };
 #pragma unroll
-        for (int h = 0; h < 2; h++) {
-            constexpr uint32_t HIGH = 0xf0f0f0f0u;
-            const uint32_t q0 = r.q[half][2 * h], q1 = r.q[half][2 * h + 1];
-            const int4_t wv = {static_cast<int>(q0 << 4 & HIGH), static_cast<int>(q0 & HIGH), static_cast<int>(q1 << 4 & HIGH),
-                               static_cast<int>(q1 & HIGH)};
-            const int4_t zero = {0, 0, 0, 0};
-            if constexpr (PER == 4) {
-                const auto pair = [](int lo, int hi) { return static_cast<long>(static_cast<uint64_t>(static_cast<uint32_t>(hi)) << 32 | static_cast<uint32_t>(lo)); };
+            for (int e = 0; e < H; e++) {
+                const float f = EARLY ? fe[e][EARLY ? u : 0] : f_of(e, u);
+                float sum[4];
 #pragma unroll
-                for (int t = 0; t < 2; t++) {
+                for (int g = 0; g < PER; g++) {
+                    const int gb = (from + e) * PER + g;  // of the block
+                    const int sx = EARLY ? se[e][EARLY ? u : 0][g] : s_of(e, u, g);
 #pragma unroll
-                    for (int u = 0; u < NT; u++)
-                        p[u] = __builtin_amdgcn_mfma_i32_16x16x32_i8(pair(wv[2 * t], wv[2 * t + 1]), pair(xv[h][u][2 * t], xv[h][u][2 * t + 1]), zero, 0, 0, 0);
-                    group_done(2 * h + t);
+                    for (int i = 0; i < 4; i++) {
+                        int q = p[e][g][i];
+                        if (ZEROS) q += __mul24(static_cast<int>(__builtin_amdgcn_sbfe(r.z[gb >> 1], (gb & 1) * 16 + 4 * i, 4)), sx);
+                        const float s = static_cast<float>(r.s[gb >> 1][(gb & 1) * 4 + i]);
+                        sum[i] = g == 0 ? s * static_cast<float>(q) : __builtin_fmaf(s, static_cast<float>(q), sum[i]);
+                    }
                 }
-            } else {
+                // (s p) f: f p by itself may leave fp32's range where W x does not
 #pragma unroll
-                for (int u = 0; u < NT; u++)
-                    p[u] = __builtin_amdgcn_mfma_i32_16x16x64_i8(wv, xv[h][u], PER == 2 || h == 0 ? zero : p[u], 0, 0, 0);
-                if (PER == 2 || h == 1) group_done(PER == 2 ? h : 0);
+                for (int i = 0; i < 4; i++) acc[u][i] = __builtin_fmaf(f, sum[i], acc[u][i]);
             }
+            if (PER == 4 && NT == 3) __builtin_amdgcn_sched_barrier(0);  // three at once do not fit the registers
         }
-        // (s p) f: f p by itself may leave fp32's range where W x does not
-#pragma unroll
-        for (int u = 0; u < NT; u++)
-#pragma unroll
-            for (int i = 0; i < 4; i++) acc[u][i] = __builtin_fmaf(f[u], sum[u][i], acc[u][i]);
     };
 
     // The wave's blocks of a tile: sub, sub + ks, ..., in rounds of DEPTH; the
     // last round loads the next tile's first ones.
     const int rounds = (blocks + ks * DEPTH - 1) / (ks * DEPTH);
-    const int hop = static_cast<int>(gridDim.x) * per_group;
-    int tile = static_cast<int>(blockIdx.x) * per_group + local;
+    const int hop = turns * per_group;
+    int tile = turn * per_group + local;
     WBlock<PER, ZEROS> ring[DEPTH];
-    // x first, as loads come back in order: pieces past HELD per thread, then
-    // HELD of them on the way together with the ring's first round.
-    constexpr int HELD = 2;
-    XUnit<PARTS> held[HELD];
-    const bool hold = a.k >= 8;
-    stage(0, hold ? HELD * G4_THREADS : 0);
-    if (hold) {
+    const auto fill = [&]() __attribute__((always_inline)) {
 #pragma unroll
-        for (int i = 0; i < HELD; i++) {
-            const int u = i * G4_THREADS + tid, v = u < units ? u : units - 1;
-            held[i] = x_load<PARTS, true>(a, v / pieces, static_cast<int64_t>(v % pieces) * 8);
+        for (int d = 0; d < DEPTH; d++) load(tile, sub + d * ks, ring[d]);
+    };
+    // x first, as loads come back in order: what a thread cannot hold, then the
+    // rest of it on the way together with the ring's first round.
+    if constexpr (MODE == G4_SELF) {
+        constexpr int HELD = 4;
+        XUnit<PARTS> held[HELD];
+        const int pieces = blocks * 32, units = pieces * m;  // of a token, of all
+        const bool hold = a.k >= 8;
+#pragma unroll 1
+        for (int u = (hold ? HELD * threads : 0) + tid; u < units; u += threads) {
+            const int t = m == 1 ? 0 : u / pieces, kc = u - t * pieces;
+            x_store<PARTS, PER, ZEROS>(x_load<PARTS, false>(a, t, kc * 8), x, a.x_type, cols, m, t, kc);
         }
-    }
+        if (hold) {
 #pragma unroll
-    for (int d = 0; d < DEPTH; d++) load(tile, sub + d * ks, ring[d]);
-    if (hold) {
-#pragma unroll
-        for (int i = 0; i < HELD; i++) {
-            const int u = i * G4_THREADS + tid;
-            if (u >= units) continue;
-            const int t = u / pieces, kc = u % pieces;
-            if (kc * 8 + 8 > a.k) x_shift<PARTS>(held[i], static_cast<int>(kc * 8 >= a.k ? 8 : kc * 8 + 8 - a.k));
-            x_store<PARTS, PER, ZEROS>(held[i], x, a.x_type, cols, m, t, kc);
+            for (int i = 0; i < HELD; i++) {
+                const int u = i * threads + tid, v = u < units ? u : units - 1, t = m == 1 ? 0 : v / pieces;
+                held[i] = x_load<PARTS, true>(a, t, static_cast<int64_t>(v - t * pieces) * 8);
+            }
         }
+        fill();
+        if (hold) {
+#pragma unroll
+            for (int i = 0; i < HELD; i++) {
+                const int u = i * threads + tid;
+                if (u >= units) continue;
+                const int t = m == 1 ? 0 : u / pieces, kc = u - t * pieces;
+                if (kc * 8 + 8 > a.k) x_shift<PARTS>(held[i], static_cast<int>(kc * 8 >= a.k ? 8 : kc * 8 + 8 - a.k));
+                x_store<PARTS, PER, ZEROS>(held[i], x, a.x_type, cols, m, t, kc);
+            }
+        }
+    } else {
+        constexpr int HELD = 8;
+        const u32x4* from = reinterpret_cast<const u32x4*>(a.image + z * chunk_bytes(a.chunk, cols, m, PER, ZEROS));
+        u32x4* to = reinterpret_cast<u32x4*>(mine);
+        const int count = static_cast<int>(chunk_bytes(blocks, cols, m, PER, ZEROS) / 16);
+        u32x4 held[HELD];
+        const auto get = [&](int base) __attribute__((always_inline)) {
+#pragma unroll
+            for (int i = 0; i < HELD; i++) {
+                const int u = base + i * threads + tid;
+                held[i] = from[u < count ? u : count - 1];
+            }
+        };
+        const auto put = [&](int base) __attribute__((always_inline)) {
+#pragma unroll
+            for (int i = 0; i < HELD; i++) {
+                const int u = base + i * threads + tid;
+                if (u < count) to[u] = held[i];
+            }
+        };
+        int base = 0;
+        for (; base + HELD * threads < count; base += HELD * threads) {
+            get(base);
+            put(base);
+        }
+        get(base);
+        fill();
+        put(base);
     }
     lds_barrier();
-    bool staged = true;  // the chunk in LDS is the next one to be used
-    for (int grp = static_cast<int>(blockIdx.x); grp < a.groups; grp += static_cast<int>(gridDim.x), tile += hop) {
+    for (int grp = turn; grp < a.groups; grp += turns, tile += hop) {
 #pragma unroll
         for (int t = 0; t < NT; t++) acc[t] = float4_t{0.f, 0.f, 0.f, 0.f};
-        int first = 0;  // of the chunk (whose length is whole rounds)
         for (int i = 0; i < rounds; i++) {
             const int s = i * ks * DEPTH + sub;
-            if (s - sub == first + a.chunk) first += a.chunk;
-            if (!a.whole && s - sub == first) {
-                if (!staged) {
-                    lds_barrier();  // the chunk before is read
-                    stage(first, 0);
-                    lds_barrier();
-                }
-                staged = false;
-            }
             const bool last = i + 1 == rounds;
             const int next = last ? tile + hop : tile, from = last ? sub : s + DEPTH * ks;
 #pragma unroll
             for (int d = 0; d < DEPTH; d++) {
                 if (tile < tiles && s + d * ks < blocks) {
-                    multiply(ring[d], 0, 2 * (s + d * ks - first));
-                    multiply(ring[d], 1, 2 * (s + d * ks - first) + 1);
+                    if constexpr (NT == 1 && PER == 1) {
+                        multiply(std::integral_constant<int, 2>{}, ring[d], 0, s + d * ks);
+                    } else {
+                        multiply(std::integral_constant<int, 1>{}, ring[d], 0, s + d * ks);
+                        __builtin_amdgcn_sched_barrier(0);  // (both halves at once do not fit the registers)
+                        multiply(std::integral_constant<int, 1>{}, ring[d], 1, s + d * ks);
+                    }
                 }
                 load(next, from + d * ks, ring[d]);
             }
         }
         // y: a token's digits of a tile's waves, added in order.  A wave that has
         // a tile by itself reads what it wrote.
-        const float digit[4] = {PARTS == 4 ? 0x1p-24f : 0x1p-16f, PARTS == 4 ? 0x1p-16f : 0x1p-8f, PARTS == 4 ? 0x1p-8f : 1.f, 1.f};
 #pragma unroll
         for (int t = 0; t < NT; t++) red[(wave * NT + t) * 64 + lane] = acc[t];
         if (ks > 1) lds_barrier();
         const float* rf = reinterpret_cast<const float*>(red);
         const int outs = (ks > 1 ? per_group : 1) * 16 * m;
-        for (int o = ks > 1 ? tid : lane; o < outs; o += ks > 1 ? G4_THREADS : 64) {
+        for (int o = ks > 1 ? tid : lane; o < outs; o += ks > 1 ? threads : 64) {
             const int r = o & 15, tt = ks > 1 ? (o >> 4) % per_group : local, t = ks > 1 ? (o >> 4) / per_group : o >> 4;
             const int64_t row = (static_cast<int64_t>(grp) * per_group + tt) * 16 + r;
             float total = 0.f;
-#pragma unroll
-            for (int h = 0; h < PARTS; h++) {
-                const int cc = PARTS * t + h;
+            for (int h = 0; h < parts; h++) {
+                const int cc = parts * t + h;
                 float sum = 0.f;
                 for (int v = 0; v < ks; v++)
                     sum += rf[(((tt * ks + v) * NT + (cc >> 4)) * 64 + (r >> 2) * 16 + (cc & 15)) * 4 + (r & 3)];
-                total = __builtin_fmaf(digit[h], sum, total);
+                total = __builtin_fmaf(total, 0x1p-8f, sum);  // digit h is worth 256 times digit h - 1
             }
-            if (row < a.rows) a.y[static_cast<int64_t>(t) * a.rows + row] = total;
+            float* y = kz > 1 ? a.partial + static_cast<int64_t>(z) * m * a.rows : a.y;
+            if (row < a.rows) y[static_cast<int64_t>(t) * a.rows + row] = total;
         }
         if (ks > 1) lds_barrier();  // red is free
     }
 }
 
-template <int PER, bool ZEROS, int PARTS>
-void g4_launch(const G4Args& a, int nt, uint32_t grid, uint32_t lds, hipStream_t st) {
-    if (nt == 1) g4_gemv_kernel<PER, ZEROS, PARTS, 1><<<grid, G4_THREADS, lds, st>>>(a);
-    else if (nt == 2) g4_gemv_kernel<PER, ZEROS, PARTS, 2><<<grid, G4_THREADS, lds, st>>>(a);
-    else if (nt == 3) g4_gemv_kernel<PER, ZEROS, PARTS, 3><<<grid, G4_THREADS, lds, st>>>(a);
-    else g4_gemv_kernel<PER, ZEROS, PARTS, 4><<<grid, G4_THREADS, lds, st>>>(a);
+// y = the chunks' sums, added in order.  (Joined by the last workgroup of a
+// tile instead, the fences around its count write back and drop a die's whole
+// L2 each time: 4096 x 14336, eight tokens, 37 us.)
+__global__ void __launch_bounds__(256) g4_join_kernel(const float* partial, float* y, int64_t n, int kz) {
+    for (int64_t i = first_item(); i < n; i += item_stride()) {
+        float total = partial[i];
+        for (int z = 1; z < kz; z++) total += partial[z * n + i];
+        y[i] = total;
+    }
 }
 
-constexpr int64_t G4_LDS = 120 << 10;  // of x in LDS, at most
-constexpr int G4_COLS = 64;            // columns of a launch, at most
+constexpr int64_t G4_LDS = 160 << 10;  // of a CU
+constexpr int64_t G4_SELF_VALUES = 16384;
+constexpr int G4_COLS = 48;  // columns of a launch, at most
 
-int g4_run(G4Args a, bool has_zeros, hipStream_t st) {
-    const int parts = a.x_type == ELEM_F32 ? 4 : 3, cols = parts * a.m, nt = (cols + 15) / 16;
-    const int per = a.l.per, depth = per == 4 ? g4_depth<4>() : g4_depth<1>();
-    const int64_t slots = (nt >= 3 ? 8 : 16) * num_cus();  // waves that are resident at once
-    a.ks = 1;
-    while (a.ks < G4_WAVES && a.l.tiles * a.ks * 2 <= slots && a.ks < a.l.blocks) a.ks *= 2;
-    // the blocks of x that LDS takes, whole rounds of the ring
-    const int64_t block_bytes = 256 * cols + 8 * a.m + (has_zeros ? 8 * per * cols : 0);
-    int64_t chunk = G4_LDS / block_bytes;
-    a.whole = chunk >= a.l.blocks;
-    while (!a.whole && a.ks > 1 && chunk < depth * a.ks) a.ks /= 2;
-    chunk = a.whole ? a.l.blocks : chunk / (depth * a.ks) * (depth * a.ks);
-    a.chunk = static_cast<int32_t>(chunk);
-    const int per_group = G4_WAVES / a.ks;
-    a.groups = static_cast<int32_t>((a.l.tiles + per_group - 1) / per_group);
-    const uint32_t lds = static_cast<uint32_t>(G4_WAVES * nt * 1024 + chunk * block_bytes);
-    const int64_t most = (lds > (80 << 10) || nt >= 3 ? 1 : 2) * num_cus();
-    const uint32_t grid = static_cast<uint32_t>(a.groups < most ? a.groups : most);
-    const bool f32 = parts == 4;
-#define G4_CASE(PER, Z)                                      \
-    if (per == PER && has_zeros == Z) {                      \
-        if (f32) g4_launch<PER, Z, 4>(a, nt, grid, lds, st); \
-        else g4_launch<PER, Z, 3>(a, nt, grid, lds, st);     \
+// How a launch of m tokens runs.
+struct G4Plan {
+    int mode, nt, ks, waves;
+    int64_t kz, chunk, groups;
+    int64_t lds;
+    int64_t partial, workspace;  // byte offset of the chunks' sums behind the image, bytes in all
+};
+
+G4Plan g4_plan(const Group4Layout& l, int64_t rows, int64_t m, int x_type, bool has_zeros) {
+    G4Plan p{};
+    const int64_t cols = (x_type == ELEM_F32 ? 4 : 3) * m;
+    p.nt = static_cast<int>((cols + 15) / 16);
+    // Chunks of k whose digits fit into LDS beside the sums.
+    const int64_t room = G4_LDS - G4_WAVES * p.nt * 1024 - 16, block = digit_bytes(cols) + table_bytes(cols, m, l.per, has_zeros);
+    p.kz = (l.blocks * block + room - 1) / room;
+    // where there are several, as many as give every CU a workgroup (4096 x 14336, eight fp16 tokens: 3 chunks 21.3 us, 4 18.8)
+    const int64_t even = (4 * num_cus() + l.tiles - 1) / l.tiles;
+    if (p.kz > 1 && p.kz < even) p.kz = even < 8 ? even : p.kz < 8 ? 8 : p.kz;
+    if (p.kz > l.blocks) p.kz = l.blocks;
+    p.chunk = (l.blocks + p.kz - 1) / p.kz;
+    p.kz = (l.blocks + p.chunk - 1) / p.chunk;
+    p.mode = p.kz == 1 && p.nt == 1 && m * l.blocks * GROUP4_K <= G4_SELF_VALUES ? G4_SELF : G4_COPY;
+    // A tile is shared by as many waves as leave each four blocks, up to eight
+    // waves a CU: more of them cost more in x staged and sums joined than they
+    // bring in loads in flight (14336 x 4096, one token: ks 1 to 8 take 9.7,
+    // 9.3, 10.5 and 14.0 us; 4096 x 4096: 9.2, 6.9, 6.1 and 6.6).
+    p.ks = 1;
+    while (p.ks < G4_WAVES && l.tiles * p.kz * p.ks * 2 <= 8 * num_cus() && p.chunk >= 8 * p.ks) p.ks *= 2;
+    // workgroups of four waves where eight would leave a quarter of the CUs without one
+    p.waves = p.ks <= 4 && l.tiles * p.kz * p.ks < 6 * num_cus() ? 4 : G4_WAVES;
+    p.groups = (l.tiles * p.ks + p.waves - 1) / p.waves;
+    p.lds = p.waves * p.nt * 1024 + chunk_bytes(p.chunk, cols, m, l.per, has_zeros);
+    p.workspace = p.mode == G4_SELF ? 0 : p.kz * chunk_bytes(p.chunk, cols, m, l.per, has_zeros);
+    if (p.kz > 1) {
+        p.partial = p.workspace;
+        p.workspace += (p.kz * m * rows * 4 + 15) / 16 * 16;
     }
-    G4_CASE(1, false)
-    G4_CASE(1, true)
-    G4_CASE(2, false)
-    G4_CASE(2, true)
-    G4_CASE(4, false)
-    G4_CASE(4, true)
-#undef G4_CASE
+    return p;
+}
+
+template <int PER, bool ZEROS>
+int g4_launch(const G4Args& a, const G4Plan& p, uint32_t grid, hipStream_t st) {
+    const uint32_t threads = 64 * p.waves, lds = static_cast<uint32_t>(p.lds);
+    if (p.mode == G4_SELF) {
+        if (a.parts == 4) g4_gemv_kernel<PER, ZEROS, 4, 1, G4_SELF><<<grid, threads, lds, st>>>(a);
+        else g4_gemv_kernel<PER, ZEROS, 3, 1, G4_SELF><<<grid, threads, lds, st>>>(a);
+        return check_launch("vb_group4_gemv");
+    }
+    const dim3 pieces(static_cast<uint32_t>((a.l.blocks * 32 + 255) / 256), static_cast<uint32_t>(a.m));
+    if (a.parts == 4) g4_image_kernel<PER, ZEROS, 4><<<pieces, 256, 0, st>>>(a);
+    else g4_image_kernel<PER, ZEROS, 3><<<pieces, 256, 0, st>>>(a);
+    if (const int rc = check_launch("vb_group4_gemv"); rc != OK) return rc;
+    if (p.nt == 1) g4_gemv_kernel<PER, ZEROS, 0, 1, G4_COPY><<<grid, threads, lds, st>>>(a);
+    else if (p.nt == 2) g4_gemv_kernel<PER, ZEROS, 0, 2, G4_COPY><<<grid, threads, lds, st>>>(a);
+    else g4_gemv_kernel<PER, ZEROS, 0, 3, G4_COPY><<<grid, threads, lds, st>>>(a);
+    if (p.kz > 1) {
+        if (const int rc = check_launch("vb_group4_gemv"); rc != OK) return rc;
+        g4_join_kernel<<<item_blocks(a.rows * a.m), 256, 0, st>>>(a.partial, a.y, a.rows * a.m, a.kz);
+    }
     return check_launch("vb_group4_gemv");
+}
+
+int g4_run(G4Args a, bool has_zeros, uint8_t* workspace, hipStream_t st) {
+    const G4Plan p = g4_plan(a.l, a.rows, a.m, a.x_type, has_zeros);
+    a.image = workspace;
+    a.partial = reinterpret_cast<float*>(workspace + p.partial);
+    a.parts = a.x_type == ELEM_F32 ? 4 : 3;
+    a.ks = p.ks;
+    a.kz = static_cast<int32_t>(p.kz);
+    a.chunk = static_cast<int32_t>(p.chunk);
+    a.groups = static_cast<int32_t>(p.groups);
+    // as many workgroups as are resident at once (16 waves a CU or 8), a share for every chunk
+    const int64_t fit = G4_LDS / p.lds, want = (g4_wide(p.nt, a.l.per, has_zeros) ? 8 : 16) / p.waves;
+    const int64_t most = ((fit < want ? fit : want) * num_cus() + p.kz - 1) / p.kz;
+    const uint32_t grid = static_cast<uint32_t>(p.kz * (p.groups < most ? p.groups : most));
+    if (a.l.per == 1) return has_zeros ? g4_launch<1, true>(a, p, grid, st) : g4_launch<1, false>(a, p, grid, st);
+    if (a.l.per == 2) return has_zeros ? g4_launch<2, true>(a, p, grid, st) : g4_launch<2, false>(a, p, grid, st);
+    return has_zeros ? g4_launch<4, true>(a, p, grid, st) : g4_launch<4, false>(a, p, grid, st);
+}
+
+// Tokens of a launch of m, in even shares.
+int64_t g4_slab(int64_t m, int x_type) {
+    const int64_t slab = G4_COLS / (x_type == ELEM_F32 ? 4 : 3), launches = (m + slab - 1) / slab;
+    return (m + launches - 1) / launches;
 }
 
 // The layout of a call's weights, or an error.
@@ -636,10 +782,21 @@ int vb_group4_dequant_rows(const void* w, float* out, int64_t rows, int64_t k, i
     return check_launch("vb_group4_dequant_rows");
 }
 
+int64_t vb_group4_workspace(int64_t m, int64_t rows, int64_t k, int32_t group, int32_t has_zeros, int32_t x_type) {
+    Group4Layout l;
+    if (m < 0 || !elem_type(x_type) || !group4_layout(rows, k, group, has_zeros != 0, &l)) return -1;
+    if (m == 0) return 0;
+    const int64_t slab = g4_slab(m, x_type), rest = m % slab;  // the last launch may be smaller
+    const int64_t need = g4_plan(l, rows, slab, x_type, has_zeros != 0).workspace;
+    const int64_t last = rest > 0 ? g4_plan(l, rows, rest, x_type, has_zeros != 0).workspace : 0;
+    return last > need ? last : need;
+}
+
 int vb_group4_gemv(const void* w, int64_t rows, int64_t k, int32_t group, int32_t has_zeros, const void* x,
-                   int32_t x_type, int64_t x_ld, int64_t m, float* y, void* stream) {
-    G4Weights g{static_cast<const uint8_t*>(w), {}, rows, k, has_zeros != 0};
-    if (const int rc = layout_of("vb_group4_gemv", rows, k, group, has_zeros, &g.l); rc != OK) return rc;
+                   int32_t x_type, int64_t x_ld, int64_t m, float* y, void* workspace, size_t workspace_bytes,
+                   void* stream) {
+    Group4Layout l;
+    if (const int rc = layout_of("vb_group4_gemv", rows, k, group, has_zeros, &l); rc != OK) return rc;
     if (!elem_type(x_type) || m < 0 || m > 0x7fffffff || (m > 1 && x_ld < 0)) {
         set_error("vb_group4_gemv: bad arguments (x type %d, m=%lld, row stride %lld)", x_type,
                   static_cast<long long>(m), static_cast<long long>(x_ld));
@@ -650,12 +807,26 @@ int vb_group4_gemv(const void* w, int64_t rows, int64_t k, int32_t group, int32_
         set_error("vb_group4_gemv: null pointer, or w not 16-byte aligned");
         return E_INVAL;
     }
-    const int64_t slab = G4_COLS / (x_type == ELEM_F32 ? 4 : 3);  // tokens of a launch
+    const int64_t need = vb_group4_workspace(m, rows, k, group, has_zeros, x_type);
+    if (static_cast<int64_t>(workspace_bytes) < need ||
+        (need > 0 && (!workspace || reinterpret_cast<uintptr_t>(workspace) % 16 != 0))) {
+        set_error("vb_group4_gemv: workspace of %zu bytes (16-byte aligned) is below the %lld needed", workspace_bytes,
+                  static_cast<long long>(need));
+        return E_INVAL;
+    }
+    const int64_t slab = g4_slab(m, x_type);
     for (int64_t t = 0; t < m; t += slab) {
-        const void* xt = static_cast<const uint8_t*>(x) + t * x_ld * elem_bytes(x_type);
-        const G4Args a{g.w, g.l, xt, y + t * rows, x_ld, rows, k, x_type, static_cast<int32_t>(m - t < slab ? m - t : slab),
-                       0, 0, 0, false};
-        if (const int rc = g4_run(a, g.has_zeros, as_stream(stream)); rc != OK) return rc;
+        G4Args a{};
+        a.w = static_cast<const uint8_t*>(w);
+        a.l = l;
+        a.x = static_cast<const uint8_t*>(x) + t * x_ld * elem_bytes(x_type);
+        a.y = y + t * rows;
+        a.x_ld = x_ld;
+        a.rows = rows;
+        a.k = k;
+        a.x_type = x_type;
+        a.m = static_cast<int32_t>(m - t < slab ? m - t : slab);
+        if (const int rc = g4_run(a, has_zeros != 0, static_cast<uint8_t*>(workspace), as_stream(stream)); rc != OK) return rc;
     }
     return OK;
 }
