@@ -18,15 +18,28 @@
 // -inf logit is never named (id -1, lp -inf).  A row with a NaN or a +inf has
 // NaN for lp, H and the alternatives' log probabilities.
 //
-// One workgroup per row.
+// One pass over the logits.  A wave walks over a slice of a row, 16 logits a
+// lane at a time, with its running maximum m, S and the entropy's sum (each
+// lane's share of them, relative to the wave's m).  The alternatives hang on a
+// threshold: the value of the last of the wave's best `top` logits so far.  A
+// batch whose every lane stays at or below it, as nearly all do after the first
+// few, costs one comparison; otherwise the logits above it are appended to a
+// buffer in LDS, and when that runs full its best `top` are ranked (each entry
+// counts those before it) and the threshold rises.  The waves of a workgroup,
+// and the workgroups of a row where there are few rows, are joined the same way.
 #include "elem_types.hpp"
+#include "vb_internal.hpp"
 #include "../../include/vbhip.h"
 
 namespace vb {
 namespace {
 
-constexpr int LP_THREADS = 256;
+constexpr int LP_WAVES = 4;
+constexpr int LP_THREADS = 64 * LP_WAVES;
 constexpr int LP_MAX_TOP = 64;
+constexpr int LP_MAX_SPLIT = 64;      // slices of a row, one per lane of the wave that joins them
+constexpr int LP_BATCH = 16;          // logits of a lane at a time
+constexpr int LP_BUF = 128;           // candidates of a wave: 64 kept, 64 new
 
 struct LpArgs {
     const void* z;
@@ -35,91 +48,377 @@ struct LpArgs {
     float* entropy;
     int32_t* top_ids;
     float* top_lp;
+    float4* stats;    // [row][split]: m, S, sum (workspace)
+    uint64_t* keys;   // [row][split][top]
     int64_t ld, rows;
-    int32_t vocab, type, token_bytes, n_tokens, top;
-    float inv_t;
+    int32_t vocab, token_bytes, n_tokens, top, splits;
+    float c, inv_t;   // log2(e) / T, 1 / T
 };
 
 // A value's place in the order of the alternatives: larger first, equal
 // values by the lower index.  0: none (NaN, -inf).
-__device__ __forceinline__ uint64_t order_key(float v, uint32_t i) {
-    if (!(v > -INFINITY)) return 0;
+__device__ __forceinline__ uint32_t order_bits(float v) {
     const uint32_t u = __float_as_uint(v + 0.f);  // -0 is 0
-    const uint32_t o = u & 0x80000000u ? ~u : u | 0x80000000u;
-    return static_cast<uint64_t>(o) << 32 | (0xffffffffu - i);
+    return u & 0x80000000u ? ~u : u | 0x80000000u;
+}
+__device__ __forceinline__ float order_value(uint32_t o) { return __uint_as_float(o & 0x80000000u ? o & 0x7fffffffu : ~o); }
+__device__ __forceinline__ uint64_t order_key(float v, uint32_t i) {
+    return v > -INFINITY ? static_cast<uint64_t>(order_bits(v)) << 32 | (0xffffffffu - i) : 0;
+}
+__device__ __forceinline__ int key_index(uint64_t k) { return static_cast<int>(0xffffffffu - static_cast<uint32_t>(k)); }
+__device__ __forceinline__ float key_value(uint64_t k) { return order_value(static_cast<uint32_t>(k >> 32)); }
+
+__device__ __forceinline__ float wave_max(float v) {
+#pragma unroll
+    for (int off = 32; off >= 1; off >>= 1) v = fmaxf(v, __shfl_xor(v, off, 64));
+    return v;
 }
 
-__device__ __forceinline__ uint64_t umax(uint64_t a, uint64_t b) { return a > b ? a : b; }
+__device__ __forceinline__ int lanes_below(uint64_t mask) {
+    return __builtin_amdgcn_mbcnt_hi(static_cast<uint32_t>(mask >> 32), __builtin_amdgcn_mbcnt_lo(static_cast<uint32_t>(mask), 0));
+}
 
-__device__ void logprob_row(const LpArgs& a, int64_t row) {
-    __shared__ float part[3][LP_THREADS / 64];
-    __shared__ uint64_t best[LP_THREADS / 64];
-    const int64_t base = row * a.ld;
-    const int wave = threadIdx.x >> 6;
-    auto key_max = [&](uint64_t below) {  // the largest key under `below`, in every thread
-        uint64_t k = 0;
-        for (int i = threadIdx.x; i < a.vocab; i += LP_THREADS) {
-            const uint64_t o = order_key(elem_ld(a.z, base + i, a.type), i);
-            if (o < below) k = umax(k, o);
+// LDS of one wave: what its lanes wrote is read by the others.
+__device__ __forceinline__ void wave_lds_fence() {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+}
+
+// A wave's best n candidates (the same in every lane, but for the buffer).
+struct Best {
+    uint64_t* buf;
+    int n, count;
+    float tau;  // no candidate at or below it is wanted (but equal values of lower index within a batch)
+
+    // The n best of the buffer, in order.
+    __device__ __forceinline__ void rank() {
+        wave_lds_fence();
+        const int lane = static_cast<int>(threadIdx.x) & 63;
+        const uint64_t a = lane < count ? buf[lane] : 0, b = lane + 64 < count ? buf[lane + 64] : 0;
+        int ra = 0, rb = 0;
+        for (int i = 0; i < count; i++) {
+            const uint64_t k = buf[i];
+            ra += k > a;
+            rb += k > b;
         }
-        for (int off = 32; off >= 1; off >>= 1) k = umax(k, __shfl_xor(k, off, 64));
-        __syncthreads();
-        if ((threadIdx.x & 63) == 0) best[wave] = k;
-        __syncthreads();
-        k = best[0];
-        for (int w = 1; w < LP_THREADS / 64; w++) k = umax(k, best[w]);
-        return k;
-    };
-    auto index_of = [](uint64_t k) { return static_cast<int>(0xffffffffu - static_cast<uint32_t>(k)); };
-    uint64_t k = key_max(~0ull);
-    const int at = k ? index_of(k) : -1;
-    const float top = k ? elem_ld(a.z, base + at, a.type) : -INFINITY, m = k ? top : 0.f;
-    float s = 0.f, t = 0.f;
-    for (int i = threadIdx.x; i < a.vocab; i += LP_THREADS) {
-        const float d = elem_ld(a.z, base + i, a.type) - m;
-        if (i == at) continue;
-        const float e = __expf(d * a.inv_t);
-        s += e;
-        t += e * fmaxf(d, -3.0e38f);
+        wave_lds_fence();
+        if (lane < count && ra < n) buf[ra] = a;
+        if (lane + 64 < count && rb < n) buf[rb] = b;
+        wave_lds_fence();
+        count = count < n ? count : n;
+        tau = count == n ? key_value(buf[n - 1]) : -INFINITY;
     }
-    s = wave_sum_dpp(s);
-    t = wave_sum_dpp(t);
-    if ((threadIdx.x & 63) == 0) {
-        part[0][wave] = s;
-        part[1][wave] = t;
+
+    __device__ __forceinline__ void append(uint64_t key, bool in) {
+        const uint64_t mask = __ballot(in);
+        if (!mask) return;
+        if (count > LP_BUF - 64) rank();
+        if (in) buf[count + lanes_below(mask)] = key;
+        count += __popcll(mask);
     }
-    __syncthreads();
-    s = part[0][0];
-    t = part[1][0];
-    for (int w = 1; w < LP_THREADS / 64; w++) {
-        s += part[0][w];
-        t += part[1][w];
+};
+
+// Maximum and sums of a set of logits: S without one place of the maximum, and
+// sum e^(z - m) (z - m), in units of log2.
+struct Stat {
+    float m, s, t;
+};
+
+// The lanes' sets as one, in every lane (an empty one: m = -inf, s = t = 0, or
+// NaN where it held one).
+__device__ __forceinline__ Stat join(Stat v, float c) {
+    const float m = wave_max(v.m);
+    const int owner = __ffsll(static_cast<unsigned long long>(__ballot(v.m == m))) - 1;
+    const int lane = static_cast<int>(threadIdx.x) & 63;
+    if (lane != owner && v.m > -INFINITY) {
+        const float d = (v.m - m) * c, f = __builtin_amdgcn_exp2f(d);
+        v.t = f * (v.t + fmaxf(d, -1e30f) * (v.s + 1.f));
+        v.s = f * (v.s + 1.f);
     }
-    if (top == INFINITY) s = t = NAN;
-    const bool empty = !k && s == 0.f;
-    const float rest = log1pf(s);
-    auto lp_of = [&](float v) { return empty ? -INFINITY : (v - m) * a.inv_t - rest; };
-    if (a.entropy && threadIdx.x == 0) a.entropy[row] = empty ? 0.f : rest - t * a.inv_t / (1.f + s);
-    for (int j = threadIdx.x; j < a.n_tokens; j += LP_THREADS) {
+    return Stat{m, wave_sum_dpp(v.s), wave_sum_dpp(v.t)};
+}
+
+// What a row's results are made from.
+struct RowResult {
+    bool empty;
+    float m, s, t, rest, inv_t;
+    __device__ __forceinline__ RowResult(Stat v, float inv_t_) : m(v.m), s(v.s), t(v.t), inv_t(inv_t_) {
+        if (m == INFINITY) s = t = NAN;
+        empty = m == -INFINITY && s == 0.f;
+        rest = log1pf(s);
+    }
+    __device__ __forceinline__ float lp(float z) const {
+        return empty ? -INFINITY : (z - m) * inv_t - rest;
+    }
+    __device__ __forceinline__ float entropy() const { return empty ? 0.f : rest - t * 0.693147180559945f / (1.f + s); }
+};
+
+template <int TYPE>
+__device__ __forceinline__ float logit(const LpArgs& a, int64_t i) {
+    return elem_ld(a.z, i, TYPE);
+}
+
+// A row's outputs by one wave; best: its alternatives in order.
+template <int TYPE>
+__device__ __forceinline__ void write_row(const LpArgs& a, int64_t row, const RowResult& r, const uint64_t* best, int count) {
+    const int lane = static_cast<int>(threadIdx.x) & 63;
+    if (a.entropy && lane == 0) a.entropy[row] = r.entropy();
+    for (int j = lane; j < a.n_tokens; j += 64) {
         const int64_t p = row * a.n_tokens + j;
         const int64_t id = a.token_bytes == 8 ? static_cast<const int64_t*>(a.tokens)[p]
                                               : static_cast<const int32_t*>(a.tokens)[p];
-        a.lp[p] = id >= 0 && id < a.vocab ? lp_of(elem_ld(a.z, base + id, a.type)) : 0.f;
+        a.lp[p] = id >= 0 && id < a.vocab ? r.lp(logit<TYPE>(a, row * a.ld + id)) : 0.f;
     }
-    for (int j = 0; j < a.top; j++) {
-        if (threadIdx.x == 0) {
-            a.top_ids[row * a.top + j] = k ? index_of(k) : -1;
-            a.top_lp[row * a.top + j] = s != s ? NAN : k ? lp_of(elem_ld(a.z, base + index_of(k), a.type)) : -INFINITY;
-        }
-        if (k && j + 1 < a.top) k = key_max(k);
+    if (lane < a.top) {
+        const uint64_t k = lane < count ? best[lane] : 0;
+        a.top_ids[row * a.top + lane] = k ? key_index(k) : -1;
+        a.top_lp[row * a.top + lane] = r.s != r.s ? NAN : k ? r.lp(key_value(k)) : -INFINITY;
     }
 }
 
-__global__ void __launch_bounds__(LP_THREADS) logprob_kernel(LpArgs a) {
-    for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
-        logprob_row(a, row);
-        __syncthreads();  // its sums are read
+template <int TYPE, bool LIST>
+struct Walk {
+    static constexpr int V = TYPE == ELEM_F32 ? 4 : 8;  // logits of a 16-byte load
+    static constexpr int U = LP_BATCH / V;              // loads of a batch
+    const LpArgs& a;
+    Best best;
+    float m, s, t, tau;  // m, tau: the wave's
+    bool first;
+
+    __device__ __forceinline__ Walk(const LpArgs& a_, uint64_t* buf)
+        : a(a_), best{buf, a_.top, 0, -INFINITY}, m(-INFINITY), s(0.f), t(0.f), tau(-INFINITY), first(true) {}
+
+    // The lanes' largest values cm hold the wave's n-th largest logit or something below it.
+    __device__ __forceinline__ float first_tau(float cm) const {
+        const uint32_t o = cm > -INFINITY ? order_bits(cm) : 0;
+        uint32_t at = 0;
+        for (int bit = 31; bit >= 12; bit--) {
+            const uint32_t up = at | 1u << bit;
+            const int count = __popcll(__ballot(o >= up));
+            if (count >= best.n) at = up;
+            if (count == best.n) break;
+        }
+        return at ? order_value(at) : -INFINITY;
     }
+
+    // Logit r of the batch, and its index in the row.
+    __device__ __forceinline__ static int index_of(int base, int r) {
+        return base + (r / V * 64 + (static_cast<int>(threadIdx.x) & 63)) * V + r % V;
+    }
+
+    __device__ __forceinline__ void above(float (&v)[LP_BATCH], float cm, int base) {
+        if constexpr (LIST) {
+            if (first) best.tau = first_tau(cm);
+            uint32_t left = 0;
+#pragma unroll
+            for (int r = 0; r < LP_BATCH; r++) left |= v[r] >= best.tau && v[r] > -INFINITY ? 1u << r : 0u;
+            while (__any(left != 0)) {
+                const int r = __ffs(left) - 1;
+                float x = v[0];
+#pragma unroll
+                for (int i = 1; i < LP_BATCH; i++) x = r == i ? v[i] : x;
+                best.append(order_key(x, static_cast<uint32_t>(index_of(base, r))), left != 0 && x >= best.tau);
+                left &= left - 1;
+            }
+            if (first) best.rank();
+            first = false;
+            tau = best.tau;
+        }
+        const float top = wave_max(cm);
+        if (top > m) {
+            // one place of the new maximum leaves the sums, the old one joins them
+            if (m > -INFINITY) {
+                const float d = (m - top) * a.c, f = __builtin_amdgcn_exp2f(d), dd = fmaxf(d, -1e30f);
+                const float back = (threadIdx.x & 63) == 0 ? 1.f : 0.f;
+                t = f * (t + dd * (s + back));
+                s = f * (s + back);
+            }
+            m = top;
+            const int owner = __ffsll(static_cast<unsigned long long>(__ballot(cm == top))) - 1;
+            bool out = (static_cast<int>(threadIdx.x) & 63) == owner;
+#pragma unroll
+            for (int r = 0; r < LP_BATCH; r++) {
+                const bool hit = out && v[r] == top;
+                v[r] = hit ? -INFINITY : v[r];
+                out = out && !hit;
+            }
+            if (!LIST) tau = m;
+        }
+    }
+
+    __device__ __forceinline__ void batch(float (&v)[LP_BATCH], int base) {
+        float cm = v[0];
+#pragma unroll
+        for (int r = 1; r < LP_BATCH; r++) cm = fmaxf(cm, v[r]);
+        if (__any(cm > tau)) above(v, cm, base);
+        const float from = m > -INFINITY ? m : 0.f;
+#pragma unroll
+        for (int r = 0; r < LP_BATCH; r++) {
+            const float d = (v[r] - from) * a.c, e = __builtin_amdgcn_exp2f(d);
+            s += e;
+            t += e * fmaxf(d, -1e30f);  // e is 0 below (and NaN for a NaN)
+        }
+    }
+
+    // The 16-byte units [u0, u1) from unit 0 at `body`, whose first logit has index i0.
+    __device__ __forceinline__ void run(const void* body, int u0, int u1, int i0) {
+        if (u0 >= u1) return;
+        const int lane = static_cast<int>(threadIdx.x) & 63;
+        const __amdgpu_buffer_rsrc_t r = make_rsrc(static_cast<const uint8_t*>(body) + static_cast<int64_t>(u0) * 16,
+                                                   static_cast<uint32_t>(u1 - u0) * 16u);
+        const int count = u1 - u0;
+        u32x4 raw[U];
+        const auto load = [&](int at) __attribute__((always_inline)) {  // units past the last read nothing
+#pragma unroll
+            for (int u = 0; u < U; u++)
+                raw[u] = __builtin_amdgcn_raw_buffer_load_b128(r, static_cast<int>(static_cast<uint32_t>(at + u * 64 + lane) * 16u), 0, 2);
+        };
+        load(0);
+        for (int at = 0; at < count; at += 64 * U) {
+            float v[LP_BATCH];
+#pragma unroll
+            for (int u = 0; u < U; u++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const uint32_t w = raw[u][i];
+                    if constexpr (TYPE == ELEM_F32) {
+                        v[u * V + i] = __uint_as_float(w);
+                    } else if constexpr (TYPE == ELEM_F16) {
+                        v[u * V + 2 * i] = f16lo(w);
+                        v[u * V + 2 * i + 1] = f16hi(w);
+                    } else {
+                        v[u * V + 2 * i] = __uint_as_float(w << 16);
+                        v[u * V + 2 * i + 1] = __uint_as_float(w & 0xffff0000u);
+                    }
+                }
+            load(at + 64 * U);
+            if (at + 64 * U > count) {
+#pragma unroll
+                for (int k = 0; k < LP_BATCH; k++)
+                    if (at + k / V * 64 + lane >= count) v[k] = -INFINITY;
+            }
+            batch(v, i0 + (u0 + at) * V);
+        }
+    }
+};
+
+// Workgroup: a slice of a row.  16-byte units from the row's first aligned one
+// on; the logits before and behind them (fewer than a unit's each) are joined
+// at the end as sets of one.
+template <int TYPE, bool LIST>
+__global__ void __launch_bounds__(LP_THREADS) logprob_kernel(LpArgs a) {
+    using W = Walk<TYPE, LIST>;
+    constexpr int SIZE = TYPE == ELEM_F32 ? 4 : 2;
+    __shared__ uint64_t bufs[LIST ? LP_WAVES : 1][LP_BUF];
+    __shared__ int counts[LP_WAVES];
+    __shared__ Stat stats[LP_WAVES];
+    const int lane = static_cast<int>(threadIdx.x) & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));
+    for (int64_t item = blockIdx.x; item < a.rows * a.splits; item += gridDim.x) {
+        const int64_t row = item / a.splits;
+        const int split = static_cast<int>(item % a.splits);
+        const uint8_t* z = static_cast<const uint8_t*>(a.z) + row * a.ld * SIZE;
+        int head = static_cast<int>((16 - (reinterpret_cast<uintptr_t>(z) & 15)) & 15) / SIZE;
+        head = head < a.vocab ? head : a.vocab;
+        const int units = (a.vocab - head) / W::V, parts = a.splits * LP_WAVES, part = split * LP_WAVES + wave;
+        const int each = ((units + parts - 1) / parts + 63) / 64 * 64;
+        const int64_t u0 = static_cast<int64_t>(part) * each, u1 = u0 + each < units ? u0 + each : units;
+        W w(a, bufs[LIST ? wave : 0]);
+        if (u0 < u1) w.run(z + head * SIZE, static_cast<int>(u0), static_cast<int>(u1), head);
+        const Stat mine{w.m, wave_sum_dpp(w.s), wave_sum_dpp(w.t)};
+        if constexpr (LIST) {
+            if (wave != 0) w.best.rank();
+        }
+        if (lane == 0) {
+            stats[wave] = mine;
+            counts[wave] = w.best.count;
+        }
+        __syncthreads();
+        if (wave == 0) {
+            // lanes 0-3: the waves; from lane 4 on: single logits
+            const int tail = head + units * W::V, single = lane - LP_WAVES;
+            const int singles = split == 0 ? head + (a.vocab - tail) : 0;
+            const int at = single < head ? single : tail + single - head;
+            Stat v{-INFINITY, 0.f, 0.f};
+            if (lane < LP_WAVES) {
+                v = stats[lane];
+            } else if (single < singles) {
+                const float x = logit<TYPE>(a, row * a.ld + at);
+                if (x > -INFINITY) v.m = x;
+                else if (x != x) v.s = v.t = NAN;
+            }
+            const Stat all = join(v, a.c);
+            if constexpr (LIST) {
+                for (int k = 1; k < LP_WAVES; k++) {
+                    const uint64_t key = lane < counts[k] ? bufs[k][lane] : 0;
+                    w.best.append(key, key != 0 && key_value(key) >= w.best.tau);
+                }
+                const bool one = single >= 0 && single < singles && v.m > -INFINITY;
+                w.best.append(order_key(v.m, static_cast<uint32_t>(at)), one && v.m >= w.best.tau);
+                w.best.rank();
+            }
+            if (a.splits == 1) {
+                write_row<TYPE>(a, row, RowResult(all, a.inv_t), bufs[0], LIST ? w.best.count : 0);
+            } else {
+                if (lane == 0) a.stats[item] = make_float4(all.m, all.s, all.t, 0.f);
+                if (LIST && lane < a.top) a.keys[item * a.top + lane] = lane < w.best.count ? bufs[0][lane] : 0;
+            }
+        }
+        __syncthreads();  // bufs and stats are free
+    }
+}
+
+// One wave: the slices of a row.  Their lists are in order, so once no slice's
+// j-th candidate is wanted none behind it is.
+template <int TYPE, bool LIST>
+__global__ void __launch_bounds__(64) logprob_join_kernel(LpArgs a) {
+    __shared__ uint64_t buf[LP_BUF];
+    const int lane = static_cast<int>(threadIdx.x);
+    for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
+        const int64_t item = row * a.splits + lane;
+        Stat v{-INFINITY, 0.f, 0.f};
+        if (lane < a.splits) {
+            const float4 p = a.stats[item];
+            v = Stat{p.x, p.y, p.z};
+        }
+        const Stat all = join(v, a.c);
+        Best best{buf, a.top, 0, -INFINITY};
+        if constexpr (LIST) {
+            for (int j = 0; j < a.top; j++) {
+                const uint64_t key = lane < a.splits ? a.keys[item * a.top + j] : 0;
+                const bool in = key != 0 && key_value(key) >= best.tau;
+                if (!__any(in)) break;
+                best.append(key, in);
+                if (best.count >= best.n) best.rank();
+            }
+            best.rank();
+        }
+        write_row<TYPE>(a, row, RowResult(all, a.inv_t), buf, best.count);
+        wave_lds_fence();
+    }
+}
+
+// Slices of a row: enough workgroups for the chip (eight a CU), each wave a batch or more.
+int64_t lp_splits(int64_t rows, int64_t vocab) {
+    const int64_t want = rows > 0 ? (8 * num_cus() + rows - 1) / rows : 1;
+    const int64_t most = (vocab + LP_THREADS * LP_BATCH - 1) / (LP_THREADS * LP_BATCH);
+    int64_t n = want < most ? want : most;
+    return n < LP_MAX_SPLIT ? n : LP_MAX_SPLIT;
+}
+
+template <int TYPE>
+int lp_launch(const LpArgs& a, hipStream_t st) {
+    const int64_t items = a.rows * a.splits;
+    const uint32_t grid = static_cast<uint32_t>(items < (1 << 20) ? items : 1 << 20);  // fewer than 2^32 threads
+    if (a.top > 0) logprob_kernel<TYPE, true><<<grid, LP_THREADS, 0, st>>>(a);
+    else logprob_kernel<TYPE, false><<<grid, LP_THREADS, 0, st>>>(a);
+    if (a.splits > 1) {
+        if (const int rc = check_launch("vb_token_logprobs"); rc != OK) return rc;
+        const uint32_t rows = static_cast<uint32_t>(a.rows < (1 << 20) ? a.rows : 1 << 20);
+        if (a.top > 0) logprob_join_kernel<TYPE, true><<<rows, 64, 0, st>>>(a);
+        else logprob_join_kernel<TYPE, false><<<rows, 64, 0, st>>>(a);
+    }
+    return check_launch("vb_token_logprobs");
 }
 
 }  // namespace
@@ -131,7 +430,8 @@ extern "C" {
 
 int64_t vb_token_logprobs_workspace(int64_t rows, int64_t vocab, int32_t top) {
     if (rows < 0 || rows > 0x7fffffff || vocab <= 0 || vocab > 0x7fffffff || top < 0 || top > LP_MAX_TOP) return -1;
-    return 0;
+    const int64_t splits = lp_splits(rows, vocab);
+    return splits > 1 ? rows * splits * (16 + 8 * top) : 0;
 }
 
 int vb_token_logprobs(const void* logits, int32_t type, int64_t ld, int64_t rows, int64_t vocab, float temperature,
@@ -164,11 +464,27 @@ int vb_token_logprobs(const void* logits, int32_t type, int64_t ld, int64_t rows
         return E_INVAL;
     }
     if (rows == 0) return OK;
-    const LpArgs a{logits, tokens, logprobs, entropy, top_ids, top_logprobs, ld, rows, static_cast<int32_t>(vocab), type,
-                   token_bytes, n_tokens, top, 1.f / temperature};
-    const uint32_t grid = static_cast<uint32_t>(rows < (1 << 20) ? rows : 1 << 20);  // fewer than 2^32 threads
-    logprob_kernel<<<dim3(grid), dim3(LP_THREADS), 0, as_stream(stream)>>>(a);
-    return check_launch("vb_token_logprobs");
+    LpArgs a{};
+    a.z = logits;
+    a.tokens = tokens;
+    a.lp = logprobs;
+    a.entropy = entropy;
+    a.top_ids = top_ids;
+    a.top_lp = top_logprobs;
+    a.ld = ld;
+    a.rows = rows;
+    a.vocab = static_cast<int32_t>(vocab);
+    a.token_bytes = token_bytes;
+    a.n_tokens = n_tokens;
+    a.top = top;
+    a.splits = static_cast<int32_t>(lp_splits(rows, vocab));
+    a.c = 1.4426950408889634f / temperature;
+    a.inv_t = 1.f / temperature;
+    a.stats = static_cast<float4*>(workspace);
+    a.keys = reinterpret_cast<uint64_t*>(a.stats + rows * a.splits);
+    if (type == ELEM_F32) return lp_launch<ELEM_F32>(a, as_stream(stream));
+    if (type == ELEM_F16) return lp_launch<ELEM_F16>(a, as_stream(stream));
+    return lp_launch<ELEM_BF16>(a, as_stream(stream));
 }
 
 }  // extern "C"
