@@ -8,9 +8,13 @@
 // y as n is computed from it are fp32 whatever the tensors' types; y and n are
 // rounded once, to the nearest, as they are stored.
 //
-// One workgroup per row.
-#include "vb_common.hpp"
+// A workgroup takes a row, and a thread its share of it into registers, in
+// pieces of four values: the branch, the stream and the gate are requested
+// together, the two sums go over the workgroup, and every value is read and
+// written once.  Rows longer than the registers of a workgroup are read again
+// for each sum (seam_long_kernel).
 #include "elem_types.hpp"
+#include "vb_internal.hpp"
 #include "../../include/vbhip.h"
 
 namespace vb {
@@ -30,55 +34,252 @@ struct SeamArgs {
     float scale, eps;
 };
 
-constexpr int SEAM_THREADS = 256;
+// ---- four neighbouring values; rows begin at any element ---------------------
 
-// The workgroup's sum of v, in every thread (waves added in order).
+template <int TYPE>
+struct Piece {
+    uint32_t u[TYPE == ELEM_F32 ? 4 : 2];
+};
+
+template <int TYPE>
+__device__ __forceinline__ Piece<TYPE> piece_ld(const void* p, int64_t i) {
+    Piece<TYPE> r;
+    if constexpr (TYPE == ELEM_F32) {
+        typedef uint32_t v4 __attribute__((ext_vector_type(4), aligned(4)));
+        const v4 v = *reinterpret_cast<const v4*>(static_cast<const float*>(p) + i);
+#pragma unroll
+        for (int j = 0; j < 4; j++) r.u[j] = v[j];
+    } else {
+        typedef uint32_t v2 __attribute__((ext_vector_type(2), aligned(2)));
+        const v2 v = *reinterpret_cast<const v2*>(static_cast<const uint16_t*>(p) + i);
+        r.u[0] = v[0];
+        r.u[1] = v[1];
+    }
+    return r;
+}
+
+template <int TYPE>
+__device__ __forceinline__ float piece_at(const Piece<TYPE>& r, int j) {
+    if constexpr (TYPE == ELEM_F32) return __uint_as_float(r.u[j]);
+    else if constexpr (TYPE == ELEM_F16) return j & 1 ? f16hi(r.u[j >> 1]) : f16lo(r.u[j >> 1]);
+    else return __uint_as_float(j & 1 ? r.u[j >> 1] & 0xffff0000u : r.u[j >> 1] << 16);
+}
+
+template <int TYPE>
+__device__ __forceinline__ void piece_st(void* p, int64_t i, const float* v) {
+    if constexpr (TYPE == ELEM_F32) {
+        typedef float v4 __attribute__((ext_vector_type(4), aligned(4)));
+        *reinterpret_cast<v4*>(static_cast<float*>(p) + i) = v4{v[0], v[1], v[2], v[3]};
+    } else {
+        typedef uint32_t v2 __attribute__((ext_vector_type(2), aligned(2)));
+        uint32_t u[2];
+#pragma unroll
+        for (int j = 0; j < 2; j++) {
+            if constexpr (TYPE == ELEM_F16) {
+                typedef _Float16 half2_t __attribute__((ext_vector_type(2)));
+                u[j] = __builtin_bit_cast(uint32_t, half2_t{static_cast<_Float16>(v[2 * j]), static_cast<_Float16>(v[2 * j + 1])});
+            } else {
+                u[j] = f32_bf16(v[2 * j]) | static_cast<uint32_t>(f32_bf16(v[2 * j + 1])) << 16;
+            }
+        }
+        *reinterpret_cast<v2*>(static_cast<uint16_t*>(p) + i) = v2{u[0], u[1]};
+    }
+}
+
+// The workgroup's sum of v, in every thread (waves added in order); part: of this sum alone.
+template <int WAVES>
 __device__ __forceinline__ float wg_sum(float v, float* part) {
     v = wave_sum_dpp(v);
-    __syncthreads();  // the last sum's readers are done
+    if constexpr (WAVES == 1) return v;
     if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = v;
     __syncthreads();
     float s = part[0];
-    for (int i = 1; i < SEAM_THREADS / 64; i++) s += part[i];
+#pragma unroll
+    for (int i = 1; i < WAVES; i++) s += part[i];
     return s;
 }
 
-__device__ __forceinline__ void seam_row(const SeamArgs& a, int64_t row, float* part) {
-    const int64_t bo = row * a.b_ld, xo = row * a.x_ld, yo = row * a.y_ld, no = row * a.n_ld, go = row * a.gate_row;
-    float inv = 1.f;
-    if (a.post_w) {
-        float s = 0.f;
-        for (int64_t i = threadIdx.x; i < a.dim; i += SEAM_THREADS) {
-            const float v = elem_ld(a.b, bo + i, a.b_type);
-            s += v * v;
-        }
-        inv = 1.f / sqrtf(wg_sum(s, part) / static_cast<float>(a.dim) + a.eps);
+// Four neighbouring values of the gate as they lie (gate_col 1), or its one value of the row.
+__device__ __forceinline__ Piece<ELEM_F32> gate_ld(const SeamArgs& a, int64_t go, int at) {
+    Piece<ELEM_F32> g;
+    if (a.gate_col == 0) {
+        g.u[0] = __float_as_uint(elem_ld(a.gate, go, a.gate_type));
+    } else if (a.gate_type == ELEM_F32) {
+        g = piece_ld<ELEM_F32>(a.gate, go + at);
+    } else {
+        const Piece<ELEM_F16> h = piece_ld<ELEM_F16>(a.gate, go + at);
+        g.u[0] = h.u[0];
+        g.u[1] = h.u[1];
     }
-    auto value = [&](int64_t i) {
-        float p = elem_ld(a.b, bo + i, a.b_type);
-        if (a.post_w) p = p * inv * a.post_w[i];
-        if (a.gate) p *= elem_ld(a.gate, go + i * a.gate_col, a.gate_type);
-        return elem_ld(a.x, xo + i, a.x_type) + a.scale * p;
-    };
-    float inv2 = 1.f;
-    if (a.pre_w) {
-        float s = 0.f;
-        for (int64_t i = threadIdx.x; i < a.dim; i += SEAM_THREADS) {
-            const float v = value(i);
-            s += v * v;
-        }
-        inv2 = 1.f / sqrtf(wg_sum(s, part) / static_cast<float>(a.dim) + a.eps);
-    }
-    for (int64_t i = threadIdx.x; i < a.dim; i += SEAM_THREADS) {
-        const float v = value(i);
-        elem_st(a.y, yo + i, a.x_type, v);
-        if (a.pre_w) elem_st(a.n, no + i, a.n_type, v * inv2 * a.pre_w[i]);
+    return g;
+}
+
+__device__ __forceinline__ float gate_at(const SeamArgs& a, const Piece<ELEM_F32>& g, int j) {
+    if (a.gate_col == 0) return __uint_as_float(g.u[0]);
+    if (a.gate_type == ELEM_F32) return __uint_as_float(g.u[j]);
+    const uint32_t w = g.u[j >> 1];
+    if (a.gate_type == ELEM_F16) return j & 1 ? f16hi(w) : f16lo(w);
+    return __uint_as_float(j & 1 ? w & 0xffff0000u : w << 16);
+}
+
+// Values skip.. of a piece (all of it as one store).
+template <int TYPE>
+__device__ __forceinline__ void piece_put(void* p, int64_t i, const float* v, int skip) {
+    if (skip == 0) {
+        piece_st<TYPE>(p, i, v);
+    } else {
+#pragma unroll
+        for (int j = 1; j < 4; j++)
+            if (j >= skip) elem_st(p, i + j, TYPE, v[j]);
     }
 }
 
-__global__ void __launch_bounds__(SEAM_THREADS) seam_kernel(SeamArgs a) {
-    __shared__ float part[SEAM_THREADS / 64];
-    for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) seam_row(a, row, part);
+// Rows of 4 to 256 * WAVES * PIECES values.  The last piece of a row is moved
+// back to end with it: its first values are another thread's, and are neither
+// summed nor stored again.
+template <int BT, int XT, int WAVES, int PIECES>
+__global__ void __launch_bounds__(64 * WAVES) seam_kernel(SeamArgs a) {
+    __shared__ float part[2][WAVES];
+    const int dim = static_cast<int>(a.dim);
+    int at[PIECES], skip[PIECES];  // a piece's first value; how many of it are not its own (4: no piece)
+#pragma unroll
+    for (int k = 0; k < PIECES; k++) {
+        const int i = (k * 64 * WAVES + static_cast<int>(threadIdx.x)) * 4;
+        at[k] = i + 4 <= dim ? i : dim - 4;
+        skip[k] = i >= dim ? 4 : i - at[k];
+    }
+    for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
+        const int64_t bo = row * a.b_ld, xo = row * a.x_ld, yo = row * a.y_ld, no = row * a.n_ld, go = row * a.gate_row;
+        Piece<ELEM_F32> g[PIECES];
+        Piece<BT> b[PIECES];
+        Piece<XT> x[PIECES];
+        if (a.gate) {
+#pragma unroll
+            for (int k = 0; k < PIECES; k++) g[k] = gate_ld(a, go, at[k]);
+        }
+#pragma unroll
+        for (int k = 0; k < PIECES; k++) b[k] = piece_ld<BT>(a.b, bo + at[k]);
+#pragma unroll
+        for (int k = 0; k < PIECES; k++) x[k] = piece_ld<XT>(a.x, xo + at[k]);
+        float inv = a.scale;
+        if (a.post_w) {
+            float s = 0.f;
+#pragma unroll
+            for (int k = 0; k < PIECES; k++)
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    const float v = piece_at<BT>(b[k], j);
+                    s += j >= skip[k] ? v * v : 0.f;
+                }
+            inv = 1.f / sqrtf(wg_sum<WAVES>(s, part[0]) / static_cast<float>(dim) + a.eps);
+        }
+        float y[PIECES][4];
+        float s = 0.f;
+#pragma unroll
+        for (int k = 0; k < PIECES; k++) {
+            float p[4];
+#pragma unroll
+            for (int j = 0; j < 4; j++) p[j] = piece_at<BT>(b[k], j) * inv;
+            if (a.post_w) {
+                const Piece<ELEM_F32> w = piece_ld<ELEM_F32>(a.post_w, at[k]);
+#pragma unroll
+                for (int j = 0; j < 4; j++) p[j] *= piece_at<ELEM_F32>(w, j) * a.scale;
+            }
+            if (a.gate) {
+#pragma unroll
+                for (int j = 0; j < 4; j++) p[j] *= gate_at(a, g[k], j);
+            }
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                y[k][j] = piece_at<XT>(x[k], j) + p[j];
+                s += j >= skip[k] ? y[k][j] * y[k][j] : 0.f;
+            }
+        }
+        // (y may be x: all of the row is read before the barrier, and stored behind it)
+        if (a.pre_w) s = wg_sum<WAVES>(s, part[1]);
+        else __syncthreads();
+        const float inv2 = 1.f / sqrtf(s / static_cast<float>(dim) + a.eps);
+#pragma unroll
+        for (int k = 0; k < PIECES; k++) {
+            if (skip[k] == 4) continue;
+            piece_put<XT>(a.y, yo + at[k], y[k], skip[k]);
+            if (a.pre_w) {
+                const Piece<ELEM_F32> w = piece_ld<ELEM_F32>(a.pre_w, at[k]);
+                float n[4];
+#pragma unroll
+                for (int j = 0; j < 4; j++) n[j] = y[k][j] * inv2 * piece_at<ELEM_F32>(w, j);
+                if (a.n_type == ELEM_F32) piece_put<ELEM_F32>(a.n, no + at[k], n, skip[k]);
+                else if (a.n_type == ELEM_F16) piece_put<ELEM_F16>(a.n, no + at[k], n, skip[k]);
+                else piece_put<ELEM_BF16>(a.n, no + at[k], n, skip[k]);
+            }
+        }
+        if (WAVES > 1) __syncthreads();  // the sums are read
+    }
+}
+
+constexpr int LONG_WAVES = 16;
+
+// Rows of any length: read again for every sum.
+__global__ void __launch_bounds__(64 * LONG_WAVES) seam_long_kernel(SeamArgs a) {
+    __shared__ float part[2][LONG_WAVES];
+    constexpr int STEP = 64 * LONG_WAVES;
+    for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
+        const int64_t bo = row * a.b_ld, xo = row * a.x_ld, yo = row * a.y_ld, no = row * a.n_ld, go = row * a.gate_row;
+        float inv = 1.f;
+        if (a.post_w) {
+            float s = 0.f;
+            for (int64_t i = threadIdx.x; i < a.dim; i += STEP) {
+                const float v = elem_ld(a.b, bo + i, a.b_type);
+                s += v * v;
+            }
+            inv = 1.f / sqrtf(wg_sum<LONG_WAVES>(s, part[0]) / static_cast<float>(a.dim) + a.eps);
+        }
+        auto value = [&](int64_t i) {
+            float p = elem_ld(a.b, bo + i, a.b_type) * inv;
+            if (a.post_w) p *= a.post_w[i];
+            p *= a.scale;
+            if (a.gate) p *= elem_ld(a.gate, go + i * a.gate_col, a.gate_type);
+            return elem_ld(a.x, xo + i, a.x_type) + p;
+        };
+        float inv2 = 1.f;
+        if (a.pre_w) {
+            float s = 0.f;
+            for (int64_t i = threadIdx.x; i < a.dim; i += STEP) {
+                const float v = value(i);
+                s += v * v;
+            }
+            inv2 = 1.f / sqrtf(wg_sum<LONG_WAVES>(s, part[1]) / static_cast<float>(a.dim) + a.eps);
+        }
+        for (int64_t i = threadIdx.x; i < a.dim; i += STEP) {
+            const float v = value(i);
+            elem_st(a.y, yo + i, a.x_type, v);
+            if (a.pre_w) elem_st(a.n, no + i, a.n_type, v * inv2 * a.pre_w[i]);
+        }
+        __syncthreads();  // the sums are read
+    }
+}
+
+template <int BT, int XT>
+void seam_launch(const SeamArgs& a, hipStream_t st) {
+    const uint32_t grid = static_cast<uint32_t>(a.rows < (1 << 20) ? a.rows : 1 << 20);  // fewer than 2^32 threads
+    // few rows: as many threads a row as it has pieces; many: four waves a row, and several rows a CU
+    const bool few = a.rows <= 2 * num_cus();
+    const int64_t d = a.dim;
+    if (d < 4 || d > 16384) seam_long_kernel<<<grid, 64 * LONG_WAVES, 0, st>>>(a);
+    else if (d <= 1024) seam_kernel<BT, XT, 4, 1><<<grid, 256, 0, st>>>(a);
+    else if (few && d <= 4096) seam_kernel<BT, XT, 16, 1><<<grid, 1024, 0, st>>>(a);
+    else if (few && d <= 8192) seam_kernel<BT, XT, 16, 2><<<grid, 1024, 0, st>>>(a);
+    else if (d <= 2048) seam_kernel<BT, XT, 4, 2><<<grid, 256, 0, st>>>(a);
+    else if (d <= 4096) seam_kernel<BT, XT, 4, 4><<<grid, 256, 0, st>>>(a);
+    else if (d <= 8192) seam_kernel<BT, XT, 4, 8><<<grid, 256, 0, st>>>(a);
+    else seam_kernel<BT, XT, 16, 4><<<grid, 1024, 0, st>>>(a);
+}
+
+template <int BT>
+void seam_launch_x(const SeamArgs& a, hipStream_t st) {
+    if (a.x_type == ELEM_F32) seam_launch<BT, ELEM_F32>(a, st);
+    else if (a.x_type == ELEM_F16) seam_launch<BT, ELEM_F16>(a, st);
+    else seam_launch<BT, ELEM_BF16>(a, st);
 }
 
 }  // namespace
@@ -113,7 +314,8 @@ extern "C" int vb_block_norm(const void* branch, int32_t branch_type, int64_t br
     if (rows == 0) return OK;
     const SeamArgs a{branch, x,      y,        n,   post_w,      pre_w,  gate,   branch_ld, x_ld,  y_ld, n_ld,
                      gate_row, gate_col, rows, dim, branch_type, x_type, n_type, gate_type, scale, eps};
-    const uint32_t grid = static_cast<uint32_t>(rows < (1 << 20) ? rows : 1 << 20);  // fewer than 2^32 threads
-    seam_kernel<<<dim3(grid), dim3(SEAM_THREADS), 0, as_stream(stream)>>>(a);
+    if (branch_type == ELEM_F32) seam_launch_x<ELEM_F32>(a, as_stream(stream));
+    else if (branch_type == ELEM_F16) seam_launch_x<ELEM_F16>(a, as_stream(stream));
+    else seam_launch_x<ELEM_BF16>(a, as_stream(stream));
     return check_launch("vb_block_norm");
 }
