@@ -269,9 +269,11 @@ void seam_launch(const SeamArgs& a, hipStream_t st) {
     else if (d <= 1024) seam_kernel<BT, XT, 4, 1><<<grid, 256, 0, st>>>(a);
     else if (few && d <= 4096) seam_kernel<BT, XT, 16, 1><<<grid, 1024, 0, st>>>(a);
     else if (few && d <= 8192) seam_kernel<BT, XT, 16, 2><<<grid, 1024, 0, st>>>(a);
-    else if (d <= 2048) seam_kernel<BT, XT, 4, 2><<<grid, 256, 0, st>>>(a);
-    else if (d <= 4096) seam_kernel<BT, XT, 4, 4><<<grid, 256, 0, st>>>(a);
-    else if (d <= 8192) seam_kernel<BT, XT, 4, 8><<<grid, 256, 0, st>>>(a);
+    else if (d <= 2048) seam_kernel<BT, XT, 8, 1><<<grid, 512, 0, st>>>(a);
+    else if (d <= 4096) seam_kernel<BT, XT, 8, 2><<<grid, 512, 0, st>>>(a);
+    else if (d <= 6144) seam_kernel<BT, XT, 8, 3><<<grid, 512, 0, st>>>(a);
+    else if (d <= 8192) seam_kernel<BT, XT, 8, 4><<<grid, 512, 0, st>>>(a);
+    else if (d <= 12288) seam_kernel<BT, XT, 16, 3><<<grid, 1024, 0, st>>>(a);
     else seam_kernel<BT, XT, 16, 4><<<grid, 1024, 0, st>>>(a);
 }
 

@@ -12,7 +12,7 @@ from __future__ import annotations
 import torch
 
 from . import _lib
-from .tensor import _as_f32_dev, _check_out, _dev, _elem, _gpu_tensor, _launch, _rows_of, _workspace
+from .tensor import _as_f32_dev, _check_out, _dev, _elem, _gpu_tensor, _launch, _rows_of
 
 __all__ = ["GroupQTensor", "group_gemv"]
 
@@ -125,11 +125,11 @@ def group_gemv(w: GroupQTensor, x: torch.Tensor, out: torch.Tensor | None = None
     xr = _rows_of(x, w.k)
     m = xr.shape[0]
     if out is None:
-        out = torch.empty((w.rows,) if x.dim() == 1 else (m, w.rows), dtype=torch.float32, device=dev)
+        out = x.new_empty((w.rows,) if x.dim() == 1 else (m, w.rows), dtype=torch.float32)
     else:
         _check_out(out, m * w.rows, dev, "group_gemv")
     nbytes = _lib.load().vb_group4_workspace(m, w.rows, w.k, w.group, int(w.zeros), kind)
-    ws = _workspace(nbytes, dev) if nbytes > 0 else None
+    ws = w.data.new_empty(nbytes) if nbytes > 0 else None
     _launch(dev, "vb_group4_gemv", w.ptr(), w.rows, w.k, w.group, int(w.zeros), xr.data_ptr(), kind, xr.stride(0), m,
-            out.data_ptr(), None if ws is None else ws.data_ptr(), max(nbytes, 0))
+            out.data_ptr(), None if ws is None else ws.data_ptr(), nbytes)
     return out

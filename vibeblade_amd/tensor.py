@@ -385,15 +385,21 @@ def _rows_of(t: torch.Tensor, dim: int) -> torch.Tensor:
     return t if t.stride(1) == 1 or dim == 1 else t.contiguous()
 
 
+# the current stream's handle without a Stream object around it, where torch has that (2 us less a call)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or \
+    (lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
 def _launch(dev: torch.device, fn: str, *args) -> None:
     """fn(*args, stream) on the current stream of the device that the tensors are on."""
-    if dev.index == torch.cuda.current_device():
-        _lib.init(dev.index)
-        _lib.call(fn, *args, torch.cuda.current_stream(dev).cuda_stream)
-        return
-    with torch.cuda.device(dev):
-        _lib.init(dev.index)
-        _lib.call(fn, *args, torch.cuda.current_stream(dev).cuda_stream)
+    index = dev.index
+    if index != torch.cuda.current_device():
+        with torch.cuda.device(index):
+            return _launch(dev, fn, *args)
+    _lib.init(index)
+    rc = getattr(_lib.load(), fn)(*args, _raw_stream(index))
+    if rc != _lib.VB_OK:
+        _lib.check(fn, rc)
 
 
 def _norm_weight(w, dim: int, dev, what: str) -> torch.Tensor | None:
@@ -444,25 +450,26 @@ def block_norm(x: torch.Tensor, branch: torch.Tensor, post_w=None, gate: torch.T
         if g.stride(1) not in (0, 1):
             g = g.contiguous()
         g_ptr, g_row, g_col = g.data_ptr(), g.stride(0), g.stride(1)
+    y_ld = dim
     if out is None:
-        out = torch.empty(x.shape, dtype=x.dtype, device=dev)
-    elif not isinstance(out, torch.Tensor) or out.dtype != x.dtype or out.device != dev or out.shape != x.shape:
-        raise ValueError(f"block_norm: out must be {tuple(x.shape)} {x.dtype} on {dev}")
-    try:
-        yr = out if out.dim() == 2 else out.view(-1, dim)
-    except RuntimeError:
-        yr = None
-    if yr is None or (yr.stride(1) != 1 and dim != 1):
-        raise ValueError("block_norm: out must be rows of unit stride")
-    n = nr = None
+        out = torch.empty_like(x, memory_format=torch.contiguous_format)
+    else:
+        if not isinstance(out, torch.Tensor) or out.dtype != x.dtype or out.device != dev or out.shape != x.shape:
+            raise ValueError(f"block_norm: out must be {tuple(x.shape)} {x.dtype} on {dev}")
+        try:
+            yr = out if out.dim() == 2 else out.view(-1, dim)
+        except RuntimeError:
+            yr = None
+        if yr is None or (yr.stride(1) != 1 and dim != 1):
+            raise ValueError("block_norm: out must be rows of unit stride")
+        y_ld = yr.stride(0)
+    n, n_ptr, n_type = None, None, 0
     if pre is not None:
-        n = torch.empty(x.shape, dtype=normed_dtype or x.dtype, device=dev)
-        nr = n.view(-1, dim)
+        n = torch.empty_like(x, dtype=normed_dtype, memory_format=torch.contiguous_format)
+        n_ptr, n_type = n.data_ptr(), _elem(n, "block_norm: normed_dtype")
     _launch(dev, "vb_block_norm", br.data_ptr(), b_type, br.stride(0), None if post is None else post.data_ptr(),
-            g_ptr, g_type, g_row, g_col, float(scale), xr.data_ptr(), x_type, xr.stride(0), yr.data_ptr(),
-            yr.stride(0), None if pre is None else pre.data_ptr(), None if nr is None else nr.data_ptr(),
-            0 if nr is None else _elem(n, "block_norm: normed_dtype"), 0 if nr is None else nr.stride(0), rows, dim,
-            float(eps))
+            g_ptr, g_type, g_row, g_col, scale, xr.data_ptr(), x_type, xr.stride(0), out.data_ptr(), y_ld,
+            None if pre is None else pre.data_ptr(), n_ptr, n_type, dim, rows, dim, eps)
     return out, n
 
 
@@ -500,13 +507,13 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor | None, top: int =
         raise ValueError(f"token_logprobs: tokens must be ({rows},) or ({rows}, t), got {tuple(tokens.shape)}")
     tokens = tokens.contiguous()
     each = tokens.shape[1] if tokens.dim() == 2 else 1
-    lp = torch.empty(tokens.shape, dtype=torch.float32, device=dev)
-    entropy = torch.empty(rows, dtype=torch.float32, device=dev)
-    ids = torch.empty((rows, top), dtype=torch.int32, device=dev)
-    best = torch.empty((rows, top), dtype=torch.float32, device=dev)
+    lp = torch.empty_like(tokens, dtype=torch.float32)
+    entropy = lp.new_empty(rows)
+    best = lp.new_empty((rows, top))
+    ids = torch.empty_like(best, dtype=torch.int32)
     nbytes = _lib.load().vb_token_logprobs_workspace(rows, vocab, top)
-    ws = _workspace(nbytes, dev) if nbytes > 0 else None
-    _launch(dev, "vb_token_logprobs", z.data_ptr(), kind, z.stride(0), rows, vocab, float(temperature),
+    ws = lp.new_empty((nbytes + 3) // 4) if nbytes > 0 else None
+    _launch(dev, "vb_token_logprobs", z.data_ptr(), kind, z.stride(0), rows, vocab, temperature,
             tokens.data_ptr(), tokens.element_size(), each, lp.data_ptr(), entropy.data_ptr(), top, ids.data_ptr(),
-            best.data_ptr(), None if ws is None else ws.data_ptr(), max(nbytes, 0))
+            best.data_ptr(), None if ws is None else ws.data_ptr(), nbytes)
     return lp, entropy, ids, best
