@@ -93,6 +93,30 @@ def test_block_norm_lengths(dim):
     check_norm(x, b, post, None, 0.5, pre, 1e-5, y, n)
 
 
+@pytest.mark.parametrize("dim", [5, 256, 257, 1025, 2048, 2050, 4095, 4097, 6145, 8191, 8193, 10241, 12287, 14337])
+@pytest.mark.parametrize("gate", [None, "full"])
+def test_block_norm_many_rows(dim, gate):
+    """More rows than CUs, lengths at and beside the borders of the pieces of a row."""
+    rows = 300
+    x, b = normal(dim, rows, dim, scale=3).cuda(), normal(dim + 1, rows, dim, dtype=F16).cuda()
+    post, pre = (1 + normal(dim + 2, dim, scale=0.1)).cuda(), (1 + normal(dim + 3, dim, scale=0.1)).cuda()
+    g = normal(dim + 4, rows, dim, dtype=BF16).cuda() if gate else None
+    y, n = block_norm(x, b, post_w=post, gate=g, pre_w=pre, normed_dtype=BF16)
+    check_norm(x, b, post, g, 1.0, pre, 1e-5, y, n)
+
+
+def test_block_norm_stores_special_values_in_16_bits():
+    """What a narrow type holds of NaN, infinities, overflow and ties: as torch rounds."""
+    v = torch.tensor([[math.nan, INF, -INF, 3.4e38, -3.4e38, 1.0 + 2 ** -8, 1.0 + 3 * 2 ** -8, 1.0 + 2 ** -11, 65519.0,
+                       65520.0, 1e-40, -1e-40, 2.0 ** -25, 0.0, -0.0, 7.0]])
+    for dtype in (F16, BF16):
+        # (a stream of 16 bits in, the branch brings the value in fp32)
+        y, _ = block_norm(torch.zeros(1, 16, dtype=dtype, device="cuda"), v.cuda())
+        want = (v + 0.0).to(dtype)
+        assert torch.equal(y.cpu().isnan(), want.isnan())
+        assert torch.equal(y.cpu().nan_to_num(5), want.nan_to_num(5))
+
+
 @pytest.mark.parametrize("xt", [F32, F16, BF16])
 @pytest.mark.parametrize("bt", [F32, F16, BF16])
 @pytest.mark.parametrize("nt", [F32, F16, BF16])

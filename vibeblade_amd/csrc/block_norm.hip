@@ -79,7 +79,7 @@ __device__ __forceinline__ void piece_st(void* p, int64_t i, const float* v) {
                 typedef _Float16 half2_t __attribute__((ext_vector_type(2)));
                 u[j] = __builtin_bit_cast(uint32_t, half2_t{static_cast<_Float16>(v[2 * j]), static_cast<_Float16>(v[2 * j + 1])});
             } else {
-                u[j] = f32_bf16(v[2 * j]) | static_cast<uint32_t>(f32_bf16(v[2 * j + 1])) << 16;
+                u[j] = f32_bf16x2(v[2 * j], v[2 * j + 1]);
             }
         }
         *reinterpret_cast<v2*>(static_cast<uint16_t*>(p) + i) = v2{u[0], u[1]};
@@ -134,20 +134,19 @@ __device__ __forceinline__ void piece_put(void* p, int64_t i, const float* v, in
     }
 }
 
-// Rows of 4 to 256 * WAVES * PIECES values.  The last piece of a row is moved
-// back to end with it: its first values are another thread's, and are neither
-// summed nor stored again.
+// Rows of at least 4 and over 256 * WAVES * (PIECES - 1) values, up to 256 *
+// WAVES * PIECES: all but a thread's last piece are whole.  The row's last
+// piece is moved back to end with it; its first values are another thread's,
+// and are neither summed nor stored again.
 template <int BT, int XT, int WAVES, int PIECES>
 __global__ void __launch_bounds__(64 * WAVES) seam_kernel(SeamArgs a) {
     __shared__ float part[2][WAVES];
     const int dim = static_cast<int>(a.dim);
-    int at[PIECES], skip[PIECES];  // a piece's first value; how many of it are not its own (4: no piece)
-#pragma unroll
-    for (int k = 0; k < PIECES; k++) {
-        const int i = (k * 64 * WAVES + static_cast<int>(threadIdx.x)) * 4;
-        at[k] = i + 4 <= dim ? i : dim - 4;
-        skip[k] = i >= dim ? 4 : i - at[k];
-    }
+    const int begin = static_cast<int>(threadIdx.x) * 4, last = begin + (PIECES - 1) * 256 * WAVES;
+    // a piece's first value, and how many of it are not its own (4: there is no piece)
+    const auto at = [&](int k) { return k < PIECES - 1 || last + 4 <= dim ? begin + k * 256 * WAVES : dim - 4; };
+    const int last_skip = last >= dim ? 4 : last + 4 <= dim ? 0 : last + 4 - dim;
+    const auto skip = [&](int k) { return k < PIECES - 1 ? 0 : last_skip; };
     for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
         const int64_t bo = row * a.b_ld, xo = row * a.x_ld, yo = row * a.y_ld, no = row * a.n_ld, go = row * a.gate_row;
         Piece<ELEM_F32> g[PIECES];
@@ -155,12 +154,12 @@ __global__ void __launch_bounds__(64 * WAVES) seam_kernel(SeamArgs a) {
         Piece<XT> x[PIECES];
         if (a.gate) {
 #pragma unroll
-            for (int k = 0; k < PIECES; k++) g[k] = gate_ld(a, go, at[k]);
+            for (int k = 0; k < PIECES; k++) g[k] = gate_ld(a, go, at(k));
         }
 #pragma unroll
-        for (int k = 0; k < PIECES; k++) b[k] = piece_ld<BT>(a.b, bo + at[k]);
+        for (int k = 0; k < PIECES; k++) b[k] = piece_ld<BT>(a.b, bo + at(k));
 #pragma unroll
-        for (int k = 0; k < PIECES; k++) x[k] = piece_ld<XT>(a.x, xo + at[k]);
+        for (int k = 0; k < PIECES; k++) x[k] = piece_ld<XT>(a.x, xo + at(k));
         float inv = a.scale;
         if (a.post_w) {
             float s = 0.f;
@@ -169,7 +168,7 @@ __global__ void __launch_bounds__(64 * WAVES) seam_kernel(SeamArgs a) {
 #pragma unroll
                 for (int j = 0; j < 4; j++) {
                     const float v = piece_at<BT>(b[k], j);
-                    s += j >= skip[k] ? v * v : 0.f;
+                    s += j >= skip(k) ? v * v : 0.f;
                 }
             inv = 1.f / sqrtf(wg_sum<WAVES>(s, part[0]) / static_cast<float>(dim) + a.eps);
         }
@@ -181,7 +180,7 @@ __global__ void __launch_bounds__(64 * WAVES) seam_kernel(SeamArgs a) {
 #pragma unroll
             for (int j = 0; j < 4; j++) p[j] = piece_at<BT>(b[k], j) * inv;
             if (a.post_w) {
-                const Piece<ELEM_F32> w = piece_ld<ELEM_F32>(a.post_w, at[k]);
+                const Piece<ELEM_F32> w = piece_ld<ELEM_F32>(a.post_w, at(k));
 #pragma unroll
                 for (int j = 0; j < 4; j++) p[j] *= piece_at<ELEM_F32>(w, j) * a.scale;
             }
@@ -192,7 +191,7 @@ __global__ void __launch_bounds__(64 * WAVES) seam_kernel(SeamArgs a) {
 #pragma unroll
             for (int j = 0; j < 4; j++) {
                 y[k][j] = piece_at<XT>(x[k], j) + p[j];
-                s += j >= skip[k] ? y[k][j] * y[k][j] : 0.f;
+                s += j >= skip(k) ? y[k][j] * y[k][j] : 0.f;
             }
         }
         // (y may be x: all of the row is read before the barrier, and stored behind it)
@@ -201,16 +200,16 @@ __global__ void __launch_bounds__(64 * WAVES) seam_kernel(SeamArgs a) {
         const float inv2 = 1.f / sqrtf(s / static_cast<float>(dim) + a.eps);
 #pragma unroll
         for (int k = 0; k < PIECES; k++) {
-            if (skip[k] == 4) continue;
-            piece_put<XT>(a.y, yo + at[k], y[k], skip[k]);
+            if (skip(k) == 4) continue;
+            piece_put<XT>(a.y, yo + at(k), y[k], skip(k));
             if (a.pre_w) {
-                const Piece<ELEM_F32> w = piece_ld<ELEM_F32>(a.pre_w, at[k]);
+                const Piece<ELEM_F32> w = piece_ld<ELEM_F32>(a.pre_w, at(k));
                 float n[4];
 #pragma unroll
                 for (int j = 0; j < 4; j++) n[j] = y[k][j] * inv2 * piece_at<ELEM_F32>(w, j);
-                if (a.n_type == ELEM_F32) piece_put<ELEM_F32>(a.n, no + at[k], n, skip[k]);
-                else if (a.n_type == ELEM_F16) piece_put<ELEM_F16>(a.n, no + at[k], n, skip[k]);
-                else piece_put<ELEM_BF16>(a.n, no + at[k], n, skip[k]);
+                if (a.n_type == ELEM_F32) piece_put<ELEM_F32>(a.n, no + at(k), n, skip(k));
+                else if (a.n_type == ELEM_F16) piece_put<ELEM_F16>(a.n, no + at(k), n, skip(k));
+                else piece_put<ELEM_BF16>(a.n, no + at(k), n, skip(k));
             }
         }
         if (WAVES > 1) __syncthreads();  // the sums are read
@@ -262,10 +261,13 @@ __global__ void __launch_bounds__(64 * LONG_WAVES) seam_long_kernel(SeamArgs a) 
 template <int BT, int XT>
 void seam_launch(const SeamArgs& a, hipStream_t st) {
     const uint32_t grid = static_cast<uint32_t>(a.rows < (1 << 20) ? a.rows : 1 << 20);  // fewer than 2^32 threads
-    // few rows: as many threads a row as it has pieces; many: four waves a row, and several rows a CU
-    const bool few = a.rows <= 2 * num_cus();
+    // A row by eight waves, in as many pieces a thread as it takes (7001 x 5121:
+    // 189 us with four waves and twice the pieces, 124 with eight); few rows by
+    // sixteen, which are on their way sooner.
+    const bool few = a.rows <= num_cus();
     const int64_t d = a.dim;
     if (d < 4 || d > 16384) seam_long_kernel<<<grid, 64 * LONG_WAVES, 0, st>>>(a);
+    else if (d <= 256) seam_kernel<BT, XT, 1, 1><<<grid, 64, 0, st>>>(a);
     else if (d <= 1024) seam_kernel<BT, XT, 4, 1><<<grid, 256, 0, st>>>(a);
     else if (few && d <= 4096) seam_kernel<BT, XT, 16, 1><<<grid, 1024, 0, st>>>(a);
     else if (few && d <= 8192) seam_kernel<BT, XT, 16, 2><<<grid, 1024, 0, st>>>(a);
@@ -273,8 +275,10 @@ void seam_launch(const SeamArgs& a, hipStream_t st) {
     else if (d <= 4096) seam_kernel<BT, XT, 8, 2><<<grid, 512, 0, st>>>(a);
     else if (d <= 6144) seam_kernel<BT, XT, 8, 3><<<grid, 512, 0, st>>>(a);
     else if (d <= 8192) seam_kernel<BT, XT, 8, 4><<<grid, 512, 0, st>>>(a);
-    else if (d <= 12288) seam_kernel<BT, XT, 16, 3><<<grid, 1024, 0, st>>>(a);
-    else seam_kernel<BT, XT, 16, 4><<<grid, 1024, 0, st>>>(a);
+    else if (d <= 10240) seam_kernel<BT, XT, 8, 5><<<grid, 512, 0, st>>>(a);
+    else if (d <= 12288) seam_kernel<BT, XT, 8, 6><<<grid, 512, 0, st>>>(a);
+    else if (d <= 14336) seam_kernel<BT, XT, 8, 7><<<grid, 512, 0, st>>>(a);
+    else seam_kernel<BT, XT, 8, 8><<<grid, 512, 0, st>>>(a);
 }
 
 template <int BT>

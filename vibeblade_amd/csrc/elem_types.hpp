@@ -12,12 +12,13 @@ inline int64_t elem_bytes(int32_t t) { return t == ELEM_F32 ? 4 : 2; }
 
 __device__ __forceinline__ float bf16_f32(uint16_t v) { return __uint_as_float(static_cast<uint32_t>(v) << 16); }
 
-// To the nearest bf16, ties to even; NaN stays NaN.
-__device__ __forceinline__ uint16_t f32_bf16(float v) {
-    const uint32_t u = __float_as_uint(v);
-    if (v != v) return static_cast<uint16_t>((u >> 16) | 0x40);
-    return static_cast<uint16_t>((u + 0x7fff + ((u >> 16) & 1)) >> 16);
+// To the nearest bf16, ties to even; NaN stays NaN (v_cvt_pk_bf16_f32).
+__device__ __forceinline__ uint32_t f32_bf16x2(float lo, float hi) {
+    typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+    typedef float f32x2 __attribute__((ext_vector_type(2)));
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{lo, hi}), bf16x2));
 }
+__device__ __forceinline__ uint16_t f32_bf16(float v) { return static_cast<uint16_t>(f32_bf16x2(v, 0.f)); }
 
 // Element i of a tensor of a type known at run time (the same in every lane).
 __device__ __forceinline__ float elem_ld(const void* p, int64_t i, int type) {
