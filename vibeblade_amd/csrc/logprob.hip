@@ -21,12 +21,15 @@
 // One pass over the logits.  A wave walks over a slice of a row, 16 logits a
 // lane at a time, with its running maximum m, S and the entropy's sum (each
 // lane's share of them, relative to the wave's m).  The alternatives hang on a
-// threshold: the value of the last of the wave's best `top` logits so far.  A
-// batch whose every lane stays at or below it, as nearly all do after the first
-// few, costs one comparison; otherwise the logits above it are appended to a
-// buffer in LDS, and when that runs full its best `top` are ranked (each entry
-// counts those before it) and the threshold rises.  The waves of a workgroup,
-// and the workgroups of a row where there are few rows, are joined the same way.
+// threshold that at least `top` logits of the row reach: at first the top-th
+// largest of the lanes' maxima over the workgroup's first batches, found by
+// bisection.  A batch whose every lane stays at or below it costs one
+// comparison; otherwise the logits that reach it are appended to a buffer in
+// LDS.  When that fills, its best `top` are ranked (each entry counts those
+// before it) and the threshold rises.  The waves' buffers, and the lists of a
+// row's slices where there are few rows, are joined and ranked once.
+#include <type_traits>
+
 #include "elem_types.hpp"
 #include "vb_internal.hpp"
 #include "../../include/vbhip.h"
@@ -62,16 +65,43 @@ __device__ __forceinline__ uint32_t order_bits(float v) {
     return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 __device__ __forceinline__ float order_value(uint32_t o) { return __uint_as_float(o & 0x80000000u ? o & 0x7fffffffu : ~o); }
+__device__ __forceinline__ float order_floor(uint32_t o) { return o > 0x007fffffu ? order_value(o) : -INFINITY; }  // (-inf's)
 __device__ __forceinline__ uint64_t order_key(float v, uint32_t i) {
     return v > -INFINITY ? static_cast<uint64_t>(order_bits(v)) << 32 | (0xffffffffu - i) : 0;
 }
 __device__ __forceinline__ int key_index(uint64_t k) { return static_cast<int>(0xffffffffu - static_cast<uint32_t>(k)); }
 __device__ __forceinline__ float key_value(uint64_t k) { return order_value(static_cast<uint32_t>(k >> 32)); }
 
+// The largest value of a wave, in every lane.
 __device__ __forceinline__ float wave_max(float v) {
+    const auto dpp = [](float x, auto ctrl, auto rows) {
+        return __int_as_float(__builtin_amdgcn_update_dpp(__float_as_int(x), __float_as_int(x), decltype(ctrl)::value,
+                                                          decltype(rows)::value, 0xF, false));
+    };
+    using std::integral_constant;
+    v = fmaxf(v, dpp(v, integral_constant<int, 0xB1>{}, integral_constant<int, 0xF>{}));   // quad_perm [1,0,3,2]
+    v = fmaxf(v, dpp(v, integral_constant<int, 0x4E>{}, integral_constant<int, 0xF>{}));   // quad_perm [2,3,0,1]
+    v = fmaxf(v, dpp(v, integral_constant<int, 0x141>{}, integral_constant<int, 0xF>{}));  // row_half_mirror
+    v = fmaxf(v, dpp(v, integral_constant<int, 0x140>{}, integral_constant<int, 0xF>{}));  // row_mirror
+    v = fmaxf(v, dpp(v, integral_constant<int, 0x142>{}, integral_constant<int, 0xA>{}));  // row_bcast:15 into rows 1, 3
+    v = fmaxf(v, dpp(v, integral_constant<int, 0x143>{}, integral_constant<int, 0xC>{}));  // row_bcast:31 into rows 2, 3
+    return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), 63));
+}
+
+// A value that at least n of the lanes' order bits reach (NV a lane, 0: none)
+// and about as few as possible; 0 where there are fewer than n.
+template <int NV>
+__device__ __forceinline__ uint32_t reached_by(const uint32_t (&o)[NV], int n) {
+    uint32_t at = 0;
+    for (int bit = 31; bit >= 12; bit--) {
+        const uint32_t up = at | 1u << bit;
+        int count = 0;
 #pragma unroll
-    for (int off = 32; off >= 1; off >>= 1) v = fmaxf(v, __shfl_xor(v, off, 64));
-    return v;
+        for (int i = 0; i < NV; i++) count += __popcll(__ballot(o[i] >= up));
+        if (count >= n) at = up;
+        if (count >= n && count <= n + (n >> 2)) break;
+    }
+    return at;
 }
 
 __device__ __forceinline__ int lanes_below(uint64_t mask) {
@@ -88,25 +118,33 @@ __device__ __forceinline__ void wave_lds_fence() {
 struct Best {
     uint64_t* buf;
     int n, count;
-    float tau;  // no candidate at or below it is wanted (but equal values of lower index within a batch)
+    float tau;  // no candidate below it is wanted
 
     // The n best of the buffer, in order.
     __device__ __forceinline__ void rank() {
         wave_lds_fence();
         const int lane = static_cast<int>(threadIdx.x) & 63;
         const uint64_t a = lane < count ? buf[lane] : 0, b = lane + 64 < count ? buf[lane + 64] : 0;
+        if (lane >= count) buf[lane] = 0;  // (the loop below reads whole groups)
+        if (lane + 64 >= count) buf[lane + 64] = 0;
+        wave_lds_fence();
         int ra = 0, rb = 0;
-        for (int i = 0; i < count; i++) {
-            const uint64_t k = buf[i];
-            ra += k > a;
-            rb += k > b;
+        for (int i = 0; i < count; i += 8) {
+            uint64_t k[8];
+#pragma unroll
+            for (int j = 0; j < 8; j++) k[j] = buf[i + j];
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                ra += k[j] > a;
+                rb += k[j] > b;
+            }
         }
         wave_lds_fence();
         if (lane < count && ra < n) buf[ra] = a;
         if (lane + 64 < count && rb < n) buf[rb] = b;
         wave_lds_fence();
         count = count < n ? count : n;
-        tau = count == n ? key_value(buf[n - 1]) : -INFINITY;
+        tau = count == n ? fmaxf(tau, key_value(buf[n - 1])) : tau;
     }
 
     __device__ __forceinline__ void append(uint64_t key, bool in) {
@@ -182,24 +220,10 @@ struct Walk {
     static constexpr int U = LP_BATCH / V;              // loads of a batch
     const LpArgs& a;
     Best best;
-    float m, s, t, tau;  // m, tau: the wave's
-    bool first;
+    float m, s, t, tau;  // m: the wave's; tau: no candidate at or below it
 
     __device__ __forceinline__ Walk(const LpArgs& a_, uint64_t* buf)
-        : a(a_), best{buf, a_.top, 0, -INFINITY}, m(-INFINITY), s(0.f), t(0.f), tau(-INFINITY), first(true) {}
-
-    // The lanes' largest values cm hold the wave's n-th largest logit or something below it.
-    __device__ __forceinline__ float first_tau(float cm) const {
-        const uint32_t o = cm > -INFINITY ? order_bits(cm) : 0;
-        uint32_t at = 0;
-        for (int bit = 31; bit >= 12; bit--) {
-            const uint32_t up = at | 1u << bit;
-            const int count = __popcll(__ballot(o >= up));
-            if (count >= best.n) at = up;
-            if (count == best.n) break;
-        }
-        return at ? order_value(at) : -INFINITY;
-    }
+        : a(a_), best{buf, a_.top, 0, -INFINITY}, m(-INFINITY), s(0.f), t(0.f), tau(-INFINITY) {}
 
     // Logit r of the batch, and its index in the row.
     __device__ __forceinline__ static int index_of(int base, int r) {
@@ -207,25 +231,45 @@ struct Walk {
     }
 
     __device__ __forceinline__ void above(float (&v)[LP_BATCH], float cm, int base) {
-        if constexpr (LIST) {
-            if (first) best.tau = first_tau(cm);
-            uint32_t left = 0;
+        if (LIST && __any(cm > tau)) {
+            const float least = fmaxf(best.tau, -3.402823466e38f);  // -inf is never a candidate
+            uint64_t reach[LP_BATCH];
+            int more = 0;
+            bool ranked = true;
 #pragma unroll
-            for (int r = 0; r < LP_BATCH; r++) left |= v[r] >= best.tau && v[r] > -INFINITY ? 1u << r : 0u;
-            while (__any(left != 0)) {
-                const int r = __ffs(left) - 1;
-                float x = v[0];
-#pragma unroll
-                for (int i = 1; i < LP_BATCH; i++) x = r == i ? v[i] : x;
-                best.append(order_key(x, static_cast<uint32_t>(index_of(base, r))), left != 0 && x >= best.tau);
-                left &= left - 1;
+            for (int r = 0; r < LP_BATCH; r++) {
+                reach[r] = __ballot(v[r] >= least);
+                more += __popcll(reach[r]);
             }
-            if (first) best.rank();
-            first = false;
-            tau = best.tau;
+            if (best.count + more <= LP_BUF) {
+#pragma unroll
+                for (int r = 0; r < LP_BATCH; r++) {
+                    if (!reach[r]) continue;
+                    if (v[r] >= least)
+                        best.buf[best.count + lanes_below(reach[r])] = order_key(v[r], static_cast<uint32_t>(index_of(base, r)));
+                    best.count += __popcll(reach[r]);
+                }
+                ranked = best.count > LP_BUF / 2 && best.count >= 2 * best.n;
+            } else {
+                uint32_t left = 0;
+#pragma unroll
+                for (int r = 0; r < LP_BATCH; r++) left |= v[r] >= least ? 1u << r : 0u;
+                while (__any(left != 0)) {
+                    const int r = __ffs(left) - 1;
+                    float x = v[0];
+#pragma unroll
+                    for (int i = 1; i < LP_BATCH; i++) x = r == i ? v[i] : x;
+                    best.append(order_key(x, static_cast<uint32_t>(index_of(base, r))), left != 0 && x >= best.tau);
+                    left &= left - 1;
+                }
+            }
+            if (ranked) {
+                best.rank();
+                if (best.count == best.n) tau = best.tau;  // equal values further on come after these
+            }
         }
-        const float top = wave_max(cm);
-        if (top > m) {
+        if (__any(cm > m)) {
+            const float top = wave_max(cm);
             // one place of the new maximum leaves the sums, the old one joins them
             if (m > -INFINITY) {
                 const float d = (m - top) * a.c, f = __builtin_amdgcn_exp2f(d), dd = fmaxf(d, -1e30f);
@@ -250,7 +294,7 @@ struct Walk {
         float cm = v[0];
 #pragma unroll
         for (int r = 1; r < LP_BATCH; r++) cm = fmaxf(cm, v[r]);
-        if (__any(cm > tau)) above(v, cm, base);
+        if (__any(cm > fminf(tau, m))) above(v, cm, base);
         const float from = m > -INFINITY ? m : 0.f;
 #pragma unroll
         for (int r = 0; r < LP_BATCH; r++) {
@@ -260,22 +304,21 @@ struct Walk {
         }
     }
 
-    // The 16-byte units [u0, u1) from unit 0 at `body`, whose first logit has index i0.
-    __device__ __forceinline__ void run(const void* body, int u0, int u1, int i0) {
-        if (u0 >= u1) return;
+    // The 16-byte units [u0, u1) from unit 0 at `body`, whose first logit has
+    // index i0.  With a list every wave of the workgroup calls this, as they
+    // share their first batches' maxima in `maxima`.
+    __device__ __forceinline__ void run(const void* body, int u0, int u1, int i0, uint32_t (*maxima)[64]) {
         const int lane = static_cast<int>(threadIdx.x) & 63;
-        const __amdgpu_buffer_rsrc_t r = make_rsrc(static_cast<const uint8_t*>(body) + static_cast<int64_t>(u0) * 16,
-                                                   static_cast<uint32_t>(u1 - u0) * 16u);
-        const int count = u1 - u0;
+        const int count = u1 > u0 ? u1 - u0 : 0;
+        const __amdgpu_buffer_rsrc_t r = make_rsrc(static_cast<const uint8_t*>(body) + static_cast<int64_t>(count ? u0 : 0) * 16,
+                                                   static_cast<uint32_t>(count) * 16u);
         u32x4 raw[U];
         const auto load = [&](int at) __attribute__((always_inline)) {  // units past the last read nothing
 #pragma unroll
             for (int u = 0; u < U; u++)
                 raw[u] = __builtin_amdgcn_raw_buffer_load_b128(r, static_cast<int>(static_cast<uint32_t>(at + u * 64 + lane) * 16u), 0, 2);
         };
-        load(0);
-        for (int at = 0; at < count; at += 64 * U) {
-            float v[LP_BATCH];
+        const auto decode = [&](float (&v)[LP_BATCH], int at) __attribute__((always_inline)) {
 #pragma unroll
             for (int u = 0; u < U; u++)
 #pragma unroll
@@ -291,12 +334,33 @@ struct Walk {
                         v[u * V + 2 * i + 1] = __uint_as_float(w & 0xffff0000u);
                     }
                 }
-            load(at + 64 * U);
             if (at + 64 * U > count) {
 #pragma unroll
                 for (int k = 0; k < LP_BATCH; k++)
                     if (at + k / V * 64 + lane >= count) v[k] = -INFINITY;
             }
+        };
+        load(0);
+        if constexpr (LIST) {
+            float v[LP_BATCH];
+            decode(v, 0);
+            float cm = v[0];
+#pragma unroll
+            for (int k = 1; k < LP_BATCH; k++) cm = fmaxf(cm, v[k]);
+            maxima[threadIdx.x >> 6][lane] = cm > -INFINITY ? order_bits(cm) : 0;
+            __syncthreads();
+            uint32_t o[LP_WAVES];
+#pragma unroll
+            for (int k = 0; k < LP_WAVES; k++) o[k] = maxima[k][lane];
+            const uint32_t at = reached_by(o, best.n);
+            best.tau = order_floor(at);
+            // the value below (of 0 not -0): what equals the threshold is a candidate
+            tau = order_floor(at == 0x80000000u ? at - 2 : at - (at > 0));
+        }
+        for (int at = 0; at < count; at += 64 * U) {
+            float v[LP_BATCH];
+            decode(v, at);
+            load(at + 64 * U);
             batch(v, i0 + (u0 + at) * V);
         }
     }
@@ -311,6 +375,7 @@ __global__ void __launch_bounds__(LP_THREADS) logprob_kernel(LpArgs a) {
     constexpr int SIZE = TYPE == ELEM_F32 ? 4 : 2;
     __shared__ uint64_t bufs[LIST ? LP_WAVES : 1][LP_BUF];
     __shared__ int counts[LP_WAVES];
+    __shared__ uint32_t maxima[LP_WAVES][64];
     __shared__ Stat stats[LP_WAVES];
     const int lane = static_cast<int>(threadIdx.x) & 63;
     const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));
@@ -324,11 +389,8 @@ __global__ void __launch_bounds__(LP_THREADS) logprob_kernel(LpArgs a) {
         const int each = ((units + parts - 1) / parts + 63) / 64 * 64;
         const int64_t u0 = static_cast<int64_t>(part) * each, u1 = u0 + each < units ? u0 + each : units;
         W w(a, bufs[LIST ? wave : 0]);
-        if (u0 < u1) w.run(z + head * SIZE, static_cast<int>(u0), static_cast<int>(u1), head);
+        w.run(z + head * SIZE, static_cast<int>(u0 < units ? u0 : units), static_cast<int>(u1), head, maxima);
         const Stat mine{w.m, wave_sum_dpp(w.s), wave_sum_dpp(w.t)};
-        if constexpr (LIST) {
-            if (wave != 0) w.best.rank();
-        }
         if (lane == 0) {
             stats[wave] = mine;
             counts[wave] = w.best.count;
@@ -349,10 +411,11 @@ __global__ void __launch_bounds__(LP_THREADS) logprob_kernel(LpArgs a) {
             }
             const Stat all = join(v, a.c);
             if constexpr (LIST) {
-                for (int k = 1; k < LP_WAVES; k++) {
-                    const uint64_t key = lane < counts[k] ? bufs[k][lane] : 0;
-                    w.best.append(key, key != 0 && key_value(key) >= w.best.tau);
-                }
+                for (int k = 1; k < LP_WAVES; k++)
+                    for (int i = 0; i < counts[k]; i += 64) {
+                        const uint64_t key = i + lane < counts[k] ? bufs[k][i + lane] : 0;
+                        w.best.append(key, key != 0 && key_value(key) >= w.best.tau);
+                    }
                 const bool one = single >= 0 && single < singles && v.m > -INFINITY;
                 w.best.append(order_key(v.m, static_cast<uint32_t>(at)), one && v.m >= w.best.tau);
                 w.best.rank();
@@ -384,12 +447,24 @@ __global__ void __launch_bounds__(64) logprob_join_kernel(LpArgs a) {
         const Stat all = join(v, a.c);
         Best best{buf, a.top, 0, -INFINITY};
         if constexpr (LIST) {
-            for (int j = 0; j < a.top; j++) {
-                const uint64_t key = lane < a.splits ? a.keys[item * a.top + j] : 0;
-                const bool in = key != 0 && key_value(key) >= best.tau;
-                if (!__any(in)) break;
-                best.append(key, in);
-                if (best.count >= best.n) best.rank();
+            // At least `top` candidates reach the q-th of every slice, q slices'
+            // worth of them being enough, or (q = 1) a bisection of the firsts.
+            const uint64_t* list = a.keys + item * a.top;
+            const int q = (a.top + a.splits - 1) / a.splits;
+            const uint64_t qth = lane < a.splits ? list[q - 1] : 0;
+            const uint32_t o[1] = {static_cast<uint32_t>(qth >> 32)};
+            const uint32_t at = reached_by(o, q == 1 ? a.top : a.splits);
+            best.tau = order_floor(at);
+            for (int j = 0; j < a.top; j += 4) {
+                uint64_t key[4];
+#pragma unroll
+                for (int i = 0; i < 4; i++) key[i] = lane < a.splits && j + i < a.top ? list[j + i] : 0;
+#pragma unroll 1
+                for (int i = 0; i < 4; i++) {
+                    const uint64_t k = i == 0 ? key[0] : i == 1 ? key[1] : i == 2 ? key[2] : key[3];
+                    best.append(k, k != 0 && key_value(k) >= best.tau);
+                }
+                if (!__any(key[3] != 0 && key_value(key[3]) >= best.tau)) break;
             }
             best.rank();
         }
