@@ -220,10 +220,14 @@ struct Walk {
     static constexpr int U = LP_BATCH / V;              // loads of a batch
     const LpArgs& a;
     Best best;
-    float m, s, t, tau;  // m: the wave's; tau: no candidate at or below it
+    float m, s, t;  // m: the wave's; s, t: the lane's sums, relative to `ref`
+    float tau;      // no candidate at or below it
+    float ref;      // c m, rounded: a term is 2^(c z - ref), one instruction for the exponent
+    bool far;       // c m is beyond fp32: 2^(c (z - m)) instead
+    bool masked;    // a term with z = -inf was met: 0 (-inf) is kept out of t
 
     __device__ __forceinline__ Walk(const LpArgs& a_, uint64_t* buf)
-        : a(a_), best{buf, a_.top, 0, -INFINITY}, m(-INFINITY), s(0.f), t(0.f), tau(-INFINITY) {}
+        : a(a_), best{buf, a_.top, 0, -INFINITY}, m(-INFINITY), s(0.f), t(0.f), tau(-INFINITY), ref(0.f), far(false), masked(false) {}
 
     // Logit r of the batch, and its index in the row.
     __device__ __forceinline__ static int index_of(int base, int r) {
@@ -271,19 +275,26 @@ struct Walk {
         if (__any(cm > m)) {
             const float top = wave_max(cm);
             // one place of the new maximum leaves the sums, the old one joins them
+            const float now = top * a.c;
+            const bool out_of = !(fabsf(now) < 1e30f);
             if (m > -INFINITY) {
-                const float d = (m - top) * a.c, f = __builtin_amdgcn_exp2f(d), dd = fmaxf(d, -1e30f);
-                const float back = (threadIdx.x & 63) == 0 ? 1.f : 0.f;
-                t = f * (t + dd * (s + back));
-                s = f * (s + back);
+                const bool any_far = far || out_of;
+                const float d = any_far ? (m - top) * a.c : ref - now, f = __builtin_amdgcn_exp2f(d), dd = fmaxf(d, -1e30f);
+                const float dm = any_far ? dd : __builtin_fmaf(m, a.c, -now);
+                const float back = (threadIdx.x & 63) == 0 ? __builtin_amdgcn_exp2f(dm) : 0.f;
+                t = f * (t + dd * s) + back * dm;
+                s = f * s + back;
             }
             m = top;
+            ref = out_of ? 0.f : now;
+            far = out_of;
             const int owner = __ffsll(static_cast<unsigned long long>(__ballot(cm == top))) - 1;
             bool out = (static_cast<int>(threadIdx.x) & 63) == owner;
+            const float gone = far ? -INFINITY : (ref - 300.f) / a.c;  // its term is 0
 #pragma unroll
             for (int r = 0; r < LP_BATCH; r++) {
                 const bool hit = out && v[r] == top;
-                v[r] = hit ? -INFINITY : v[r];
+                v[r] = hit ? gone : v[r];
                 out = out && !hit;
             }
             if (!LIST) tau = m;
@@ -295,17 +306,38 @@ struct Walk {
 #pragma unroll
         for (int r = 1; r < LP_BATCH; r++) cm = fmaxf(cm, v[r]);
         if (__any(cm > fminf(tau, m))) above(v, cm, base);
-        const float from = m > -INFINITY ? m : 0.f;
+        if (!far && !masked) {
+            float s1 = s, t1 = t;
+#pragma unroll
+            for (int r = 0; r < LP_BATCH; r++) {
+                const float d = __builtin_fmaf(v[r], a.c, -ref), e = __builtin_amdgcn_exp2f(d);
+                s1 += e;
+                t1 = __builtin_fmaf(e, d, t1);
+            }
+            if (!__any(t1 != t1)) {
+                s = s1;
+                t = t1;
+                return;
+            }
+            masked = true;
+        }
+        const float from = far ? m : 0.f;
 #pragma unroll
         for (int r = 0; r < LP_BATCH; r++) {
-            const float d = (v[r] - from) * a.c, e = __builtin_amdgcn_exp2f(d);
+            const float d = __builtin_fmaf(v[r] - from, a.c, -ref), e = __builtin_amdgcn_exp2f(d);
             s += e;
-            t += e * fmaxf(d, -1e30f);  // e is 0 below (and NaN for a NaN)
+            t = __builtin_fmaf(e, fmaxf(d, -1e30f), t);  // e is 0 below (and NaN for a NaN)
         }
     }
 
-    // The 16-byte units [u0, u1) from unit 0 at `body`, whose first logit has
-    // index i0.  With a list every wave of the workgroup calls this, as they
+    // The wave's set, relative to m itself.
+    __device__ __forceinline__ Stat stat() const {
+        const float lo = far || !(m > -INFINITY) ? 0.f : __builtin_fmaf(m, a.c, -ref), f = __builtin_amdgcn_exp2f(-lo);
+        return Stat{m, wave_sum_dpp(s * f), wave_sum_dpp((t - lo * s) * f)};
+    }
+
+    // The workgroup's 16-byte units [u0, u1) from unit 0 at `body`, whose first
+    // logit has index i0: its waves take batches in turn.  With a list every wave of the workgroup calls this, as they
     // share their first batches' maxima in `maxima`.
     __device__ __forceinline__ void run(const void* body, int u0, int u1, int i0, uint32_t (*maxima)[64]) {
         const int lane = static_cast<int>(threadIdx.x) & 63;
@@ -340,10 +372,11 @@ struct Walk {
                     if (at + k / V * 64 + lane >= count) v[k] = -INFINITY;
             }
         };
-        load(0);
+        const int begin = static_cast<int>(threadIdx.x >> 6) * 64 * U, step = LP_WAVES * 64 * U;
+        load(begin);
         if constexpr (LIST) {
             float v[LP_BATCH];
-            decode(v, 0);
+            decode(v, begin);
             float cm = v[0];
 #pragma unroll
             for (int k = 1; k < LP_BATCH; k++) cm = fmaxf(cm, v[k]);
@@ -357,10 +390,10 @@ struct Walk {
             // the value below (of 0 not -0): what equals the threshold is a candidate
             tau = order_floor(at == 0x80000000u ? at - 2 : at - (at > 0));
         }
-        for (int at = 0; at < count; at += 64 * U) {
+        for (int at = __builtin_amdgcn_readfirstlane(begin); at < count; at += step) {
             float v[LP_BATCH];
             decode(v, at);
-            load(at + 64 * U);
+            load(at + step);
             batch(v, i0 + (u0 + at) * V);
         }
     }
@@ -385,12 +418,12 @@ __global__ void __launch_bounds__(LP_THREADS) logprob_kernel(LpArgs a) {
         const uint8_t* z = static_cast<const uint8_t*>(a.z) + row * a.ld * SIZE;
         int head = static_cast<int>((16 - (reinterpret_cast<uintptr_t>(z) & 15)) & 15) / SIZE;
         head = head < a.vocab ? head : a.vocab;
-        const int units = (a.vocab - head) / W::V, parts = a.splits * LP_WAVES, part = split * LP_WAVES + wave;
-        const int each = ((units + parts - 1) / parts + 63) / 64 * 64;
-        const int64_t u0 = static_cast<int64_t>(part) * each, u1 = u0 + each < units ? u0 + each : units;
+        const int units = (a.vocab - head) / W::V;
+        const int each = ((units + a.splits - 1) / a.splits + 63) / 64 * 64;
+        const int64_t u0 = static_cast<int64_t>(split) * each, u1 = u0 + each < units ? u0 + each : units;
         W w(a, bufs[LIST ? wave : 0]);
         w.run(z + head * SIZE, static_cast<int>(u0 < units ? u0 : units), static_cast<int>(u1), head, maxima);
-        const Stat mine{w.m, wave_sum_dpp(w.s), wave_sum_dpp(w.t)};
+        const Stat mine = w.stat();
         if (lane == 0) {
             stats[wave] = mine;
             counts[wave] = w.best.count;
