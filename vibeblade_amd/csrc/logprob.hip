@@ -129,14 +129,24 @@ struct Best {
         if (lane + 64 >= count) buf[lane + 64] = 0;
         wave_lds_fence();
         int ra = 0, rb = 0;
-        for (int i = 0; i < count; i += 8) {
-            uint64_t k[8];
+        if (count <= 64) {
+            for (int i = 0; i < count; i += 8) {
+                uint64_t k[8];
 #pragma unroll
-            for (int j = 0; j < 8; j++) k[j] = buf[i + j];
+                for (int j = 0; j < 8; j++) k[j] = buf[i + j];
 #pragma unroll
-            for (int j = 0; j < 8; j++) {
-                ra += k[j] > a;
-                rb += k[j] > b;
+                for (int j = 0; j < 8; j++) ra += k[j] > a;
+            }
+        } else {
+            for (int i = 0; i < count; i += 8) {
+                uint64_t k[8];
+#pragma unroll
+                for (int j = 0; j < 8; j++) k[j] = buf[i + j];
+#pragma unroll
+                for (int j = 0; j < 8; j++) {
+                    ra += k[j] > a;
+                    rb += k[j] > b;
+                }
             }
         }
         wave_lds_fence();
@@ -237,23 +247,32 @@ struct Walk {
     __device__ __forceinline__ void above(float (&v)[LP_BATCH], float cm, int base) {
         if (LIST && __any(cm > tau)) {
             const float least = fmaxf(best.tau, -3.402823466e38f);  // -inf is never a candidate
-            uint64_t reach[LP_BATCH];
             int more = 0;
             bool ranked = true;
 #pragma unroll
-            for (int r = 0; r < LP_BATCH; r++) {
-                reach[r] = __ballot(v[r] >= least);
-                more += __popcll(reach[r]);
+            for (int g = 0; g < LP_BATCH; g += 4) {  // most fours have none
+                const uint64_t any = __ballot(fmaxf(fmaxf(v[g], v[g + 1]), fmaxf(v[g + 2], v[g + 3])) >= least);
+                more += 4 * __popcll(any);
+            }
+            if (best.count + more > LP_BUF) {
+                more = 0;
+#pragma unroll
+                for (int r = 0; r < LP_BATCH; r++) more += __popcll(__ballot(v[r] >= least));
             }
             if (best.count + more <= LP_BUF) {
 #pragma unroll
-                for (int r = 0; r < LP_BATCH; r++) {
-                    if (!reach[r]) continue;
-                    if (v[r] >= least)
-                        best.buf[best.count + lanes_below(reach[r])] = order_key(v[r], static_cast<uint32_t>(index_of(base, r)));
-                    best.count += __popcll(reach[r]);
+                for (int g = 0; g < LP_BATCH; g += 4) {
+                    if (!__any(fmaxf(fmaxf(v[g], v[g + 1]), fmaxf(v[g + 2], v[g + 3])) >= least)) continue;
+#pragma unroll
+                    for (int r = g; r < g + 4; r++) {
+                        const uint64_t reach = __ballot(v[r] >= least);
+                        if (!reach) continue;
+                        if (v[r] >= least)
+                            best.buf[best.count + lanes_below(reach)] = order_key(v[r], static_cast<uint32_t>(index_of(base, r)));
+                        best.count += __popcll(reach);
+                    }
                 }
-                ranked = best.count > LP_BUF / 2 && best.count >= 2 * best.n;
+                ranked = best.count >= 2 * best.n && best.count >= 24;
             } else {
                 uint32_t left = 0;
 #pragma unroll
@@ -506,11 +525,16 @@ __global__ void __launch_bounds__(64) logprob_join_kernel(LpArgs a) {
     }
 }
 
-// Slices of a row: enough workgroups for the chip (eight a CU), each wave a batch or more.
+// Slices of a row.  A row is one workgroup's from two rows a CU on, as slices
+// have a threshold and a list each and the launch that joins them (512 x 128256
+// fp32, five alternatives: 50 us whole, 54 halved, 55 in four; without a list
+// 43, 46, 48); fewer rows make three workgroups a CU (64 rows: 24 us with two,
+// 21 with three or four, 25 with eight).  Each wave has a batch or more.
 int64_t lp_splits(int64_t rows, int64_t vocab) {
-    const int64_t want = rows > 0 ? (8 * num_cus() + rows - 1) / rows : 1;
+    if (rows <= 0 || rows >= 2 * num_cus()) return 1;
+    const int64_t want = (3 * num_cus() + rows - 1) / rows;
     const int64_t most = (vocab + LP_THREADS * LP_BATCH - 1) / (LP_THREADS * LP_BATCH);
-    int64_t n = want < most ? want : most;
+    const int64_t n = want < most ? want : most;
     return n < LP_MAX_SPLIT ? n : LP_MAX_SPLIT;
 }
 
