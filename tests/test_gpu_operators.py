@@ -425,7 +425,7 @@ def test_group4_products_of_many_rows(rows, m):
 
 
 @pytest.mark.parametrize("dtype", [F32, F16, BF16])
-@pytest.mark.parametrize("m", [1, 3])
+@pytest.mark.parametrize("m", [1, 3, 8])
 def test_group4_activations_of_every_size(dtype, m):
     """Outliers, tiny and huge values, a row of zeros, subnormals: each block of 128 keeps its own precision."""
     k = 1024
@@ -445,6 +445,33 @@ def test_group4_activations_of_every_size(dtype, m):
     b = x64.abs().view(m, -1, 128).max(2, keepdim=True).values.expand(m, -1, 128).reshape(m, k)
     mag = x64.abs() @ w64.abs().T
     close(y, x64 @ w64.T, (4 * U + (k / 32 + 32) * U) * mag + 2.0 ** -38 * (b @ w64.abs().T))
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("m", [5, 6, 16])
+@pytest.mark.parametrize("zeros", [False, True])
+def test_group4_subnormal_activations(dtype, m, zeros):
+    """Every value below the type's smallest normal one; those are fp32's own subnormals in bf16."""
+    packed, s, z, w64 = parts(9, 40, 512, 64, zeros)
+    w = GroupQTensor.from_packed(packed, s, z, k=512, group=64)
+    f = torch.finfo(dtype)
+    x = (torch.from_numpy(np.random.default_rng(m).integers(-100, 101, (m, 512))).double() * (f.tiny * f.eps)).to(dtype)
+    assert (x != 0).any() and x.abs().double().max() < f.tiny
+    y = group_gemv(w, x.cuda())
+    mag = x.double().abs() @ w64.abs().T
+    close(y, x.double() @ w64.T, (4 * U + (512 / 32 + 32) * U) * mag + 2.0 ** -146)  # and sixteen roundings below the normal range
+
+
+def test_group4_activations_of_a_few_tokens_without_bounds_stay_in_theirs():
+    packed, s, z, w64 = parts(7, 50, 300, 64, True)
+    w = GroupQTensor.from_packed(packed, s, z, k=300, group=64)
+    for dtype in (F16, BF16):
+        x = normal(8, 9, 300, dtype=dtype)
+        x[1, 7], x[2, 299] = float("nan"), INF
+        y = group_gemv(w, x.cuda()).cpu()
+        assert torch.isnan(y[1]).all() and not torch.isfinite(y[2]).any()
+        rest = [0, 3, 4, 5, 6, 7, 8]
+        check_product(w, w64, x[rest], y[rest])
 
 
 def test_group4_activations_without_bounds_stay_in_their_token():

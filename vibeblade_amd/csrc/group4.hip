@@ -139,7 +139,14 @@ __global__ void __launch_bounds__(256) g4_quantize_kernel(const void* src, int32
 // of a token meet at the end.  A block with a NaN or an infinity has the power
 // NaN, which stays in its token.  Columns past the tokens repeat the last one
 // and are dropped.
-typedef _Float16 half4_t __attribute__((ext_vector_type(4)));
+//
+// More than a few 16-bit tokens would take two or three such sets of columns, so
+// they go to v_mfma_f32_16x16x32_f16 as they are, a column each: fp16 values
+// unchanged, bf16 ones brought to |x| < 2^15 by a power of two for each block of
+// 128 (exact down to 2^-29 of its largest, cut there to multiples of 2^-39 of
+// it).  The weights' codes become fp16 integers q - z, exactly; a group's
+// products are summed in fp32.
+typedef _Float16 half2_t __attribute__((ext_vector_type(2)));
 typedef _Float16 half8_t __attribute__((ext_vector_type(8)));
 typedef float float4_t __attribute__((ext_vector_type(4)));
 typedef int int4_t __attribute__((ext_vector_type(4)));
@@ -155,7 +162,7 @@ struct G4Args {
     float* partial;  // [chunk][token][row]: sums of a chunk, where there are several
     float* y;
     int64_t x_ld, rows, k;
-    int32_t x_type, parts;  // digits of a value
+    int32_t x_type, parts;  // digits of a value (1: fp16 operands)
     int32_t m;              // tokens of this launch
     int32_t ks;             // waves of a workgroup that share a row tile
     int32_t kz, chunk;      // chunks of k, each a workgroup's of its own, and their blocks
@@ -210,7 +217,7 @@ __device__ __forceinline__ void x_shift(XUnit<PARTS>& r, int by) {  // values `b
 #pragma unroll
         for (int i = 0; i < N; i++) r.u[i] = i + b < N ? r.u[i + b] : 0u;
     }
-    if (PARTS == 3 && (by & 1)) {
+    if (PARTS != 4 && (by & 1)) {
 #pragma unroll
         for (int i = 0; i < N; i++) r.u[i] = r.u[i] >> 16 | (i + 1 < N ? r.u[i + 1] << 16 : 0u);
     }
@@ -225,6 +232,9 @@ __device__ __forceinline__ int dpp_i(int v) {
 //   digits  [step][half][c][col] of 16 bytes: the B operand's bytes of k = 64 half + 8 c + 0..7 and + 32
 //   power   [step][token] the block's power of two (with the weights' 1/16 and the top digit's 256^(PARTS-1))
 //   sums    [step][group][col] -16 sum X
+// As fp16 operands
+//   digits  [step][t][c][token] of 16 bytes: the values of k = 32 t + 8 c + 0, 4, 1, 5, 2, 6, 3, 7
+//   power   [step][token] the block's power of two
 struct XImage {
     uint8_t* digits;
     float* power;
@@ -232,27 +242,54 @@ struct XImage {
 };
 
 // Bytes of a block's 256 k: digits, power and sums.
-__host__ __device__ constexpr int64_t digit_bytes(int64_t cols) { return 256 * cols; }
-__host__ __device__ constexpr int64_t table_bytes(int64_t cols, int64_t m, int64_t per, bool zeros) {
-    return 8 * m + (zeros ? 8 * per * cols : 0);
+__host__ __device__ constexpr int64_t digit_bytes(int64_t parts, int64_t m) { return parts == 1 ? 512 * m : 256 * parts * m; }
+__host__ __device__ constexpr int64_t table_bytes(int64_t parts, int64_t m, int64_t per, bool zeros) {
+    return 8 * m + (zeros && parts > 1 ? 8 * per * parts * m : 0);
 }
 
 // Bytes of a chunk in LDS and in the image.
-__host__ __device__ constexpr int64_t chunk_bytes(int64_t blocks, int64_t cols, int64_t m, int64_t per, bool zeros) {
-    return (blocks * (digit_bytes(cols) + table_bytes(cols, m, per, zeros)) + 15) / 16 * 16;
+__host__ __device__ constexpr int64_t chunk_bytes(int64_t blocks, int64_t parts, int64_t m, int64_t per, bool zeros) {
+    return (blocks * (digit_bytes(parts, m) + table_bytes(parts, m, per, zeros)) + 15) / 16 * 16;
 }
 
-__device__ __forceinline__ XImage x_image(uint8_t* at, int blocks, int cols, int m) {
+__device__ __forceinline__ XImage x_image(uint8_t* at, int blocks, int parts, int m) {
     XImage x;
     x.digits = at;
-    x.power = reinterpret_cast<float*>(at + digit_bytes(cols) * blocks);
+    x.power = reinterpret_cast<float*>(at + digit_bytes(parts, m) * blocks);
     x.sums = reinterpret_cast<int*>(x.power + 2 * blocks * m);
     return x;
 }
 
 // One piece (eight values; piece kc of the chunk, 16 to a block in 16 neighbouring lanes) of a token.
 template <int PARTS, int PER, bool ZEROS>
-__device__ __forceinline__ void x_store(const XUnit<PARTS>& r, const XImage& x, int type, int cols, int m, int token, int kc) {
+__device__ __forceinline__ void x_store(const XUnit<PARTS>& r, const XImage& x, int type, int m, int token, int kc) {
+    if constexpr (PARTS == 1) {
+        u32x4 h;  // values i and i + 4 side by side, as their codes come out of the weights
+#pragma unroll
+        for (int i = 0; i < 4; i++) h[i] = __builtin_amdgcn_perm(r.u[2 + i / 2], r.u[i / 2], i & 1 ? 0x07060302u : 0x05040100u);
+        float power = 1.f;
+        if (type == ELEM_BF16) {
+            typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+            u16x2 most = {0, 0};
+#pragma unroll
+            for (int i = 0; i < 4; i++) most = __builtin_elementwise_max(most, __builtin_bit_cast(u16x2, h[i] & 0x7fff7fffu));
+            int big = max(most[0], most[1]);
+            big = max(big, dpp_i<0xB1>(big));
+            big = max(big, dpp_i<0x4E>(big));
+            big = max(big, dpp_i<0x141>(big));
+            big = max(big, dpp_i<0x140>(big));
+            const int e = max(big >> 7, 1) - 127;  // |v| < 2^(e + 1)
+            power = big >= 0x7f80 ? NAN : __builtin_ldexpf(1.f, e - 14);
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+                h[i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(__builtin_ldexpf(__uint_as_float(h[i] << 16), 14 - e),
+                                                                               __builtin_ldexpf(__uint_as_float(h[i] & 0xffff0000u), 14 - e)));
+        }
+        *reinterpret_cast<u32x4*>(x.digits + kc * m * 16 + token * 16) = h;
+        if ((kc & 15) == 0) x.power[(kc >> 4) * m + token] = power;
+        return;
+    }
+    const int cols = PARTS * m;
     float v[8];
     if constexpr (PARTS == 4) {
 #pragma unroll
@@ -337,14 +374,14 @@ struct WBlock {
 // x of a launch as digits into the workspace, one thread per piece.
 template <int PER, bool ZEROS, int PARTS>
 __global__ void __launch_bounds__(256) g4_image_kernel(G4Args a) {
-    const int cols = PARTS * a.m, t = static_cast<int>(blockIdx.y);
+    const int t = static_cast<int>(blockIdx.y);
     const int64_t at = first_item();
     if (at >= a.l.blocks * 32) return;
     const int64_t z = at / (a.chunk * 32);
     const int64_t left = a.l.blocks - z * a.chunk;
     const int blocks = static_cast<int>(left < a.chunk ? left : a.chunk);
-    const XImage x = x_image(a.image + z * chunk_bytes(a.chunk, cols, a.m, PER, ZEROS), blocks, cols, a.m);
-    x_store<PARTS, PER, ZEROS>(x_load<PARTS, false>(a, t, at * 8), x, a.x_type, cols, a.m, t,
+    const XImage x = x_image(a.image + z * chunk_bytes(a.chunk, PARTS, a.m, PER, ZEROS), blocks, PARTS, a.m);
+    x_store<PARTS, PER, ZEROS>(x_load<PARTS, false>(a, t, at * 8), x, a.x_type, a.m, t,
                                static_cast<int>(at - z * a.chunk * 32));
 }
 
@@ -354,11 +391,13 @@ enum { G4_SELF, G4_COPY };
 constexpr int G4_DEPTH = 2;  // blocks in flight per wave
 
 // Kernels that take the registers of 8 waves a CU, not 16.
-__host__ __device__ constexpr bool g4_wide(int nt, int per, bool zeros) { return nt > 1 || (per == 4 && zeros); }
+__host__ __device__ constexpr bool g4_wide(int parts, int nt, int per, bool zeros) {
+    return nt > 1 || (per == 4 && (zeros || parts == 1));
+}
 
 // PARTS 0: a.parts (no code but the staging depends on it).
 template <int PER, bool ZEROS, int PARTS, int NT, int MODE>
-__global__ void __launch_bounds__(64 * G4_WAVES, g4_wide(NT, PER, ZEROS) ? 2 : 4) g4_gemv_kernel(G4Args a) {
+__global__ void __launch_bounds__(64 * G4_WAVES, g4_wide(PARTS, NT, PER, ZEROS) ? 2 : 4) g4_gemv_kernel(G4Args a) {
     constexpr int DEPTH = G4_DEPTH;
     extern __shared__ uint4 lds[];
     const int tid = static_cast<int>(threadIdx.x), lane = tid & 63, n = lane & 15, c = lane >> 4;
@@ -366,14 +405,14 @@ __global__ void __launch_bounds__(64 * G4_WAVES, g4_wide(NT, PER, ZEROS) ? 2 : 4
     const int waves = static_cast<int>(blockDim.x) >> 6, threads = static_cast<int>(blockDim.x);
     const int parts = PARTS ? PARTS : a.parts, m = a.m, cols = parts * m;
     const int ks = a.ks, sub = wave % ks, local = wave / ks, per_group = waves / ks;
-    const int kz = MODE == G4_SELF ? 1 : a.kz, z = static_cast<int>(blockIdx.x) % kz;
+    const int kz = MODE == G4_SELF && PARTS != 1 ? 1 : a.kz, z = static_cast<int>(blockIdx.x) % kz;
     const int turn = static_cast<int>(blockIdx.x) / kz, turns = static_cast<int>(gridDim.x) / kz;
     const int64_t row_blocks = a.l.blocks, first = static_cast<int64_t>(z) * a.chunk;
     const int tiles = static_cast<int>(a.l.tiles);
     const int blocks = static_cast<int>(row_blocks - first < a.chunk ? row_blocks - first : a.chunk);
     float4_t* red = reinterpret_cast<float4_t*>(lds);  // [wave][nt][lane]
     uint8_t* const mine = reinterpret_cast<uint8_t*>(lds + waves * NT * 64);
-    const XImage x = x_image(mine, blocks, cols, m);
+    const XImage x = x_image(mine, blocks, parts, m);
 
     int col[NT], token[NT];
 #pragma unroll
@@ -399,7 +438,7 @@ __global__ void __launch_bounds__(64 * G4_WAVES, g4_wide(NT, PER, ZEROS) ? 2 : 4
 #pragma unroll
         for (int g = 0; g < PER; g++) r.s[g] = __builtin_bit_cast(half8_t, ld(2048 + c * (16 * PER) + 16 * g));
         if constexpr (ZEROS) {
-            const uint32_t zo = 2048 + 64 * PER + c * (4 * PER);
+            const uint32_t zo = 2048 + 64 * PER + (PARTS == 1 ? n >> 2 : c) * (4 * PER);
             if constexpr (PER == 4) {
                 const u32x4 v = ld(zo);
 #pragma unroll
@@ -415,6 +454,51 @@ __global__ void __launch_bounds__(64 * G4_WAVES, g4_wide(NT, PER, ZEROS) ? 2 : 4
         __builtin_amdgcn_sched_barrier(0);  // slot after slot, as they are waited for
     };
     float4_t acc[NT];
+    // Half `from` of a block with fp16 operands.  A code q is made from the bits
+    // of 1024 + q, or where it lies four bits higher of 1024 + 16 q, and its zero
+    // point taken off, two at a time and exactly.
+    auto multiply_half = [&](const WBlock<PER, ZEROS>& r, int from, int at) __attribute__((always_inline)) {
+        const int step = 2 * at + from;
+        const uint4* xs = reinterpret_cast<const uint4*>(x.digits) + (step * 16 + c) * m + col[0];
+        half8_t xv[4];
+#pragma unroll
+        for (int t = 0; t < 4; t++) xv[t] = __builtin_bit_cast(half8_t, xs[4 * t * m]);
+        const float f = x.power[step * m + token[0]];
+        float4_t p[PER];
+#pragma unroll
+        for (int t = 0; t < 4; t++) {
+            const int g = t * PER / 4, gb = from * PER + g;
+            uint32_t low = 0xe408e408u, high = 0xd480d480u;  // -(1024 + z), -(64 + z)
+            if constexpr (ZEROS) {
+                const uint32_t zz = ((r.z[gb >> 1] >> ((gb & 1) * 16 + (n & 3) * 4)) & 15) * 0x10001u;
+                low ^= zz;
+                high ^= zz << 4;
+            }
+            half8_t wv;
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const uint32_t word = r.q[from][t] >> (i & 2) * 4;
+                const uint32_t bits = i & 1 ? (word & 0x00f000f0u) ^ 0x64806480u : (word & 0x000f000fu) ^ 0x64086408u;
+                const half2_t v = __builtin_bit_cast(half2_t, bits);
+                const half2_t w = i & 1 ? __builtin_elementwise_fma(v, half2_t{0x1p-4f16, 0x1p-4f16}, __builtin_bit_cast(half2_t, high))
+                                        : v + __builtin_bit_cast(half2_t, low);
+                wv[2 * i] = w[0];
+                wv[2 * i + 1] = w[1];
+            }
+            const float4_t before = t * PER % 4 == 0 ? float4_t{0.f, 0.f, 0.f, 0.f} : p[g];
+            p[g] = __builtin_amdgcn_mfma_f32_16x16x32_f16(wv, xv[t], before, 0, 0, 0);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            float sum = 0.f;
+#pragma unroll
+            for (int g = 0; g < PER; g++) {
+                const int gb = from * PER + g;
+                sum = __builtin_fmaf(static_cast<float>(r.s[gb >> 1][(gb & 1) * 4 + i]), p[g][i], sum);
+            }
+            acc[0][i] = __builtin_fmaf(f, sum, acc[0][i]);
+        }
+    };
     // H halves of a block from half `from` on.
     auto multiply = [&](auto halves, const WBlock<PER, ZEROS>& r, int from, int at) __attribute__((always_inline)) {
         constexpr int H = decltype(halves)::value;
@@ -512,38 +596,54 @@ __global__ void __launch_bounds__(64 * G4_WAVES, g4_wide(NT, PER, ZEROS) ? 2 : 4
     // x first, as loads come back in order: what a thread cannot hold, then the
     // rest of it on the way together with the ring's first round.
     if constexpr (MODE == G4_SELF) {
-        constexpr int HELD = 4;
+        constexpr int HELD = PARTS == 1 ? 8 : 4;
         XUnit<PARTS> held[HELD];
         const int pieces = blocks * 32, units = pieces * m;  // of a token, of all
-        const bool hold = a.k >= 8;
-#pragma unroll 1
-        for (int u = (hold ? HELD * threads : 0) + tid; u < units; u += threads) {
-            const int t = m == 1 ? 0 : u / pieces, kc = u - t * pieces;
-            x_store<PARTS, PER, ZEROS>(x_load<PARTS, false>(a, t, kc * 8), x, a.x_type, cols, m, t, kc);
-        }
-        if (hold) {
+        const int64_t k0 = first * GROUP4_K;
+        const float share = 1.f / static_cast<float>(pieces);
+        const auto token_of = [&](int u) __attribute__((always_inline)) {  // u / pieces: u < 2^14, so half a piece is more than the rounding
+            return m == 1 ? 0 : static_cast<int>((static_cast<float>(u) + 0.5f) * share);
+        };
+        const auto get = [&](int base) __attribute__((always_inline)) {
 #pragma unroll
             for (int i = 0; i < HELD; i++) {
-                const int u = i * threads + tid, v = u < units ? u : units - 1, t = m == 1 ? 0 : v / pieces;
-                held[i] = x_load<PARTS, true>(a, t, static_cast<int64_t>(v - t * pieces) * 8);
+                const int u = base + i * threads + tid, v = u < units ? u : units - 1, t = token_of(v);
+                held[i] = x_load<PARTS, true>(a, t, k0 + static_cast<int64_t>(v - t * pieces) * 8);
             }
-        }
-        fill();
-        if (hold) {
+        };
+        const auto put = [&](int base) __attribute__((always_inline)) {
 #pragma unroll
             for (int i = 0; i < HELD; i++) {
-                const int u = i * threads + tid;
+                const int u = base + i * threads + tid;
                 if (u >= units) continue;
-                const int t = m == 1 ? 0 : u / pieces, kc = u - t * pieces;
-                if (kc * 8 + 8 > a.k) x_shift<PARTS>(held[i], static_cast<int>(kc * 8 >= a.k ? 8 : kc * 8 + 8 - a.k));
-                x_store<PARTS, PER, ZEROS>(held[i], x, a.x_type, cols, m, t, kc);
+                const int t = token_of(u), kc = u - t * pieces;
+                const int64_t at = k0 + kc * 8;
+                if (at + 8 > a.k) x_shift<PARTS>(held[i], static_cast<int>(at >= a.k ? 8 : at + 8 - a.k));
+                x_store<PARTS, PER, ZEROS>(held[i], x, a.x_type, m, t, kc);
             }
+        };
+        if (a.k >= 8) {
+            int base = 0;
+#pragma unroll 1
+            for (; base + HELD * threads < units; base += HELD * threads) {
+                get(base);
+                put(base);
+            }
+            get(base);
+            fill();
+            put(base);
+        } else {
+            for (int u = tid; u < units; u += threads) {
+                const int t = u / pieces, kc = u - t * pieces;
+                x_store<PARTS, PER, ZEROS>(x_load<PARTS, false>(a, t, kc * 8), x, a.x_type, m, t, kc);
+            }
+            fill();
         }
     } else {
         constexpr int HELD = 8;
-        const u32x4* from = reinterpret_cast<const u32x4*>(a.image + z * chunk_bytes(a.chunk, cols, m, PER, ZEROS));
+        const u32x4* from = reinterpret_cast<const u32x4*>(a.image + z * chunk_bytes(a.chunk, parts, m, PER, ZEROS));
         u32x4* to = reinterpret_cast<u32x4*>(mine);
-        const int count = static_cast<int>(chunk_bytes(blocks, cols, m, PER, ZEROS) / 16);
+        const int count = static_cast<int>(chunk_bytes(blocks, parts, m, PER, ZEROS) / 16);
         u32x4 held[HELD];
         const auto get = [&](int base) __attribute__((always_inline)) {
 #pragma unroll
@@ -579,7 +679,10 @@ __global__ void __launch_bounds__(64 * G4_WAVES, g4_wide(NT, PER, ZEROS) ? 2 : 4
 #pragma unroll
             for (int d = 0; d < DEPTH; d++) {
                 if (tile < tiles && s + d * ks < blocks) {
-                    if constexpr (NT == 1 && PER == 1) {
+                    if constexpr (PARTS == 1) {
+                        multiply_half(ring[d], 0, s + d * ks);
+                        multiply_half(ring[d], 1, s + d * ks);
+                    } else if constexpr (NT == 1 && PER == 1) {
                         multiply(std::integral_constant<int, 2>{}, ring[d], 0, s + d * ks);
                     } else {
                         multiply(std::integral_constant<int, 1>{}, ring[d], 0, s + d * ks);
@@ -632,7 +735,7 @@ constexpr int G4_COLS = 48;  // columns of a launch, at most
 
 // How a launch of m tokens runs.
 struct G4Plan {
-    int mode, nt, ks, waves;
+    int mode, parts, nt, ks, waves;
     int64_t kz, chunk, groups;
     int64_t lds;
     int64_t partial, workspace;  // byte offset of the chunks' sums behind the image, bytes in all
@@ -640,10 +743,18 @@ struct G4Plan {
 
 G4Plan g4_plan(const Group4Layout& l, int64_t rows, int64_t m, int x_type, bool has_zeros) {
     G4Plan p{};
-    const int64_t cols = (x_type == ELEM_F32 ? 4 : 3) * m;
-    p.nt = static_cast<int>((cols + 15) / 16);
+    // Tokens of 16 bits as fp16 operands: from the sixth on, whose digits take a
+    // second set of columns (six to sixteen tokens of 14336 x 4096: 20 us as
+    // digits, 13.3 so); and fp16 tokens from the third where what a workgroup
+    // stages counts for more than what it decodes, at up to four row tiles a CU
+    // (digits and fp16: 14336 x 4096, two tokens 9.3 and 9.9 us, four 10.5 and
+    // 10.1; 4096 x 4096, three 8.2 and 6.4; 4096 x 14336, five 15.2 and 13.7;
+    // 128256 x 4096, five 56.8 and 62.8).  bf16 tokens take longer to stage
+    // (three 10.0 and 10.7, five of 4096 x 14336 15.1 and 16.0).
+    p.parts = x_type == ELEM_F32 ? 4 : m > 5 || (x_type == ELEM_F16 && m > 2 && l.tiles <= 4 * num_cus()) ? 1 : 3;
+    p.nt = static_cast<int>((p.parts * m + 15) / 16);
     // Chunks of k whose digits fit into LDS beside the sums.
-    const int64_t room = G4_LDS - G4_WAVES * p.nt * 1024 - 16, block = digit_bytes(cols) + table_bytes(cols, m, l.per, has_zeros);
+    const int64_t room = G4_LDS - G4_WAVES * p.nt * 1024 - 16, block = digit_bytes(p.parts, m) + table_bytes(p.parts, m, l.per, has_zeros);
     p.kz = (l.blocks * block + room - 1) / room;
     // where there are several, as many as give every CU a workgroup (4096 x 14336, eight fp16 tokens: 3 chunks 21.3 us, 4 18.8)
     const int64_t even = (4 * num_cus() + l.tiles - 1) / l.tiles;
@@ -651,7 +762,7 @@ G4Plan g4_plan(const Group4Layout& l, int64_t rows, int64_t m, int x_type, bool 
     if (p.kz > l.blocks) p.kz = l.blocks;
     p.chunk = (l.blocks + p.kz - 1) / p.kz;
     p.kz = (l.blocks + p.chunk - 1) / p.chunk;
-    p.mode = p.kz == 1 && p.nt == 1 && m * l.blocks * GROUP4_K <= G4_SELF_VALUES ? G4_SELF : G4_COPY;
+    p.mode = p.parts == 1 || (p.kz == 1 && p.nt == 1 && m * l.blocks * GROUP4_K <= G4_SELF_VALUES) ? G4_SELF : G4_COPY;
     // A tile is shared by as many waves as leave each four blocks, up to eight
     // waves a CU: more of them cost more in x staged and sums joined than they
     // bring in loads in flight (14336 x 4096, one token: ks 1 to 8 take 9.7,
@@ -659,10 +770,11 @@ G4Plan g4_plan(const Group4Layout& l, int64_t rows, int64_t m, int x_type, bool 
     p.ks = 1;
     while (p.ks < G4_WAVES && l.tiles * p.kz * p.ks * 2 <= 8 * num_cus() && p.chunk >= 8 * p.ks) p.ks *= 2;
     // workgroups of four waves where eight would leave a quarter of the CUs without one
-    p.waves = p.ks <= 4 && l.tiles * p.kz * p.ks < 6 * num_cus() ? 4 : G4_WAVES;
+    // (fp16 operands are quick to multiply, and all eight stage them: 1024 x 4096, eight tokens 9.4 us and 8.8)
+    p.waves = p.parts != 1 && p.ks <= 4 && l.tiles * p.kz * p.ks < 6 * num_cus() ? 4 : G4_WAVES;
     p.groups = (l.tiles * p.ks + p.waves - 1) / p.waves;
-    p.lds = p.waves * p.nt * 1024 + chunk_bytes(p.chunk, cols, m, l.per, has_zeros);
-    p.workspace = p.mode == G4_SELF ? 0 : p.kz * chunk_bytes(p.chunk, cols, m, l.per, has_zeros);
+    p.lds = p.waves * p.nt * 1024 + chunk_bytes(p.chunk, p.parts, m, l.per, has_zeros);
+    p.workspace = p.mode == G4_SELF ? 0 : p.kz * chunk_bytes(p.chunk, p.parts, m, l.per, has_zeros);
     if (p.kz > 1) {
         p.partial = p.workspace;
         p.workspace += (p.kz * m * rows * 4 + 15) / 16 * 16;
@@ -674,17 +786,18 @@ template <int PER, bool ZEROS>
 int g4_launch(const G4Args& a, const G4Plan& p, uint32_t grid, hipStream_t st) {
     const uint32_t threads = 64 * p.waves, lds = static_cast<uint32_t>(p.lds);
     if (p.mode == G4_SELF) {
-        if (a.parts == 4) g4_gemv_kernel<PER, ZEROS, 4, 1, G4_SELF><<<grid, threads, lds, st>>>(a);
+        if (a.parts == 1) g4_gemv_kernel<PER, ZEROS, 1, 1, G4_SELF><<<grid, threads, lds, st>>>(a);
+        else if (a.parts == 4) g4_gemv_kernel<PER, ZEROS, 4, 1, G4_SELF><<<grid, threads, lds, st>>>(a);
         else g4_gemv_kernel<PER, ZEROS, 3, 1, G4_SELF><<<grid, threads, lds, st>>>(a);
-        return check_launch("vb_group4_gemv");
+    } else {
+        const dim3 pieces(static_cast<uint32_t>((a.l.blocks * 32 + 255) / 256), static_cast<uint32_t>(a.m));
+        if (a.parts == 4) g4_image_kernel<PER, ZEROS, 4><<<pieces, 256, 0, st>>>(a);
+        else g4_image_kernel<PER, ZEROS, 3><<<pieces, 256, 0, st>>>(a);
+        if (const int rc = check_launch("vb_group4_gemv"); rc != OK) return rc;
+        if (p.nt == 1) g4_gemv_kernel<PER, ZEROS, 0, 1, G4_COPY><<<grid, threads, lds, st>>>(a);
+        else if (p.nt == 2) g4_gemv_kernel<PER, ZEROS, 0, 2, G4_COPY><<<grid, threads, lds, st>>>(a);
+        else g4_gemv_kernel<PER, ZEROS, 0, 3, G4_COPY><<<grid, threads, lds, st>>>(a);
     }
-    const dim3 pieces(static_cast<uint32_t>((a.l.blocks * 32 + 255) / 256), static_cast<uint32_t>(a.m));
-    if (a.parts == 4) g4_image_kernel<PER, ZEROS, 4><<<pieces, 256, 0, st>>>(a);
-    else g4_image_kernel<PER, ZEROS, 3><<<pieces, 256, 0, st>>>(a);
-    if (const int rc = check_launch("vb_group4_gemv"); rc != OK) return rc;
-    if (p.nt == 1) g4_gemv_kernel<PER, ZEROS, 0, 1, G4_COPY><<<grid, threads, lds, st>>>(a);
-    else if (p.nt == 2) g4_gemv_kernel<PER, ZEROS, 0, 2, G4_COPY><<<grid, threads, lds, st>>>(a);
-    else g4_gemv_kernel<PER, ZEROS, 0, 3, G4_COPY><<<grid, threads, lds, st>>>(a);
     if (p.kz > 1) {
         if (const int rc = check_launch("vb_group4_gemv"); rc != OK) return rc;
         g4_join_kernel<<<item_blocks(a.rows * a.m), 256, 0, st>>>(a.partial, a.y, a.rows * a.m, a.kz);
@@ -696,13 +809,13 @@ int g4_run(G4Args a, bool has_zeros, uint8_t* workspace, hipStream_t st) {
     const G4Plan p = g4_plan(a.l, a.rows, a.m, a.x_type, has_zeros);
     a.image = workspace;
     a.partial = reinterpret_cast<float*>(workspace + p.partial);
-    a.parts = a.x_type == ELEM_F32 ? 4 : 3;
+    a.parts = p.parts;
     a.ks = p.ks;
     a.kz = static_cast<int32_t>(p.kz);
     a.chunk = static_cast<int32_t>(p.chunk);
     a.groups = static_cast<int32_t>(p.groups);
     // as many workgroups as are resident at once (16 waves a CU or 8), a share for every chunk
-    const int64_t fit = G4_LDS / p.lds, want = (g4_wide(p.nt, a.l.per, has_zeros) ? 8 : 16) / p.waves;
+    const int64_t fit = G4_LDS / p.lds, want = (g4_wide(p.parts, p.nt, a.l.per, has_zeros) ? 8 : 16) / p.waves;
     const int64_t most = ((fit < want ? fit : want) * num_cus() + p.kz - 1) / p.kz;
     const uint32_t grid = static_cast<uint32_t>(p.kz * (p.groups < most ? p.groups : most));
     if (a.l.per == 1) return has_zeros ? g4_launch<1, true>(a, p, grid, st) : g4_launch<1, false>(a, p, grid, st);
