@@ -596,7 +596,9 @@ __global__ void __launch_bounds__(64 * G4_WAVES, g4_wide(PARTS, NT, PER, ZEROS) 
     // x first, as loads come back in order: what a thread cannot hold, then the
     // rest of it on the way together with the ring's first round.
     if constexpr (MODE == G4_SELF) {
-        constexpr int HELD = PARTS == 1 ? 8 : 4;
+        // Digits take long code, which a launch fetches anew: two at a time (one, two
+        // and four: 4096 x 4096, one token 6.3, 5.9 and 6.1 us).
+        constexpr int HELD = PARTS == 1 ? 8 : 2;
         XUnit<PARTS> held[HELD];
         const int pieces = blocks * 32, units = pieces * m;  // of a token, of all
         const int64_t k0 = first * GROUP4_K;
@@ -770,8 +772,7 @@ G4Plan g4_plan(const Group4Layout& l, int64_t rows, int64_t m, int x_type, bool 
     p.ks = 1;
     while (p.ks < G4_WAVES && l.tiles * p.kz * p.ks * 2 <= 8 * num_cus() && p.chunk >= 8 * p.ks) p.ks *= 2;
     // workgroups of four waves where eight would leave a quarter of the CUs without one
-    // (fp16 operands are quick to multiply, and all eight stage them: 1024 x 4096, eight tokens 9.4 us and 8.8)
-    p.waves = p.parts != 1 && p.ks <= 4 && l.tiles * p.kz * p.ks < 6 * num_cus() ? 4 : G4_WAVES;
+    p.waves = p.ks <= 4 && l.tiles * p.kz * p.ks < 6 * num_cus() ? 4 : G4_WAVES;
     p.groups = (l.tiles * p.ks + p.waves - 1) / p.waves;
     p.lds = p.waves * p.nt * 1024 + chunk_bytes(p.chunk, p.parts, m, l.per, has_zeros);
     p.workspace = p.mode == G4_SELF ? 0 : p.kz * chunk_bytes(p.chunk, p.parts, m, l.per, has_zeros);
