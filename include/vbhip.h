@@ -435,9 +435,11 @@ int vb_group4_dequant_rows(const void* w, float* out, int64_t rows, int64_t k, i
 /* y[t * rows + n] = sum_i W[n, i] x[t, i] for the m activation rows of x (row
  * stride x_ld, element type as above), fp32.  Per token and 128 consecutive k,
  * activations are taken as integers of 30 bits (fp32) or 22 bits (fp16, bf16)
- * below a power of two that holds the largest of them, the products with the
- * codes are summed exactly in a group, and groups in fp32.  A token with a NaN
- * or an infinity gives NaN.  workspace: at least vb_group4_workspace(...) bytes
+ * below a power of two that holds the largest of them, and the products with
+ * the codes are summed exactly in a group; or, where there are several tokens
+ * of 16 bits, as fp16 values below such a power (fp16 ones as they are), summed
+ * in fp32.  Groups are summed in fp32.  A NaN or an infinity gives its token NaN
+ * or infinities, no other one.  workspace: at least vb_group4_workspace(...) bytes
  * (0: none), 16-byte aligned, free again when the call's work is done. */
 int64_t vb_group4_workspace(int64_t m, int64_t rows, int64_t k, int32_t group, int32_t has_zeros, int32_t x_type);
 int vb_group4_gemv(const void* w, int64_t rows, int64_t k, int32_t group, int32_t has_zeros, const void* x,

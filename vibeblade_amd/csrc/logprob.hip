@@ -52,7 +52,7 @@ struct LpArgs {
     int32_t* top_ids;
     float* top_lp;
     float4* stats;    // [row][split]: m, S, sum (workspace)
-    uint64_t* keys;   // [row][split][top]
+    uint64_t* keys;   // [row][place][split]
     int64_t ld, rows;
     int32_t vocab, token_bytes, n_tokens, top, splits;
     float c, inv_t;   // log2(e) / T, 1 / T
@@ -476,24 +476,36 @@ __global__ void __launch_bounds__(LP_THREADS) logprob_kernel(LpArgs a) {
                 write_row<TYPE>(a, row, RowResult(all, a.inv_t), bufs[0], LIST ? w.best.count : 0);
             } else {
                 if (lane == 0) a.stats[item] = make_float4(all.m, all.s, all.t, 0.f);
-                if (LIST && lane < a.top) a.keys[item * a.top + lane] = lane < w.best.count ? bufs[0][lane] : 0;
+                if (LIST && lane < a.top)
+                    a.keys[(row * a.top + lane) * a.splits + split] = lane < w.best.count ? bufs[0][lane] : 0;
             }
         }
         __syncthreads();  // bufs and stats are free
     }
 }
 
-// One wave: the slices of a row.  Their lists are in order, so once no slice's
-// j-th candidate is wanted none behind it is.
+// One wave: the slices of a row.  Their lists are in order and lie place by
+// place, so once no slice's candidate of a place is wanted none behind it is.
+// Eight candidates a lane come at once (slice by slice, four places at a time:
+// eight rows of 32003 with 64 alternatives 25.9 us a call, so 18.2; 200 rows of
+// 32000 with 20 alternatives 22.2 and 19.1).
 template <int TYPE, bool LIST>
 __global__ void __launch_bounds__(64) logprob_join_kernel(LpArgs a) {
     __shared__ uint64_t buf[LP_BUF];
     const int lane = static_cast<int>(threadIdx.x);
     for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
-        const int64_t item = row * a.splits + lane;
+        constexpr int BATCH = 8;
+        uint64_t key[BATCH];
+        const uint64_t* list = a.keys + row * a.top * a.splits;
+        const int total = a.top * a.splits;
+        const auto load = [&](int base) __attribute__((always_inline)) {
+#pragma unroll
+            for (int i = 0; i < BATCH; i++) key[i] = base + i * 64 + lane < total ? list[base + i * 64 + lane] : 0;
+        };
+        if constexpr (LIST) load(0);
         Stat v{-INFINITY, 0.f, 0.f};
         if (lane < a.splits) {
-            const float4 p = a.stats[item];
+            const float4 p = a.stats[row * a.splits + lane];
             v = Stat{p.x, p.y, p.z};
         }
         const Stat all = join(v, a.c);
@@ -501,22 +513,23 @@ __global__ void __launch_bounds__(64) logprob_join_kernel(LpArgs a) {
         if constexpr (LIST) {
             // At least `top` candidates reach the q-th of every slice, q slices'
             // worth of them being enough, or (q = 1) a bisection of the firsts.
-            const uint64_t* list = a.keys + item * a.top;
             const int q = (a.top + a.splits - 1) / a.splits;
-            const uint64_t qth = lane < a.splits ? list[q - 1] : 0;
+            const uint64_t qth = lane < a.splits ? list[(q - 1) * a.splits + lane] : 0;
             const uint32_t o[1] = {static_cast<uint32_t>(qth >> 32)};
             const uint32_t at = reached_by(o, q == 1 ? a.top : a.splits);
             best.tau = order_floor(at);
-            for (int j = 0; j < a.top; j += 4) {
-                uint64_t key[4];
-#pragma unroll
-                for (int i = 0; i < 4; i++) key[i] = lane < a.splits && j + i < a.top ? list[j + i] : 0;
+            for (int base = 0; base < total;) {
+                uint64_t k = key[0];
 #pragma unroll 1
-                for (int i = 0; i < 4; i++) {
-                    const uint64_t k = i == 0 ? key[0] : i == 1 ? key[1] : i == 2 ? key[2] : key[3];
+                for (int i = 0; i < BATCH; i++) {
                     best.append(k, k != 0 && key_value(k) >= best.tau);
+#pragma unroll
+                    for (int j = 1; j < BATCH; j++) k = i + 1 == j ? key[j] : k;
                 }
-                if (!__any(key[3] != 0 && key_value(key[3]) >= best.tau)) break;
+                // the last place that is here from every slice
+                if (!__any(lane >= 64 - a.splits && key[BATCH - 1] != 0 && key_value(key[BATCH - 1]) >= best.tau)) break;
+                base += 64 * BATCH;
+                load(base);
             }
             best.rank();
         }
