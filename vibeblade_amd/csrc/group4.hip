@@ -233,7 +233,8 @@ __device__ __forceinline__ int dpp_i(int v) {
 //   power   [step][token] the block's power of two (with the weights' 1/16 and the top digit's 256^(PARTS-1))
 //   sums    [step][group][col] -16 sum X
 // As fp16 operands
-//   digits  [step][t][c][token] of 16 bytes: the values of k = 32 t + 8 c + 0, 4, 1, 5, 2, 6, 3, 7
+//   digits  [step][t][c][token, of an odd number] of 16 bytes: the values of k = 32 t + 8 c + 0, 4, 1, 5, 2, 6, 3, 7
+//           (an odd number: neighbouring lanes store neighbouring k, and meet different banks)
 //   power   [step][token] the block's power of two
 struct XImage {
     uint8_t* digits;
@@ -242,7 +243,7 @@ struct XImage {
 };
 
 // Bytes of a block's 256 k: digits, power and sums.
-__host__ __device__ constexpr int64_t digit_bytes(int64_t parts, int64_t m) { return parts == 1 ? 512 * m : 256 * parts * m; }
+__host__ __device__ constexpr int64_t digit_bytes(int64_t parts, int64_t m) { return parts == 1 ? 512 * (m | 1) : 256 * parts * m; }
 __host__ __device__ constexpr int64_t table_bytes(int64_t parts, int64_t m, int64_t per, bool zeros) {
     return 8 * m + (zeros && parts > 1 ? 8 * per * parts * m : 0);
 }
@@ -285,7 +286,7 @@ __device__ __forceinline__ void x_store(const XUnit<PARTS>& r, const XImage& x, 
                 h[i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(__builtin_ldexpf(__uint_as_float(h[i] << 16), 14 - e),
                                                                                __builtin_ldexpf(__uint_as_float(h[i] & 0xffff0000u), 14 - e)));
         }
-        *reinterpret_cast<u32x4*>(x.digits + kc * m * 16 + token * 16) = h;
+        *reinterpret_cast<u32x4*>(x.digits + (kc * (m | 1) + token) * 16) = h;
         if ((kc & 15) == 0) x.power[(kc >> 4) * m + token] = power;
         return;
     }
@@ -459,10 +460,10 @@ __global__ void __launch_bounds__(64 * G4_WAVES, g4_wide(PARTS, NT, PER, ZEROS) 
     // point taken off, two at a time and exactly.
     auto multiply_half = [&](const WBlock<PER, ZEROS>& r, int from, int at) __attribute__((always_inline)) {
         const int step = 2 * at + from;
-        const uint4* xs = reinterpret_cast<const uint4*>(x.digits) + (step * 16 + c) * m + col[0];
+        const uint4* xs = reinterpret_cast<const uint4*>(x.digits) + (step * 16 + c) * (m | 1) + col[0];
         half8_t xv[4];
 #pragma unroll
-        for (int t = 0; t < 4; t++) xv[t] = __builtin_bit_cast(half8_t, xs[4 * t * m]);
+        for (int t = 0; t < 4; t++) xv[t] = __builtin_bit_cast(half8_t, xs[4 * t * (m | 1)]);
         const float f = x.power[step * m + token[0]];
         float4_t p[PER];
 #pragma unroll
