@@ -34,7 +34,13 @@ struct SeamArgs {
     float scale, eps;
 };
 
+// Where element i of a tensor is.
+__device__ __forceinline__ uint8_t* elem_at(const void* p, int64_t i, int type) {
+    return static_cast<uint8_t*>(const_cast<void*>(p)) + i * (type == ELEM_F32 ? 4 : 2);
+}
+
 // ---- four neighbouring values; rows begin at any element ---------------------
+// (a row is the same in all of a wave: one address and an offset of 32 bits a lane)
 
 template <int TYPE>
 struct Piece {
@@ -44,17 +50,17 @@ struct Piece {
 // ONCE: past the caches' usual order, as this launch is the last to read it
 // (8192 x 4096 fp32: 84 to 78 us, 4096 x 8192: 106 to 88).
 template <int TYPE, bool ONCE = false>
-__device__ __forceinline__ Piece<TYPE> piece_ld(const void* p, int64_t i) {
+__device__ __forceinline__ Piece<TYPE> piece_ld(const void* p, uint32_t i) {
     Piece<TYPE> r;
     if constexpr (TYPE == ELEM_F32) {
         typedef uint32_t v4 __attribute__((ext_vector_type(4), aligned(4)));
-        const v4* q = reinterpret_cast<const v4*>(static_cast<const float*>(p) + i);
+        const v4* q = reinterpret_cast<const v4*>(static_cast<const uint8_t*>(p) + i * 4);
         const v4 v = ONCE ? __builtin_nontemporal_load(q) : *q;
 #pragma unroll
         for (int j = 0; j < 4; j++) r.u[j] = v[j];
     } else {
         typedef uint32_t v2 __attribute__((ext_vector_type(2), aligned(2)));
-        const v2* q = reinterpret_cast<const v2*>(static_cast<const uint16_t*>(p) + i);
+        const v2* q = reinterpret_cast<const v2*>(static_cast<const uint8_t*>(p) + i * 2);
         const v2 v = ONCE ? __builtin_nontemporal_load(q) : *q;
         r.u[0] = v[0];
         r.u[1] = v[1];
@@ -70,10 +76,10 @@ __device__ __forceinline__ float piece_at(const Piece<TYPE>& r, int j) {
 }
 
 template <int TYPE>
-__device__ __forceinline__ void piece_st(void* p, int64_t i, const float* v) {
+__device__ __forceinline__ void piece_st(void* p, uint32_t i, const float* v) {
     if constexpr (TYPE == ELEM_F32) {
         typedef float v4 __attribute__((ext_vector_type(4), aligned(4)));
-        *reinterpret_cast<v4*>(static_cast<float*>(p) + i) = v4{v[0], v[1], v[2], v[3]};
+        *reinterpret_cast<v4*>(static_cast<uint8_t*>(p) + i * 4) = v4{v[0], v[1], v[2], v[3]};
     } else {
         typedef uint32_t v2 __attribute__((ext_vector_type(2), aligned(2)));
         uint32_t u[2];
@@ -86,7 +92,7 @@ __device__ __forceinline__ void piece_st(void* p, int64_t i, const float* v) {
                 u[j] = f32_bf16x2(v[2 * j], v[2 * j + 1]);
             }
         }
-        *reinterpret_cast<v2*>(static_cast<uint16_t*>(p) + i) = v2{u[0], u[1]};
+        *reinterpret_cast<v2*>(static_cast<uint8_t*>(p) + i * 2) = v2{u[0], u[1]};
     }
 }
 
@@ -104,14 +110,14 @@ __device__ __forceinline__ float wg_sum(float v, float* part) {
 }
 
 // Four neighbouring values of the gate as they lie (gate_col 1), or its one value of the row.
-__device__ __forceinline__ Piece<ELEM_F32> gate_ld(const SeamArgs& a, int64_t go, int at) {
+__device__ __forceinline__ Piece<ELEM_F32> gate_ld(const SeamArgs& a, const void* gate, uint32_t at) {
     Piece<ELEM_F32> g;
     if (a.gate_col == 0) {
-        g.u[0] = __float_as_uint(elem_ld(a.gate, go, a.gate_type));
+        g.u[0] = __float_as_uint(elem_ld(gate, 0, a.gate_type));
     } else if (a.gate_type == ELEM_F32) {
-        g = piece_ld<ELEM_F32, true>(a.gate, go + at);
+        g = piece_ld<ELEM_F32, true>(gate, at);
     } else {
-        const Piece<ELEM_F16> h = piece_ld<ELEM_F16, true>(a.gate, go + at);
+        const Piece<ELEM_F16> h = piece_ld<ELEM_F16, true>(gate, at);
         g.u[0] = h.u[0];
         g.u[1] = h.u[1];
     }
@@ -128,7 +134,7 @@ __device__ __forceinline__ float gate_at(const SeamArgs& a, const Piece<ELEM_F32
 
 // Values skip.. of a piece (all of it as one store).
 template <int TYPE>
-__device__ __forceinline__ void piece_put(void* p, int64_t i, const float* v, int skip) {
+__device__ __forceinline__ void piece_put(void* p, uint32_t i, const float* v, int skip) {
     if (skip == 0) {
         piece_st<TYPE>(p, i, v);
     } else {
@@ -147,23 +153,30 @@ __global__ void __launch_bounds__(64 * WAVES) seam_kernel(SeamArgs a) {
     __shared__ float part[2][WAVES];
     const int dim = static_cast<int>(a.dim);
     const int begin = static_cast<int>(threadIdx.x) * 4, last = begin + (PIECES - 1) * 256 * WAVES;
-    // a piece's first value, and how many of it are not its own (4: there is no piece)
-    const auto at = [&](int k) { return k < PIECES - 1 || last + 4 <= dim ? begin + k * 256 * WAVES : dim - 4; };
+    // how many values of a piece are not its own (4: there is no piece)
     const int last_skip = last >= dim ? 4 : last + 4 <= dim ? 0 : last + 4 - dim;
     const auto skip = [&](int k) { return k < PIECES - 1 ? 0 : last_skip; };
     for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
-        const int64_t bo = row * a.b_ld, xo = row * a.x_ld, yo = row * a.y_ld, no = row * a.n_ld, go = row * a.gate_row;
+        const uint8_t* rb = elem_at(a.b, row * a.b_ld, BT);
+        const uint8_t* rx = elem_at(a.x, row * a.x_ld, XT);
+        const uint8_t* rg = elem_at(a.gate, row * a.gate_row, a.gate_type);
+        uint8_t* ry = elem_at(a.y, row * a.y_ld, XT);
+        uint8_t* rn = elem_at(a.n, row * a.n_ld, a.n_type);
+        // a piece's first value (made anew in each turn: an address a piece would take the registers of half a row)
+        uint32_t start = begin, end = last + 4 <= dim ? last : dim - 4;
+        asm volatile("" : "+v"(start), "+v"(end));
+        const auto at = [&](int k) { return k < PIECES - 1 ? start + k * 256 * WAVES : end; };
         Piece<ELEM_F32> g[PIECES];
         Piece<BT> b[PIECES];
         Piece<XT> x[PIECES];
         if (a.gate) {
 #pragma unroll
-            for (int k = 0; k < PIECES; k++) g[k] = gate_ld(a, go, at(k));
+            for (int k = 0; k < PIECES; k++) g[k] = gate_ld(a, rg, at(k));
         }
 #pragma unroll
-        for (int k = 0; k < PIECES; k++) b[k] = piece_ld<BT, true>(a.b, bo + at(k));
+        for (int k = 0; k < PIECES; k++) b[k] = piece_ld<BT, true>(rb, at(k));
 #pragma unroll
-        for (int k = 0; k < PIECES; k++) x[k] = piece_ld<XT, true>(a.x, xo + at(k));
+        for (int k = 0; k < PIECES; k++) x[k] = piece_ld<XT, true>(rx, at(k));
         float inv = a.scale;
         if (a.post_w) {
             float s = 0.f;
@@ -205,15 +218,15 @@ __global__ void __launch_bounds__(64 * WAVES) seam_kernel(SeamArgs a) {
 #pragma unroll
         for (int k = 0; k < PIECES; k++) {
             if (skip(k) == 4) continue;
-            piece_put<XT>(a.y, yo + at(k), y[k], skip(k));
+            piece_put<XT>(ry, at(k), y[k], skip(k));
             if (a.pre_w) {
                 const Piece<ELEM_F32> w = piece_ld<ELEM_F32>(a.pre_w, at(k));
                 float n[4];
 #pragma unroll
                 for (int j = 0; j < 4; j++) n[j] = y[k][j] * inv2 * piece_at<ELEM_F32>(w, j);
-                if (a.n_type == ELEM_F32) piece_put<ELEM_F32>(a.n, no + at(k), n, skip(k));
-                else if (a.n_type == ELEM_F16) piece_put<ELEM_F16>(a.n, no + at(k), n, skip(k));
-                else piece_put<ELEM_BF16>(a.n, no + at(k), n, skip(k));
+                if (a.n_type == ELEM_F32) piece_put<ELEM_F32>(rn, at(k), n, skip(k));
+                else if (a.n_type == ELEM_F16) piece_put<ELEM_F16>(rn, at(k), n, skip(k));
+                else piece_put<ELEM_BF16>(rn, at(k), n, skip(k));
             }
         }
         if (WAVES > 1) __syncthreads();  // the sums are read
