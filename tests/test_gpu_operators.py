@@ -105,6 +105,22 @@ def test_block_norm_many_rows(dim, gate):
     check_norm(x, b, post, g, 1.0, pre, 1e-5, y, n)
 
 
+@pytest.mark.parametrize("rows,dims", [
+    (1100, [4, 5, 257, 512, 513, 768, 769, 1024, 1025, 1536, 1537, 2048, 2049, 2560, 2561, 3000, 3100, 4096, 4097, 5120, 5121]),
+    (400, [300, 1024, 1100, 2000, 2049, 4096, 4100, 6144, 14336]),
+    (2, [257, 1025, 4097, 8192, 8193, 12288, 12289, 14337, 16383, 16385])])
+def test_block_norm_rows_by_waves(rows, dims):
+    """Each number of waves and pieces that a row may take, in place and with a gate of each row."""
+    for dim in dims:
+        x, b = normal(dim, rows, dim, scale=2, dtype=BF16).cuda(), normal(dim + 1, rows, dim).cuda()
+        post, pre = (1 + normal(dim + 2, dim, scale=0.1)).cuda(), (1 + normal(dim + 3, dim, scale=0.1)).cuda()
+        g = normal(dim + 4, rows, 1, dtype=F16).cuda()
+        was = x.clone()
+        y, n = block_norm(x, b, post_w=post, gate=g, pre_w=pre, normed_dtype=F16, out=x)
+        assert y.data_ptr() == x.data_ptr()
+        check_norm(was, b, post, g, 1.0, pre, 1e-5, y, n)
+
+
 def test_block_norm_stores_special_values_in_16_bits():
     """What a narrow type holds of NaN, infinities, overflow and ties: as torch rounds."""
     v = torch.tensor([[math.nan, INF, -INF, 3.4e38, -3.4e38, 1.0 + 2 ** -8, 1.0 + 3 * 2 ** -8, 1.0 + 2 ** -11, 65519.0,

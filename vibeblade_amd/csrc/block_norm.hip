@@ -278,24 +278,40 @@ __global__ void __launch_bounds__(64 * LONG_WAVES) seam_long_kernel(SeamArgs a) 
 template <int BT, int XT>
 void seam_launch(const SeamArgs& a, hipStream_t st) {
     const uint32_t grid = static_cast<uint32_t>(a.rows < (1 << 20) ? a.rows : 1 << 20);  // fewer than 2^32 threads
-    // A row by eight waves, in as many pieces a thread as it takes (7001 x 5121:
-    // 189 us with four waves and twice the pieces, 124 with eight); few rows by
-    // sixteen, which are on their way sooner.
-    const bool few = a.rows <= num_cus();
+    // Few rows (a CU or less for each) are on their way soonest with sixteen
+    // waves and short shares.  With many, bytes in flight count: as few waves as
+    // hold a row in up to five pieces a thread, and lengths that leave few
+    // threads idle (bf16, eight waves and two pieces against the many's: 8192 x
+    // 2560 49 us and 37, 16384 x 2048 73 and 51, 65536 x 512 113 and 53, 8192 x
+    // 4096 55 and 52).  Between them eight waves (512 x 4096 6.7 us, four 7.3;
+    // 1024 rows 10.9 and 9.8).  Over 5120 eight waves again (7001 x 5121: four
+    // 111 us, eight 105), and sixteen where eight no longer fit twice (2048 x
+    // 16384: eight 97 us, sixteen 86).
+    const bool few = a.rows <= num_cus(), many = a.rows > 2 * num_cus();
     const int64_t d = a.dim;
     if (d < 4 || d > 16384) seam_long_kernel<<<grid, 64 * LONG_WAVES, 0, st>>>(a);
     else if (d <= 256) seam_kernel<BT, XT, 1, 1><<<grid, 64, 0, st>>>(a);
+    else if (many && d <= 512) seam_kernel<BT, XT, 1, 2><<<grid, 64, 0, st>>>(a);
+    else if (many && d <= 768) seam_kernel<BT, XT, 1, 3><<<grid, 64, 0, st>>>(a);
+    else if (many && d <= 1024) seam_kernel<BT, XT, 2, 2><<<grid, 128, 0, st>>>(a);
+    else if (many && d <= 1536) seam_kernel<BT, XT, 2, 3><<<grid, 128, 0, st>>>(a);
+    else if (many && d <= 2048) seam_kernel<BT, XT, 4, 2><<<grid, 256, 0, st>>>(a);
+    else if (many && d <= 2560) seam_kernel<BT, XT, 2, 5><<<grid, 128, 0, st>>>(a);
+    else if (many && d <= 3072) seam_kernel<BT, XT, 4, 3><<<grid, 256, 0, st>>>(a);
+    else if (many && d <= 4096) seam_kernel<BT, XT, 4, 4><<<grid, 256, 0, st>>>(a);
+    else if (many && d <= 5120) seam_kernel<BT, XT, 4, 5><<<grid, 256, 0, st>>>(a);
     else if (d <= 1024) seam_kernel<BT, XT, 4, 1><<<grid, 256, 0, st>>>(a);
     else if (few && d <= 4096) seam_kernel<BT, XT, 16, 1><<<grid, 1024, 0, st>>>(a);
     else if (few && d <= 8192) seam_kernel<BT, XT, 16, 2><<<grid, 1024, 0, st>>>(a);
+    else if (few && d <= 12288) seam_kernel<BT, XT, 16, 3><<<grid, 1024, 0, st>>>(a);
     else if (d <= 2048) seam_kernel<BT, XT, 8, 1><<<grid, 512, 0, st>>>(a);
     else if (d <= 4096) seam_kernel<BT, XT, 8, 2><<<grid, 512, 0, st>>>(a);
     else if (d <= 6144) seam_kernel<BT, XT, 8, 3><<<grid, 512, 0, st>>>(a);
     else if (d <= 8192) seam_kernel<BT, XT, 8, 4><<<grid, 512, 0, st>>>(a);
     else if (d <= 10240) seam_kernel<BT, XT, 8, 5><<<grid, 512, 0, st>>>(a);
     else if (d <= 12288) seam_kernel<BT, XT, 8, 6><<<grid, 512, 0, st>>>(a);
-    else if (d <= 14336) seam_kernel<BT, XT, 8, 7><<<grid, 512, 0, st>>>(a);
-    else seam_kernel<BT, XT, 8, 8><<<grid, 512, 0, st>>>(a);
+    else if (!few && d <= 14336) seam_kernel<BT, XT, 8, 7><<<grid, 512, 0, st>>>(a);
+    else seam_kernel<BT, XT, 16, 4><<<grid, 1024, 0, st>>>(a);
 }
 
 template <int BT>
