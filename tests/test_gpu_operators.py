@@ -396,7 +396,8 @@ def parts(seed, rows, k, group, zeros):
 
 
 def check_product(w, w64, x, y):
-    """x's two halves keep 22 bits; a group's sum is one chain of instructions of 32 products each."""
+    """Activations keep 22 bits or more below a block's largest (digits) or are exact (fp16 operands); a group's sum
+    is exact, or one chain of instructions of 32 products each."""
     x64 = x.cpu().double().reshape(-1, w64.shape[1])
     mag = x64.abs() @ w64.abs().T
     want = x64 @ w64.T

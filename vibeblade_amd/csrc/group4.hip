@@ -121,9 +121,16 @@ __global__ void __launch_bounds__(256) g4_quantize_kernel(const void* src, int32
 // 16-byte load per lane brings half a block's codes in the order of the A operand of
 // v_mfma_i32_16x16x64_i8 (group4.hpp).  The operand needs no more than a shift
 // and two masks per eight codes: a nibble in the high half of a byte, as int8,
-// is 16 (q - 8).  Fp16 operands would take five times the instructions, and
+// is 16 (q - 8).  Fp16 operands take five times the instructions, and
 // instructions are what bounds a wave here: at the memory's rate a CU has about
 // 100 issue slots for a step's 1 KB.
+//
+// Bound by memory where the weights are large (one token, us and TB/s of weights:
+// 128256 x 4096 44 and 6.2, 128256 x 14336 145 and 6.5); below that by what comes
+// before and behind the stream (14336 x 4096 9.2 and 3.3, 4096 x 4096 5.9, of which a launch is
+// 1.9, the first loads, digits and barrier about 2 and the sums over waves 0.5);
+// with more tokens by staging them and, in groups of 32, by the multiplications
+// and sums of each group (128256 x 4096, five tokens 56).
 //
 // The B operand's 16 columns are the activations as integers: each block of 128
 // of a token, brought by a power of two to |X| < 2^30 (fp32 x) or 2^22 (16-bit
@@ -733,6 +740,10 @@ __global__ void __launch_bounds__(256) g4_join_kernel(const float* partial, floa
 }
 
 constexpr int64_t G4_LDS = 160 << 10;  // of a CU
+// Activations that every workgroup turns into digits itself; more are made once,
+// by a launch of their own, and copied (itself and once: 4096 x 4096, one token
+// 5.9 and 7.8 us, four 9.2 and 9.7; 4096 x 8192, three 10.8 and 10.7; 4096 x
+// 14336, two 14.3 and 13.2).
 constexpr int64_t G4_SELF_VALUES = 16384;
 constexpr int G4_COLS = 48;  // columns of a launch, at most
 
