@@ -388,8 +388,8 @@ int vb_block_norm(const void* branch, int32_t branch_type, int64_t branch_ld, co
                   int64_t rows, int64_t dim, float eps, void* stream);
 
 /* ---- log probabilities ------------------------------------------------------
- * logits: `rows` rows of `vocab` values (row stride ld, element type as
- * above); z = logits / temperature (in [1e-30, 1e30]).
+ * logits: `rows` rows of `vocab` (up to 2^28) values (row stride ld of 0 or
+ * more, element type as above); z = logits / temperature (in [1e-30, 1e30]).
  *   logprobs[r, j] = log softmax(z_r)[tokens[r, j]], j < n_tokens; an id
  *       outside [0, vocab) gives 0 (a padded position);
  *   entropy[r] = - sum p log p (optional, may be NULL);
@@ -439,8 +439,9 @@ int vb_group4_dequant_rows(const void* w, float* out, int64_t rows, int64_t k, i
  * the codes are summed exactly in a group; or, where there are several tokens
  * of 16 bits, as fp16 values below such a power (fp16 ones as they are), summed
  * in fp32.  Groups are summed in fp32.  A NaN or an infinity gives its token NaN
- * or infinities, no other one.  workspace: at least vb_group4_workspace(...) bytes
- * (0: none), 16-byte aligned, free again when the call's work is done. */
+ * or infinities, no other one.  y overlaps neither x nor w.  workspace: at least
+ * vb_group4_workspace(...) bytes (0: none), 16-byte aligned, free again when the
+ * call's work is done. */
 int64_t vb_group4_workspace(int64_t m, int64_t rows, int64_t k, int32_t group, int32_t has_zeros, int32_t x_type);
 int vb_group4_gemv(const void* w, int64_t rows, int64_t k, int32_t group, int32_t has_zeros, const void* x,
                    int32_t x_type, int64_t x_ld, int64_t m, float* y, void* workspace, size_t workspace_bytes,

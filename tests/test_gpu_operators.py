@@ -12,7 +12,7 @@ import numpy as np
 import pytest
 import torch
 
-from vibeblade_amd import ggml
+from vibeblade_amd import _lib, ggml
 from vibeblade_amd.group4 import GroupQTensor, group_gemv
 from vibeblade_amd.quant import pack_nibbles
 from vibeblade_amd.tensor import QTensor, activation, block_norm, embed_rows, gemm, token_logprobs
@@ -623,6 +623,96 @@ class Step:
 
     def inputs(self, seed, t):
         return pick(seed, 1, t, self.V)[0].to(torch.int32), normal(seed, t, self.H).cuda(), pick(seed + 1, 1, t, self.V)[0]
+
+
+def far_rows(t, apart=1_200_000_000):
+    """t's rows, 2.4 GB apart (16-bit types): the third begins behind 2^31 elements and 2^32 bytes."""
+    buf = torch.empty((t.shape[0] - 1) * apart + t.shape[1], dtype=t.dtype, device="cuda")
+    far = buf.as_strided(t.shape, (apart, 1))
+    far.copy_(t)
+    return far
+
+
+def test_rows_far_apart():
+    x, b = normal(1, 3, 5003, dtype=BF16), normal(2, 3, 5003, dtype=F16)
+    pre = (1 + normal(3, 5003, scale=0.1)).cuda()
+    fx, fb = far_rows(x), far_rows(b)
+    y, n = block_norm(fx, fb, pre_w=pre, out=fx)
+    check_norm(x, b, None, None, 1.0, pre, 1e-5, y, n)
+    z, tok = normal(4, 3, 9001, scale=4, dtype=F16), torch.tensor([0, 9000, 77])
+    check_logprobs(far_rows(z), tok.cuda(), top=3)
+    packed, s, zp, w64 = parts(5, 40, 5003, 128, True)
+    w = GroupQTensor.from_packed(packed, s, zp, k=5003, group=128)
+    for dtype in (F16, BF16):
+        v = normal(6, 3, 5003, dtype=dtype)
+        check_product(w, w64, v, group_gemv(w, far_rows(v)))
+
+
+def test_group4_weights_past_4_gb():
+    k, rows, last = 16384, 560000, 48
+    packed, s, z, w64 = parts(11, last, k, 64, True)
+    small = GroupQTensor.from_packed(packed, s, z, k=k, group=64)
+    data = torch.zeros(small.nbytes // last * rows, dtype=torch.uint8, device="cuda")
+    data[-small.nbytes:] = small.data
+    assert data.numel() > 2 ** 32
+    w = GroupQTensor(data, rows, k, 64, True)
+    for m, dtype in ((1, F32), (2, BF16), (9, F16)):
+        x = normal(m, m, k, dtype=dtype).cuda()
+        y = group_gemv(w, x)
+        assert (y[:, :-last] == 0).all()
+        check_product(small, w64, x, y[:, -last:])
+
+
+def test_logits_of_one_row_for_all():
+    z = normal(21, 1, 4099, scale=4)
+    tok = torch.arange(700, dtype=torch.int32).reshape(-1, 1).cuda()
+    check_logprobs(z.cuda().expand(700, 4099), tok, top=2)
+
+
+@pytest.mark.parametrize("m,dtype", [(1, F32), (2, BF16), (6, F32), (9, F16), (9, BF16)])
+def test_group4_products_over_a_very_long_k(m, dtype):
+    """More chunks of k than one launch holds at a time."""
+    k = 262144 + 100
+    packed, s, z, w64 = parts(m, 20, k, 128, True)
+    w = GroupQTensor.from_packed(packed, s, z, k=k, group=128)
+    x = normal(m, m, k, dtype=dtype).cuda()
+    check_product(w, w64, x, group_gemv(w, x))
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("group,zeros", [(32, True), (128, False)])
+def test_group4_chunks_of_k_fit(dtype, group, zeros):
+    """Every number of blocks of k near those that a workgroup holds, for each number of tokens."""
+    for m in range(1, 17):
+        for blocks in (9, 10, 11, 15, 17, 18, 19, 21, 33, 34, 35, 37, 41, 51, 67, 68, 69, 103, 137, 205):
+            k = 256 * blocks - blocks % 3
+            data = torch.randint(0, 256, (_lib.load().vb_group4_bytes(20, k, group, zeros),), dtype=torch.uint8,
+                                 device="cuda", generator=torch.Generator("cuda").manual_seed(blocks)) & 0x3b  # finite scales
+            w = GroupQTensor(data, 20, k, group, zeros)
+            x = torch.randn(m, k, device="cuda", generator=torch.Generator("cuda").manual_seed(m)).to(dtype)
+            w64, x64 = w.dequantize().double(), x.double()
+            off = (group_gemv(w, x).double() - x64 @ w64.T).abs() - (k / 32 + 36) * U * (x64.abs() @ w64.abs().T)
+            assert off.max() <= 0, (m, blocks)
+
+
+@pytest.mark.parametrize("dim", [300, 5121, 16385, 40000])
+def test_block_norm_of_the_stream_itself(dim):
+    x, pre = normal(dim, 5, dim).cuda(), (1 + normal(1, dim, scale=0.1)).cuda()
+    was = x.clone()
+    y, n = block_norm(x, x, post_w=pre, pre_w=pre, scale=0.5, out=x)
+    check_norm(was, was, pre, None, 0.5, pre, 1e-5, y, n)
+
+
+def test_group4_refuses_out_over_x():
+    packed, s, z, _ = parts(3, 128, 128, 32, False)
+    w = GroupQTensor.from_packed(packed, s, z, k=128, group=32)
+    buf = torch.zeros(400, device="cuda")
+    for x, out in ((buf[:128], buf[:128]), (buf[:128], buf[100:228]), (buf[100:228], buf[:128]),
+                   (buf[:384].view(3, 128)[:, :], buf[:384].view(3, 128))):
+        with pytest.raises(ValueError, match="overlaps"):
+            group_gemv(w, x, out=out)
+    group_gemv(w, buf[:128], out=buf[128:256])
+    group_gemv(w, buf[:0].view(0, 128), out=buf[:0].view(0, 128))
 
 
 @pytest.mark.parametrize("t", [1, 5])

@@ -61,6 +61,12 @@ def test_token_logprobs_refuses(lib, bad):
     assert b"vb_token_logprobs" in lib.vb_last_error()
 
 
+def test_token_logprobs_vocabulary_within_a_slice_offset(lib):
+    assert lib.vb_token_logprobs_workspace(600, 1 << 28, 1) >= 0
+    assert lib.vb_token_logprobs_workspace(600, (1 << 28) + 1, 1) == -1
+    assert lib.vb_token_logprobs(*lp_args(vocab=(1 << 28) + 1, ld=0)) == INVAL
+
+
 def test_token_logprobs_workspace(lib):
     for bad in ((-1, 10, 1), (1, 0, 1), (1, 1 << 31, 1), (1, 10, 65), (1, 10, -1)):
         assert lib.vb_token_logprobs_workspace(*bad) == -1

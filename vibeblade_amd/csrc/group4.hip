@@ -769,7 +769,8 @@ G4Plan g4_plan(const Group4Layout& l, int64_t rows, int64_t m, int x_type, bool 
     p.nt = static_cast<int>((p.parts * m + 15) / 16);
     // Chunks of k whose digits fit into LDS beside the sums.
     const int64_t room = G4_LDS - G4_WAVES * p.nt * 1024 - 16, block = digit_bytes(p.parts, m) + table_bytes(p.parts, m, l.per, has_zeros);
-    p.kz = (l.blocks * block + room - 1) / room;
+    const int64_t fit = room / block;  // 146 blocks of one fp32 token, 10 of twelve
+    p.kz = (l.blocks + fit - 1) / fit;
     // where there are several, as many as give every CU a workgroup (4096 x 14336, eight fp16 tokens: 3 chunks 21.3 us, 4 18.8)
     const int64_t even = (4 * num_cus() + l.tiles - 1) / l.tiles;
     if (p.kz > 1 && p.kz < even) p.kz = even < 8 ? even : p.kz < 8 ? 8 : p.kz;

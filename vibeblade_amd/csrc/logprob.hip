@@ -45,6 +45,7 @@ namespace {
 constexpr int LP_WAVES = 4;
 constexpr int LP_THREADS = 64 * LP_WAVES;
 constexpr int LP_MAX_TOP = 64;
+constexpr int LP_MAX_VOCAB = 1 << 28; // a slice's offsets are 32 bits
 constexpr int LP_MAX_SPLIT = 64;      // slices of a row, one per lane of the wave that joins them
 constexpr int LP_BATCH = 16;          // logits of a lane at a time
 constexpr int LP_BUF = 128;           // candidates of a wave: 64 kept, 64 new
@@ -580,7 +581,7 @@ using namespace vb;
 extern "C" {
 
 int64_t vb_token_logprobs_workspace(int64_t rows, int64_t vocab, int32_t top) {
-    if (rows < 0 || rows > 0x7fffffff || vocab <= 0 || vocab > 0x7fffffff || top < 0 || top > LP_MAX_TOP) return -1;
+    if (rows < 0 || rows > 0x7fffffff || vocab <= 0 || vocab > LP_MAX_VOCAB || top < 0 || top > LP_MAX_TOP) return -1;
     const int64_t splits = lp_splits(rows, vocab);
     return splits > 1 ? rows * splits * (16 + 8 * top) : 0;
 }

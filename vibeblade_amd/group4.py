@@ -115,7 +115,8 @@ class GroupQTensor:
 
 def group_gemv(w: GroupQTensor, x: torch.Tensor, out: torch.Tensor | None = None) -> torch.Tensor:
     """y = W x for one activation vector (k,) -> (rows,) or a few of them (m, k) -> (m, rows), fp32
-    (vb_group4_gemv).  x: float32, float16 or bfloat16 on w's device, rows of any stride."""
+    (vb_group4_gemv).  x: float32, float16 or bfloat16 on w's device, rows of any stride.  out: contiguous
+    float32, apart from x."""
     dev = _gpu_tensor(x, "group_gemv: x")
     if dev != w.device:
         raise ValueError(f"group_gemv: x is on {dev}, W on {w.device}")
@@ -128,6 +129,9 @@ def group_gemv(w: GroupQTensor, x: torch.Tensor, out: torch.Tensor | None = None
         out = x.new_empty((w.rows,) if x.dim() == 1 else (m, w.rows), dtype=torch.float32)
     else:
         _check_out(out, m * w.rows, dev, "group_gemv")
+        end = xr.data_ptr() + ((m - 1) * xr.stride(0) + w.k) * xr.element_size()
+        if m > 0 and out.data_ptr() < end and xr.data_ptr() < out.data_ptr() + out.numel() * 4:
+            raise ValueError("group_gemv: out overlaps x, which is read until the call's end")
     nbytes = _lib.load().vb_group4_workspace(m, w.rows, w.k, w.group, int(w.zeros), kind)
     ws = w.data.new_empty(nbytes) if nbytes > 0 else None
     _launch(dev, "vb_group4_gemv", w.ptr(), w.rows, w.k, w.group, int(w.zeros), xr.data_ptr(), kind, xr.stride(0), m,
