@@ -413,8 +413,8 @@ __global__ void __launch_bounds__(64 * G4_WAVES, g4_wide(PARTS, NT, PER, ZEROS) 
     const int waves = static_cast<int>(blockDim.x) >> 6, threads = static_cast<int>(blockDim.x);
     const int parts = PARTS ? PARTS : a.parts, m = a.m, cols = parts * m;
     const int ks = a.ks, sub = wave % ks, local = wave / ks, per_group = waves / ks;
-    const int kz = MODE == G4_SELF && PARTS != 1 ? 1 : a.kz, z = static_cast<int>(blockIdx.x) % kz;
-    const int turn = static_cast<int>(blockIdx.x) / kz, turns = static_cast<int>(gridDim.x) / kz;
+    const int kz = a.kz, z = static_cast<int>(blockIdx.x);
+    const int turn = static_cast<int>(blockIdx.y), turns = static_cast<int>(gridDim.y);
     const int64_t row_blocks = a.l.blocks, first = static_cast<int64_t>(z) * a.chunk;
     const int tiles = static_cast<int>(a.l.tiles);
     const int blocks = static_cast<int>(row_blocks - first < a.chunk ? row_blocks - first : a.chunk);
@@ -774,10 +774,17 @@ G4Plan g4_plan(const Group4Layout& l, int64_t rows, int64_t m, int x_type, bool 
     // where there are several, as many as give every CU a workgroup (4096 x 14336, eight fp16 tokens: 3 chunks 21.3 us, 4 18.8)
     const int64_t even = (4 * num_cus() + l.tiles - 1) / l.tiles;
     if (p.kz > 1 && p.kz < even) p.kz = even < 8 ? even : p.kz < 8 ? 8 : p.kz;
+    // and where the row tiles leave CUs without work, if there is enough of it to
+    // pay for the launch that joins them (whole and split: 549 x 12800, one token
+    // 12.3 us and 9.0; 1024 x 4096, four 9.0 and 7.6, but two 6.5 and 6.9)
+    if (p.kz == 1 && m * l.blocks >= 48) {
+        const int64_t idle = num_cus() / l.tiles, pairs = l.blocks / 2, most = idle < pairs ? idle : pairs;
+        p.kz = most < 1 ? 1 : most < 8 ? most : 8;
+    }
     if (p.kz > l.blocks) p.kz = l.blocks;
     p.chunk = (l.blocks + p.kz - 1) / p.kz;
     p.kz = (l.blocks + p.chunk - 1) / p.chunk;
-    p.mode = p.parts == 1 || (p.kz == 1 && p.nt == 1 && m * l.blocks * GROUP4_K <= G4_SELF_VALUES) ? G4_SELF : G4_COPY;
+    p.mode = p.parts == 1 || (p.nt == 1 && m * p.chunk * GROUP4_K <= G4_SELF_VALUES) ? G4_SELF : G4_COPY;
     // A tile is shared by as many waves as leave each four blocks, up to eight
     // waves a CU: more of them cost more in x staged and sums joined than they
     // bring in loads in flight (14336 x 4096, one token: ks 1 to 8 take 9.7,
@@ -797,7 +804,7 @@ G4Plan g4_plan(const Group4Layout& l, int64_t rows, int64_t m, int x_type, bool 
 }
 
 template <int PER, bool ZEROS>
-int g4_launch(const G4Args& a, const G4Plan& p, uint32_t grid, hipStream_t st) {
+int g4_launch(const G4Args& a, const G4Plan& p, dim3 grid, hipStream_t st) {
     const uint32_t threads = 64 * p.waves, lds = static_cast<uint32_t>(p.lds);
     if (p.mode == G4_SELF) {
         if (a.parts == 1) g4_gemv_kernel<PER, ZEROS, 1, 1, G4_SELF><<<grid, threads, lds, st>>>(a);
@@ -831,7 +838,7 @@ int g4_run(G4Args a, bool has_zeros, uint8_t* workspace, hipStream_t st) {
     // as many workgroups as are resident at once (16 waves a CU or 8), a share for every chunk
     const int64_t fit = G4_LDS / p.lds, want = (g4_wide(p.parts, p.nt, a.l.per, has_zeros) ? 8 : 16) / p.waves;
     const int64_t most = ((fit < want ? fit : want) * num_cus() + p.kz - 1) / p.kz;
-    const uint32_t grid = static_cast<uint32_t>(p.kz * (p.groups < most ? p.groups : most));
+    const dim3 grid(static_cast<uint32_t>(p.kz), static_cast<uint32_t>(p.groups < most ? p.groups : most));
     if (a.l.per == 1) return has_zeros ? g4_launch<1, true>(a, p, grid, st) : g4_launch<1, false>(a, p, grid, st);
     if (a.l.per == 2) return has_zeros ? g4_launch<2, true>(a, p, grid, st) : g4_launch<2, false>(a, p, grid, st);
     return has_zeros ? g4_launch<4, true>(a, p, grid, st) : g4_launch<4, false>(a, p, grid, st);
