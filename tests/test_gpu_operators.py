@@ -106,7 +106,8 @@ def test_block_norm_many_rows(dim, gate):
 
 
 @pytest.mark.parametrize("rows,dims", [
-    (1100, [4, 5, 257, 512, 513, 768, 769, 1024, 1025, 1536, 1537, 2048, 2049, 2560, 2561, 3000, 3100, 4096, 4097, 5120, 5121]),
+    (1100, [4, 5, 257, 512, 513, 768, 769, 1024, 1025, 1536, 1537, 2048, 2049, 2560, 2561, 3000, 3100, 4096, 4097, 5120, 5121,
+            5632, 5633, 6144, 6145, 6657, 7168, 7169]),
     (400, [300, 1024, 1100, 2000, 2049, 4096, 4100, 6144, 14336]),
     (2, [257, 1025, 4097, 8192, 8193, 12288, 12289, 14337, 16383, 16385])])
 def test_block_norm_rows_by_waves(rows, dims):

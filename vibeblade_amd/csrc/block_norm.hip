@@ -15,8 +15,9 @@
 // for each sum (seam_long_kernel).
 //
 // Memory bounds it: fp32 rows run at 6.0 to 6.3 TB/s of what is read and written
-// (8192 x 4096 79 us, 4096 x 8192 86), 16-bit ones at 5.2 (8192 x 4096 51 us),
-// rows of odd length at 4.9 (7001 x 5121, a full gate: 103 us).  One row of 4096 takes
+// (4096 x 8192 86 us, 8192 x 4096 with fp16 n 73), 16-bit ones at 5.2 to 5.8
+// (8192 x 4096 46 us), rows of odd length at 4.9 (7001 x 5121, a full gate: 103
+// us; 7001 x 5120 81).  One row of 4096 takes
 // 3.4 us in a graph, of which a launch is 1.9.
 #include "elem_types.hpp"
 #include "vb_internal.hpp"
@@ -155,6 +156,9 @@ __device__ __forceinline__ void piece_put(void* p, uint32_t i, const float* v, i
 // and are neither summed nor stored again.
 template <int BT, int XT, int WAVES, int PIECES>
 __global__ void __launch_bounds__(64 * WAVES) seam_kernel(SeamArgs a) {
+    // the weights come with the rest (8192 x 4096 fp32 78 us and 73, 7001 x 5120 91 and 81), where that leaves
+    // the registers for as many workgroups (eight waves, three pieces: 101 us and 106)
+    constexpr bool EARLY = WAVES <= 4 || (WAVES == 8 && PIECES <= 2);
     __shared__ float part[2][WAVES];
     const int dim = static_cast<int>(a.dim);
     const int begin = static_cast<int>(threadIdx.x) * 4, last = begin + (PIECES - 1) * 256 * WAVES;
@@ -182,6 +186,14 @@ __global__ void __launch_bounds__(64 * WAVES) seam_kernel(SeamArgs a) {
         for (int k = 0; k < PIECES; k++) b[k] = piece_ld<BT, true>(rb, at(k));
 #pragma unroll
         for (int k = 0; k < PIECES; k++) x[k] = piece_ld<XT, true>(rx, at(k));
+        Piece<ELEM_F32> post[EARLY ? PIECES : 1], pre[EARLY ? PIECES : 1];
+        if constexpr (EARLY) {
+#pragma unroll
+            for (int k = 0; k < PIECES; k++) {
+                if (a.post_w) post[k] = piece_ld<ELEM_F32>(a.post_w, at(k));
+                if (a.pre_w) pre[k] = piece_ld<ELEM_F32>(a.pre_w, at(k));
+            }
+        }
         float inv = a.scale;
         if (a.post_w) {
             float s = 0.f;
@@ -202,7 +214,7 @@ __global__ void __launch_bounds__(64 * WAVES) seam_kernel(SeamArgs a) {
 #pragma unroll
             for (int j = 0; j < 4; j++) p[j] = piece_at<BT>(b[k], j) * inv;
             if (a.post_w) {
-                const Piece<ELEM_F32> w = piece_ld<ELEM_F32>(a.post_w, at(k));
+                const Piece<ELEM_F32> w = EARLY ? post[EARLY ? k : 0] : piece_ld<ELEM_F32>(a.post_w, at(k));
 #pragma unroll
                 for (int j = 0; j < 4; j++) p[j] *= piece_at<ELEM_F32>(w, j) * a.scale;
             }
@@ -225,7 +237,7 @@ __global__ void __launch_bounds__(64 * WAVES) seam_kernel(SeamArgs a) {
             if (skip(k) == 4) continue;
             piece_put<XT>(ry, at(k), y[k], skip(k));
             if (a.pre_w) {
-                const Piece<ELEM_F32> w = piece_ld<ELEM_F32>(a.pre_w, at(k));
+                const Piece<ELEM_F32> w = EARLY ? pre[EARLY ? k : 0] : piece_ld<ELEM_F32>(a.pre_w, at(k));
                 float n[4];
 #pragma unroll
                 for (int j = 0; j < 4; j++) n[j] = y[k][j] * inv2 * piece_at<ELEM_F32>(w, j);
@@ -285,13 +297,14 @@ void seam_launch(const SeamArgs& a, hipStream_t st) {
     const uint32_t grid = static_cast<uint32_t>(a.rows < (1 << 20) ? a.rows : 1 << 20);  // fewer than 2^32 threads
     // Few rows (a CU or less for each) are on their way soonest with sixteen
     // waves and short shares.  With many, bytes in flight count: as few waves as
-    // hold a row in up to five pieces a thread, and lengths that leave few
+    // hold a row in up to seven pieces a thread, and lengths that leave few
     // threads idle (bf16, eight waves and two pieces against the many's: 8192 x
-    // 2560 49 us and 37, 16384 x 2048 73 and 51, 65536 x 512 113 and 53, 8192 x
-    // 4096 55 and 52).  Between them eight waves (512 x 4096 6.7 us, four 7.3;
-    // 1024 rows 10.9 and 9.8).  Over 5120 eight waves again (7001 x 5121: four
-    // 111 us, eight 105), and sixteen where eight no longer fit twice (2048 x
-    // 16384: eight 97 us, sixteen 86).
+    // 2560 49 us and 35, 16384 x 2048 73 and 51, 65536 x 512 113 and 44, 8192 x
+    // 4096 55 and 46; six pieces half of whose last is there, 7001 x 6144: 66 and
+    // 60, seven, 5000 x 7168: 59 and 52, but 7001 x 5121 101 and 105).  Between
+    // them eight waves (512 x 4096 6.7 us, four 7.3; 1024 rows 10.9 and 9.8).
+    // Over 7168 eight waves again (4096 x 8192 fp32: 86 us, four 89), and sixteen
+    // where eight no longer fit twice (2048 x 16384: eight 97 us, sixteen 86).
     const bool few = a.rows <= num_cus(), many = a.rows > 2 * num_cus();
     const int64_t d = a.dim;
     if (d < 4 || d > 16384) seam_long_kernel<<<grid, 64 * LONG_WAVES, 0, st>>>(a);
@@ -305,6 +318,8 @@ void seam_launch(const SeamArgs& a, hipStream_t st) {
     else if (many && d <= 3072) seam_kernel<BT, XT, 4, 3><<<grid, 256, 0, st>>>(a);
     else if (many && d <= 4096) seam_kernel<BT, XT, 4, 4><<<grid, 256, 0, st>>>(a);
     else if (many && d <= 5120) seam_kernel<BT, XT, 4, 5><<<grid, 256, 0, st>>>(a);
+    else if (many && d > 5632 && d <= 6144) seam_kernel<BT, XT, 4, 6><<<grid, 256, 0, st>>>(a);
+    else if (many && d > 6656 && d <= 7168) seam_kernel<BT, XT, 4, 7><<<grid, 256, 0, st>>>(a);
     else if (d <= 1024) seam_kernel<BT, XT, 4, 1><<<grid, 256, 0, st>>>(a);
     else if (few && d <= 4096) seam_kernel<BT, XT, 16, 1><<<grid, 1024, 0, st>>>(a);
     else if (few && d <= 8192) seam_kernel<BT, XT, 16, 2><<<grid, 1024, 0, st>>>(a);
