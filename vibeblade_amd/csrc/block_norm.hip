@@ -17,8 +17,8 @@
 // Memory bounds it: fp32 rows run at 6.0 to 6.3 TB/s of what is read and written
 // (4096 x 8192 86 us, 8192 x 4096 with fp16 n 73), 16-bit ones at 5.2 to 5.8
 // (8192 x 4096 46 us), rows of odd length at 4.9 (7001 x 5121, a full gate: 103
-// us; 7001 x 5120 81).  One row of 4096 takes
-// 3.4 us in a graph, of which a launch is 1.9.
+// us; 7001 x 5120 82).  One row of 4096 takes 3.4 us in a graph, of which a
+// launch is 1.9.
 #include "elem_types.hpp"
 #include "vb_internal.hpp"
 #include "../../include/vbhip.h"
@@ -307,30 +307,31 @@ void seam_launch(const SeamArgs& a, hipStream_t st) {
     // where eight no longer fit twice (2048 x 16384: eight 97 us, sixteen 86).
     const bool few = a.rows <= num_cus(), many = a.rows > 2 * num_cus();
     const int64_t d = a.dim;
-    if (d < 4 || d > 16384) seam_long_kernel<<<grid, 64 * LONG_WAVES, 0, st>>>(a);
-    else if (d <= 256) seam_kernel<BT, XT, 1, 1><<<grid, 64, 0, st>>>(a);
-    else if (many && d <= 512) seam_kernel<BT, XT, 1, 2><<<grid, 64, 0, st>>>(a);
-    else if (many && d <= 768) seam_kernel<BT, XT, 1, 3><<<grid, 64, 0, st>>>(a);
-    else if (many && d <= 1024) seam_kernel<BT, XT, 2, 2><<<grid, 128, 0, st>>>(a);
-    else if (many && d <= 1536) seam_kernel<BT, XT, 2, 3><<<grid, 128, 0, st>>>(a);
-    else if (many && d <= 2048) seam_kernel<BT, XT, 4, 2><<<grid, 256, 0, st>>>(a);
-    else if (many && d <= 2560) seam_kernel<BT, XT, 2, 5><<<grid, 128, 0, st>>>(a);
-    else if (many && d <= 3072) seam_kernel<BT, XT, 4, 3><<<grid, 256, 0, st>>>(a);
-    else if (many && d <= 4096) seam_kernel<BT, XT, 4, 4><<<grid, 256, 0, st>>>(a);
-    else if (many && d <= 5120) seam_kernel<BT, XT, 4, 5><<<grid, 256, 0, st>>>(a);
-    else if (many && d > 5632 && d <= 6144) seam_kernel<BT, XT, 4, 6><<<grid, 256, 0, st>>>(a);
-    else if (many && d > 6656 && d <= 7168) seam_kernel<BT, XT, 4, 7><<<grid, 256, 0, st>>>(a);
-    else if (d <= 1024) seam_kernel<BT, XT, 4, 1><<<grid, 256, 0, st>>>(a);
-    else if (few && d <= 4096) seam_kernel<BT, XT, 16, 1><<<grid, 1024, 0, st>>>(a);
-    else if (few && d <= 8192) seam_kernel<BT, XT, 16, 2><<<grid, 1024, 0, st>>>(a);
-    else if (few && d <= 12288) seam_kernel<BT, XT, 16, 3><<<grid, 1024, 0, st>>>(a);
-    else if (d <= 2048) seam_kernel<BT, XT, 8, 1><<<grid, 512, 0, st>>>(a);
-    else if (d <= 4096) seam_kernel<BT, XT, 8, 2><<<grid, 512, 0, st>>>(a);
-    else if (d <= 6144) seam_kernel<BT, XT, 8, 3><<<grid, 512, 0, st>>>(a);
-    else if (d <= 8192) seam_kernel<BT, XT, 8, 4><<<grid, 512, 0, st>>>(a);
-    else if (d <= 10240) seam_kernel<BT, XT, 8, 5><<<grid, 512, 0, st>>>(a);
-    else if (d <= 12288) seam_kernel<BT, XT, 8, 6><<<grid, 512, 0, st>>>(a);
-    else if (!few && d <= 14336) seam_kernel<BT, XT, 8, 7><<<grid, 512, 0, st>>>(a);
+    const auto within = [d](int64_t waves, int64_t pieces) { return d <= 256 * waves * pieces; };
+    if (d < 4 || !within(16, 4)) seam_long_kernel<<<grid, 64 * LONG_WAVES, 0, st>>>(a);
+    else if (within(1, 1)) seam_kernel<BT, XT, 1, 1><<<grid, 64, 0, st>>>(a);
+    else if (many && within(1, 2)) seam_kernel<BT, XT, 1, 2><<<grid, 64, 0, st>>>(a);
+    else if (many && within(1, 3)) seam_kernel<BT, XT, 1, 3><<<grid, 64, 0, st>>>(a);
+    else if (many && within(2, 2)) seam_kernel<BT, XT, 2, 2><<<grid, 128, 0, st>>>(a);
+    else if (many && within(2, 3)) seam_kernel<BT, XT, 2, 3><<<grid, 128, 0, st>>>(a);
+    else if (many && within(4, 2)) seam_kernel<BT, XT, 4, 2><<<grid, 256, 0, st>>>(a);
+    else if (many && within(2, 5)) seam_kernel<BT, XT, 2, 5><<<grid, 128, 0, st>>>(a);
+    else if (many && within(4, 3)) seam_kernel<BT, XT, 4, 3><<<grid, 256, 0, st>>>(a);
+    else if (many && within(4, 4)) seam_kernel<BT, XT, 4, 4><<<grid, 256, 0, st>>>(a);
+    else if (many && within(4, 5)) seam_kernel<BT, XT, 4, 5><<<grid, 256, 0, st>>>(a);
+    else if (many && d > 5632 && within(4, 6)) seam_kernel<BT, XT, 4, 6><<<grid, 256, 0, st>>>(a);
+    else if (many && d > 6656 && within(4, 7)) seam_kernel<BT, XT, 4, 7><<<grid, 256, 0, st>>>(a);
+    else if (within(4, 1)) seam_kernel<BT, XT, 4, 1><<<grid, 256, 0, st>>>(a);
+    else if (few && within(16, 1)) seam_kernel<BT, XT, 16, 1><<<grid, 1024, 0, st>>>(a);
+    else if (few && within(16, 2)) seam_kernel<BT, XT, 16, 2><<<grid, 1024, 0, st>>>(a);
+    else if (few && within(16, 3)) seam_kernel<BT, XT, 16, 3><<<grid, 1024, 0, st>>>(a);
+    else if (within(8, 1)) seam_kernel<BT, XT, 8, 1><<<grid, 512, 0, st>>>(a);
+    else if (within(8, 2)) seam_kernel<BT, XT, 8, 2><<<grid, 512, 0, st>>>(a);
+    else if (within(8, 3)) seam_kernel<BT, XT, 8, 3><<<grid, 512, 0, st>>>(a);
+    else if (within(8, 4)) seam_kernel<BT, XT, 8, 4><<<grid, 512, 0, st>>>(a);
+    else if (within(8, 5)) seam_kernel<BT, XT, 8, 5><<<grid, 512, 0, st>>>(a);
+    else if (within(8, 6)) seam_kernel<BT, XT, 8, 6><<<grid, 512, 0, st>>>(a);
+    else if (!few && within(8, 7)) seam_kernel<BT, XT, 8, 7><<<grid, 512, 0, st>>>(a);
     else seam_kernel<BT, XT, 16, 4><<<grid, 1024, 0, st>>>(a);
 }
 
