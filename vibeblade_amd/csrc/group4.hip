@@ -406,7 +406,7 @@ __host__ __device__ constexpr bool g4_wide(int parts, int nt, int per, bool zero
 // PARTS 0: a.parts (no code but the staging depends on it).
 template <int PER, bool ZEROS, int PARTS, int NT, int MODE>
 __global__ void __launch_bounds__(64 * G4_WAVES, g4_wide(PARTS, NT, PER, ZEROS) ? 2 : 4) g4_gemv_kernel(G4Args a) {
-    constexpr int DEPTH = G4_DEPTH;
+    constexpr int DEPTH = NT == 3 && PER == 4 && ZEROS ? 1 : G4_DEPTH;  // (two do not fit the registers)
     extern __shared__ uint4 lds[];
     const int tid = static_cast<int>(threadIdx.x), lane = tid & 63, n = lane & 15, c = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -771,9 +771,11 @@ G4Plan g4_plan(const Group4Layout& l, int64_t rows, int64_t m, int x_type, bool 
     const int64_t room = G4_LDS - G4_WAVES * p.nt * 1024 - 16, block = digit_bytes(p.parts, m) + table_bytes(p.parts, m, l.per, has_zeros);
     const int64_t fit = room / block;  // 146 blocks of one fp32 token, 10 of twelve
     p.kz = (l.blocks + fit - 1) / fit;
-    // where there are several, as many as give every CU a workgroup (4096 x 14336, eight fp16 tokens: 3 chunks 21.3 us, 4 18.8)
+    // where there are several, as many as give every CU a workgroup (4096 x 14336, eight tokens as
+    // digits: 3 chunks 21.3 us, 4 18.8)
     const int64_t even = (4 * num_cus() + l.tiles - 1) / l.tiles;
-    if (p.kz > 1 && p.kz < even) p.kz = even < 8 ? even : p.kz < 8 ? 8 : p.kz;
+    // or all of them the same number (nine fp32 tokens, groups of 32: 5 chunks 53.7 us, 8 31.9)
+    if (p.kz > 1) p.kz = even <= 8 ? (p.kz + even - 1) / even * even : p.kz < 8 ? 8 : p.kz;
     // and where the row tiles leave CUs without work, if there is enough of it to
     // pay for the launch that joins them (whole and split: 549 x 12800, one token
     // 12.3 us and 9.0; 1024 x 4096, four 9.0 and 7.6, but two 6.5 and 6.9)
