@@ -127,10 +127,10 @@ __global__ void __launch_bounds__(256) g4_quantize_kernel(const void* src, int32
 //
 // Bound by memory where the weights are large (one token, us and TB/s of weights:
 // 128256 x 4096 44 and 6.2, 128256 x 14336 145 and 6.5); below that by what comes
-// before and behind the stream (14336 x 4096 9.2 and 3.3, 4096 x 4096 5.9, of which a launch is
-// 1.9, the first loads, digits and barrier about 2 and the sums over waves 0.5);
-// with more tokens by staging them and, in groups of 32, by the multiplications
-// and sums of each group (128256 x 4096, five tokens 56).
+// before and behind the stream (14336 x 4096 9.2 and 3.3, 4096 x 4096 5.9, of
+// which a launch is 1.9, the first loads, digits and barrier about 2 and the
+// sums over waves 0.5); with more tokens by staging them and, in groups of 32,
+// by the multiplications and sums of each group (128256 x 4096, five tokens 56).
 //
 // The B operand's 16 columns are the activations as integers: each block of 128
 // of a token, brought by a power of two to |X| < 2^30 (fp32 x) or 2^22 (16-bit
@@ -611,7 +611,8 @@ __global__ void __launch_bounds__(64 * G4_WAVES, g4_wide(PARTS, NT, PER, ZEROS) 
         const int pieces = blocks * 32, units = pieces * m;  // of a token, of all
         const int64_t k0 = first * GROUP4_K;
         const float share = 1.f / static_cast<float>(pieces);
-        const auto token_of = [&](int u) __attribute__((always_inline)) {  // u / pieces: u < 2^14, so half a piece is more than the rounding
+        // u / pieces: u < 2^14, so half a piece is more than the rounding
+        const auto token_of = [&](int u) __attribute__((always_inline)) {
             return m == 1 ? 0 : static_cast<int>((static_cast<float>(u) + 0.5f) * share);
         };
         const auto get = [&](int base) __attribute__((always_inline)) {
