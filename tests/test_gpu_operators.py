@@ -783,3 +783,47 @@ def test_calls_on_two_streams_at_once():
     torch.cuda.synchronize()
     for g, w in zip(got, want):
         assert all(torch.equal(a, b) for a, b in zip(g, w))
+
+
+@pytest.mark.parametrize("temperature", [1e-7, 1e-8, 3e-9, 1e-9, 1e-12, 1e-20, 1e-25, 1e-29, 1e-30])
+@pytest.mark.parametrize("rows,vocab,top", [(3, 20000, 6), (40, 4096, 0), (600, 3001, 3)])
+def test_token_logprobs_low_temperatures(temperature, rows, vocab, top):
+    """Near-greedy sampling: log2(e) / T times a logit passes 2^31, and its rounding any exponent that fp32 holds.
+    (A temperature that fp32 holds, so that its own rounding is none of the result's.)"""
+    z = normal(31, rows, vocab, scale=3)
+    z[1, 7] = z[1, vocab - 2] = z[1].max()  # two places of the maximum
+    check_logprobs(z.cuda(), pick(31, rows, 2, vocab), top=top, temperature=float(np.float32(temperature)))
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("fill", [-1e9, -1e10, -1e15, -1e20, -1e30, 8e9])
+@pytest.mark.parametrize("rows,vocab,top", [(5, 333, 4), (5, 40000, 9), (5, 40000, 0), (520, 5000, 9)])
+def test_token_logprobs_finite_masks(dtype, fill, rows, vocab, top):
+    """Rows that an additive mask leaves at a large finite value: all of them, but for one, but for the last few,
+    but for a stretch in between, and every second."""
+    for temperature in (1.0, 0.75, 0.3, 0.1):
+        z = normal(32, rows, vocab, scale=2, dtype=dtype)
+        z[0] = fill
+        z[1, torch.arange(vocab) != vocab // 3] = fill
+        z[2, :vocab - 20] = fill
+        z[3, :vocab // 4] = fill
+        z[3, vocab // 2:] = fill
+        z[4, ::2] = fill
+        tokens = torch.tensor([[0, vocab // 3, vocab - 1, vocab // 2 - 1]]).expand(rows, 4)
+        check_logprobs(z.cuda(), tokens.cuda(), top=top, temperature=float(np.float32(temperature)))
+
+
+@pytest.mark.parametrize("sign", [1, -1])
+@pytest.mark.parametrize("exponent", [20, 22, 23, 24, 25, 26])
+@pytest.mark.parametrize("vocab", [300, 9000, 50001])
+def test_token_logprobs_far_from_zero(sign, exponent, vocab):
+    """Logits whose common part, times log2(e), is a power of two with many places left behind the point: whichever
+    way the sums are kept, terms on both sides of the border count."""
+    step = 2.0 ** (exponent - 24)
+    base = round(sign * 2.0 ** exponent * math.log(2) / step) * step
+    off = (normal(33, 4, vocab, scale=2) / step).round() * step
+    off[1], off[2] = off[1].sort().values, off[2].sort(descending=True).values
+    off[3] = torch.linspace(-6, 6, vocab).div(step).round() * step
+    z = (base + off.double()).float()
+    for top in (0, 5):
+        check_logprobs(z.cuda(), pick(34, 4, 3, vocab), top=top)

@@ -49,6 +49,11 @@ constexpr int LP_MAX_VOCAB = 1 << 28; // a slice's offsets are 32 bits
 constexpr int LP_MAX_SPLIT = 64;      // slices of a row, one per lane of the wave that joins them
 constexpr int LP_BATCH = 16;          // logits of a lane at a time
 constexpr int LP_BUF = 128;           // candidates of a wave: 64 kept, 64 new
+// |c m| up to which sums are kept relative to c m rounded: its rounding is an
+// exponent of at most 1/2 there, which costs no range (from 2^31 on it may be 128
+// and more, and a term no number of fp32's).  The form for larger ones takes an
+// instruction more a logit.
+constexpr float LP_NEAR = 0x1p24f;
 
 struct LpArgs {
     const void* z;
@@ -239,7 +244,7 @@ struct Walk {
     float m, s, t;  // m: the wave's; s, t: the lane's sums, relative to `ref`
     float tau;      // no candidate at or below it
     float ref;      // c m, rounded: a term is 2^(c z - ref), one instruction for the exponent
-    bool far;       // c m is beyond fp32: 2^(c (z - m)) instead
+    bool far;       // |c m| from LP_NEAR on: ref is 0, a term is 2^(c (z - m))
     bool masked;    // a term with z = -inf was met: 0 (-inf) is kept out of t
 
     __device__ __forceinline__ Walk(const LpArgs& a_, uint64_t* buf)
@@ -301,11 +306,12 @@ struct Walk {
             const float top = wave_max(cm);
             // one place of the new maximum leaves the sums, the old one joins them
             const float now = top * a.c;
-            const bool out_of = !(fabsf(now) < 1e30f);
+            const bool out_of = !(fabsf(now) < LP_NEAR);
             if (m > -INFINITY) {
-                const bool any_far = far || out_of;
-                const float d = any_far ? (m - top) * a.c : ref - now, f = __builtin_amdgcn_exp2f(d), dd = fmaxf(d, -1e30f);
-                const float dm = any_far ? dd : __builtin_fmaf(m, a.c, -now);
+                // the old reference and the old maximum, from the new reference
+                const float back_at = out_of ? (m - top) * a.c : __builtin_fmaf(m, a.c, -now);
+                const float d = far ? back_at : out_of ? __builtin_fmaf(-top, a.c, ref) : ref - now;
+                const float f = __builtin_amdgcn_exp2f(d), dd = fmaxf(d, -1e30f), dm = fmaxf(back_at, -1e30f);
                 const float back = (threadIdx.x & 63) == 0 ? __builtin_amdgcn_exp2f(dm) : 0.f;
                 t = f * (t + dd * s) + back * dm;
                 s = f * s + back;
