@@ -380,7 +380,8 @@ int vb_softmax(const float* x, float* y, int64_t rows, int64_t n, void* stream);
  * tensor starts at element r * its stride (branch_ld, x_ld of 0 or more, y_ld,
  * n_ld at least dim, where rows > 1).  Element i of the gate of row r is
  * gate[r * gate_row + i * gate_col], gate_col 0 or 1.  post_w, pre_w: dim
- * fp32.  y may be x (same stride); no other overlap.  Any alignment of whole
+ * fp32.  y may be x, branch or (gate_col 1) the gate value for value, of one
+ * address, element size and stride; no other overlap.  Any alignment of whole
  * elements. */
 int vb_block_norm(const void* branch, int32_t branch_type, int64_t branch_ld, const float* post_w, const void* gate,
                   int32_t gate_type, int64_t gate_row, int64_t gate_col, float scale, const void* x, int32_t x_type,

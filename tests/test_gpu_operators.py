@@ -827,3 +827,30 @@ def test_token_logprobs_far_from_zero(sign, exponent, vocab):
     z = (base + off.double()).float()
     for top in (0, 5):
         check_logprobs(z.cuda(), pick(34, 4, 3, vocab), top=top)
+
+
+@pytest.mark.parametrize("dim", [300, 771, 5121, 16385, 40000])
+@pytest.mark.parametrize("rows", [1, 5, 300, 1100])
+def test_block_norm_over_the_branch_or_the_gate(dim, rows):
+    if rows * dim > 6 << 20:
+        rows = 40
+    x, b, g = normal(1, rows, dim).cuda(), normal(2, rows, dim).cuda(), normal(3, rows, dim).cuda()
+    post, pre = (1 + normal(4, dim, scale=0.1)).cuda(), (1 + normal(5, dim, scale=0.1)).cuda()
+    want = block_norm(x, b, post_w=post, gate=g, pre_w=pre)
+    for over in (x, b, g):
+        kept = over.clone()
+        y, n = block_norm(x, b, post_w=post, gate=g, pre_w=pre, out=over)
+        assert y is over and torch.equal(y, want[0]) and torch.equal(n, want[1])
+        over.copy_(kept)
+
+
+def test_block_norm_in_columns_of_one_buffer():
+    """x, branch, gate and out side by side in a wider buffer: their ranges of memory meet, their rows do not."""
+    wide = normal(6, 7, 4 * 130).cuda()
+    x, b, g, out = (wide[:, i * 130:(i + 1) * 130] for i in range(4))
+    pre = (1 + normal(7, 130, scale=0.1)).cuda()
+    want = block_norm(x, b, post_w=pre, gate=g, pre_w=pre)
+    y, n = block_norm(x, b, post_w=pre, gate=g, pre_w=pre, out=out)
+    assert torch.equal(y, want[0]) and torch.equal(n, want[1])
+    with pytest.raises(ValueError, match="overlaps"):
+        block_norm(x, b, out=wide[:, 129:259])

@@ -163,3 +163,60 @@ def test_ctypes_signatures_have_the_header_s_argument_count():
             want = ctypes.c_void_p if "*" in a else ctypes.c_float if "float" in a else \
                 ctypes.c_size_t if "size_t" in a else ctypes.c_int64 if "int64_t" in a else ctypes.c_int32
             assert c is want, (name, a)
+
+
+@pytest.fixture
+def launches(monkeypatch):
+    """Calls on CPU tensors up to their launches, which are written down and not made."""
+    from vibeblade_amd import group4, tensor
+    made = []
+    for module in (tensor, group4):
+        monkeypatch.setattr(module, "_gpu_tensor", lambda t, what: t.device)
+        monkeypatch.setattr(module, "_launch", lambda dev, fn, *args: made.append((fn, args)))
+    return made
+
+
+def test_block_norm_refuses_out_over_what_other_rows_read(launches):
+    buf = torch.zeros(40, 64)
+    x, b, w = torch.zeros(6, 64), torch.ones(6, 64), torch.ones(64)
+    row = torch.zeros(6, 200)
+    for x_, branch, kw in (
+            (buf[:6], b, dict(out=buf[1:7])),                                # shifted by a row
+            (buf[1:7], b, dict(out=buf[:6])),
+            (buf.view(-1)[:384].view(6, 64), b, dict(out=buf.view(-1)[1:385].view(6, 64))),  # by a value
+            (buf[:12:2], b, dict(out=buf[:6])),                              # another row stride
+            (buf[:1].expand(6, 64), b, dict(out=buf[:6])),
+            (x, buf[:6], dict(out=buf[5:11])),
+            (x, buf[3].expand(6, 64), dict(out=buf[:6])),
+            (x, buf[:6].view(torch.bfloat16)[:, 64:], dict(out=buf[:6])),    # half of each row, another type
+            (x, b, dict(out=buf[:6], gate=buf[2])),
+            (x, b, dict(out=buf[:6], gate=buf[:6, :1])),
+            (x, b, dict(out=buf[:6], gate=buf[1:7])),
+            (x, b, dict(out=buf[:6], post_w=buf[5])),
+            (x, b, dict(out=buf[:6], pre_w=buf[0])),
+            (x[:1], b[:1], dict(out=buf[:1], post_w=buf[0])),
+            (x[:1], b[:1], dict(out=buf[:1], pre_w=buf[0])),                 # read once y is stored
+            (row[:, :64], b, dict(out=row[:, 63:127])),
+            (row.as_strided((5, 64), (200, 1), 140), b[:5], dict(out=row[:5, :64])),  # ends in the next row
+            (buf[:2], b[:2], dict(out=buf.view(-1)[10:138].view(2, 64))),
+            (buf[0], b[0], dict(out=buf.view(-1)[1:65]))):
+        with pytest.raises(ValueError, match="overlaps"):
+            block_norm(x_, branch, **kw)
+    assert not launches
+
+
+def test_block_norm_takes_out_beside_or_over_its_operands(launches):
+    buf, wide = torch.zeros(40, 64), torch.zeros(6, 256)
+    x, b, w = torch.zeros(6, 64), torch.ones(6, 64), torch.ones(64)
+    for x_, branch, kw in (
+            (x, b, dict(out=x)), (x, x, dict(out=x)), (x, b, dict(out=b)), (x, b, dict(out=x, gate=x)),
+            (buf[:1], b[:1], dict(out=buf[1:2], gate=buf[1])),
+            (buf[:6], buf[6:12], dict(out=buf[12:18], gate=buf[18], post_w=buf[19], pre_w=buf[20])),
+            (wide[:, :64], wide[:, 64:128], dict(out=wide[:, 128:192], gate=wide[:, 192:])),  # columns of one buffer
+            (wide[:, :64], wide[:, 64:128], dict(out=wide[:, :64], gate=wide[:, 192:193])),
+            (buf[1:13:2], b, dict(out=buf[:12:2])),                            # every second row and the others
+            (wide[1:2, :64], b[:1], dict(out=wide.view(-1)[256:320].view(1, 64))),  # one row, two strides
+            (x[:0], x[:0], dict(out=x[:0])), (x.t()[:6, :6], b[:, :6], dict(out=x[:, :6]))):
+        launches.clear()
+        y, _ = block_norm(x_, branch, **kw)
+        assert y is kw["out"] and [fn for fn, _ in launches] == ["vb_block_norm"]

@@ -385,6 +385,20 @@ def _rows_of(t: torch.Tensor, dim: int) -> torch.Tensor:
     return t if t.stride(1) == 1 or dim == 1 else t.contiguous()
 
 
+def _rows_meet(p: int, p_ld: int, p_width: int, rows: int, q: int, q_ld: int, q_width: int, q_rows: int) -> bool:
+    """Whether rows at p (each p_width bytes, p_ld >= p_width apart) share a byte with rows at q."""
+    if rows == 0 or q_rows == 0 or p >= q + (q_rows - 1) * q_ld + q_width or q >= p + (rows - 1) * p_ld + p_width:
+        return False
+    if rows == q_rows == 1:
+        return True
+    # per row of q: the first of p's rows that ends behind its begin, the last that begins before its end
+    begin = q - p + np.arange(q_rows, dtype=np.int64) * q_ld
+    step = max(p_ld, p_width)
+    first = np.maximum((begin - p_width) // step + 1, 0)
+    last = np.minimum((begin + q_width - 1) // step, rows - 1)
+    return bool((first <= last).any())
+
+
 # the current stream's handle without a Stream object around it, where torch has that (2 us less a call)
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or \
     (lambda index: torch.cuda.current_stream(index).cuda_stream)
@@ -419,7 +433,7 @@ def block_norm(x: torch.Tensor, branch: torch.Tensor, post_w=None, gate: torch.T
     residual stream ``x`` and the stream is normalised for the next block.  Returns ``(y, n)``:
 
         p = rms_norm(branch, post_w, eps)   (branch itself without post_w)
-        y = x + scale * gate * p            (x's type; ``out``, which may be x, or a new tensor)
+        y = x + scale * gate * p            (x's type; ``out``, which may be x or branch, or a new tensor)
         n = rms_norm(y, pre_w, eps)         (``normed_dtype``, x's type by default; None without pre_w)
 
     x and branch: (..., dim) of one shape, float32 / float16 / bfloat16 each, rows of any stride.  ``gate``
@@ -463,6 +477,24 @@ def block_norm(x: torch.Tensor, branch: torch.Tensor, post_w=None, gate: torch.T
         if yr is None or (yr.stride(1) != 1 and dim != 1):
             raise ValueError("block_norm: out must be rows of unit stride")
         y_ld = yr.stride(0)
+        # operands that lie under out value for value are read before they are stored over; no others are
+        size, y_ptr = out.element_size(), out.data_ptr()
+        y_end = y_ptr + ((rows - 1) * y_ld + dim) * size
+        for what, t, ptr, ld, width, count in (
+                ("x", xr, xr.data_ptr(), xr.stride(0), dim, rows), ("branch", br, br.data_ptr(), br.stride(0), dim, rows),
+                ("gate", gate, g_ptr, g_row, dim if g_col else 1, rows if g_row else 1),
+                ("post_w", post, None if post is None else post.data_ptr(), 0, dim, 1),
+                ("pre_w", pre, None if pre is None else pre.data_ptr(), 0, dim, 1)):
+            if ptr is None or ptr >= y_end:
+                continue
+            each = t.element_size()
+            if y_ptr >= ptr + ((count - 1) * ld + width) * each:
+                continue
+            if ptr == y_ptr and each == size and width == dim and count == rows and (rows == 1 or ld == y_ld) \
+                    and t is not post and t is not pre:
+                continue
+            if _rows_meet(y_ptr, y_ld * size, dim * size, rows, ptr, ld * each, width * each, count):
+                raise ValueError(f"block_norm: out overlaps {what}, which other rows read")
     n, n_ptr, n_type = None, None, 0
     if pre is not None:
         n = torch.empty_like(x, dtype=normed_dtype, memory_format=torch.contiguous_format)
