@@ -220,3 +220,25 @@ def test_block_norm_takes_out_beside_or_over_its_operands(launches):
         launches.clear()
         y, _ = block_norm(x_, branch, **kw)
         assert y is kw["out"] and [fn for fn, _ in launches] == ["vb_block_norm"]
+
+
+def host_weights(rows, k, group=32, zeros=False):
+    """A GroupQTensor's fields around bytes on the host (for calls that make no launch)."""
+    w = object.__new__(GroupQTensor)
+    w.data = torch.zeros(_lib.load().vb_group4_bytes(rows, k, group, int(zeros)) + 64, dtype=torch.uint8)
+    w.rows, w.k, w.group, w.zeros = rows, k, group, zeros
+    return w
+
+
+def test_group_gemv_takes_out_between_the_rows_of_x(launches):
+    w, buf = host_weights(16, 32), torch.zeros(3, 100)
+    x = buf[:, :32]
+    for out in (buf[0, 32:80], buf[1, 40:88], buf.view(-1)[252:300]):
+        launches.clear()
+        group_gemv(w, x, out=out)
+        assert [fn for fn, _ in launches] == ["vb_group4_gemv"]
+    launches.clear()
+    for out in (buf[0, 31:79], buf.view(-1)[60:108], buf.view(-1)[180:228], buf.view(-1)[231:279]):
+        with pytest.raises(ValueError, match="overlaps"):
+            group_gemv(w, x, out=out)
+    assert not launches

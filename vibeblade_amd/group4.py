@@ -12,7 +12,7 @@ from __future__ import annotations
 import torch
 
 from . import _lib
-from .tensor import _as_f32_dev, _check_out, _dev, _elem, _gpu_tensor, _launch, _rows_of
+from .tensor import _as_f32_dev, _check_out, _dev, _elem, _gpu_tensor, _launch, _rows_meet, _rows_of
 
 __all__ = ["GroupQTensor", "group_gemv"]
 
@@ -129,8 +129,8 @@ def group_gemv(w: GroupQTensor, x: torch.Tensor, out: torch.Tensor | None = None
         out = x.new_empty((w.rows,) if x.dim() == 1 else (m, w.rows), dtype=torch.float32)
     else:
         _check_out(out, m * w.rows, dev, "group_gemv")
-        end = xr.data_ptr() + ((m - 1) * xr.stride(0) + w.k) * xr.element_size()
-        if m > 0 and out.data_ptr() < end and xr.data_ptr() < out.data_ptr() + out.numel() * 4:
+        each = xr.element_size()
+        if _rows_meet(out.data_ptr(), 0, out.numel() * 4, 1, xr.data_ptr(), xr.stride(0) * each, w.k * each, m):
             raise ValueError("group_gemv: out overlaps x, which is read until the call's end")
     nbytes = _lib.load().vb_group4_workspace(m, w.rows, w.k, w.group, int(w.zeros), kind)
     ws = w.data.new_empty(nbytes) if nbytes > 0 else None
