@@ -242,3 +242,16 @@ def test_group_gemv_takes_out_between_the_rows_of_x(launches):
         with pytest.raises(ValueError, match="overlaps"):
             group_gemv(w, x, out=out)
     assert not launches
+
+
+def test_group_gemv_refuses_out_over_the_weights(launches):
+    w = host_weights(16, 32)
+    used = _lib.load().vb_group4_bytes(16, 32, 32, 0)
+    w.data, spare = w.data[:used], w.data.view(torch.float32)
+    x = torch.zeros(32)
+    for at in (0, 10, used // 4 - 1):
+        with pytest.raises(ValueError, match="overlaps"):
+            group_gemv(w, x, out=spare[at:at + 16])
+    assert not launches
+    group_gemv(w, x, out=spare[used // 4:used // 4 + 16])
+    assert launches

@@ -116,7 +116,7 @@ class GroupQTensor:
 def group_gemv(w: GroupQTensor, x: torch.Tensor, out: torch.Tensor | None = None) -> torch.Tensor:
     """y = W x for one activation vector (k,) -> (rows,) or a few of them (m, k) -> (m, rows), fp32
     (vb_group4_gemv).  x: float32, float16 or bfloat16 on w's device, rows of any stride.  out: contiguous
-    float32, apart from x."""
+    float32, apart from x and w."""
     dev = _gpu_tensor(x, "group_gemv: x")
     if dev != w.device:
         raise ValueError(f"group_gemv: x is on {dev}, W on {w.device}")
@@ -132,6 +132,8 @@ def group_gemv(w: GroupQTensor, x: torch.Tensor, out: torch.Tensor | None = None
         each = xr.element_size()
         if _rows_meet(out.data_ptr(), 0, out.numel() * 4, 1, xr.data_ptr(), xr.stride(0) * each, w.k * each, m):
             raise ValueError("group_gemv: out overlaps x, which is read until the call's end")
+        if m > 0 and w.ptr() - out.numel() * 4 < out.data_ptr() < w.ptr() + w.nbytes:
+            raise ValueError("group_gemv: out overlaps the weights")
     nbytes = _lib.load().vb_group4_workspace(m, w.rows, w.k, w.group, int(w.zeros), kind)
     ws = w.data.new_empty(nbytes) if nbytes > 0 else None
     _launch(dev, "vb_group4_gemv", w.ptr(), w.rows, w.k, w.group, int(w.zeros), xr.data_ptr(), kind, xr.stride(0), m,
