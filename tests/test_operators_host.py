@@ -170,6 +170,7 @@ def launches(monkeypatch):
     """Calls on CPU tensors up to their launches, which are written down and not made."""
     from vibeblade_amd import group4, tensor
     made = []
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: None)  # a CPU device's index
     for module in (tensor, group4):
         monkeypatch.setattr(module, "_gpu_tensor", lambda t, what: t.device)
         monkeypatch.setattr(module, "_launch", lambda dev, fn, *args: made.append((fn, args)))
@@ -255,3 +256,37 @@ def test_group_gemv_refuses_out_over_the_weights(launches):
     assert not launches
     group_gemv(w, x, out=spare[used // 4:used // 4 + 16])
     assert launches
+
+
+def test_workspaces_are_sized_on_the_device_that_runs_the_call(monkeypatch):
+    """The entry points size a workspace by the CUs of the current device: that of the tensors, for both calls."""
+    from contextlib import contextmanager
+    from types import SimpleNamespace
+    from vibeblade_amd import group4, tensor
+    current, seen = [0], []
+
+    @contextmanager
+    def device(index):
+        was, current[0] = current[0], index
+        yield
+        current[0] = was
+
+    def entry(name):
+        return lambda *args: seen.append((name, current[0])) or (32 if name.endswith("workspace") else 0)
+
+    fake = SimpleNamespace(**{name: entry(name) for name in ("vb_token_logprobs_workspace", "vb_token_logprobs",
+                                                             "vb_group4_workspace", "vb_group4_gemv")})
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: current[0])
+    monkeypatch.setattr(torch.cuda, "device", device)
+    monkeypatch.setattr(_lib, "load", lambda: fake)
+    monkeypatch.setattr(_lib, "init", lambda index: None)
+    monkeypatch.setattr(tensor, "_raw_stream", lambda index: 0)
+    for module in (tensor, group4):
+        monkeypatch.setattr(module, "_gpu_tensor", lambda t, what: torch.device("cuda", 1))
+    token_logprobs(torch.zeros(2, 10), torch.zeros(2, dtype=torch.int64))
+    w = SimpleNamespace(device=torch.device("cuda", 1), data=torch.zeros(1, dtype=torch.uint8), rows=4, k=10, group=32,
+                        zeros=False, ptr=lambda: 0)
+    group_gemv(w, torch.zeros(10))
+    assert seen == [(name, 1) for name in ("vb_token_logprobs_workspace", "vb_token_logprobs", "vb_group4_workspace",
+                                           "vb_group4_gemv")]
+    assert current == [0]

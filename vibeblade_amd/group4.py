@@ -12,7 +12,8 @@ from __future__ import annotations
 import torch
 
 from . import _lib
-from .tensor import _as_f32_dev, _check_out, _dev, _elem, _gpu_tensor, _launch, _rows_meet, _rows_of
+from .tensor import (_as_f32_dev, _check_out, _dev, _elem, _gpu_tensor, _launch, _rows_meet, _rows_of,
+                     _workspace_bytes)
 
 __all__ = ["GroupQTensor", "group_gemv"]
 
@@ -134,7 +135,7 @@ def group_gemv(w: GroupQTensor, x: torch.Tensor, out: torch.Tensor | None = None
             raise ValueError("group_gemv: out overlaps x, which is read until the call's end")
         if m > 0 and w.ptr() - out.numel() * 4 < out.data_ptr() < w.ptr() + w.nbytes:
             raise ValueError("group_gemv: out overlaps the weights")
-    nbytes = _lib.load().vb_group4_workspace(m, w.rows, w.k, w.group, int(w.zeros), kind)
+    nbytes = _workspace_bytes(dev, "vb_group4_workspace", m, w.rows, w.k, w.group, int(w.zeros), kind)
     ws = w.data.new_empty(nbytes) if nbytes > 0 else None
     _launch(dev, "vb_group4_gemv", w.ptr(), w.rows, w.k, w.group, int(w.zeros), xr.data_ptr(), kind, xr.stride(0), m,
             out.data_ptr(), None if ws is None else ws.data_ptr(), nbytes)

@@ -416,6 +416,14 @@ def _launch(dev: torch.device, fn: str, *args) -> None:
         _lib.check(fn, rc)
 
 
+def _workspace_bytes(dev: torch.device, fn: str, *args) -> int:
+    """fn(*args), which sizes a workspace by the current device's CUs, on the device of the launch."""
+    if dev.index != torch.cuda.current_device():
+        with torch.cuda.device(dev.index):
+            return getattr(_lib.load(), fn)(*args)
+    return getattr(_lib.load(), fn)(*args)
+
+
 def _norm_weight(w, dim: int, dev, what: str) -> torch.Tensor | None:
     if w is None:
         return None
@@ -543,7 +551,7 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor | None, top: int =
     entropy = lp.new_empty(rows)
     best = lp.new_empty((rows, top))
     ids = torch.empty_like(best, dtype=torch.int32)
-    nbytes = _lib.load().vb_token_logprobs_workspace(rows, vocab, top)
+    nbytes = _workspace_bytes(dev, "vb_token_logprobs_workspace", rows, vocab, top)
     ws = lp.new_empty((nbytes + 3) // 4) if nbytes > 0 else None
     _launch(dev, "vb_token_logprobs", z.data_ptr(), kind, z.stride(0), rows, vocab, temperature,
             tokens.data_ptr(), tokens.element_size(), each, lp.data_ptr(), entropy.data_ptr(), top, ids.data_ptr(),
