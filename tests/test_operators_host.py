@@ -290,3 +290,16 @@ def test_workspaces_are_sized_on_the_device_that_runs_the_call(monkeypatch):
     assert seen == [(name, 1) for name in ("vb_token_logprobs_workspace", "vb_token_logprobs", "vb_group4_workspace",
                                            "vb_group4_gemv")]
     assert current == [0]
+
+
+@pytest.mark.parametrize("group", [(1 << 32) + 128, (1 << 32) + 32, 1 << 32, 1 << 31, (1 << 40) + 256])
+def test_group4_refuses_groups_past_32_bits(launches, group):
+    """The entry points take 32 bits, of which ctypes would pass the low ones: another group, with more scales."""
+    packed, scales = torch.zeros((2, 512), dtype=torch.uint8), torch.zeros((2, 1), dtype=torch.float16)
+    with pytest.raises(ValueError, match="group"):
+        GroupQTensor.from_packed(packed, scales, k=1024, group=group)
+    with pytest.raises(ValueError, match="group"):
+        GroupQTensor(packed, 2, 1024, group, False)
+    assert not launches
+
+

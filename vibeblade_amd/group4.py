@@ -19,8 +19,8 @@ __all__ = ["GroupQTensor", "group_gemv"]
 
 
 def _groups(k: int, group: int) -> int:
-    if group not in (32, 64) and (group <= 0 or group % 128):
-        raise ValueError(f"group must be 32, 64 or a multiple of 128, got {group}")
+    if group not in (32, 64) and (group <= 0 or group % 128 or group >= 1 << 31):
+        raise ValueError(f"group must be 32, 64 or a multiple of 128 below 2^31, got {group}")
     return -(-k // group)
 
 
@@ -28,6 +28,7 @@ class GroupQTensor:
     """A 4-bit weight matrix (rows outputs x k inputs) with group scales, resident on one GPU."""
 
     def __init__(self, data: torch.Tensor, rows: int, k: int, group: int, zeros: bool):
+        _groups(k, group)
         if not isinstance(data, torch.Tensor) or data.dtype != torch.uint8 or data.device.type != "cuda":
             raise ValueError("GroupQTensor data must be a cuda uint8 tensor")
         nbytes = _lib.load().vb_group4_bytes(rows, k, group, int(zeros))
