@@ -303,3 +303,8 @@ def test_group4_refuses_groups_past_32_bits(launches, group):
     assert not launches
 
 
+def test_token_logprobs_refuses_more_tokens_than_32_bits_count(launches):
+    for t in ((1 << 31), (1 << 32) + 1):
+        with pytest.raises(ValueError, match="tokens"):
+            token_logprobs(torch.zeros(1, 10), torch.zeros((1, 1), dtype=torch.int32).expand(1, t))
+    assert not launches

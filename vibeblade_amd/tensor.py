@@ -545,8 +545,10 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor | None, top: int =
         raise ValueError(f"token_logprobs: tokens must be int32 or int64, got {tokens.dtype}")
     if tokens.dim() not in (1, 2) or tokens.shape[0] != rows:
         raise ValueError(f"token_logprobs: tokens must be ({rows},) or ({rows}, t), got {tuple(tokens.shape)}")
-    tokens = tokens.contiguous()
     each = tokens.shape[1] if tokens.dim() == 2 else 1
+    if each >= 1 << 31:
+        raise ValueError(f"token_logprobs: {each} tokens per row (fewer than 2^31)")
+    tokens = tokens.contiguous()
     lp = torch.empty_like(tokens, dtype=torch.float32)
     entropy = lp.new_empty(rows)
     best = lp.new_empty((rows, top))
