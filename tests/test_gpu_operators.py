@@ -854,3 +854,12 @@ def test_block_norm_in_columns_of_one_buffer():
     assert torch.equal(y, want[0]) and torch.equal(n, want[1])
     with pytest.raises(ValueError, match="overlaps"):
         block_norm(x, b, out=wide[:, 129:259])
+
+
+def test_block_norm_gates_of_few_values_at_any_stride():
+    for rows, dim in ((1, 1), (4, 1), (0, 64), (1, 64)):
+        x, b = normal(1, rows, dim).cuda(), normal(2, rows, dim).cuda()
+        pre = (1 + normal(3, dim, scale=0.1)).cuda()
+        for gate in (normal(4, rows, 5 * dim).cuda()[:, ::5], normal(5, 5 * dim).cuda()[::5]):
+            y, n = block_norm(x, b, gate=gate, pre_w=pre)
+            check_norm(x, b, None, gate.expand(rows, dim), 1.0, pre, 1e-5, y, n)

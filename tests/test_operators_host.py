@@ -308,3 +308,15 @@ def test_token_logprobs_refuses_more_tokens_than_32_bits_count(launches):
         with pytest.raises(ValueError, match="tokens"):
             token_logprobs(torch.zeros(1, 10), torch.zeros((1, 1), dtype=torch.int32).expand(1, t))
     assert not launches
+
+
+@pytest.mark.parametrize("rows,dim", [(1, 1), (0, 64), (0, 1), (4, 1), (1, 64), (4, 64)])
+def test_block_norm_hands_over_gates_of_any_stride(launches, rows, dim):
+    """Columns apart, also where there are too few values for torch to call such a gate strided."""
+    x = torch.zeros(rows, dim)
+    for gate in (torch.zeros(rows, 5 * dim)[:, ::5], torch.zeros(5 * dim)[::5], torch.zeros(dim, rows).t(),
+                 torch.zeros(rows, 1, 7)[:, :, 3], torch.zeros(3, rows, dim).permute(1, 2, 0)[:, :, 1]):
+        launches.clear()
+        block_norm(x, x.clone(), gate=gate)
+        (_, args), = launches
+        assert args[6] >= 0 and args[7] in (0, 1)  # gate_row, gate_col

@@ -471,7 +471,8 @@ def block_norm(x: torch.Tensor, branch: torch.Tensor, post_w=None, gate: torch.T
             g = g.reshape(-1, dim)
         if g.stride(1) not in (0, 1):
             g = g.contiguous()
-        g_ptr, g_row, g_col = g.data_ptr(), g.stride(0), g.stride(1)
+        # (a column, or no rows at all, is contiguous to torch at any stride along the row)
+        g_ptr, g_row, g_col = g.data_ptr(), g.stride(0), min(g.stride(1), 1)
     y_ld = dim
     if out is None:
         out = torch.empty_like(x, memory_format=torch.contiguous_format)
