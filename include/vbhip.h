@@ -427,7 +427,8 @@ int vb_group4_pack(const uint8_t* packed, const void* scales, const uint8_t* zer
 /* The parts of a weight matrix src (rows x k, row stride ld, element type as
  * above).  Symmetric (zeros NULL): s = fp16(max |w| / 7).  With zeros: over
  * the group's range stretched to hold 0, s = fp16((hi - lo) / 15), z =
- * round(-lo / s).  q = round(w / s) + z, clamped to 0..15. */
+ * round(-lo / s).  s is 65504 at most.  q = round(w / s) + z, clamped to
+ * 0..15.  A group that holds a NaN or an infinity has the scale NaN. */
 int vb_group4_quantize(const void* src, int32_t type, int64_t ld, int64_t rows, int64_t k, int32_t group,
                        uint8_t* packed, void* scales, uint8_t* zeros, void* stream);
 /* out[n * k + i] = W[n, i] of packed weights w, fp32 (exact). */

@@ -863,3 +863,24 @@ def test_block_norm_gates_of_few_values_at_any_stride():
         for gate in (normal(4, rows, 5 * dim).cuda()[:, ::5], normal(5, 5 * dim).cuda()[::5]):
             y, n = block_norm(x, b, gate=gate, pre_w=pre)
             check_norm(x, b, None, gate.expand(rows, dim), 1.0, pre, 1e-5, y, n)
+
+
+@pytest.mark.parametrize("zeros", [False, True])
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("group", [32, 128])
+def test_group4_quantize_keeps_what_is_no_number(dtype, zeros, group):
+    """A NaN or an infinity has no code: its group is NaN, and no other one changes."""
+    src = normal(41, 9, 300, scale=0.02, dtype=dtype)
+    want = GroupQTensor.quantize(src.cuda(), group=group, zeros=zeros).dequantize().cpu()
+    bad = {(1, 0): math.nan, (2, group - 1): INF, (3, group): -INF, (4, 299): math.nan, (5, 298): INF}
+    for (r, c), v in bad.items():
+        src[r, c] = v
+        want[r, c // group * group:(c // group + 1) * group] = math.nan
+    src[6, 4], src[6, 5] = INF, -INF
+    want[6, :group] = math.nan
+    w = GroupQTensor.quantize(src.cuda(), group=group, zeros=zeros)
+    got = w.dequantize().cpu()
+    assert torch.equal(got.isnan(), want.isnan()) and torch.equal(got.nan_to_num(7), want.nan_to_num(7))
+    for m, xt in ((1, F32), (3, BF16), (8, F16)):
+        y = group_gemv(w, normal(m, m, 300, dtype=xt).cuda()).cpu()
+        assert y[:, 1:7].isnan().all() and y[:, [0, 7, 8]].isfinite().all()

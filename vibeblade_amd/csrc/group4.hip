@@ -85,20 +85,24 @@ __global__ void __launch_bounds__(256) g4_dequant_kernel(G4Weights g, float* out
 
 // One thread per group of a row.  Symmetric: s = absmax / 7, codes 1..15
 // around 8.  With zeros: the range is stretched to hold 0, s = (hi - lo) / 15,
-// z = round(-lo / s).  s is rounded to fp16 first and the codes go by that.
+// z = round(-lo / s).  s is rounded to fp16 first (at most 65504, and weights
+// past its codes take the last one) and the codes go by that.  A NaN or an
+// infinity has no code: its group's scale is NaN.
 __global__ void __launch_bounds__(256) g4_quantize_kernel(const void* src, int32_t type, int64_t ld, int64_t rows,
                                                           int64_t k, int32_t group, int64_t groups, uint8_t* codes,
                                                           _Float16* scales, uint8_t* zeros) {
     for (int64_t i = first_item(); i < rows * groups; i += item_stride()) {
         const int64_t row = i / groups, k0 = i % groups * group, end = k0 + group < k ? k0 + group : k;
         float lo = 0.f, hi = 0.f;
+        bool finite = true;
         for (int64_t j = k0; j < end; j++) {
             const float v = elem_ld(src, row * ld + j, type);
+            finite = finite && fabsf(v) < INFINITY;
             lo = fminf(lo, v);
             hi = fmaxf(hi, v);
         }
         const float want = zeros ? (hi - lo) / 15.f : fmaxf(hi, -lo) / 7.f;
-        const _Float16 sh = static_cast<_Float16>(fminf(want, 65504.f));
+        const _Float16 sh = static_cast<_Float16>(finite ? fminf(want, 65504.f) : NAN);
         const float s = static_cast<float>(sh);
         const float z = !zeros ? 8.f : s > 0.f ? fminf(fmaxf(rintf(-lo / s), 0.f), 15.f) : 0.f;
         scales[i] = sh;

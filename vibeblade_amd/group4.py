@@ -88,7 +88,8 @@ class GroupQTensor:
 
     @classmethod
     def quantize(cls, w, group: int = 128, zeros: bool = True, device=None) -> "GroupQTensor":
-        """Quantize a (rows, k) matrix on the device (vb_group4_quantize)."""
+        """Quantize a (rows, k) matrix on the device (vb_group4_quantize).  A group that holds a NaN or an infinity
+        becomes NaN."""
         if isinstance(w, torch.Tensor) and w.is_cuda and device is None:
             dev, src = w.device, w
             _elem(src, "GroupQTensor.quantize: w")
