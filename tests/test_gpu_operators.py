@@ -884,3 +884,12 @@ def test_group4_quantize_keeps_what_is_no_number(dtype, zeros, group):
     for m, xt in ((1, F32), (3, BF16), (8, F16)):
         y = group_gemv(w, normal(m, m, 300, dtype=xt).cuda()).cpu()
         assert y[:, 1:7].isnan().all() and y[:, [0, 7, 8]].isfinite().all()
+
+
+def test_group4_refuses_zero_points_past_four_bits():
+    packed, s, z, _ = parts(16, 20, 100, 32, True)
+    z[19, 3] = 16
+    with pytest.raises(ValueError, match="zero points"):
+        GroupQTensor.from_packed(packed, s, z, k=100, group=32)
+    z[19, 3] = 15
+    GroupQTensor.from_packed(packed, s, z, k=100, group=32)

@@ -320,3 +320,13 @@ def test_block_norm_hands_over_gates_of_any_stride(launches, rows, dim):
         block_norm(x, x.clone(), gate=gate)
         (_, args), = launches
         assert args[6] >= 0 and args[7] in (0, 1)  # gate_row, gate_col
+
+
+def test_group4_refuses_zero_points_past_four_bits(launches):
+    packed, scales = torch.zeros((3, 32), dtype=torch.uint8), torch.zeros((3, 2), dtype=torch.float16)
+    for bad in (16, 255):
+        zeros = torch.full((3, 2), 15, dtype=torch.uint8)
+        zeros[2, 1] = bad
+        with pytest.raises(ValueError, match="zero points"):
+            GroupQTensor.from_packed(packed, scales, zeros, k=64, group=32)
+    assert not launches

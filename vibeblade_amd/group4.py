@@ -61,7 +61,7 @@ class GroupQTensor:
                     group: int = 128) -> "GroupQTensor":
         """From device tensors: packed (rows, ceil(k / 2)) uint8 with code 2i of a row in the low half of its byte
         i (``quant.pack_nibbles`` order), scales (rows, ceil(k / group)) float16, zeros of that shape, uint8 in
-        0..15 (None: 8 everywhere).  The parts are not kept."""
+        0..15 (None: 8 everywhere; the check of these values waits for the device).  The parts are not kept."""
         dev = _gpu_tensor(packed, "GroupQTensor: packed")
         k, group = int(k), int(group)
         if packed.dim() != 2 or packed.dtype != torch.uint8 or packed.shape[0] == 0 or k <= 0 \
@@ -76,6 +76,13 @@ class GroupQTensor:
             if _gpu_tensor(t, f"GroupQTensor: {name}") != dev or t.dtype != dtype or tuple(t.shape) != want:
                 raise ValueError(f"GroupQTensor: {name} must be {want} {dtype} on {dev}, got {tuple(t.shape)} "
                                  f"{t.dtype} on {t.device}")
+        if zeros is not None and bool((zeros > 15).any()):
+            raise ValueError("GroupQTensor: zero points must be 0 to 15")
+        return cls._pack(packed, scales, zeros, k, group)
+
+    @classmethod
+    def _pack(cls, packed, scales, zeros, k: int, group: int) -> "GroupQTensor":
+        rows, dev = packed.shape[0], packed.device
         packed, scales = packed.contiguous(), scales.contiguous()
         zeros = None if zeros is None else zeros.contiguous()
         nbytes = _lib.load().vb_group4_bytes(rows, k, group, int(zeros is not None))
@@ -106,7 +113,7 @@ class GroupQTensor:
         z = torch.empty((rows, groups), dtype=torch.uint8, device=dev) if zeros else None
         _launch(dev, "vb_group4_quantize", src.data_ptr(), _elem(src, "GroupQTensor.quantize: w"), src.stride(0), rows, k,
                 int(group), packed.data_ptr(), scales.data_ptr(), None if z is None else z.data_ptr())
-        return cls.from_packed(packed, scales, z, k=k, group=group)
+        return cls._pack(packed, scales, z, k, int(group))
 
     def dequantize(self) -> torch.Tensor:
         """The weights in fp32 (rows, k), exact (vb_group4_dequant_rows)."""
