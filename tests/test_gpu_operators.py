@@ -893,3 +893,40 @@ def test_group4_refuses_zero_points_past_four_bits():
         GroupQTensor.from_packed(packed, s, z, k=100, group=32)
     z[19, 3] = 15
     GroupQTensor.from_packed(packed, s, z, k=100, group=32)
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("m", [1, 2, 4, 8, 16])
+@pytest.mark.parametrize("group,zeros", [(32, True), (64, False), (128, True)])
+def test_group4_small_activations_beside_large_ones(dtype, m, group, zeros):
+    """Each output is one activation times one weight (every other code is the zero point), so what is lost of a
+    value beside an outlier of its block of 128 is seen by itself.  With `big` the block's largest magnitude: fp32 is
+    exact from 2^-6 big on and below within 2^-30 big, 16-bit digits from 2^-14 (bf16) or 2^-11 (fp16) on and within
+    2^-22, fp16 operands throughout, bf16 ones brought to fp16 from 2^-31 on and within 2^-38."""
+    k = 384
+    rng = np.random.default_rng(m)
+    z = rng.integers(0, 16, (k, -(-k // group)), dtype=np.uint8) if zeros else None
+    at = np.arange(k) // group
+    q = (z[:, at] if zeros else np.full((k, k), 8)).astype(np.int64)
+    diag = np.arange(k)
+    own = q[diag, diag]
+    q[diag, diag] = np.where(own < 8, own + 3, own - 3)
+    s = np.full((k, -(-k // group)), 0.5, dtype=np.float16)
+    packed = np.stack([pack_nibbles(r.astype(np.uint8)) for r in q])
+    w = GroupQTensor.from_packed(torch.from_numpy(packed).cuda(), torch.from_numpy(s).cuda(),
+                                 torch.from_numpy(z).cuda() if zeros else None, k=k, group=group)
+    gain = torch.from_numpy(np.where(own < 8, 1.5, -1.5))
+    small = 2.0 ** -14 if dtype == F16 else 2.0 ** -30
+    x = normal(m, m, k) * torch.from_numpy(small ** rng.uniform(0, 1, (m, k))).float()
+    x[:, 200] = torch.from_numpy(rng.uniform(500, 4000, m)).float()  # the second block's outlier
+    x[:, 256:] *= 2.0 ** -6                                          # the third has its own scale
+    x = x.to(dtype)
+    as_fp16 = m > 5 or (dtype == F16 and m > 2)
+    exact, lost = {F32: (6, 30), F16: (99, 99) if as_fp16 else (11, 22), BF16: (31, 38) if as_fp16 else (14, 22)}[dtype]
+    v = x.double()
+    big = v.abs().view(m, 3, 128).amax(2, keepdim=True).expand(m, 3, 128).reshape(m, k)
+    tol = torch.where(v.abs() >= 2.0 ** -exact * big, 0.0, 2.0 ** -lost * big) + 8 * U * v.abs()
+    close(group_gemv(w, x.cuda()), v * gain, tol * 1.5)
+    if lost < 99:  # a few bits fewer would be seen
+        step = 2.0 ** (4 - lost) * big.log2().floor().exp2()
+        assert (((v / step).round() * step - v).abs() > tol).any()
