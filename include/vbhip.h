@@ -401,8 +401,9 @@ int vb_block_norm(const void* branch, int32_t branch_type, int64_t branch_ld, co
  * log probabilities -inf and entropy 0; a -inf logit is not named among the
  * alternatives (id -1, log probability -inf); a row with a NaN or +inf has
  * NaN for its log probabilities and entropy.  workspace: at least
- * vb_token_logprobs_workspace(rows, vocab, top) bytes (0: none), 16-byte
- * aligned, free again when the call's work is done. */
+ * vb_token_logprobs_workspace(rows, vocab, top) bytes (0: none; asked on the
+ * device of the call), 16-byte aligned, free again when the call's work is
+ * done. */
 int64_t vb_token_logprobs_workspace(int64_t rows, int64_t vocab, int32_t top);
 int vb_token_logprobs(const void* logits, int32_t type, int64_t ld, int64_t rows, int64_t vocab, float temperature,
                       const void* tokens, int32_t token_bytes, int32_t n_tokens, float* logprobs, float* entropy,
@@ -440,10 +441,12 @@ int vb_group4_dequant_rows(const void* w, float* out, int64_t rows, int64_t k, i
  * below a power of two that holds the largest of them, and the products with
  * the codes are summed exactly in a group; or, where there are several tokens
  * of 16 bits, as fp16 values below such a power (fp16 ones as they are), summed
- * in fp32.  Groups are summed in fp32.  A NaN or an infinity gives its token NaN
- * or infinities, no other one.  y overlaps neither x nor w.  workspace: at least
- * vb_group4_workspace(...) bytes (0: none), 16-byte aligned, free again when the
- * call's work is done. */
+ * in fp32.  Groups are summed in fp32.  Which form is taken, and the order of
+ * the groups, go by m and rows: a token's last bits may depend on how many come
+ * with it.  A NaN or an infinity gives its token NaN or infinities, no other
+ * one.  y overlaps neither x nor w.  workspace: at least vb_group4_workspace(...)
+ * bytes (0: none; asked on the device of the call), 16-byte aligned, free again
+ * when the call's work is done. */
 int64_t vb_group4_workspace(int64_t m, int64_t rows, int64_t k, int32_t group, int32_t has_zeros, int32_t x_type);
 int vb_group4_gemv(const void* w, int64_t rows, int64_t k, int32_t group, int32_t has_zeros, const void* x,
                    int32_t x_type, int64_t x_ld, int64_t m, float* y, void* workspace, size_t workspace_bytes,

@@ -14,7 +14,7 @@
 // written once.  Rows longer than the registers of a workgroup are read again
 // for each sum (seam_long_kernel).
 //
-// Memory bounds it: fp32 rows run at 6.0 to 6.3 TB/s of what is read and written
+// Memory bounds it: fp32 rows run at 6.0 to 6.5 TB/s of what is read and written
 // (4096 x 8192 86 us, 8192 x 4096 with fp16 n 73), 16-bit ones at 5.2 to 5.8
 // (8192 x 4096 46 us), rows of odd length at 4.9 (7001 x 5121, a full gate: 103
 // us; 7001 x 5120 82).  One row of 4096 takes 3.4 us in a graph, of which a

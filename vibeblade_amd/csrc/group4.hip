@@ -130,18 +130,18 @@ __global__ void __launch_bounds__(256) g4_quantize_kernel(const void* src, int32
 // 100 issue slots for a step's 1 KB.
 //
 // Bound by memory where the weights are large (one token, us and TB/s of weights:
-// 128256 x 4096 44 and 6.2, 128256 x 14336 145 and 6.5); below that by what comes
-// before and behind the stream (14336 x 4096 9.2 and 3.3, 4096 x 4096 5.9, of
+// 128256 x 4096 44 and 6.2, 128256 x 14336 147 and 6.5); below that by what comes
+// before and behind the stream (14336 x 4096 9.0 and 3.4, 4096 x 4096 5.9, of
 // which a launch is 1.9, the first loads, digits and barrier about 2 and the
 // sums over waves 0.5); with more tokens by staging them and, in groups of 32,
-// by the multiplications and sums of each group (128256 x 4096, five tokens 56).
+// by the multiplications and sums of each group (128256 x 4096, five tokens 54).
 //
 // The B operand's 16 columns are the activations as integers: each block of 128
 // of a token, brought by a power of two to |X| < 2^30 (fp32 x) or 2^22 (16-bit
 // x) and rounded, is split into 4 or 3 signed digits to the base 256, one
 // column each.  fp32 values keep all their bits down to 2^-6 of the block's
 // largest, bf16 and fp16 ones down to 2^-14 and 2^-11; what is lost below is at
-// most 2^-31 (2^-23) of the largest.  Sums over a group are exact:
+// most 2^-30 (2^-22) of the largest.  Sums over a group are exact:
 //
 //   sum (q - z) X = sum (q - 8) X - (z - 8) sum X
 //
@@ -154,8 +154,8 @@ __global__ void __launch_bounds__(256) g4_quantize_kernel(const void* src, int32
 // More than a few 16-bit tokens would take two or three such sets of columns, so
 // they go to v_mfma_f32_16x16x32_f16 as they are, a column each: fp16 values
 // unchanged, bf16 ones brought to |x| < 2^15 by a power of two for each block of
-// 128 (exact down to 2^-29 of its largest, cut there to multiples of 2^-39 of
-// it).  The weights' codes become fp16 integers q - z, exactly; a group's
+// 128 (exact down to 2^-31 of its largest, below that cut to multiples of fp16's
+// 2^-24, at most 2^-38 of it).  The weights' codes become fp16 integers q - z, exactly; a group's
 // products are summed in fp32.
 typedef _Float16 half2_t __attribute__((ext_vector_type(2)));
 typedef _Float16 half8_t __attribute__((ext_vector_type(8)));

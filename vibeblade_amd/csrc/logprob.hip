@@ -29,10 +29,11 @@
 // before it) and the threshold rises.  The waves' buffers, and the lists of a
 // row's slices where there are few rows, are joined and ranked once.
 //
-// Memory bounds many rows (512 x 128256 fp32 43 us, 6.1 TB/s, with five
-// alternatives 49; 1500 x 151669 bf16 73, 6.2 TB/s); few rows wait for the two
+// Memory bounds many rows (512 x 128256 fp32 41 us, 6.4 TB/s, with five
+// alternatives 45; 1500 x 151669 bf16 73, 6.2 TB/s); few rows wait for the two
 // launches, and with alternatives for the threshold and the ranking in each
-// (1 x 128256: 5.6 us, with twenty 11.6).
+// (1 x 128256: 5.7 us, with twenty 11.8).  No vector register is spilled; with
+// alternatives 46 scalar ones are kept in lanes of vector registers.
 #include <type_traits>
 
 #include "elem_types.hpp"
@@ -553,9 +554,10 @@ __global__ void __launch_bounds__(64) logprob_join_kernel(LpArgs a) {
 
 // Slices of a row.  A row is one workgroup's from two rows a CU on, as slices
 // have a threshold and a list each and the launch that joins them (512 x 128256
-// fp32, five alternatives: 50 us whole, 54 halved, 55 in four; without a list
-// 43, 46, 48); fewer rows make three workgroups a CU (64 rows: 24 us with two,
-// 21 with three or four, 25 with eight).  Each wave has a batch or more.
+// fp32, five alternatives: 45 us whole, 49 halved, 52 in four; without a list
+// 41, 44, 46); fewer rows make three workgroups a CU (256 rows, five
+// alternatives: 36 us with one, 30 with two to four; 64, twenty: 23 with two, 22
+// with three, 21 with four, 23 with eight).  Each wave has a batch or more.
 int64_t lp_splits(int64_t rows, int64_t vocab) {
     if (rows <= 0 || rows >= 2 * num_cus()) return 1;
     const int64_t want = (3 * num_cus() + rows - 1) / rows;

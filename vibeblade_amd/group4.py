@@ -126,7 +126,15 @@ class GroupQTensor:
 def group_gemv(w: GroupQTensor, x: torch.Tensor, out: torch.Tensor | None = None) -> torch.Tensor:
     """y = W x for one activation vector (k,) -> (rows,) or a few of them (m, k) -> (m, rows), fp32
     (vb_group4_gemv).  x: float32, float16 or bfloat16 on w's device, rows of any stride.  out: contiguous
-    float32, apart from x and w."""
+    float32, apart from x and w.
+
+    Products with the codes are exact and summed in fp32 or wider, but of an activation much smaller than the
+    largest of its 128 neighbours (blocks of 128 along k) the last bits are dropped: fp32 keeps all of them from
+    2^-6 of that largest on and loses at most 2^-30 of it below; 16-bit types from 2^-14 (bfloat16) or 2^-11
+    (float16) on and at most 2^-22; with more than a few tokens float16 goes in as it is and bfloat16 loses at most
+    2^-38.  Which of the two forms 16-bit tokens take, and in which order groups are summed, depends on their number
+    and the number of rows: the same token in another batch may differ in its last bits.  The same call gives the
+    same bits.  A NaN or an infinity makes its own token's results NaN or infinite."""
     dev = _gpu_tensor(x, "group_gemv: x")
     if dev != w.device:
         raise ValueError(f"group_gemv: x is on {dev}, W on {w.device}")
