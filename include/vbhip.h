@@ -443,7 +443,8 @@ int vb_group4_dequant_rows(const void* w, float* out, int64_t rows, int64_t k, i
  * of 16 bits, as fp16 values below such a power (fp16 ones as they are), summed
  * in fp32.  Groups are summed in fp32.  Which form is taken, and the order of
  * the groups, go by m and rows: a token's last bits may depend on how many come
- * with it.  A NaN or an infinity gives its token NaN or infinities, no other
+ * with it.  Results are finite while 4 sum |W| max |x| (the maximum of each 128)
+ * is below 2^128.  A NaN or an infinity gives its token NaN or infinities, no other
  * one.  y overlaps neither x nor w.  workspace: at least vb_group4_workspace(...)
  * bytes (0: none; asked on the device of the call), 16-byte aligned, free again
  * when the call's work is done. */

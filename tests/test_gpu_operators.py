@@ -930,3 +930,19 @@ def test_group4_small_activations_beside_large_ones(dtype, m, group, zeros):
     if lost < 99:  # a few bits fewer would be seen
         step = 2.0 ** (4 - lost) * big.log2().floor().exp2()
         assert (((v / step).round() * step - v).abs() > tol).any()
+
+
+@pytest.mark.parametrize("dtype,m", [(F32, 1), (F32, 2), (F32, 9), (BF16, 3), (BF16, 8)])
+@pytest.mark.parametrize("zeros", [False, True])
+def test_group4_largest_activations(dtype, m, zeros):
+    """Up to the range that the header gives: 4 sum |W| max |x| just below 2^128."""
+    k = 384
+    packed, s, z, w64 = parts(61, 40, k, 128, zeros)
+    w = GroupQTensor.from_packed(packed, s, z, k=k, group=128)
+    x = normal(62, m, k).double()
+    top = x.abs().view(m, 3, 128).amax(2)  # per block
+    bound = 4 * torch.einsum("nb,mb->mn", w64.abs().view(40, 3, 128).sum(2), top).amax(1, keepdim=True)
+    x = (x * (0.98 * 2.0 ** 128 / bound)).to(dtype)
+    y = group_gemv(w, x.cuda())
+    assert y.isfinite().all()
+    check_product(w, w64, x, y)

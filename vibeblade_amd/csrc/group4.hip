@@ -147,7 +147,9 @@ __global__ void __launch_bounds__(256) g4_quantize_kernel(const void* src, int32
 //
 // with sum X found once as x is staged.  Then, in fp32, a group's sum is
 // multiplied by its scale and the block's power of two and added up; the digits
-// of a token meet at the end.  A block with a NaN or an infinity has the power
+// of a token meet at the end.  Until then each digit counts as the top one, so a
+// sum may be up to 4 sum |W| max |x| (over each block) and has to stay below
+// 2^128.  A block with a NaN or an infinity has the power
 // NaN, which stays in its token.  Columns past the tokens repeat the last one
 // and are dropped.
 //
