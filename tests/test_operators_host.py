@@ -330,3 +330,21 @@ def test_group4_refuses_zero_points_past_four_bits(launches):
         with pytest.raises(ValueError, match="zero points"):
             GroupQTensor.from_packed(packed, scales, zeros, k=64, group=32)
     assert not launches
+
+
+def test_rows_meet_as_their_bytes_do():
+    import random
+    from vibeblade_amd.tensor import _rows_meet
+    rng = random.Random(0)
+    seen = [0, 0]
+    for _ in range(20000):
+        width, q_width = rng.randint(1, 9), rng.randint(1, 9)
+        rows, q_rows = rng.randint(0, 5), rng.randint(0, 5)
+        p_ld, q_ld = width + rng.randint(0, 12), rng.randint(0, 20)
+        p, q = rng.randint(100, 160), rng.randint(100, 160)
+        ours = {p + i * p_ld + j for i in range(rows) for j in range(width)}
+        theirs = {q + i * q_ld + j for i in range(q_rows) for j in range(q_width)}
+        want = bool(ours & theirs)
+        seen[want] += 1
+        assert _rows_meet(p, p_ld, width, rows, q, q_ld, q_width, q_rows) == want
+    assert min(seen) > 2000
