@@ -946,3 +946,13 @@ def test_group4_largest_activations(dtype, m, zeros):
     y = group_gemv(w, x.cuda())
     assert y.isfinite().all()
     check_product(w, w64, x, y)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("vocab", [30, 9000])
+def test_token_logprobs_of_opposite_ends_of_the_range(dtype, vocab):
+    """z - max leaves fp32's range where the log probability, over a temperature, does not."""
+    z = normal(71, 2, vocab, scale=1e38).clamp(-3e38, 3e38).to(dtype)
+    z[0, 3], z[0, 20], z[1, 7], z[1, 8] = 3.2e38, -3.2e38, -3.2e38, 3.3e38
+    for temperature in (4.0, 1024.0, float(np.float32(1e30))):
+        check_logprobs(z.cuda(), torch.tensor([[3, 20, 5], [7, 8, 1]]).cuda(), top=20, temperature=temperature)

@@ -208,7 +208,8 @@ struct RowResult {
         rest = log1pf(s);
     }
     __device__ __forceinline__ float lp(float z) const {
-        return empty ? -INFINITY : (z - m) * inv_t - rest;
+        // (halves, as z - m itself may leave fp32's range)
+        return empty ? -INFINITY : (0.5f * z - 0.5f * m) * (2.f * inv_t) - rest;
     }
     __device__ __forceinline__ float entropy() const { return empty ? 0.f : rest - t * 0.693147180559945f / (1.f + s); }
 };
