@@ -255,7 +255,7 @@ def _plain_route(case, z, bias):
 
 def _plain_int8(case, x, w):
     """The quantizing in 64 bits (a value next to the border of two codes), the product in 32."""
-    scale = (x.float().abs().max(1, keepdim=True).values / 127).clamp(min=2.0 ** -126)
+    scale = (x.abs().max(1, keepdim=True).values.double() / 127).float().clamp(min=2.0 ** -126)
     codes = torch.round(x.double() / scale.double()).float()
     y = (codes @ w["codes"].float().T) * scale * w["scales"]
     return (y if w["bias"] is None else y + w["bias"]).to(DTYPES[case["out"]])
@@ -371,7 +371,7 @@ def _exact_route(case, s):
 
 def _exact_int8(case, s):
     x, out = s["x"].double(), []
-    scale = torch.clamp((s["x"].float().abs().amax(1) / 127), min=2.0 ** -126).double()  # kept in float32
+    scale = torch.clamp((x.abs().amax(1) / 127).float(), min=2.0 ** -126).double()  # kept in float32
     codes = (x / scale[:, None]).round()
     for w in s["mats"]:
         y = torch.empty((case["m"], case["n"]), dtype=torch.float64, device=x.device)
