@@ -347,6 +347,18 @@ int vb_moe_grouped_ffn_types(const void* const* wg, const void* const* wu, const
                              int32_t gate_up_type, int32_t down_type, void* workspace, size_t workspace_bytes,
                              void* stream);
 
+/* vb_moe_grouped_ffn_types with the routing given (vb_route_experts, or a
+ * program's own) in place of the router's logits: idx and weights[t *
+ * routing_ld + j], j < topk, routing_ld >= topk.  The call's experts are
+ * first_expert ... first_expert + n_exp - 1; any other id (-1, or an expert of
+ * another call) is no slot and adds nothing to y.  Layers past the limits (n_exp,
+ * topk, slots) run in several calls whose y are added. */
+int vb_moe_grouped_ffn_routed(const void* const* wg, const void* const* wu, const void* const* wd,
+                              int32_t n_exp, const float* x, int32_t n_tokens, const int32_t* idx,
+                              const float* weights, int64_t routing_ld, int32_t first_expert, int32_t topk,
+                              float* y, int64_t h, int64_t i, int32_t gate_up_type, int32_t down_type,
+                              void* workspace, size_t workspace_bytes, void* stream);
+
 /* Routing only: out_idx / out_w (n_tokens x topk) as vb_moe_grouped_ffn
  * computes them (ExpertRouter.route, vibeblade/moe.py:170-206, with the
  * selected experts ordered by descending weight). */
@@ -452,6 +464,80 @@ int64_t vb_group4_workspace(int64_t m, int64_t rows, int64_t k, int32_t group, i
 int vb_group4_gemv(const void* w, int64_t rows, int64_t k, int32_t group, int32_t has_zeros, const void* x,
                    int32_t x_type, int64_t x_ld, int64_t m, float* y, void* workspace, size_t workspace_bytes,
                    void* stream);
+
+/* ---- experts of a token ---------------------------------------------------------
+ * For each of n_tokens tokens with n_exp (at most 512) logits z (row stride ld,
+ * element type as above), s_e = softmax(z)_e (scores 0) or sigmoid(z_e) (1):
+ *   c_e = s_e + bias[e]; without a bias z_e, which is of the same order;
+ *   of `groups` (at most 64) groups of n_exp / groups consecutive experts the
+ *       groups_kept best stay, by the largest c of each (group_score 0) or by
+ *       the sum of its two largest s + bias (1; one alone counts for itself);
+ *   out_idx[t, 0..topk) = the best topk (at most 64, at most the experts that
+ *       stay) of their experts by c, in descending order, equal ones (and
+ *       equal groups) by the lower id;
+ *   out_w[t, j] = scale * s of it, over the sum of the chosen s with renorm.
+ * Scores, choices and sums are 64 bits.  An expert whose logit or bias is -inf
+ * is never chosen; where too few are left the id is -1, the weight 0.  A token
+ * with a NaN logit or choice, or +inf under softmax, has ids -1 and weights
+ * NaN.  (vb_moe_route keeps the reference's routing, whose logits are clamped.) */
+int vb_route_experts(const void* logits, int32_t type, int64_t ld, int64_t n_tokens, int32_t n_exp, int32_t topk,
+                     int32_t scores, const float* bias, int32_t groups, int32_t groups_kept, int32_t group_score,
+                     int32_t renorm, float scale, int32_t* out_idx, float* out_w, void* stream);
+
+/* ---- products in 8-bit integers ----------------------------------------------------
+ * A matrix of codes q[r, k] (8 bits, signed) and a scale s[r] per row: weights
+ * (rows = output channels) and activations (rows = tokens) alike, in one packed
+ * layout of vb_int8_bytes(rows, k) bytes (16-byte aligned; k at most 131071, so
+ * that sums of products stay within 32 bits; -1 for other shapes).
+ *
+ * vb_int8_pack lays out codes (row stride ld) and fp32 scales that a program
+ * has.  vb_int8_quantize makes them of src (row stride ld, element type as
+ * above): s[r] = max(max |src[r]| / 127, 2^-126) (0 for a row of zeros), q =
+ * src / s to the nearest integer, ties to even.  A row with a NaN or an
+ * infinity has the scale NaN.  vb_int8_dequant_rows: out[r * k + i] = q s. */
+int64_t vb_int8_bytes(int64_t rows, int64_t k);
+int vb_int8_pack(const int8_t* codes, int64_t ld, const float* scales, void* w, int64_t rows, int64_t k, void* stream);
+int vb_int8_quantize(const void* src, int32_t type, int64_t ld, int64_t rows, int64_t k, void* w, void* stream);
+int vb_int8_dequant_rows(const void* w, float* out, int64_t rows, int64_t k, void* stream);
+/* y[t * rows + n] = s_x[t] s_w[n] sum_i q_x[t, i] q_w[n, i] (+ bias[n], fp32) for
+ * the m tokens of x, y of the element type y_type.  x_type 0 to 2: x has row
+ * stride x_ld and is quantized in the call, as vb_int8_quantize does; 3: x is
+ * packed (m rows of k).  Sums are exact; they are converted to fp32 once,
+ * multiplied by s_x, then by s_w, and the result is rounded to y_type.  A NaN or
+ * an infinity of x makes its own token's results NaN.  y overlaps no operand.
+ * workspace: at least vb_int8_workspace(...) bytes (asked on the device of the
+ * call), 16-byte aligned, free again when the call's work is done. */
+int64_t vb_int8_workspace(int64_t m, int64_t rows, int64_t k, int32_t x_type);
+int vb_int8_gemm(const void* w, int64_t rows, int64_t k, const void* x, int32_t x_type, int64_t x_ld, int64_t m,
+                 const float* bias, void* y, int32_t y_type, void* workspace, size_t workspace_bytes, void* stream);
+
+/* ---- drafted tokens against a target ------------------------------------------------
+ * For each of n_seqs sequences: n_drafts (at most 63) drafted ids, the target's
+ * logits of n_drafts + 1 positions and, unless draft is NULL, the drafter's of
+ * n_drafts (both of the element type `type`, vocab up to 2^28; element (s, j, i)
+ * at s * ..._seq + j * ..._row + i).  p = softmax(target / temperature), q =
+ * softmax(draft / draft_temperature), or 1 at the drafted id without draft.
+ * With u = uniforms[s * uniforms_row + 0..n_drafts], in [0, 1), draft j is
+ * accepted while u[j] q_j(id) < p_j(id).  The next token is the first id whose
+ * sum of weights exceeds u[n_drafts] times that of all, the weights being
+ * max(p - q, 0) at the first refused draft (p, where that is 0 everywhere; a
+ * difference below 2^-45 p is rounding and counts as 0) and p behind the last.
+ *   lengths (optional): drafts of each sequence (cut to 0..n_drafts); an id
+ *       outside the vocabulary ends them too.
+ *   tokens[s, 0..n_drafts]: the accepted ids, the next token, then -1.
+ *   accepted[s]: their number.
+ * Sums are 64 bits.  A row that holds NaN or +inf, or a target row of nothing but
+ * -inf, ends its sequence with the token -1; rows behind the first refused
+ * draft are without effect.  drafted: ids of token_bytes (4 or 8), row stride
+ * drafted_row; outputs contiguous.  workspace: at least
+ * vb_verify_draft_workspace(...) bytes (asked on the device of the call),
+ * 16-byte aligned, free again when the call's work is done. */
+int64_t vb_verify_draft_workspace(int64_t n_seqs, int32_t n_drafts, int64_t vocab, int32_t has_draft);
+int vb_verify_draft(const void* target, int32_t type, int64_t target_seq, int64_t target_row, const void* draft,
+                    int64_t draft_seq, int64_t draft_row, const void* drafted, int32_t token_bytes, int64_t drafted_row,
+                    const int32_t* lengths, const float* uniforms, int64_t uniforms_row, int64_t n_seqs, int32_t n_drafts,
+                    int64_t vocab, float temperature, float draft_temperature, int32_t* tokens, int32_t* accepted,
+                    void* workspace, size_t workspace_bytes, void* stream);
 
 /* ---- GGUF ingestion --------------------------------------------------------
  * A .gguf file mapped read-only and parsed (header, metadata, tensor table).

@@ -7,9 +7,12 @@ The device work is hand-written HIP in ``csrc/`` built into ``libvbhip.so``
 * ``tensor``        -- ``QTensor`` (GGUF weights resident in HBM) and the ops
                        on it: gemv, gemm, sparse_ffn, topk_indices,
                        moe_grouped_ffn, moe_route; the steps around them:
-                       block_norm, token_logprobs
+                       block_norm, token_logprobs, route_experts,
+                       verify_draft
 * ``group4``        -- ``GroupQTensor`` (4-bit weights with group scales) and
                        group_gemv
+* ``int8``          -- ``Int8QTensor`` (8-bit integers with a scale per row),
+                       quantize_tokens and int8_gemm
 * ``sparse``        -- drop-in for vibeblade/sparse.py (TurboSparse FFN)
 * ``moe``           -- drop-in for vibeblade/moe.py (router, experts, MoE FFN)
 * ``moe_executor``  -- drop-in for vibeblade/moe_executor.py (HotColdExecutor)
@@ -23,5 +26,5 @@ and selects the device (there is no CPU fallback).
 """
 from . import ggml  # noqa: F401
 
-__all__ = ["ggml", "tensor", "group4", "sparse", "moe", "moe_executor", "moe_profiler", "gpu", "quant"]
+__all__ = ["ggml", "tensor", "group4", "int8", "sparse", "moe", "moe_executor", "moe_profiler", "gpu", "quant"]
 __version__ = "0.1.0"

@@ -61,6 +61,8 @@ SIGNATURES = {
                                           _i64, _i32, _vp, _sz, _vp]),
     "vb_moe_grouped_ffn_types": (ctypes.c_int, [_vp, _vp, _vp, _i32, _vp, _i32, _vp, _i32, _vp, _vp, _vp,
                                                 _i64, _i64, _i32, _i32, _vp, _sz, _vp]),
+    "vb_moe_grouped_ffn_routed": (ctypes.c_int, [_vp, _vp, _vp, _i32, _vp, _i32, _vp, _vp, _i64, _i32, _i32, _vp, _i64,
+                                                 _i64, _i32, _i32, _vp, _sz, _vp]),
     "vb_moe_route": (ctypes.c_int, [_vp, _i32, _i32, _i32, _vp, _vp, _vp]),
     "vb_activation": (ctypes.c_int, [_vp, _vp, _i64, _i32, _vp]),
     "vb_rms_norm": (ctypes.c_int, [_vp, _vp, _vp, _i64, _i64, ctypes.c_float, _vp]),
@@ -76,6 +78,17 @@ SIGNATURES = {
     "vb_group4_dequant_rows": (ctypes.c_int, [_vp, _vp, _i64, _i64, _i32, _i32, _vp]),
     "vb_group4_workspace": (_i64, [_i64, _i64, _i64, _i32, _i32, _i32]),
     "vb_group4_gemv": (ctypes.c_int, [_vp, _i64, _i64, _i32, _i32, _vp, _i32, _i64, _i64, _vp, _vp, _sz, _vp]),
+    "vb_route_experts": (ctypes.c_int, [_vp, _i32, _i64, _i64, _i32, _i32, _i32, _vp, _i32, _i32, _i32, _i32,
+                                        ctypes.c_float, _vp, _vp, _vp]),
+    "vb_int8_bytes": (_i64, [_i64, _i64]),
+    "vb_int8_pack": (ctypes.c_int, [_vp, _i64, _vp, _vp, _i64, _i64, _vp]),
+    "vb_int8_quantize": (ctypes.c_int, [_vp, _i32, _i64, _i64, _i64, _vp, _vp]),
+    "vb_int8_dequant_rows": (ctypes.c_int, [_vp, _vp, _i64, _i64, _vp]),
+    "vb_int8_workspace": (_i64, [_i64, _i64, _i64, _i32]),
+    "vb_int8_gemm": (ctypes.c_int, [_vp, _i64, _i64, _vp, _i32, _i64, _i64, _vp, _vp, _i32, _vp, _sz, _vp]),
+    "vb_verify_draft_workspace": (_i64, [_i64, _i32, _i64, _i32]),
+    "vb_verify_draft": (ctypes.c_int, [_vp, _i32, _i64, _i64, _vp, _i64, _i64, _vp, _i32, _i64, _vp, _vp, _i64, _i64, _i32,
+                                       _i64, ctypes.c_float, ctypes.c_float, _vp, _vp, _vp, _sz, _vp]),
     "vb_gguf_open": (ctypes.c_int, [ctypes.c_char_p, ctypes.POINTER(_vp)]),
     "vb_gguf_close": (ctypes.c_int, [_vp]),
     "vb_gguf_info": (ctypes.c_int, [_vp, ctypes.POINTER(ctypes.c_uint32), ctypes.POINTER(ctypes.c_uint64),

@@ -321,8 +321,28 @@ __device__ __forceinline__ void slot_lists(ListCounts& l, int eq, int e_n, int32
     if (eq >= 0 && eq < e_n) elist[l.off[eq] + l.cnt[wave][eq] + pos] = q;
 }
 
+// Routing that the caller has: ids (first ... first + n_exp - 1 are this call's
+// experts, others no slot) and weights, ld apart per token.
+struct GivenRouting {
+    const int32_t* idx = nullptr;
+    const float* w = nullptr;
+    int64_t ld = 0;
+    int32_t first = 0;
+};
+
+__device__ __forceinline__ void take_routing(const GivenRouting& g, int t, int e_n, int topk, int32_t* __restrict__ ridx,
+                                             float* __restrict__ rw, int* __restrict__ sexp) {
+    const int lane = threadIdx.x & 63;
+    if (lane >= topk) return;
+    const int64_t e = static_cast<int64_t>(g.idx[t * g.ld + lane]) - g.first;
+    const int id = e >= 0 && e < e_n ? static_cast<int>(e) : -1;
+    ridx[lane] = id;
+    rw[lane] = g.w[t * g.ld + lane];
+    if (sexp) sexp[lane] = id;
+}
+
 __global__ void __launch_bounds__(PREP_THREADS) moe_prep_kernel(
-        const float* __restrict__ x, const float* __restrict__ logits, int t_n, int e_n, int topk, int64_t nx,
+        const float* __restrict__ x, const float* __restrict__ logits, GivenRouting given, int t_n, int e_n, int topk, int64_t nx,
         _Float16* __restrict__ xh, int32_t* __restrict__ ridx, float* __restrict__ rw, int32_t* __restrict__ eoff,
         int32_t* __restrict__ elist, float* __restrict__ yzero, int32_t* __restrict__ out_idx,
         float* __restrict__ out_w, int rblocks) {
@@ -350,10 +370,15 @@ __global__ void __launch_bounds__(PREP_THREADS) moe_prep_kernel(
     int32_t* const cidx = yzero ? out_idx : nullptr;
     float* const cw = yzero ? out_w : nullptr;
     for (int t = static_cast<int>(blockIdx.x) * (PREP_THREADS / 64) + static_cast<int>(threadIdx.x >> 6); t < t_n;
-         t += PREP_THREADS / 64 * rblocks)
+         t += PREP_THREADS / 64 * rblocks) {
+        if (given.idx) {
+            take_routing(given, t, e_n, topk, ridx + t * topk, rw + t * topk, rblocks == 1 ? sexp + t * topk : nullptr);
+            continue;
+        }
         route_token_wave(logits + static_cast<int64_t>(t) * e_n, e_n, topk, ridx + t * topk, rw + t * topk,
                          rblocks == 1 ? sexp + t * topk : nullptr, cidx ? cidx + t * topk : nullptr,
                          cw ? cw + t * topk : nullptr);
+    }
     if (rblocks > 1) return;  // the lists follow in moe_lists_kernel
     __syncthreads();
     if (nslots > 64) {
@@ -561,15 +586,15 @@ bool moe_quant_type(int32_t t) {
 }
 }  // namespace
 
-extern "C" int vb_moe_grouped_ffn_types(const void* const* wg, const void* const* wu, const void* const* wd,
-                                        int32_t n_exp, const float* x, int32_t n_tokens, const float* router_logits,
-                                        int32_t topk, float* y, int32_t* out_idx, float* out_w, int64_t h, int64_t i,
-                                        int32_t gate_up_type, int32_t down_type, void* workspace,
-                                        size_t workspace_bytes, void* stream) {
+namespace {
+int moe_grouped_ffn(const void* const* wg, const void* const* wu, const void* const* wd, int32_t n_exp, const float* x,
+                    int32_t n_tokens, const float* router_logits, const GivenRouting& given, int32_t topk, float* y,
+                    int32_t* out_idx, float* out_w, int64_t h, int64_t i, int32_t gate_up_type, int32_t down_type,
+                    void* workspace, size_t workspace_bytes, void* stream) {
     hipStream_t st = as_stream(stream);
-    if (n_exp <= 0 || n_exp > MOE_MAX_EXPERTS || topk <= 0 || topk > MOE_MAX_TOPK || topk > n_exp ||
+    if (n_exp <= 0 || n_exp > MOE_MAX_EXPERTS || topk <= 0 || topk > MOE_MAX_TOPK || (topk > n_exp && !given.idx) ||
         n_tokens < 0 || static_cast<int64_t>(n_tokens) * topk > MOE_MAX_SLOTS || h <= 0 || i <= 0 || !wg ||
-        !wu || !wd || (n_tokens > 0 && (!x || !router_logits || !y))) {
+        !wu || !wd || (n_tokens > 0 && (!x || !(router_logits || (given.idx && given.w)) || !y))) {
         set_error("vb_moe_grouped_ffn: bad arguments (n_exp<=%d, topk<=%d, tokens*topk<=%d)", MOE_MAX_EXPERTS,
                   MOE_MAX_TOPK, MOE_MAX_SLOTS);
         return E_INVAL;
@@ -627,8 +652,8 @@ extern "C" int vb_moe_grouped_ffn_types(const void* const* wg, const void* const
     // weighted output into y (zeroed here), so no combine launch follows
     const bool fused_combine = !f32 && topk <= 2;
     float* yacc = fused_combine ? y : nullptr;
-    moe_prep_kernel<<<prep, dim3(PREP_THREADS), 0, st>>>(x, router_logits, n_tokens, n_exp, topk, nx, xh, ridx, rw,
-                                                         eoff, elist, yacc, out_idx, out_w, rblocks);
+    moe_prep_kernel<<<prep, dim3(PREP_THREADS), 0, st>>>(x, router_logits, given, n_tokens, n_exp, topk, nx, xh, ridx,
+                                                         rw, eoff, elist, yacc, out_idx, out_w, rblocks);
     int rc = check_launch("vb_moe_grouped_ffn");
     if (rc != OK) return rc;
     if (rblocks > 1) {
@@ -693,6 +718,29 @@ extern "C" int vb_moe_grouped_ffn_types(const void* const* wg, const void* const
     moe_combine_routed<<<dim3(static_cast<uint32_t>(n_tokens), static_cast<uint32_t>((h + 1023) / 1024)), dim3(256), 0,
                          st>>>(obuf, ridx, rw, topk, h, y, out_idx, out_w);
     return check_launch("vb_moe_grouped_ffn");
+}
+}  // namespace
+
+extern "C" int vb_moe_grouped_ffn_types(const void* const* wg, const void* const* wu, const void* const* wd,
+                                        int32_t n_exp, const float* x, int32_t n_tokens, const float* router_logits,
+                                        int32_t topk, float* y, int32_t* out_idx, float* out_w, int64_t h, int64_t i,
+                                        int32_t gate_up_type, int32_t down_type, void* workspace,
+                                        size_t workspace_bytes, void* stream) {
+    return moe_grouped_ffn(wg, wu, wd, n_exp, x, n_tokens, router_logits, GivenRouting{}, topk, y, out_idx, out_w, h, i,
+                           gate_up_type, down_type, workspace, workspace_bytes, stream);
+}
+
+extern "C" int vb_moe_grouped_ffn_routed(const void* const* wg, const void* const* wu, const void* const* wd,
+                                         int32_t n_exp, const float* x, int32_t n_tokens, const int32_t* idx,
+                                         const float* weights, int64_t routing_ld, int32_t first_expert, int32_t topk,
+                                         float* y, int64_t h, int64_t i, int32_t gate_up_type, int32_t down_type,
+                                         void* workspace, size_t workspace_bytes, void* stream) {
+    if (n_tokens > 0 && (!idx || !weights || routing_ld < topk || first_expert < 0)) {
+        set_error("vb_moe_grouped_ffn_routed: null routing, its row stride below topk, or a negative first expert");
+        return E_INVAL;
+    }
+    return moe_grouped_ffn(wg, wu, wd, n_exp, x, n_tokens, nullptr, GivenRouting{idx, weights, routing_ld, first_expert},
+                           topk, y, nullptr, nullptr, h, i, gate_up_type, down_type, workspace, workspace_bytes, stream);
 }
 
 extern "C" int vb_moe_grouped_ffn(const void* const* wg, const void* const* wu, const void* const* wd,

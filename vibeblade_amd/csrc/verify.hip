@@ -1,0 +1,477 @@
+// Verification of drafted tokens against a target's logits, from given random
+// numbers.  Of a sequence with k drafted tokens d_j, the target's logits of
+// k + 1 positions and a drafter's of k, let
+//
+//   p_j = softmax(target_j / T)      q_j = softmax(draft_j / T')
+//
+// (without the drafter's logits q_j is 1 at d_j).  With u_j in [0, 1), d_j is
+// accepted while u_j q_j(d_j) < p_j(d_j).  At the first that is not, a token
+// from max(p_j - q_j, 0) (from p_j, where that is 0 everywhere) takes its
+// place; behind k accepted ones a token from p_k follows.  That token is the
+// first i with C_i > u C_V, C_i the sum of the weights up to i and u the
+// sequence's last random number: the tokens are distributed as the target's own.
+//
+// Exponentials and sums are 64 bits.  A token is an id, found by comparing a
+// random number with a sum over a vocabulary; in fp32 the order of the
+// additions would decide about one in a hundred of them.
+//
+//   stats    (row, slice): the maximum and the sum of 2^(c (z - max)), c =
+//            log2(e) / T, of each slice of each row that a decision may need
+//   rest     (sequence, slice), with a drafter's logits: the sequence's
+//            decision from these, and the slice's sum of the weights of its token
+//   token    one workgroup a sequence: the decision, the slice that the random
+//            number falls into, then the place in it
+//
+// A row with a NaN or +inf (target's or drafter's) ends the sequence at its
+// position: its token is -1, as it is where a mask leaves the target nothing.
+// An id outside the vocabulary ends the drafts there, as a length does.
+#include "elem_types.hpp"
+#include "vb_internal.hpp"
+#include "wave64.hpp"
+#include "../../include/vbhip.h"
+
+namespace vb {
+namespace {
+
+constexpr int VF_MAX_DRAFTS = 63;    // one a lane, and one lane more
+constexpr int VF_MAX_SLICES = 64;    // one a lane
+constexpr int VF_MAX_VOCAB = 1 << 28;
+constexpr int VF_THREADS = 256;      // of the passes over rows
+constexpr int VF_PIECE = 8;          // logits of a load
+constexpr int VF_WIDE = 1024;        // threads of a sequence's last step
+constexpr double LOG2E = 1.4426950408889634;
+
+struct VerifyArgs {
+    const void* target;
+    const void* draft;
+    const void* drafted;
+    const int32_t* lengths;
+    const float* u;
+    int32_t* tokens;
+    int32_t* accepted;
+    double2* stats;  // [sequence][row][slice]: maximum, sum
+    double* rest;    // [sequence][slice]
+    int64_t target_seq, target_row, draft_seq, draft_row, drafted_row, u_row;
+    int32_t seqs, drafts, vocab, token_bytes, slices, slice, rests, rest_slice;
+    double c, cd;  // log2(e) / T of the target and of the drafter
+};
+
+// Drafts of a sequence that count: up to its length and the first id outside
+// the vocabulary.  Every wave of a workgroup computes the same.
+__device__ __forceinline__ int drafts_of(const VerifyArgs& a, int seq) {
+    const int lane = static_cast<int>(threadIdx.x) & 63;
+    const int given = a.lengths ? a.lengths[seq] : a.drafts;
+    bool in = lane < a.drafts && lane < given;
+    if (in) {
+        const int64_t p = seq * a.drafted_row + lane;
+        const int64_t id = a.token_bytes == 8 ? static_cast<const int64_t*>(a.drafted)[p]
+                                              : static_cast<const int32_t*>(a.drafted)[p];
+        in = id >= 0 && id < a.vocab;
+    }
+    return __ffsll(static_cast<unsigned long long>(~__ballot(in))) - 1;
+}
+
+__device__ __forceinline__ int drafted_id(const VerifyArgs& a, int seq, int j) {
+    const int64_t p = seq * a.drafted_row + j;
+    return a.token_bytes == 8 ? static_cast<int>(static_cast<const int64_t*>(a.drafted)[p])
+                              : static_cast<const int32_t*>(a.drafted)[p];
+}
+
+// 2^(c (z - m)); 0 for z = -inf (m finite).
+__device__ __forceinline__ double term(float z, double m, double c) {
+    return exp2_64((static_cast<double>(z) - m) * c);
+}
+
+// Sum over a workgroup of up to 16 waves, in every thread; buf: one place a wave.
+__device__ __forceinline__ double group_sum(double v, double* buf) {
+    const int wave = static_cast<int>(threadIdx.x) >> 6, waves = static_cast<int>(blockDim.x) >> 6;
+    v = wave_sum64(v);
+    __syncthreads();
+    buf[wave] = v;
+    __syncthreads();
+    const int lane = static_cast<int>(threadIdx.x) & 63;
+    return wave_sum64(lane < waves ? buf[lane] : 0.0);
+}
+
+// ---- stats ------------------------------------------------------------------
+
+template <int TYPE>
+__global__ void __launch_bounds__(VF_THREADS) verify_stats_kernel(VerifyArgs a) {
+    __shared__ float tops[VF_THREADS / 64];
+    __shared__ double sums[VF_THREADS / 64];
+    const int rows = a.drafts + 1 + (a.draft ? a.drafts : 0);
+    const int lane = static_cast<int>(threadIdx.x) & 63, wave = static_cast<int>(threadIdx.x) >> 6;
+    for (int64_t item = blockIdx.x; item < static_cast<int64_t>(a.seqs) * rows * a.slices; item += gridDim.x) {
+        const int slice = static_cast<int>(item % a.slices), row = static_cast<int>(item / a.slices % rows);
+        const int seq = static_cast<int>(item / a.slices / rows);
+        const int count = drafts_of(a, seq);
+        const bool of_target = row <= a.drafts;
+        const int j = of_target ? row : row - a.drafts - 1;
+        if (j > count || (!of_target && j == count)) continue;  // no decision asks for it
+        const void* z = of_target ? a.target : a.draft;
+        const int64_t at = of_target ? seq * a.target_seq + j * a.target_row : seq * a.draft_seq + j * a.draft_row;
+        const double c = of_target ? a.c : a.cd;
+        const int begin = slice * a.slice, end = a.vocab - begin < a.slice ? a.vocab : begin + a.slice;
+        float top = -INFINITY;
+        double sum = 0.0;
+        bool bad = false;
+        for (int i = begin + static_cast<int>(threadIdx.x); i < end; i += VF_THREADS) {
+            const float v = elem_ld(z, at + i, TYPE);
+            bad = bad || !(v < INFINITY);
+            if (v > top) {
+                sum = top > -INFINITY ? sum * term(top, v, c) : 0.0;
+                top = v;
+            }
+            sum += v > -INFINITY ? term(v, top, c) : 0.0;
+        }
+        const float all = wave_largest(top);
+        sum = wave_sum64(top > -INFINITY ? sum * term(top, all, c) : 0.0);
+        if (__any(bad)) sum = NAN;
+        if (lane == 0) {
+            tops[wave] = all;
+            sums[wave] = sum;
+        }
+        __syncthreads();
+        if (threadIdx.x == 0) {
+            float m = tops[0];
+            for (int w = 1; w < VF_THREADS / 64; w++) m = fmaxf(m, tops[w]);
+            double s = 0.0;
+            for (int w = 0; w < VF_THREADS / 64; w++)
+                s += sums[w] != sums[w] ? NAN : tops[w] > -INFINITY ? sums[w] * term(tops[w], m, c) : 0.0;
+            a.stats[item] = make_double2(static_cast<double>(m), s);
+        }
+        __syncthreads();
+    }
+}
+
+// ---- the decision -------------------------------------------------------------
+
+// A row's maximum and sum from its slices, by a wave, in every lane.
+__device__ __forceinline__ double2 row_stats(const VerifyArgs& a, int seq, int row, double c) {
+    const int lane = static_cast<int>(threadIdx.x) & 63;
+    const int rows = a.drafts + 1 + (a.draft ? a.drafts : 0);
+    double2 v = make_double2(-INFINITY, 0.0);
+    if (lane < a.slices) v = a.stats[(static_cast<int64_t>(seq) * rows + row) * a.slices + lane];
+    const double m = wave_largest(v.x);
+    const double s = v.y != v.y ? NAN : v.x > -INFINITY ? v.y * exp2_64((v.x - m) * c) : 0.0;
+    return make_double2(m, wave_sum64(s));
+}
+
+// What a sequence's token is drawn from.
+struct Source {
+    int accepted;  // drafted tokens
+    bool bad;      // the token is -1
+    bool refused;  // from max(p - q, 0), else from p
+    int without;   // q is 1 at this id (no drafter's logits), or -1
+    int64_t p, q;  // rows: first logit
+    double pm, ps, qm, qs;  // their maxima and reciprocal sums
+};
+
+// Weight of id i, before the sum of them all divides it.  Of equal p and q the
+// roundings of two sums may leave some 2^-52 p, which is no weight.
+template <int TYPE>
+__device__ __forceinline__ double weight(const VerifyArgs& a, const Source& s, bool refused, int i) {
+    const float zp = elem_ld(a.target, s.p + i, TYPE);
+    double r = zp > -INFINITY ? term(zp, s.pm, a.c) * s.ps : 0.0;
+    if (refused && a.draft) {
+        const float zq = elem_ld(a.draft, s.q + i, TYPE);
+        const double q = zq > -INFINITY ? term(zq, s.qm, a.cd) * s.qs : 0.0;
+        r = r - q > 0x1p-45 * r ? r - q : 0.0;
+    }
+    return refused && i == s.without ? 0.0 : r;
+}
+
+// The decision of a sequence, by a workgroup; verdicts: a place per draft.
+template <int TYPE>
+__device__ __forceinline__ Source decide(const VerifyArgs& a, int seq, int* verdicts) {
+    const int wave = static_cast<int>(threadIdx.x) >> 6, waves = static_cast<int>(blockDim.x) >> 6;
+    const int count = drafts_of(a, seq);
+    // 0: accepted, 1: refused, 2: a row that holds NaN or +inf
+    for (int j = wave; j <= count; j += waves) {
+        const double2 p = row_stats(a, seq, j, a.c);
+        int verdict = p.y != p.y ? 2 : 1;
+        if (j < count) {
+            const int d = drafted_id(a, seq, j);
+            const float zp = elem_ld(a.target, seq * a.target_seq + j * a.target_row + d, TYPE);
+            const double pd = zp > -INFINITY ? term(zp, p.x, a.c) : 0.0;
+            double qd = 1.0, qs = 1.0;
+            if (a.draft) {
+                const double2 q = row_stats(a, seq, a.drafts + 1 + j, a.cd);
+                const float zq = elem_ld(a.draft, seq * a.draft_seq + j * a.draft_row + d, TYPE);
+                qd = zq > -INFINITY ? term(zq, q.x, a.cd) : 0.0;
+                qs = q.y > 0.0 ? q.y : 1.0;
+                if (q.y != q.y) verdict = 2;
+            }
+            if (verdict == 1 && static_cast<double>(a.u[seq * a.u_row + j]) * qd * p.y < pd * qs) verdict = 0;
+        }
+        verdicts[j] = verdict;
+    }
+    __syncthreads();
+    Source s{};
+    s.accepted = 0;
+    while (s.accepted < count && verdicts[s.accepted] == 0) s.accepted++;
+    s.bad = verdicts[s.accepted] == 2;
+    s.refused = s.accepted < count;
+    s.without = s.refused && !a.draft ? drafted_id(a, seq, s.accepted) : -1;
+    const double2 p = row_stats(a, seq, s.accepted, a.c);
+    s.p = seq * a.target_seq + s.accepted * a.target_row;
+    s.pm = p.x;
+    s.ps = p.y > 0.0 ? 1.0 / p.y : 0.0;
+    if (!(p.y > 0.0)) s.bad = true;  // nothing is left, or NaN
+    if (s.refused && a.draft) {
+        const double2 q = row_stats(a, seq, a.drafts + 1 + s.accepted, a.cd);
+        s.q = seq * a.draft_seq + s.accepted * a.draft_row;
+        s.qm = q.x;
+        s.qs = q.y > 0.0 ? 1.0 / q.y : 0.0;
+    }
+    return s;
+}
+
+// ---- rest ---------------------------------------------------------------------
+
+template <int TYPE>
+__global__ void __launch_bounds__(VF_THREADS) verify_rest_kernel(VerifyArgs a) {
+    __shared__ int verdicts[VF_MAX_DRAFTS + 1];
+    __shared__ double sums[VF_THREADS / 64];
+    for (int64_t item = blockIdx.x; item < static_cast<int64_t>(a.seqs) * a.rests; item += gridDim.x) {
+        const int slice = static_cast<int>(item % a.rests), seq = static_cast<int>(item / a.rests);
+        const Source s = decide<TYPE>(a, seq, verdicts);
+        const int begin = slice * a.rest_slice;
+        const int end = a.vocab - begin < a.rest_slice ? a.vocab : begin + a.rest_slice;
+        double sum = 0.0;
+        if (!s.bad)
+            for (int i = begin + static_cast<int>(threadIdx.x); i < end; i += VF_THREADS)
+                sum += weight<TYPE>(a, s, s.refused, i);
+        sum = group_sum(sum, sums);
+        if (threadIdx.x == 0) a.rest[item] = sum;
+        __syncthreads();
+    }
+}
+
+// ---- token --------------------------------------------------------------------
+
+// The first id of [begin, end) whose sum of weights, from `carry` on, exceeds
+// `goal`; the last id of a weight where rounding leaves none; -1 without weights.
+// By a workgroup of VF_WIDE threads.
+template <int TYPE>
+__device__ __forceinline__ int locate(const VerifyArgs& a, const Source& s, bool refused, int begin, int end, double carry,
+                                      double goal, double* buf, int* found) {
+    constexpr int WAVES = VF_WIDE / 64;
+    const int lane = static_cast<int>(threadIdx.x) & 63, wave = static_cast<int>(threadIdx.x) >> 6;
+    const int share = ((end - begin + WAVES - 1) / WAVES + 63) / 64 * 64;
+    const int lo = begin + wave * share < end ? begin + wave * share : end, hi = lo + share < end ? lo + share : end;
+    double sum = 0.0;
+    for (int i = lo + lane; i < hi; i += 64) sum += weight<TYPE>(a, s, refused, i);
+    sum = wave_sum64(sum);
+    __syncthreads();
+    buf[wave] = sum;
+    if (threadIdx.x == 0) *found = -1;
+    __syncthreads();
+    // the wave whose share the goal falls into, or the last with a weight
+    int owner = -1;
+    double before = carry, at = carry;
+    for (int w = 0; w < WAVES; w++) {
+        if (buf[w] > 0.0) {
+            owner = w;
+            before = at;
+        }
+        at += buf[w];
+        if (at > goal && buf[w] > 0.0) break;
+    }
+    if (owner == wave) {
+        int last = -1;
+        for (int i0 = lo; i0 < hi; i0 += 64) {
+            const double w = i0 + lane < hi ? weight<TYPE>(a, s, refused, i0 + lane) : 0.0;
+            double c = w;
+#pragma unroll
+            for (int o = 1; o < 64; o <<= 1) {
+                const double v = __shfl_up(c, o, 64);
+                if (lane >= o) c += v;
+            }
+            const uint64_t some = __ballot(w > 0.0), past = __ballot(w > 0.0 && before + c > goal);
+            if (past) {
+                last = i0 + __ffsll(static_cast<unsigned long long>(past)) - 1;
+                break;
+            }
+            if (some) last = i0 + 63 - __clzll(static_cast<long long>(some));
+            before += lane_value(c, 63);
+        }
+        if (lane == 0) *found = last;
+    }
+    __syncthreads();
+    return *found;
+}
+
+template <int TYPE>
+__global__ void __launch_bounds__(VF_WIDE) verify_token_kernel(VerifyArgs a) {
+    __shared__ int verdicts[VF_MAX_DRAFTS + 1];
+    __shared__ double buf[VF_WIDE / 64];
+    __shared__ double parts[VF_MAX_SLICES];
+    __shared__ int found;
+    const int lane = static_cast<int>(threadIdx.x) & 63;
+    const int rows = a.drafts + 1 + (a.draft ? a.drafts : 0);
+    for (int seq = static_cast<int>(blockIdx.x); seq < a.seqs; seq += static_cast<int>(gridDim.x)) {
+        const Source s = decide<TYPE>(a, seq, verdicts);
+        const double u = static_cast<double>(a.u[seq * a.u_row + a.drafts]);
+        int token = -1;
+        if (!s.bad) {
+            // each slice's weights: summed by the pass before, or the target's own sums
+            const int slices = a.draft ? a.rests : a.slices, size = a.draft ? a.rest_slice : a.slice;
+            if (lane < slices && threadIdx.x < 64) {
+                double v;
+                if (a.draft) {
+                    v = a.rest[static_cast<int64_t>(seq) * slices + lane];
+                } else {
+                    const double2 p = a.stats[(static_cast<int64_t>(seq) * rows + s.accepted) * slices + lane];
+                    v = p.x > -INFINITY ? p.y * exp2_64((p.x - s.pm) * a.c) * s.ps : 0.0;
+                }
+                parts[lane] = v;
+            }
+            __syncthreads();
+            if (s.without >= 0) {  // the slice of the refused token, without it (the difference of sums would lose digits)
+                const int slice = s.without / size, begin = slice * size, end = a.vocab - begin < size ? a.vocab : begin + size;
+                double sum = 0.0;
+                for (int i = begin + static_cast<int>(threadIdx.x); i < end; i += VF_WIDE) sum += weight<TYPE>(a, s, true, i);
+                sum = group_sum(sum, buf);
+                if (threadIdx.x == 0) parts[slice] = sum;
+                __syncthreads();
+            }
+            double total = 0.0;
+            for (int i = 0; i < slices; i++) total += parts[i];
+            if (total > 0.0) {
+                const double goal = u * total;
+                int owner = -1;
+                double before = 0.0, at = 0.0;
+                for (int i = 0; i < slices; i++) {
+                    if (parts[i] > 0.0) {
+                        owner = i;
+                        before = at;
+                    }
+                    at += parts[i];
+                    if (at > goal && parts[i] > 0.0) break;
+                }
+                const int begin = owner * size, end = a.vocab - begin < size ? a.vocab : begin + size;
+                token = locate<TYPE>(a, s, s.refused, begin, end, before, goal, buf, &found);
+            } else {  // nothing is left of p behind q: from p itself (whose sum is 1)
+                token = locate<TYPE>(a, s, false, 0, a.vocab, 0.0, u, buf, &found);
+            }
+        }
+        for (int j = static_cast<int>(threadIdx.x); j <= a.drafts; j += VF_WIDE)
+            a.tokens[static_cast<int64_t>(seq) * (a.drafts + 1) + j] =
+                j < s.accepted ? drafted_id(a, seq, j) : j == s.accepted ? token : -1;
+        if (threadIdx.x == 0) a.accepted[seq] = s.accepted;
+        __syncthreads();
+    }
+}
+
+struct VerifyPlan {
+    int64_t slices, slice, rests, rest_slice, workspace;
+};
+
+VerifyPlan verify_plan(int64_t seqs, int64_t drafts, int64_t vocab, bool draft) {
+    const int64_t rows = seqs * (drafts + 1 + (draft ? drafts : 0));
+    const auto cut = [&](int64_t n, int64_t groups, int64_t* slices, int64_t* slice) {
+        const int64_t most = (vocab + VF_THREADS * VF_PIECE - 1) / (VF_THREADS * VF_PIECE);
+        int64_t want = (groups * num_cus() + n - 1) / (n > 0 ? n : 1);
+        want = want < 1 ? 1 : want < VF_MAX_SLICES ? want : VF_MAX_SLICES;
+        want = want < most ? want : most;
+        *slice = ((vocab + want - 1) / want + VF_PIECE - 1) / VF_PIECE * VF_PIECE;
+        *slices = (vocab + *slice - 1) / *slice;
+    };
+    VerifyPlan p{};
+    cut(rows, 8, &p.slices, &p.slice);
+    cut(seqs, 4, &p.rests, &p.rest_slice);
+    if (!draft) p.rests = 0;
+    p.workspace = rows * p.slices * 16 + seqs * p.rests * 8;
+    return p;
+}
+
+template <int TYPE>
+int verify_launch(const VerifyArgs& a, hipStream_t st) {
+    const auto grid = [](int64_t n) { return static_cast<uint32_t>(n < (1 << 20) ? n : 1 << 20); };
+    verify_stats_kernel<TYPE><<<grid(static_cast<int64_t>(a.seqs) * (a.drafts + 1 + (a.draft ? a.drafts : 0)) * a.slices),
+                                VF_THREADS, 0, st>>>(a);
+    if (const int rc = check_launch("vb_verify_draft"); rc != OK) return rc;
+    if (a.draft) {
+        verify_rest_kernel<TYPE><<<grid(static_cast<int64_t>(a.seqs) * a.rests), VF_THREADS, 0, st>>>(a);
+        if (const int rc = check_launch("vb_verify_draft"); rc != OK) return rc;
+    }
+    verify_token_kernel<TYPE><<<grid(a.seqs), VF_WIDE, 0, st>>>(a);
+    return check_launch("vb_verify_draft");
+}
+
+}  // namespace
+}  // namespace vb
+
+using namespace vb;
+
+extern "C" {
+
+int64_t vb_verify_draft_workspace(int64_t n_seqs, int32_t n_drafts, int64_t vocab, int32_t has_draft) {
+    if (n_seqs < 0 || n_seqs > 1 << 24 || n_drafts < 0 || n_drafts > VF_MAX_DRAFTS || vocab <= 0 || vocab > VF_MAX_VOCAB)
+        return -1;
+    if (n_seqs == 0) return 0;
+    return verify_plan(n_seqs, n_drafts, vocab, has_draft != 0 && n_drafts > 0).workspace;
+}
+
+int vb_verify_draft(const void* target, int32_t type, int64_t target_seq, int64_t target_row, const void* draft,
+                    int64_t draft_seq, int64_t draft_row, const void* drafted, int32_t token_bytes, int64_t drafted_row,
+                    const int32_t* lengths, const float* uniforms, int64_t uniforms_row, int64_t n_seqs, int32_t n_drafts,
+                    int64_t vocab, float temperature, float draft_temperature, int32_t* tokens, int32_t* accepted,
+                    void* workspace, size_t workspace_bytes, void* stream) {
+    if (n_drafts == 0) draft = nullptr;
+    const int64_t need = vb_verify_draft_workspace(n_seqs, n_drafts, vocab, draft != nullptr);
+    if (!elem_type(type) || need < 0 || target_seq < 0 || target_row < 0 || draft_seq < 0 || draft_row < 0 ||
+        drafted_row < 0 || uniforms_row < 0) {
+        set_error("vb_verify_draft: bad arguments (type %d, %lld sequences, %d of at most %d drafts, vocab=%lld, or a "
+                  "negative stride)", type, static_cast<long long>(n_seqs), n_drafts, VF_MAX_DRAFTS,
+                  static_cast<long long>(vocab));
+        return E_INVAL;
+    }
+    if (!(temperature >= 1e-30f && temperature <= 1e30f && draft_temperature >= 1e-30f && draft_temperature <= 1e30f)) {
+        set_error("vb_verify_draft: temperatures must be in [1e-30, 1e30]");
+        return E_INVAL;
+    }
+    if (n_seqs == 0) return OK;
+    if (!target || !uniforms || !tokens || !accepted || (n_drafts > 0 && (!drafted || (token_bytes != 4 && token_bytes != 8)))) {
+        set_error("vb_verify_draft: null pointer, or token ids of %d bytes (4 or 8)", token_bytes);
+        return E_INVAL;
+    }
+    if (static_cast<int64_t>(workspace_bytes) < need || !workspace || reinterpret_cast<uintptr_t>(workspace) % 16 != 0) {
+        set_error("vb_verify_draft: workspace of %zu bytes (16-byte aligned) is below the %lld needed", workspace_bytes,
+                  static_cast<long long>(need));
+        return E_INVAL;
+    }
+    const VerifyPlan p = verify_plan(n_seqs, n_drafts, vocab, draft != nullptr);
+    VerifyArgs a{};
+    a.target = target;
+    a.draft = draft;
+    a.drafted = drafted;
+    a.lengths = lengths;
+    a.u = uniforms;
+    a.tokens = tokens;
+    a.accepted = accepted;
+    a.target_seq = target_seq;
+    a.target_row = target_row;
+    a.draft_seq = draft_seq;
+    a.draft_row = draft_row;
+    a.drafted_row = drafted_row;
+    a.u_row = uniforms_row;
+    a.seqs = static_cast<int32_t>(n_seqs);
+    a.drafts = n_drafts;
+    a.vocab = static_cast<int32_t>(vocab);
+    a.token_bytes = token_bytes;
+    a.slices = static_cast<int32_t>(p.slices);
+    a.slice = static_cast<int32_t>(p.slice);
+    a.rests = static_cast<int32_t>(p.rests);
+    a.rest_slice = static_cast<int32_t>(p.rest_slice);
+    a.c = LOG2E / static_cast<double>(temperature);
+    a.cd = LOG2E / static_cast<double>(draft_temperature);
+    a.stats = static_cast<double2*>(workspace);
+    a.rest = reinterpret_cast<double*>(a.stats + n_seqs * (n_drafts + 1 + (draft ? n_drafts : 0)) * p.slices);
+    if (type == ELEM_F32) return verify_launch<ELEM_F32>(a, as_stream(stream));
+    if (type == ELEM_F16) return verify_launch<ELEM_F16>(a, as_stream(stream));
+    return verify_launch<ELEM_BF16>(a, as_stream(stream));
+}
+
+}  // extern "C"

@@ -21,7 +21,8 @@ from dataclasses import dataclass
 import numpy as np
 import torch
 
-from .tensor import QTensor, as_qtensor, gemv, moe_route, moe_grouped_ffn, sparse_ffn, ACT_SILU, DOWN_GGUF
+from .tensor import (QTensor, as_qtensor, gemv, moe_route, moe_grouped_ffn, route_experts, sparse_ffn, ACT_SILU,
+                     DOWN_GGUF)
 
 __all__ = [
     "MoEConfig", "ExpertRouter", "MoEExpertSet", "detect_moe_config", "moe_ffn_silu",
@@ -104,14 +105,37 @@ class MoEConfig:
 class ExpertRouter:
     """Top-k expert router (vibeblade/moe.py:151-216): logits = x @ W_router on
     the GPU, then softmax (logits clamped to +-50), top-k and renormalisation
-    in one device kernel."""
+    in one device kernel.  With any of ``route_experts``' keywords (scores,
+    bias, groups, groups_kept, group_score, renorm, scale), which the reference
+    has not, that routing takes its place, for up to 512 experts."""
 
-    def __init__(self, router_weight: np.ndarray, topk: int = 2):
+    def __init__(self, router_weight: np.ndarray, topk: int = 2, **options):
         self.weight = np.asarray(router_weight, dtype=np.float32)
         self.topk = int(topk)
         self.num_experts = int(self.weight.shape[1])
         self.shared_dim = int(self.weight.shape[0])
         self._dev_w: QTensor | None = None
+        unknown = set(options) - {"scores", "bias", "groups", "groups_kept", "group_score", "renorm", "scale"}
+        if unknown:
+            raise TypeError(f"ExpertRouter: unknown options {sorted(unknown)}")
+        self.options = options
+        if options.get("bias") is not None:
+            bias = np.asarray(options["bias"], dtype=np.float32).reshape(-1)
+            if bias.size != self.num_experts:
+                raise ValueError(f"ExpertRouter: bias has {bias.size} values, {self.num_experts} expected")
+            self.options = dict(options, bias=bias)
+        self._dev_bias: torch.Tensor | None = None
+
+    def _route_dev(self, logits: torch.Tensor):
+        """(indices, weights) on the device."""
+        if not self.options:
+            return moe_route(logits, self.topk)
+        options = dict(self.options)
+        if options.get("bias") is not None:
+            if self._dev_bias is None:
+                self._dev_bias = torch.from_numpy(options["bias"]).to(logits.device)
+            options["bias"] = self._dev_bias
+        return route_experts(logits, self.topk, **options)
 
     def _wdev(self) -> QTensor:
         if self._dev_w is None:
@@ -129,7 +153,7 @@ class ExpertRouter:
     def route(self, x: np.ndarray):
         squeeze = np.asarray(x).ndim == 1
         x2 = np.atleast_2d(np.asarray(x, dtype=np.float32))
-        idx, w = moe_route(self._logits_dev(x2), self.topk)
+        idx, w = self._route_dev(self._logits_dev(x2))
         idx = idx.cpu().numpy().astype(np.int64)
         w = w.cpu().numpy().astype(np.float32)
         if squeeze:
@@ -242,14 +266,22 @@ class MoEExpertSet:
                 as_qtensor(np.ascontiguousarray(self.down[idx])))
 
 
-def grouped_ffn(experts: MoEExpertSet, x2d: np.ndarray, logits: torch.Tensor, topk: int):
-    """Route every token and run the grouped expert FFN on the GPU.
+def given_routing(router, logits: torch.Tensor):
+    """The routing of a router that has options (``ExpertRouter``), None where the experts' op routes itself."""
+    return router._route_dev(logits) if getattr(router, "options", None) else None
+
+
+def grouped_ffn(experts: MoEExpertSet, x2d: np.ndarray, logits: torch.Tensor | None, topk: int, routing=None):
+    """Route every token (or take its routing) and run the grouped expert FFN on the GPU.
     Returns (out (T, shared_dim) fp32 numpy, indices, weights)."""
     gs, us, ds, hp = experts.device_experts()
     h = experts.shared_dim
     xp = np.zeros((x2d.shape[0], hp), dtype=np.float32)
     xp[:, :h] = x2d
-    y, idx, w = moe_grouped_ffn(gs, us, ds, torch.from_numpy(xp), logits, topk)
+    if routing is not None:
+        y, idx, w = moe_grouped_ffn(gs, us, ds, torch.from_numpy(xp), routing=routing)
+    else:
+        y, idx, w = moe_grouped_ffn(gs, us, ds, torch.from_numpy(xp), logits, topk)
     return y[:, :h].cpu().numpy(), idx.cpu().numpy().astype(np.int64), w.cpu().numpy()
 
 
@@ -343,7 +375,7 @@ def moe_ffn_silu(x: np.ndarray, router: ExpertRouter, experts: MoEExpertSet, sha
     squeeze = np.asarray(x).ndim == 1
     x2 = np.atleast_2d(np.asarray(x, dtype=np.float32))
     logits = router._logits_dev(x2)
-    moe_out, indices, weights = grouped_ffn(experts, x2, logits, router.topk)
+    moe_out, indices, weights = grouped_ffn(experts, x2, logits, router.topk, given_routing(router, logits))
     has_shared = shared_expert_gate is not None
     if has_shared:
         moe_out = moe_out + np.atleast_2d(_dense_ffn(x2, shared_expert_gate, shared_expert_up, shared_expert_down))

@@ -21,7 +21,7 @@ from dataclasses import dataclass
 import numpy as np
 import torch
 
-from .moe import grouped_ffn, _dense_ffn, _sanitize
+from .moe import given_routing, grouped_ffn, _dense_ffn, _sanitize
 
 __all__ = ["ExecutorStats", "HotColdExecutor"]
 
@@ -122,7 +122,7 @@ class HotColdExecutor:
         cpu_ms = self._upload(layer_idx)
         t0 = time.perf_counter()
         logits = router._logits_dev(x2)
-        out, indices, weights = grouped_ffn(expert_set, x2, logits, router.topk)
+        out, indices, weights = grouped_ffn(expert_set, x2, logits, router.topk, given_routing(router, logits))
         t1 = time.perf_counter()
         shared = self._shared.get(layer_idx)
         if shared is not None and shared[0] is not None:
@@ -131,6 +131,7 @@ class HotColdExecutor:
         t2 = time.perf_counter()
 
         routed = np.asarray(indices).reshape(-1)
+        routed = routed[routed >= 0]  # (-1: a mask left a token too few experts)
         hits = int(np.count_nonzero(np.isin(routed, list(self._hot_map.hot_experts.get(layer_idx, ())))))
         per = ExecutorStats(gpu_hits=hits, cpu_falls=int(routed.size) - hits, gpu_latency_ms=(t1 - t0) * 1000.0,
                             cpu_latency_ms=cpu_ms, sync_latency_ms=(t2 - t1) * 1000.0)

@@ -313,13 +313,21 @@ def moe_route(logits: torch.Tensor, topk: int):
     return idx, w
 
 
-def moe_grouped_ffn(gates, ups, downs, x: torch.Tensor, logits: torch.Tensor, topk: int):
+def moe_grouped_ffn(gates, ups, downs, x: torch.Tensor, logits: torch.Tensor | None = None, topk: int | None = None,
+                    routing=None):
     """Top-k MoE over experts (lists of QTensors: gate/up i x h, down h x i;
-    gate/up of one ggml type, down of the same or another).  Returns (y (T, h) fp32, indices (T, topk) int32, weights (T, topk) fp32)."""
+    gate/up of one ggml type, down of the same or another).  Returns (y (T, h) fp32, indices (T, topk) int32, weights (T, topk) fp32).
+
+    The experts come from ``logits`` and ``topk`` (the reference's routing, as ``moe_route``; at most 64 experts, 8 of
+    them a token, 1024 slots), or from ``routing=(indices int32, weights float32)``, (T, topk) each, as
+    ``route_experts`` gives them, of any size: an index that names no expert (-1) adds nothing, and layers past those
+    limits run in several calls whose results are added."""
     import ctypes
     n_exp = len(gates)
     if not (len(ups) == len(downs) == n_exp) or n_exp == 0:
         raise ValueError("moe_grouped_ffn: need the same number of gate/up/down experts")
+    if (routing is None) == (logits is None) or (routing is None) == (topk is None):
+        raise ValueError("moe_grouped_ffn: takes logits and topk, or routing")
     g0 = gates[0]
     h, i = g0.k, g0.rows
     gu_type, dn_type = g0.qtype, downs[0].qtype
@@ -334,22 +342,64 @@ def moe_grouped_ffn(gates, ups, downs, x: torch.Tensor, logits: torch.Tensor, to
     if x.dim() == 1:
         x = x.reshape(1, -1)
     t = x.shape[0]
+    vp = ctypes.c_void_p
+
+    def pointers(qs):
+        return ctypes.cast((vp * len(qs))(*[q.ptr() for q in qs]), vp)
+
+    if routing is not None:
+        return _moe_routed(gates, ups, downs, x, routing, pointers)
     logits = _as_f32_dev(logits, dev).reshape(t, n_exp)
     y = torch.empty((t, h), dtype=torch.float32, device=dev)
     idx = torch.empty((t, topk), dtype=torch.int32, device=dev)
     w = torch.empty((t, topk), dtype=torch.float32, device=dev)
-    arr = ctypes.c_void_p * n_exp
-    pg = arr(*[g.ptr() for g in gates])
-    pu = arr(*[u.ptr() for u in ups])
-    pd = arr(*[d.ptr() for d in downs])
     nbytes = _lib.load().vb_moe_workspace(t, topk, h, i)
     if nbytes < 0:
         raise ValueError("moe_grouped_ffn: bad shape")
     ws = _workspace(nbytes, dev)
-    vp = ctypes.c_void_p
-    _lib.call("vb_moe_grouped_ffn_types", ctypes.cast(pg, vp), ctypes.cast(pu, vp), ctypes.cast(pd, vp), n_exp,
+    _lib.call("vb_moe_grouped_ffn_types", pointers(gates), pointers(ups), pointers(downs), n_exp,
               x.data_ptr(), t, logits.data_ptr(), topk, y.data_ptr(), idx.data_ptr(), w.data_ptr(), h, i,
               gu_type, dn_type, ws.data_ptr(), ws.numel(), _stream())
+    return y, idx, w
+
+
+_MOE_EXPERTS, _MOE_TOPK, _MOE_SLOTS = 64, 8, 1024  # of one vb_moe_grouped_ffn_routed
+
+
+def _moe_routed(gates, ups, downs, x, routing, pointers):
+    dev, h, i = x.device, gates[0].k, gates[0].rows
+    idx, w = routing
+    t = x.shape[0]
+    for r, dtype in ((idx, torch.int32), (w, torch.float32)):
+        if not isinstance(r, torch.Tensor) or r.device != dev or r.dtype != dtype or r.dim() != 2 or r.shape[0] != t \
+                or r.shape != idx.shape or r.shape[1] == 0:
+            raise ValueError(f"moe_grouped_ffn: routing must be (indices int32, weights float32), ({t}, topk) each on {dev}")
+    if x.shape[1] != h:
+        raise ValueError(f"moe_grouped_ffn: x has {x.shape[1]} columns, {h} expected")
+    idx, w = idx.contiguous(), w.contiguous()
+    topk = idx.shape[1]
+    y = torch.empty((t, h), dtype=torch.float32, device=dev)
+    step = min(topk, _MOE_TOPK)
+    tokens = max(1, min(t, _MOE_SLOTS // step))
+    nbytes = _lib.load().vb_moe_workspace(tokens, step, h, i)
+    if nbytes < 0:
+        raise ValueError("moe_grouped_ffn: bad shape")
+    ws = _workspace(nbytes, dev)
+    part = None
+    for first in range(0, t, tokens):
+        n, to = min(tokens, t - first), y[first:first + tokens]
+        for k in range(0, topk, step):
+            for e in range(0, len(gates), _MOE_EXPERTS):
+                some = slice(e, min(e + _MOE_EXPERTS, len(gates)))
+                if (k, e) != (0, 0):  # a further part of these tokens' results
+                    part = torch.empty((tokens, h), dtype=torch.float32, device=dev) if part is None else part
+                    to = part[:n]
+                at = 4 * (first * topk + k)
+                _launch(dev, "vb_moe_grouped_ffn_routed", pointers(gates[some]), pointers(ups[some]), pointers(downs[some]),
+                        some.stop - e, x.data_ptr() + 4 * first * h, n, idx.data_ptr() + at, w.data_ptr() + at, topk, e,
+                        min(step, topk - k), to.data_ptr(), h, i, gates[0].qtype, downs[0].qtype, ws.data_ptr(), ws.numel())
+                if (k, e) != (0, 0):
+                    y[first:first + n] += to
     return y, idx, w
 
 
@@ -560,3 +610,117 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor | None, top: int =
             tokens.data_ptr(), tokens.element_size(), each, lp.data_ptr(), entropy.data_ptr(), top, ids.data_ptr(),
             best.data_ptr(), None if ws is None else ws.data_ptr(), nbytes)
     return lp, entropy, ids, best
+
+
+EXPERTS_MAX = 512  # logits per token of route_experts
+
+
+def route_experts(logits: torch.Tensor, topk: int, *, scores: str = "softmax", bias: torch.Tensor | None = None,
+                  groups: int = 1, groups_kept: int | None = None, group_score: str = "max", renorm: bool = True,
+                  scale: float = 1.0):
+    """Experts of every token and their weights from router logits (tokens, experts), float32 / float16 / bfloat16
+    with rows of any stride and at most 512 experts (vb_route_experts).  Returns ``(indices int32, weights
+    float32)``, (tokens, topk) each, the best expert first:
+
+        s = softmax(logits) or sigmoid(logits)          (``scores``)
+        c = s + bias                                    (float32 (experts,); without a bias c is the logit)
+        experts in ``groups`` equal runs: the ``groups_kept`` best ones stay, by the largest c of each
+            (``group_score="max"``) or by the sum of its two largest s + bias (``"top2"``)
+        the topk largest c of those, equal ones (and equal groups) by the lower id
+        weight = scale * s, over the sum of the chosen s with ``renorm``
+
+    Scores are compared in 64 bits.  A logit or bias of -inf keeps an expert from being chosen: where too few are
+    left the index is -1 and the weight 0.  A token with a NaN (or, under softmax, +inf) has indices -1 and weights
+    NaN.  ``moe_grouped_ffn(..., routing=(indices, weights))`` runs the experts; ``moe_route`` keeps the reference's
+    routing, which clamps the logits to +-50."""
+    dev = _gpu_tensor(logits, "route_experts: logits")
+    if logits.dim() != 2 or not 0 < logits.shape[1] <= EXPERTS_MAX:
+        raise ValueError(f"route_experts: logits must be (tokens, experts) with 1 to {EXPERTS_MAX} experts, got "
+                         f"{tuple(logits.shape)}")
+    kind = _elem(logits, "route_experts: logits")
+    tokens, experts = logits.shape
+    topk, groups = int(topk), int(groups)
+    kept = groups if groups_kept is None else int(groups_kept)
+    if scores not in ("softmax", "sigmoid") or group_score not in ("max", "top2"):
+        raise ValueError(f"route_experts: scores={scores!r} is softmax or sigmoid, group_score={group_score!r} max or top2")
+    if not 1 <= groups <= 64 or experts % groups or not 1 <= kept <= groups:
+        raise ValueError(f"route_experts: {kept} of {groups} groups (1 to 64, of equal size) of {experts} experts")
+    if not 1 <= topk <= min(64, kept * (experts // groups)):
+        raise ValueError(f"route_experts: topk={topk} is out of range (1 to {min(64, kept * (experts // groups))})")
+    if bias is not None:
+        if _gpu_tensor(bias, "route_experts: bias") != dev or bias.dtype != torch.float32 or bias.numel() != experts:
+            raise ValueError(f"route_experts: bias must be ({experts},) float32 on {dev}, got {tuple(bias.shape)} "
+                             f"{bias.dtype} on {bias.device}")
+        bias = bias.contiguous()
+    z = _rows_of(logits, experts)
+    idx = torch.empty((tokens, topk), dtype=torch.int32, device=dev)
+    w = torch.empty_like(idx, dtype=torch.float32)
+    _launch(dev, "vb_route_experts", z.data_ptr(), kind, z.stride(0), tokens, experts, topk, int(scores == "sigmoid"),
+            None if bias is None else bias.data_ptr(), groups, kept, int(group_score == "top2"), int(bool(renorm)), scale,
+            idx.data_ptr(), w.data_ptr())
+    return idx, w
+
+
+DRAFTS_MAX = 63  # drafted tokens per sequence of verify_draft
+
+
+def verify_draft(target: torch.Tensor, drafted: torch.Tensor, uniforms: torch.Tensor, draft: torch.Tensor | None = None,
+                 lengths: torch.Tensor | None = None, temperature: float = 1.0, draft_temperature: float | None = None):
+    """Drafted tokens against the target's probabilities, and the token that follows them (vb_verify_draft).
+    Returns ``(tokens (seqs, k + 1) int32, accepted (seqs,) int32)``: the accepted drafts, the next token, then -1.
+
+    target: (seqs, k + 1, vocab) logits, float32 / float16 / bfloat16, as ``gemm`` leaves them for the verified
+    positions; drafted: (seqs, k) ids, int32 or int64, k at most 63; uniforms: (seqs, k + 1) float32 in [0, 1), one
+    per draft and one for the next token.  draft: the drafter's logits (seqs, k, vocab), of the target's type (None: the
+    drafts came without probabilities, a lookup's say).  With p and q their softmax over ``temperature`` and
+    ``draft_temperature`` (the same by default), q = 1 at the draft without ``draft``:
+
+        draft j is accepted while u_j q_j(d_j) < p_j(d_j)
+        at the first that is not, the next token is drawn from max(p_j - q_j, 0), behind k accepted ones from p_k:
+        the first id whose sum of weights exceeds the last random number times the sum of all
+
+    so that the tokens are distributed as the target's own.  ``lengths`` (seqs,) int32: how many drafts of each
+    sequence count (an id outside the vocabulary ends them too).  Logits of -inf are never drawn.  A row with a NaN or
+    +inf, or a target row of -inf only, ends its sequence with the token -1."""
+    dev = _gpu_tensor(target, "verify_draft: target")
+    if target.dim() != 3 or target.shape[1] == 0 or target.shape[2] == 0:
+        raise ValueError(f"verify_draft: target must be (seqs, k + 1, vocab), got {tuple(target.shape)}")
+    kind = _elem(target, "verify_draft: target")
+    seqs, k, vocab = target.shape[0], target.shape[1] - 1, target.shape[2]
+    if k > DRAFTS_MAX:
+        raise ValueError(f"verify_draft: {k} drafts per sequence (at most {DRAFTS_MAX})")
+    if _gpu_tensor(drafted, "verify_draft: drafted") != dev or drafted.dtype not in (torch.int32, torch.int64) \
+            or tuple(drafted.shape) != (seqs, k):
+        raise ValueError(f"verify_draft: drafted must be ({seqs}, {k}) int32 or int64 on {dev}, got "
+                         f"{tuple(drafted.shape)} {drafted.dtype} on {drafted.device}")
+    if _gpu_tensor(uniforms, "verify_draft: uniforms") != dev or uniforms.dtype != torch.float32 \
+            or tuple(uniforms.shape) != (seqs, k + 1):
+        raise ValueError(f"verify_draft: uniforms must be ({seqs}, {k + 1}) float32 on {dev}, got "
+                         f"{tuple(uniforms.shape)} {uniforms.dtype} on {uniforms.device}")
+    if draft is not None and (_gpu_tensor(draft, "verify_draft: draft") != dev or draft.dtype != target.dtype
+                              or tuple(draft.shape) != (seqs, k, vocab)):
+        raise ValueError(f"verify_draft: draft must be ({seqs}, {k}, {vocab}) {target.dtype} on {dev}, got "
+                         f"{tuple(draft.shape)} {draft.dtype} on {draft.device}")
+    if lengths is not None:
+        if _gpu_tensor(lengths, "verify_draft: lengths") != dev or lengths.dtype != torch.int32 \
+                or tuple(lengths.shape) != (seqs,):
+            raise ValueError(f"verify_draft: lengths must be ({seqs},) int32 on {dev}, got {tuple(lengths.shape)} "
+                             f"{lengths.dtype} on {lengths.device}")
+        lengths = lengths.contiguous()
+    unit = lambda t: t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()  # noqa: E731
+    target, drafted, uniforms = unit(target), unit(drafted), unit(uniforms)
+    draft = None if draft is None or k == 0 else unit(draft)
+    if draft_temperature is None:
+        draft_temperature = temperature
+    tokens = torch.empty((seqs, k + 1), dtype=torch.int32, device=dev)
+    accepted = tokens.new_empty(seqs)
+    nbytes = _workspace_bytes(dev, "vb_verify_draft_workspace", seqs, k, vocab, int(draft is not None))
+    if nbytes < 0:
+        raise ValueError(f"verify_draft: no workspace for {seqs} sequences of {vocab} ids")
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+    _launch(dev, "vb_verify_draft", target.data_ptr(), kind, target.stride(0), target.stride(1),
+            None if draft is None else draft.data_ptr(), 0 if draft is None else draft.stride(0),
+            0 if draft is None else draft.stride(1), drafted.data_ptr(), drafted.element_size(), drafted.stride(0),
+            None if lengths is None else lengths.data_ptr(), uniforms.data_ptr(), uniforms.stride(0), seqs, k, vocab,
+            temperature, draft_temperature, tokens.data_ptr(), accepted.data_ptr(), ws.data_ptr(), nbytes)
+    return tokens, accepted
