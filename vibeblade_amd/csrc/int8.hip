@@ -113,47 +113,219 @@ __global__ void __launch_bounds__(256) i8_dequant_kernel(const uint8_t* w, Int8L
 }
 
 // ---- products ---------------------------------------------------------------
+//
+// A workgroup makes a tile of weight rows by tokens from stages of one block of
+// k (64): its blocks of both operands go by DMA into one of STAGES images in
+// LDS, each wave bringing its share of whole 1 KB blocks, and every wave reads
+// the blocks of its own rows and tokens, a conflict-free 16 bytes a lane each.
+// An image is filled STAGES - 1 stages before it is read, and one barrier a
+// stage says both that an image has landed and that the one behind is free.
+// A block is an operand as it lies in memory, so nothing is shuffled anywhere.
+//
+// A operands are the weights, B the tokens: a lane's four results are then four
+// neighbouring outputs of one token.
 
 struct I8Args {
     const uint8_t* w;
     const uint8_t* x;  // packed
     const float* bias;
     void* y;
+    int32_t* partial;  // [chunk of k][token][row of the last tile too], or null: y
     Int8Layout wl, xl;
     int64_t n, m;
     int32_t out_type;
+    int32_t chunk;     // blocks of k of a chunk
 };
 
-__device__ __forceinline__ void i8_store(const I8Args& a, int64_t t, int64_t n, int sum) {
-    const float sx = reinterpret_cast<const float*>(a.x + a.xl.scales)[t], sw = reinterpret_cast<const float*>(a.w + a.wl.scales)[n];
-    float v = static_cast<float>(sum) * sx * sw;
-    if (a.bias) v += a.bias[n];
-    elem_st(a.y, t * a.n + n, a.out_type, v);
+template <int N>
+__device__ __forceinline__ void wait_loads_barrier() {
+    // all but the wave's last N loads have landed, then everyone's
+    __builtin_amdgcn_sched_barrier(0);
+    __builtin_amdgcn_s_waitcnt(0x0F70 | (N & 15) | ((N >> 4) << 14));
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
 }
 
-// 16 rows of the weights by 16 tokens a workgroup, k over its four waves.
-__global__ void __launch_bounds__(256) i8_gemm_kernel(I8Args a) {
-    __shared__ i32x4 part[4][64];
-    const int lane = static_cast<int>(threadIdx.x) & 63, wave = static_cast<int>(threadIdx.x) >> 6;
-    for (int64_t item = blockIdx.x; item < a.wl.tiles * a.xl.tiles; item += gridDim.x) {
-        const int64_t tile = item % a.wl.tiles, cols = item / a.wl.tiles;
-        const i32x4* pw = reinterpret_cast<const i32x4*>(a.w) + tile * a.wl.blocks * 64 + lane;
-        const i32x4* px = reinterpret_cast<const i32x4*>(a.x) + cols * a.wl.blocks * 64 + lane;
-        i32x4 acc = {0, 0, 0, 0};
-        for (int64_t b = wave; b < a.wl.blocks; b += 4) acc = mfma_i8(pw[b * 64], px[b * 64], acc);
-        part[wave][lane] = acc;
-        __syncthreads();
-        if (wave == 0) {
-            const i32x4 sum = (part[0][lane] + part[1][lane]) + (part[2][lane] + part[3][lane]);
-            const int64_t t = cols * 16 + (lane & 15);
+// The results of four neighbouring rows n ... n + 3 and a token.
+__device__ __forceinline__ void i8_store4(const I8Args& a, int64_t t, int64_t n, i32x4 sum, float sx, float4 sw, bool vec) {
+    float v[4] = {static_cast<float>(sum[0]) * sx * sw.x, static_cast<float>(sum[1]) * sx * sw.y,
+                  static_cast<float>(sum[2]) * sx * sw.z, static_cast<float>(sum[3]) * sx * sw.w};
+    if (a.bias) {
 #pragma unroll
-            for (int r = 0; r < 4; r++) {
-                const int64_t n = tile * 16 + 4 * (lane >> 4) + r;
-                if (t < a.m && n < a.n) i8_store(a, t, n, sum[r]);
+        for (int r = 0; r < 4; r++) v[r] += n + r < a.n ? a.bias[n + r] : 0.f;
+    }
+    const int64_t at = t * a.n + n;
+    if (vec && n + 4 <= a.n) {
+        if (a.out_type == ELEM_F32) {
+            *reinterpret_cast<float4*>(static_cast<float*>(a.y) + at) = make_float4(v[0], v[1], v[2], v[3]);
+        } else {
+            uint2 u;
+            if (a.out_type == ELEM_BF16) {
+                u = make_uint2(f32_bf16x2(v[0], v[1]), f32_bf16x2(v[2], v[3]));
+            } else {
+                typedef _Float16 h4 __attribute__((ext_vector_type(4)));
+                const h4 h = {static_cast<_Float16>(v[0]), static_cast<_Float16>(v[1]), static_cast<_Float16>(v[2]),
+                              static_cast<_Float16>(v[3])};
+                u = __builtin_bit_cast(uint2, h);
+            }
+            *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.y) + at) = u;
+        }
+        return;
+    }
+#pragma unroll
+    for (int r = 0; r < 4; r++)
+        if (n + r < a.n) elem_st(a.y, at + r, a.out_type, v[r]);
+}
+
+// Whether rows of y take whole stores of four values.
+__device__ __forceinline__ bool i8_vec(const I8Args& a) {
+    return (a.n & 3) == 0 && (reinterpret_cast<uintptr_t>(a.y) & (a.out_type == ELEM_F32 ? 15 : 7)) == 0;
+}
+
+// Tile of (16 FR WR) weight rows by (16 FT WT) tokens by WR x WT waves, FR x FT
+// operands each.
+template <int FR, int FT, int WR, int WT, int STAGES>
+__global__ void __launch_bounds__(64 * WR * WT) i8_tile_kernel(I8Args a, int32_t row_tiles, int32_t col_tiles) {
+    constexpr int AR = FR * WR, AT = FT * WT, WAVES = WR * WT, SHARE = (AR + AT) / WAVES;
+    static_assert((AR + AT) % WAVES == 0 && STAGES == 4, "whole blocks a wave; the images below");
+    __shared__ i32x4 image0[(AR + AT) * 64], image1[(AR + AT) * 64], image2[(AR + AT) * 64], image3[(AR + AT) * 64];
+    const int lane = static_cast<int>(threadIdx.x) & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int wr = wave / WT, wt = wave % WT;
+    const int64_t blocks = a.wl.blocks;
+    const int item = static_cast<int>(blockIdx.x);
+    const int64_t row0 = static_cast<int64_t>(item % row_tiles) * AR, col0 = static_cast<int64_t>(item / row_tiles) * AT;
+    const int64_t first = static_cast<int64_t>(blockIdx.y) * a.chunk;
+    const int count = static_cast<int>(blocks - first < a.chunk ? blocks - first : a.chunk);
+    // past the matrix, the last rows of blocks again: their results are dropped
+    const int64_t rows_here = a.wl.tiles - row0 < AR ? a.wl.tiles - row0 : AR, cols_here = a.xl.tiles - col0 < AT ? a.xl.tiles - col0 : AT;
+    const auto ws = make_rsrc(a.w + row0 * blocks * INT8_BLOCK, static_cast<uint32_t>(rows_here * blocks * INT8_BLOCK));
+    const auto xs = make_rsrc(a.x + col0 * blocks * INT8_BLOCK, static_cast<uint32_t>(cols_here * blocks * INT8_BLOCK));
+    typedef __attribute__((address_space(3))) void* lds_ptr;
+    const auto stage_in = [&](int s, i32x4* image) __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = 0; i < SHARE; i++) {
+            const int b = wave * SHARE + i, last = static_cast<int>(b < AR ? rows_here : cols_here) - 1;
+            const int tile = (b < AR ? b : b - AR) < last ? (b < AR ? b : b - AR) : last;
+            const uint32_t at = static_cast<uint32_t>((tile * blocks + first + (s < count ? s : count - 1)) * INT8_BLOCK);
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(b < AR ? ws : xs, (lds_ptr)(image + b * 64), 16, 16 * lane,
+                                                     static_cast<int>(at), 0, 0);
+        }
+    };
+    i32x4 acc[FR][FT];
+#pragma unroll
+    for (int r = 0; r < FR; r++)
+#pragma unroll
+        for (int t = 0; t < FT; t++) acc[r][t] = i32x4{0, 0, 0, 0};
+    const auto multiply = [&](const i32x4* image) __attribute__((always_inline)) {
+        const i32x4* pa = image + wr * FR * 64 + lane;
+        const i32x4* pb = image + (AR + wt * FT) * 64 + lane;
+        i32x4 fb[FT], fa[FR];
+#pragma unroll
+        for (int t = 0; t < FT; t++) fb[t] = pb[t * 64];
+#pragma unroll
+        for (int r = 0; r < FR; r++) fa[r] = pa[r * 64];
+#pragma unroll
+        for (int r = 0; r < FR; r++)
+#pragma unroll
+            for (int t = 0; t < FT; t++) acc[r][t] = mfma_i8(fa[r], fb[t], acc[r][t]);
+    };
+    stage_in(0, image0);
+    stage_in(1, image1);
+    stage_in(2, image2);
+    for (int s = 0; s < count; s += 4) {
+        wait_loads_barrier<2 * SHARE>();
+        stage_in(s + 3, image3);
+        multiply(image0);
+        wait_loads_barrier<2 * SHARE>();
+        stage_in(s + 4, image0);
+        if (s + 1 < count) multiply(image1);
+        wait_loads_barrier<2 * SHARE>();
+        stage_in(s + 5, image1);
+        if (s + 2 < count) multiply(image2);
+        wait_loads_barrier<2 * SHARE>();
+        stage_in(s + 6, image2);
+        if (s + 3 < count) multiply(image3);
+    }
+    const bool vec = i8_vec(a);
+#pragma unroll
+    for (int t = 0; t < FT; t++) {
+        const int64_t token = (col0 + wt * FT + t) * 16 + (lane & 15);
+        if (token >= a.m) continue;
+        const float sx = reinterpret_cast<const float*>(a.x + a.xl.scales)[token];
+#pragma unroll
+        for (int r = 0; r < FR; r++) {
+            const int64_t n = (row0 + wr * FR + r) * 16 + 4 * (lane >> 4);
+            if (n >= a.n) continue;
+            if (a.partial) {
+                reinterpret_cast<i32x4*>(a.partial)[((static_cast<int64_t>(blockIdx.y) * a.m + token) * a.wl.tiles * 16 + n) >> 2] = acc[r][t];
+            } else {
+                i8_store4(a, token, n, acc[r][t], sx, *reinterpret_cast<const float4*>(a.w + a.wl.scales + 4 * n), vec);
             }
         }
-        __syncthreads();
     }
+}
+
+// The chunks' sums of four neighbouring rows and a token a thread.
+__global__ void __launch_bounds__(256) i8_join_kernel(I8Args a, int32_t chunks) {
+    const int64_t fours = a.wl.tiles * 4, all = a.m * fours;
+    const bool vec = i8_vec(a);
+    for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < all; i += static_cast<int64_t>(gridDim.x) * 256) {
+        const int64_t t = i / fours, n = i % fours * 4;
+        if (n >= a.n) continue;
+        const i32x4* p = reinterpret_cast<const i32x4*>(a.partial) + i;
+        i32x4 sum = p[0];
+        for (int c = 1; c < chunks; c++) sum += p[c * all];
+        i8_store4(a, t, n, sum, reinterpret_cast<const float*>(a.x + a.xl.scales)[t],
+                  *reinterpret_cast<const float4*>(a.w + a.wl.scales + 4 * n), vec);
+    }
+}
+
+struct I8Plan {
+    int shape;       // of the tiles
+    int64_t chunks;  // of k
+    int64_t chunk;   // blocks of k
+    int64_t packed, workspace;
+};
+
+constexpr int I8_SHAPE_ROWS[] = {256, 128, 128}, I8_SHAPE_COLS[] = {256, 128, 64};
+
+I8Plan i8_plan(const Int8Layout& wl, const Int8Layout& xl, int64_t m, bool packed) {
+    I8Plan p{};
+    const auto tiles = [&](int s) {
+        return ((wl.tiles * 16 + I8_SHAPE_ROWS[s] - 1) / I8_SHAPE_ROWS[s]) * ((xl.tiles * 16 + I8_SHAPE_COLS[s] - 1) / I8_SHAPE_COLS[s]);
+    };
+    p.shape = tiles(0) >= 2 * num_cus() ? 0 : xl.tiles > 4 ? 1 : 2;
+    if (const char* e = getenv("I8_SHAPE")) p.shape = atoi(e);
+    p.chunks = 1;
+    while (p.chunks < 16 && tiles(p.shape) * p.chunks * 2 <= 2 * num_cus() && wl.blocks >= 16 * p.chunks) p.chunks *= 2;
+    if (const char* e = getenv("I8_CHUNKS")) p.chunks = atoi(e);
+    p.chunk = (wl.blocks + p.chunks - 1) / p.chunks;
+    p.chunks = (wl.blocks + p.chunk - 1) / p.chunk;
+    p.packed = packed ? 0 : xl.total;
+    p.workspace = p.packed + (p.chunks > 1 ? p.chunks * m * wl.tiles * 64 : 0);
+    return p;
+}
+
+template <int FR, int FT, int WR, int WT>
+int i8_tile(const I8Args& a, const I8Plan& p, hipStream_t st) {
+    const int64_t rows = (a.wl.tiles + FR * WR - 1) / (FR * WR), cols = (a.xl.tiles + FT * WT - 1) / (FT * WT);
+    const dim3 grid(static_cast<uint32_t>(rows * cols), static_cast<uint32_t>(p.chunks));
+    i8_tile_kernel<FR, FT, WR, WT, 4><<<grid, 64 * WR * WT, 0, st>>>(a, static_cast<int32_t>(rows), static_cast<int32_t>(cols));
+    return check_launch("vb_int8_gemm");
+}
+
+int i8_run(I8Args a, const I8Plan& p, hipStream_t st) {
+    a.chunk = static_cast<int32_t>(p.chunk);
+    if (p.chunks == 1) a.partial = nullptr;
+    int rc = OK;
+    if (p.shape == 0) rc = i8_tile<8, 4, 2, 4>(a, p, st);
+    else if (p.shape == 1) rc = i8_tile<4, 4, 2, 2>(a, p, st);
+    else rc = i8_tile<4, 2, 2, 2>(a, p, st);
+    if (rc != OK || p.chunks == 1) return rc;
+    i8_join_kernel<<<i8_grid((a.m * a.wl.tiles * 4 + 255) / 256), 256, 0, st>>>(a, static_cast<int32_t>(p.chunks));
+    return check_launch("vb_int8_gemm");
 }
 
 int i8_quantize(const I8Rows& a, int32_t type, hipStream_t st) {
@@ -224,8 +396,8 @@ int vb_int8_dequant_rows(const void* w, float* out, int64_t rows, int64_t k, voi
 int64_t vb_int8_workspace(int64_t m, int64_t rows, int64_t k, int32_t x_type) {
     Int8Layout wl, xl;
     if (m < 0 || m > 0x7fffffff - 255 || (x_type != I8_PACKED && !elem_type(x_type)) || !int8_layout(rows, k, &wl)) return -1;
-    if (m == 0 || x_type == I8_PACKED) return 0;
-    return int8_layout(m, k, &xl) ? xl.total : -1;
+    if (m == 0) return 0;
+    return int8_layout(m, k, &xl) ? i8_plan(wl, xl, m, x_type == I8_PACKED).workspace : -1;
 }
 
 int vb_int8_gemm(const void* w, int64_t rows, int64_t k, const void* x, int32_t x_type, int64_t x_ld, int64_t m,
@@ -252,6 +424,7 @@ int vb_int8_gemm(const void* w, int64_t rows, int64_t k, const void* x, int32_t 
     a.w = static_cast<const uint8_t*>(w);
     a.wl = l;
     int8_layout(m, k, &a.xl);
+    const I8Plan p = i8_plan(l, a.xl, m, x_type == I8_PACKED);
     a.x = static_cast<const uint8_t*>(x);
     if (x_type != I8_PACKED) {
         a.x = static_cast<const uint8_t*>(workspace);
@@ -259,13 +432,13 @@ int vb_int8_gemm(const void* w, int64_t rows, int64_t k, const void* x, int32_t 
             rc != OK)
             return rc;
     }
+    a.partial = reinterpret_cast<int32_t*>(static_cast<uint8_t*>(workspace) + p.packed);
     a.bias = bias;
     a.y = y;
     a.n = rows;
     a.m = m;
     a.out_type = y_type;
-    i8_gemm_kernel<<<i8_grid(a.wl.tiles * a.xl.tiles), 256, 0, as_stream(stream)>>>(a);
-    return check_launch("vb_int8_gemm");
+    return i8_run(a, p, as_stream(stream));
 }
 
 }  // extern "C"
