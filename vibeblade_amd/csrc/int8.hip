@@ -115,12 +115,15 @@ __global__ void __launch_bounds__(256) i8_dequant_kernel(const uint8_t* w, Int8L
 // ---- products ---------------------------------------------------------------
 //
 // A workgroup makes a tile of weight rows by tokens from stages of one block of
-// k (64): its blocks of both operands go by DMA into one of STAGES images in
-// LDS, each wave bringing its share of whole 1 KB blocks, and every wave reads
-// the blocks of its own rows and tokens, a conflict-free 16 bytes a lane each.
-// An image is filled STAGES - 1 stages before it is read, and one barrier a
-// stage says both that an image has landed and that the one behind is free.
-// A block is an operand as it lies in memory, so nothing is shuffled anywhere.
+// k (64): its blocks of both operands go by DMA into one of four images in LDS,
+// each wave bringing its share of whole 1 KB blocks, and every wave reads the
+// blocks of its own rows and tokens, a conflict-free 16 bytes a lane each.  A
+// block is an operand as it lies in memory, so nothing is shuffled anywhere.
+//
+// While a wave multiplies a stage's operands it reads the next stage's from
+// their image and requests the blocks of the fourth stage on, into the image that
+// all have read: one barrier a stage says that an image has landed and that
+// another is free.
 //
 // A operands are the weights, B the tokens: a lane's four results are then four
 // neighbouring outputs of one token.
@@ -137,15 +140,28 @@ struct I8Args {
     int32_t chunk;     // blocks of k of a chunk
 };
 
+// The wave's LDS reads and all but its last N loads have landed, then everyone's.
 template <int N>
-__device__ __forceinline__ void wait_loads_barrier() {
-    // all but the wave's last N loads have landed, then everyone's
+__device__ __forceinline__ void landed_barrier() {
     __builtin_amdgcn_sched_barrier(0);
-    __builtin_amdgcn_s_waitcnt(0x0F70 | (N & 15) | ((N >> 4) << 14));
+    __builtin_amdgcn_s_waitcnt(0x0070 | (N & 15) | ((N >> 4) << 14));
     asm volatile("" ::: "memory");
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
     __builtin_amdgcn_sched_barrier(0);
+}
+
+// 16 bytes a lane from a buffer's at + 16 * lane into the 1 KB of LDS at `lds`.  In
+// asm, as the compiler would wait for other images' DMA before it reads one; the
+// waits are landed_barrier's.  (Writing M0 takes a wait state before its use.)
+__device__ __forceinline__ void dma_block(u32x4 rsrc, uint32_t lds, uint32_t lane16, uint32_t at) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds"
+                 :: "s"(lds), "v"(lane16), "s"(rsrc), "s"(at) : "memory");
+}
+
+__device__ __forceinline__ u32x4 buffer_of(const void* base, uint32_t bytes) {
+    const uint64_t p = reinterpret_cast<uintptr_t>(base);
+    return u32x4{static_cast<uint32_t>(p), static_cast<uint32_t>(p >> 32) & 0xffffu, bytes, 0x00020000u};
 }
 
 // The results of four neighbouring rows n ... n + 3 and a token.
@@ -186,11 +202,12 @@ __device__ __forceinline__ bool i8_vec(const I8Args& a) {
 
 // Tile of (16 FR WR) weight rows by (16 FT WT) tokens by WR x WT waves, FR x FT
 // operands each.
-template <int FR, int FT, int WR, int WT, int STAGES>
+template <int FR, int FT, int WR, int WT>
 __global__ void __launch_bounds__(64 * WR * WT) i8_tile_kernel(I8Args a, int32_t row_tiles, int32_t col_tiles) {
-    constexpr int AR = FR * WR, AT = FT * WT, WAVES = WR * WT, SHARE = (AR + AT) / WAVES;
-    static_assert((AR + AT) % WAVES == 0 && STAGES == 4, "whole blocks a wave; the images below");
-    __shared__ i32x4 image0[(AR + AT) * 64], image1[(AR + AT) * 64], image2[(AR + AT) * 64], image3[(AR + AT) * 64];
+    constexpr int AR = FR * WR, AT = FT * WT, WAVES = WR * WT, SA = AR / WAVES, SHARE = (AR + AT) / WAVES;
+    static_assert(AR % WAVES == 0 && AT % WAVES == 0, "whole blocks of each operand a wave");
+    constexpr int IMAGE = (AR + AT) * INT8_BLOCK;
+    __shared__ i32x4 images[4 * IMAGE / 16];
     const int lane = static_cast<int>(threadIdx.x) & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wr = wave / WT, wt = wave % WT;
     const int64_t blocks = a.wl.blocks;
@@ -200,54 +217,68 @@ __global__ void __launch_bounds__(64 * WR * WT) i8_tile_kernel(I8Args a, int32_t
     const int count = static_cast<int>(blocks - first < a.chunk ? blocks - first : a.chunk);
     // past the matrix, the last rows of blocks again: their results are dropped
     const int64_t rows_here = a.wl.tiles - row0 < AR ? a.wl.tiles - row0 : AR, cols_here = a.xl.tiles - col0 < AT ? a.xl.tiles - col0 : AT;
-    const auto ws = make_rsrc(a.w + row0 * blocks * INT8_BLOCK, static_cast<uint32_t>(rows_here * blocks * INT8_BLOCK));
-    const auto xs = make_rsrc(a.x + col0 * blocks * INT8_BLOCK, static_cast<uint32_t>(cols_here * blocks * INT8_BLOCK));
-    typedef __attribute__((address_space(3))) void* lds_ptr;
-    const auto stage_in = [&](int s, i32x4* image) __attribute__((always_inline)) {
+    const u32x4 ws = buffer_of(a.w + row0 * blocks * INT8_BLOCK, static_cast<uint32_t>(rows_here * blocks * INT8_BLOCK));
+    const u32x4 xs = buffer_of(a.x + col0 * blocks * INT8_BLOCK, static_cast<uint32_t>(cols_here * blocks * INT8_BLOCK));
+    typedef __attribute__((address_space(3))) i32x4* lds_ptr;
+    const uint32_t lds = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((lds_ptr)images)), lane16 = 16u * lane;
+    // the wave's block i of an image, from its first stage on
+    uint32_t from[SHARE];
 #pragma unroll
-        for (int i = 0; i < SHARE; i++) {
-            const int b = wave * SHARE + i, last = static_cast<int>(b < AR ? rows_here : cols_here) - 1;
-            const int tile = (b < AR ? b : b - AR) < last ? (b < AR ? b : b - AR) : last;
-            const uint32_t at = static_cast<uint32_t>((tile * blocks + first + (s < count ? s : count - 1)) * INT8_BLOCK);
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(b < AR ? ws : xs, (lds_ptr)(image + b * 64), 16, 16 * lane,
-                                                     static_cast<int>(at), 0, 0);
-        }
+    for (int i = 0; i < SHARE; i++) {
+        const int tile = i < SA ? wave * SA + i : wave * (SHARE - SA) + i - SA;
+        const int last = static_cast<int>(i < SA ? rows_here : cols_here) - 1;
+        from[i] = static_cast<uint32_t>(((tile < last ? tile : last) * blocks + first) * INT8_BLOCK);
+    }
+    // block i of stage s (the last one again past the end) into image q
+    const auto request = [&](int s, int q, int i) __attribute__((always_inline)) {
+        const int to = i < SA ? wave * SA + i : AR + wave * (SHARE - SA) + i - SA;
+        dma_block(i < SA ? ws : xs, lds + q * IMAGE + to * INT8_BLOCK, lane16,
+                  from[i] + static_cast<uint32_t>(s < count ? s : count - 1) * INT8_BLOCK);
     };
-    i32x4 acc[FR][FT];
+    i32x4 acc[FR][FT], fr[2][FR], ft[2][FT];
 #pragma unroll
     for (int r = 0; r < FR; r++)
 #pragma unroll
         for (int t = 0; t < FT; t++) acc[r][t] = i32x4{0, 0, 0, 0};
-    const auto multiply = [&](const i32x4* image) __attribute__((always_inline)) {
-        const i32x4* pa = image + wr * FR * 64 + lane;
-        const i32x4* pb = image + (AR + wt * FT) * 64 + lane;
-        i32x4 fb[FT], fa[FR];
-#pragma unroll
-        for (int t = 0; t < FT; t++) fb[t] = pb[t * 64];
-#pragma unroll
-        for (int r = 0; r < FR; r++) fa[r] = pa[r * 64];
-#pragma unroll
-        for (int r = 0; r < FR; r++)
-#pragma unroll
-            for (int t = 0; t < FT; t++) acc[r][t] = mfma_i8(fa[r], fb[t], acc[r][t]);
+    const i32x4* mine_r = images + wr * FR * 64 + lane;
+    const i32x4* mine_t = images + (AR + wt * FT) * 64 + lane;
+    // operand i (tokens, then rows) from image q
+    const auto read = [&](int q, int p, int i) __attribute__((always_inline)) {
+        if (i < FT) ft[p][i] = mine_t[q * (IMAGE / 16) + i * 64];
+        else fr[p][i - FT] = mine_r[q * (IMAGE / 16) + (i - FT) * 64];
     };
-    stage_in(0, image0);
-    stage_in(1, image1);
-    stage_in(2, image2);
-    for (int s = 0; s < count; s += 4) {
-        wait_loads_barrier<2 * SHARE>();
-        stage_in(s + 3, image3);
-        multiply(image0);
-        wait_loads_barrier<2 * SHARE>();
-        stage_in(s + 4, image0);
-        if (s + 1 < count) multiply(image1);
-        wait_loads_barrier<2 * SHARE>();
-        stage_in(s + 5, image1);
-        if (s + 2 < count) multiply(image2);
-        wait_loads_barrier<2 * SHARE>();
-        stage_in(s + 6, image2);
-        if (s + 3 < count) multiply(image3);
+    // stage s, whose image was q, with the operands of parity p
+    const auto step = [&](int s, int q, int p) __attribute__((always_inline)) {
+        landed_barrier<2 * SHARE>();
+#pragma unroll
+        for (int r = 0; r < FR; r++) {
+#pragma unroll
+            for (int i = r * (FR + FT) / FR; i < (r + 1) * (FR + FT) / FR; i++) read((q + 1) & 3, p ^ 1, i);
+#pragma unroll
+            for (int i = r * SHARE / FR; i < (r + 1) * SHARE / FR; i++) request(s + 4, q, i);
+#pragma unroll
+            for (int t = 0; t < FT; t++) acc[r][t] = mfma_i8(fr[p][r], ft[p][t], acc[r][t]);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    };
+#pragma unroll
+    for (int q = 0; q < 4; q++)
+#pragma unroll
+        for (int i = 0; i < SHARE; i++) request(q, q, i);
+    landed_barrier<3 * SHARE>();
+#pragma unroll
+    for (int i = 0; i < FR + FT; i++) read(0, 0, i);
+    for (int s = 0;; s += 4) {
+        step(s, 0, 0);
+        if (s + 1 >= count) break;
+        step(s + 1, 1, 1);
+        if (s + 2 >= count) break;
+        step(s + 2, 2, 0);
+        if (s + 3 >= count) break;
+        step(s + 3, 3, 1);
+        if (s + 4 >= count) break;
     }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // no DMA is left when the workgroup's LDS goes
     const bool vec = i8_vec(a);
 #pragma unroll
     for (int t = 0; t < FT; t++) {
@@ -289,7 +320,7 @@ struct I8Plan {
     int64_t packed, workspace;
 };
 
-constexpr int I8_SHAPE_ROWS[] = {256, 128, 128}, I8_SHAPE_COLS[] = {256, 128, 64};
+constexpr int I8_SHAPE_ROWS[] = {256, 128, 128, 256}, I8_SHAPE_COLS[] = {256, 128, 64, 256};
 
 I8Plan i8_plan(const Int8Layout& wl, const Int8Layout& xl, int64_t m, bool packed) {
     I8Plan p{};
@@ -312,7 +343,7 @@ template <int FR, int FT, int WR, int WT>
 int i8_tile(const I8Args& a, const I8Plan& p, hipStream_t st) {
     const int64_t rows = (a.wl.tiles + FR * WR - 1) / (FR * WR), cols = (a.xl.tiles + FT * WT - 1) / (FT * WT);
     const dim3 grid(static_cast<uint32_t>(rows * cols), static_cast<uint32_t>(p.chunks));
-    i8_tile_kernel<FR, FT, WR, WT, 4><<<grid, 64 * WR * WT, 0, st>>>(a, static_cast<int32_t>(rows), static_cast<int32_t>(cols));
+    i8_tile_kernel<FR, FT, WR, WT><<<grid, 64 * WR * WT, 0, st>>>(a, static_cast<int32_t>(rows), static_cast<int32_t>(cols));
     return check_launch("vb_int8_gemm");
 }
 
@@ -321,6 +352,7 @@ int i8_run(I8Args a, const I8Plan& p, hipStream_t st) {
     if (p.chunks == 1) a.partial = nullptr;
     int rc = OK;
     if (p.shape == 0) rc = i8_tile<8, 4, 2, 4>(a, p, st);
+    else if (p.shape == 3) rc = i8_tile<8, 8, 2, 2>(a, p, st);
     else if (p.shape == 1) rc = i8_tile<4, 4, 2, 2>(a, p, st);
     else rc = i8_tile<4, 2, 2, 2>(a, p, st);
     if (rc != OK || p.chunks == 1) return rc;
