@@ -165,39 +165,57 @@ __device__ __forceinline__ u32x4 buffer_of(const void* base, uint32_t bytes) {
 }
 
 // The results of four neighbouring rows n ... n + 3 and a token.
-__device__ __forceinline__ void i8_store4(const I8Args& a, int64_t t, int64_t n, i32x4 sum, float sx, float4 sw, bool vec) {
-    float v[4] = {static_cast<float>(sum[0]) * sx * sw.x, static_cast<float>(sum[1]) * sx * sw.y,
-                  static_cast<float>(sum[2]) * sx * sw.z, static_cast<float>(sum[3]) * sx * sw.w};
+__device__ __forceinline__ float4 i8_results(const I8Args& a, int64_t n, i32x4 sum, float sx, float4 sw) {
+    float4 v = make_float4(static_cast<float>(sum[0]) * sx * sw.x, static_cast<float>(sum[1]) * sx * sw.y,
+                           static_cast<float>(sum[2]) * sx * sw.z, static_cast<float>(sum[3]) * sx * sw.w);
     if (a.bias) {
-#pragma unroll
-        for (int r = 0; r < 4; r++) v[r] += n + r < a.n ? a.bias[n + r] : 0.f;
+        v.x += n < a.n ? a.bias[n] : 0.f;
+        v.y += n + 1 < a.n ? a.bias[n + 1] : 0.f;
+        v.z += n + 2 < a.n ? a.bias[n + 2] : 0.f;
+        v.w += n + 3 < a.n ? a.bias[n + 3] : 0.f;
     }
+    return v;
+}
+
+// Four results as bf16 or fp16.
+__device__ __forceinline__ uint2 i8_halves(const I8Args& a, float4 v) {
+    if (a.out_type == ELEM_BF16) return make_uint2(f32_bf16x2(v.x, v.y), f32_bf16x2(v.z, v.w));
+    typedef _Float16 h4 __attribute__((ext_vector_type(4)));
+    const h4 h = {static_cast<_Float16>(v.x), static_cast<_Float16>(v.y), static_cast<_Float16>(v.z), static_cast<_Float16>(v.w)};
+    return __builtin_bit_cast(uint2, h);
+}
+
+__device__ __forceinline__ void i8_store4(const I8Args& a, int64_t t, int64_t n, i32x4 sum, float sx, float4 sw, bool vec) {
+    const float4 v = i8_results(a, n, sum, sx, sw);
     const int64_t at = t * a.n + n;
     if (vec && n + 4 <= a.n) {
-        if (a.out_type == ELEM_F32) {
-            *reinterpret_cast<float4*>(static_cast<float*>(a.y) + at) = make_float4(v[0], v[1], v[2], v[3]);
-        } else {
-            uint2 u;
-            if (a.out_type == ELEM_BF16) {
-                u = make_uint2(f32_bf16x2(v[0], v[1]), f32_bf16x2(v[2], v[3]));
-            } else {
-                typedef _Float16 h4 __attribute__((ext_vector_type(4)));
-                const h4 h = {static_cast<_Float16>(v[0]), static_cast<_Float16>(v[1]), static_cast<_Float16>(v[2]),
-                              static_cast<_Float16>(v[3])};
-                u = __builtin_bit_cast(uint2, h);
-            }
-            *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.y) + at) = u;
-        }
+        if (a.out_type == ELEM_F32) *reinterpret_cast<float4*>(static_cast<float*>(a.y) + at) = v;
+        else *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.y) + at) = i8_halves(a, v);
         return;
     }
+    const float u[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
     for (int r = 0; r < 4; r++)
-        if (n + r < a.n) elem_st(a.y, at + r, a.out_type, v[r]);
+        if (n + r < a.n) elem_st(a.y, at + r, a.out_type, u[r]);
 }
 
 // Whether rows of y take whole stores of four values.
 __device__ __forceinline__ bool i8_vec(const I8Args& a) {
     return (a.n & 3) == 0 && (reinterpret_cast<uintptr_t>(a.y) & (a.out_type == ELEM_F32 ? 15 : 7)) == 0;
+}
+
+// The tile of this workgroup, or x < 0: none.  Workgroups go to the eight dies in
+// turn, and each die has an L2 of its own: a die takes one run of the tiles, in
+// panels of PANEL column tiles, so that the 32 that it has at once share both
+// their rows and their columns.
+constexpr int I8_DIES = 8, I8_PANEL = 4;
+__device__ __forceinline__ int2 tile_of(int rows, int cols) {
+    const int all = rows * cols, each = (all + I8_DIES - 1) / I8_DIES;
+    const int b = static_cast<int>(blockIdx.x), at = b % I8_DIES * each + b / I8_DIES;
+    if (b / I8_DIES >= each || at >= all) return make_int2(-1, 0);
+    const int panel = at / (rows * I8_PANEL), in = at % (rows * I8_PANEL);
+    const int wide = cols - panel * I8_PANEL < I8_PANEL ? cols - panel * I8_PANEL : I8_PANEL;
+    return make_int2(in / wide, panel * I8_PANEL + in % wide);
 }
 
 // Tile of (16 FR WR) weight rows by (16 FT WT) tokens by WR x WT waves, FR x FT
@@ -211,8 +229,9 @@ __global__ void __launch_bounds__(64 * WR * WT) i8_tile_kernel(I8Args a, int32_t
     const int lane = static_cast<int>(threadIdx.x) & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wr = wave / WT, wt = wave % WT;
     const int64_t blocks = a.wl.blocks;
-    const int item = static_cast<int>(blockIdx.x);
-    const int64_t row0 = static_cast<int64_t>(item % row_tiles) * AR, col0 = static_cast<int64_t>(item / row_tiles) * AT;
+    const int2 at = tile_of(row_tiles, col_tiles);
+    if (at.x < 0) return;
+    const int64_t row0 = static_cast<int64_t>(at.x) * AR, col0 = static_cast<int64_t>(at.y) * AT;
     const int64_t first = static_cast<int64_t>(blockIdx.y) * a.chunk;
     const int count = static_cast<int>(blocks - first < a.chunk ? blocks - first : a.chunk);
     // past the matrix, the last rows of blocks again: their results are dropped
@@ -278,23 +297,63 @@ __global__ void __launch_bounds__(64 * WR * WT) i8_tile_kernel(I8Args a, int32_t
         step(s + 3, 3, 1);
         if (s + 4 >= count) break;
     }
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // no DMA is left when the workgroup's LDS goes
-    const bool vec = i8_vec(a);
+    // No DMA is in flight, and all have read their last operands: the images are
+    // free.  A lane's results are four rows of a token, and 16 rows of 16 tokens
+    // would be pieces of 32 bytes: the wave's go through its share of LDS, 16
+    // tokens at a time, and out as whole runs of its rows.
+    landed_barrier<0>();
+    const int size = a.partial || a.out_type == ELEM_F32 ? 4 : 2, pitch = 16 * FR * size + 16;
+    uint8_t* mine = reinterpret_cast<uint8_t*>(images) + wave * (16 * (64 * FR + 16));
+    static_assert(WAVES * 16 * (64 * FR + 16) <= 4 * IMAGE, "the waves' shares");
+    const int64_t n0 = (row0 + wr * FR) * 16, width = a.partial ? a.wl.tiles * 16 : a.n;
+    uint8_t* const y = a.partial ? reinterpret_cast<uint8_t*>(a.partial) + static_cast<int64_t>(blockIdx.y) * a.m * width * 4
+                                 : static_cast<uint8_t*>(a.y);
+    const bool vec = (width * size & 15) == 0 && (reinterpret_cast<uintptr_t>(y) & 15) == 0;
 #pragma unroll
     for (int t = 0; t < FT; t++) {
-        const int64_t token = (col0 + wt * FT + t) * 16 + (lane & 15);
-        if (token >= a.m) continue;
+        const int64_t t0 = (col0 + wt * FT + t) * 16;
+        if (t0 >= a.m) break;
+        const int64_t token = t0 + (lane & 15) < a.m ? t0 + (lane & 15) : a.m - 1;
         const float sx = reinterpret_cast<const float*>(a.x + a.xl.scales)[token];
 #pragma unroll
         for (int r = 0; r < FR; r++) {
-            const int64_t n = (row0 + wr * FR + r) * 16 + 4 * (lane >> 4);
-            if (n >= a.n) continue;
+            const int64_t n = n0 + r * 16 + 4 * (lane >> 4);
+            uint8_t* to = mine + (lane & 15) * pitch + (r * 16 + 4 * (lane >> 4)) * size;
             if (a.partial) {
-                reinterpret_cast<i32x4*>(a.partial)[((static_cast<int64_t>(blockIdx.y) * a.m + token) * a.wl.tiles * 16 + n) >> 2] = acc[r][t];
+                *reinterpret_cast<i32x4*>(to) = acc[r][t];
             } else {
-                i8_store4(a, token, n, acc[r][t], sx, *reinterpret_cast<const float4*>(a.w + a.wl.scales + 4 * n), vec);
+                const bool in = n < a.wl.tiles * 16;
+                const float4 v = i8_results(a, n, acc[r][t], sx,
+                                            in ? *reinterpret_cast<const float4*>(a.w + a.wl.scales + 4 * n) : make_float4(0.f, 0.f, 0.f, 0.f));
+                if (size == 4) *reinterpret_cast<float4*>(to) = v;
+                else *reinterpret_cast<uint2*>(to) = i8_halves(a, v);
             }
         }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        const int pieces = FR * size;  // of 16 bytes, of a token
+        for (int i = lane; i < 16 * pieces; i += 64) {
+            const int row = i / pieces, piece = i % pieces;
+            const int64_t n = n0 + piece * 16 / size;
+            if (t0 + row >= a.m || n >= width) continue;
+            const uint4 v = *reinterpret_cast<const uint4*>(mine + row * pitch + piece * 16);
+            uint8_t* to = y + ((t0 + row) * width + n) * size;
+            if (vec) {
+                *reinterpret_cast<uint4*>(to) = v;
+            } else {
+                const uint32_t u[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+                for (int j = 0; j < 8; j++) {
+                    if (size == 2) {
+                        if (n + j < width) reinterpret_cast<uint16_t*>(to)[j] = static_cast<uint16_t>(u[j >> 1] >> 16 * (j & 1));
+                    } else if (j < 4 && n + j < width) {
+                        reinterpret_cast<uint32_t*>(to)[j] = u[j];
+                    }
+                }
+            }
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
     }
 }
 
@@ -342,7 +401,7 @@ I8Plan i8_plan(const Int8Layout& wl, const Int8Layout& xl, int64_t m, bool packe
 template <int FR, int FT, int WR, int WT>
 int i8_tile(const I8Args& a, const I8Plan& p, hipStream_t st) {
     const int64_t rows = (a.wl.tiles + FR * WR - 1) / (FR * WR), cols = (a.xl.tiles + FT * WT - 1) / (FT * WT);
-    const dim3 grid(static_cast<uint32_t>(rows * cols), static_cast<uint32_t>(p.chunks));
+    const dim3 grid(static_cast<uint32_t>((rows * cols + I8_DIES - 1) / I8_DIES * I8_DIES), static_cast<uint32_t>(p.chunks));
     i8_tile_kernel<FR, FT, WR, WT><<<grid, 64 * WR * WT, 0, st>>>(a, static_cast<int32_t>(rows), static_cast<int32_t>(cols));
     return check_launch("vb_int8_gemm");
 }
@@ -352,7 +411,6 @@ int i8_run(I8Args a, const I8Plan& p, hipStream_t st) {
     if (p.chunks == 1) a.partial = nullptr;
     int rc = OK;
     if (p.shape == 0) rc = i8_tile<8, 4, 2, 4>(a, p, st);
-    else if (p.shape == 3) rc = i8_tile<8, 8, 2, 2>(a, p, st);
     else if (p.shape == 1) rc = i8_tile<4, 4, 2, 2>(a, p, st);
     else rc = i8_tile<4, 2, 2, 2>(a, p, st);
     if (rc != OK || p.chunks == 1) return rc;
