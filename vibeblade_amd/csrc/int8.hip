@@ -33,16 +33,106 @@ __device__ __forceinline__ float scale_of(float big) {
     return big > 0.f ? fmaxf(big / 127.f, 0x1p-126f) : 0.f;
 }
 
-// v / s to the nearest integer, ties to even: the quotient of fp32's division may
-// have been rounded onto a tie, which the remainder tells.
+// v / s to the nearest integer, ties to even, with inv = 1 / s rounded: the
+// remainder v - q s, exact in the fma, tells a q that is not the nearest.
 __device__ __forceinline__ int code_of(float v, float s, float inv) {
-    float q = rintf(v * inv);
-    // v - q s is exact in the fma; a code that is not the nearest is off by one
-    const float r = __builtin_fmaf(-q, s, v), half = 0.5f * s;
-    if (r > half || (r == half && (static_cast<int>(q) & 1))) q += 1.f;
-    else if (r < -half || (r == -half && (static_cast<int>(q) & 1))) q -= 1.f;
-    return static_cast<int>(q);
+    const float q = rintf(v * inv), r = __builtin_fmaf(-q, s, v), twice = r + r;
+    const int c = static_cast<int>(q);
+    // one further where more than half a step is left, or half of one behind an odd code
+    const bool off = fabsf(twice) > s || (fabsf(twice) == s && (c & 1));
+    return off ? c + (r > 0.f ? 1 : -1) : c;
 }
+
+// 16 consecutive values of a row, from k0 on (0 past the row's end).
+template <int TYPE>
+struct Values {
+    float v[16];
+    // whole: rows begin at multiples of 16 bytes
+    __device__ __forceinline__ void load(const void* row, int64_t k0, int64_t k, bool whole) {
+        if (whole && k0 + 16 <= k) {
+            if constexpr (TYPE == ELEM_F32) {
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const float4 f = reinterpret_cast<const float4*>(static_cast<const float*>(row) + k0)[i];
+                    v[4 * i] = f.x, v[4 * i + 1] = f.y, v[4 * i + 2] = f.z, v[4 * i + 3] = f.w;
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < 2; i++) {
+                    const uint4 q = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(row) + k0)[i];
+                    const uint32_t u[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+                    for (int j = 0; j < 8; j++) {
+                        const uint32_t h = u[j >> 1] >> 16 * (j & 1) & 0xffffu;
+                        v[8 * i + j] = TYPE == ELEM_BF16 ? __uint_as_float(h << 16)
+                                                         : static_cast<float>(__builtin_bit_cast(_Float16, static_cast<uint16_t>(h)));
+                    }
+                }
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 16; i++) v[i] = k0 + i < k ? elem_ld(row, k0 + i, TYPE) : 0.f;
+        }
+    }
+    // the largest magnitude as bits: infinities and NaN from 0x7f800000 on
+    __device__ __forceinline__ uint32_t largest() const {
+        uint32_t b = 0;
+#pragma unroll
+        for (int i = 0; i < 16; i++) {
+            const uint32_t m = __float_as_uint(v[i]) & 0x7fffffffu;
+            b = m > b ? m : b;
+        }
+        return b;
+    }
+    // The low byte of v / s + 3 * 2^22, rounded by one fma, is the code, unless the
+    // remainder of one of the sixteen says that its quotient is not the nearest
+    // (or a tie): then all by code_of.
+    __device__ __forceinline__ uint4 codes(float s, float inv) const {
+        if (!(s > 0.f)) return make_uint4(0, 0, 0, 0);
+        uint32_t t[16], w[4];
+        float most = 0.f;
+#pragma unroll
+        for (int i = 0; i < 16; i++) {
+            const float q = __builtin_fmaf(v[i], inv, 12582912.f);
+            t[i] = __float_as_uint(q);
+            most = fmaxf(most, fabsf(__builtin_fmaf(12582912.f - q, s, v[i])));
+        }
+        if (!(most + most < s)) {
+#pragma unroll
+            for (int i = 0; i < 16; i++) t[i] = static_cast<uint32_t>(code_of(v[i], s, inv));
+        }
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            // bytes 0 of two values, twice
+            const uint32_t lo = __builtin_amdgcn_perm(t[4 * i + 1], t[4 * i], 0x0c0c0400u);
+            w[i] = __builtin_amdgcn_perm(t[4 * i + 3], t[4 * i + 2], 0x04000c0cu) | lo;
+        }
+        return make_uint4(w[0], w[1], w[2], w[3]);
+    }
+};
+
+__device__ __forceinline__ uint32_t wave_max_bits(uint32_t v) {
+    const auto take = [&](uint32_t u) { v = u > v ? u : v; };
+    take(__builtin_amdgcn_update_dpp(v, v, 0xB1, 0xF, 0xF, false));   // quad_perm [1,0,3,2]
+    take(__builtin_amdgcn_update_dpp(v, v, 0x4E, 0xF, 0xF, false));   // quad_perm [2,3,0,1]
+    take(__builtin_amdgcn_update_dpp(v, v, 0x141, 0xF, 0xF, false));  // row_half_mirror
+    take(__builtin_amdgcn_update_dpp(v, v, 0x140, 0xF, 0xF, false));  // row_mirror
+    take(__builtin_amdgcn_update_dpp(v, v, 0x142, 0xA, 0xF, false));  // row_bcast:15 into rows 1, 3
+    take(__builtin_amdgcn_update_dpp(v, v, 0x143, 0xC, 0xF, false));  // row_bcast:31 into rows 2, 3
+    return __builtin_amdgcn_readlane(v, 63);
+}
+
+// The scale of a row by the bits of its largest magnitude: codes by s (0: all
+// 0), and what is stored.
+struct RowScale {
+    float s, inv, stored;
+    __device__ __forceinline__ explicit RowScale(uint32_t bits) {
+        const bool bad = bits >= 0x7f800000u;
+        s = bad ? 0.f : scale_of(__uint_as_float(bits));
+        inv = s > 0.f ? 1.f / s : 0.f;
+        stored = bad ? NAN : s;
+    }
+};
 
 // Byte k of row r in the codes.
 __device__ __forceinline__ int64_t code_at(int64_t blocks, int64_t r, int64_t k) {
@@ -54,34 +144,66 @@ struct I8Rows {
     uint8_t* w;
     Int8Layout l;
     int64_t ld, rows, k;
+    bool whole;  // rows of src begin at multiples of 16 bytes
 };
 
-// One workgroup a row (rows to the end of the last tile: zeros).
-template <int TYPE>
-__global__ void __launch_bounds__(256) i8_quantize_kernel(I8Rows a) {
-    __shared__ float bigs[4];
-    const int wave = static_cast<int>(threadIdx.x) >> 6;
-    for (int64_t row = blockIdx.x; row < a.l.tiles * INT8_ROWS; row += gridDim.x) {
-        float big = 0.f;
-        bool bad = false;
-        if (row < a.rows)
-            for (int64_t i = threadIdx.x; i < a.k; i += 256) {
-                const float v = fabsf(elem_ld(a.src, row * a.ld + i, TYPE));
-                bad = bad || !(v < INFINITY);
-                big = fmaxf(big, v);
-            }
+// A row by a wave (WAVES = 1; eight rows a workgroup) or by a workgroup of 16
+// waves, which few rows need; a thread's first HELD pieces of 16 values are
+// read once, longer rows again for their codes.  Rows to the end of the last
+// tile are zeros.
+template <int TYPE, int WAVES>
+__global__ void __launch_bounds__(WAVES == 1 ? 512 : 1024) i8_quantize_kernel(I8Rows a) {
+    __shared__ uint32_t bigs[16];
+    const int lane = static_cast<int>(threadIdx.x) & 63, wave = static_cast<int>(threadIdx.x) >> 6;
+    const int at = WAVES == 1 ? lane : static_cast<int>(threadIdx.x);
+    constexpr int SPAN = 64 * WAVES, HELD = WAVES == 1 ? 4 : 1, ROWS = WAVES == 1 ? 8 : 1;
+    const int64_t pieces = a.l.blocks * 4, all = a.l.tiles * INT8_ROWS;
+    for (int64_t r0 = static_cast<int64_t>(blockIdx.x) * ROWS; r0 < all; r0 += static_cast<int64_t>(gridDim.x) * ROWS) {
+        const int64_t row = WAVES == 1 ? r0 + wave : r0;
+        const bool in = row < a.rows;
+        const uint8_t* src = static_cast<const uint8_t*>(a.src) + (in ? row * a.ld * (TYPE == ELEM_F32 ? 4 : 2) : 0);
+        Values<TYPE> held[HELD];
+        uint32_t big = 0;
 #pragma unroll
-        for (int o = 32; o >= 1; o >>= 1) big = fmaxf(big, __shfl_xor(big, o, 64));
-        if ((threadIdx.x & 63) == 0) bigs[wave] = big;
-        bad = __syncthreads_or(bad);
-        big = fmaxf(fmaxf(bigs[0], bigs[1]), fmaxf(bigs[2], bigs[3]));
-        const float s = bad ? 0.f : scale_of(big), inv = s > 0.f ? 1.f / s : 0.f;
-        for (int64_t i = threadIdx.x; i < a.l.blocks * INT8_K; i += 256) {
-            const float v = s > 0.f && i < a.k ? elem_ld(a.src, row * a.ld + i, TYPE) : 0.f;
-            a.w[code_at(a.l.blocks, row, i)] = static_cast<uint8_t>(code_of(v, s, inv));
+        for (int h = 0; h < HELD; h++) {
+            const int64_t p = at + h * SPAN;
+            if (in && p < pieces) {
+                held[h].load(src, p * 16, a.k, a.whole);
+                const uint32_t b = held[h].largest();
+                big = b > big ? b : big;
+            }
         }
-        if (threadIdx.x == 0) reinterpret_cast<float*>(a.w + a.l.scales)[row] = bad ? NAN : s;
-        __syncthreads();
+        for (int64_t p = at + HELD * SPAN; in && p < pieces; p += SPAN) {
+            Values<TYPE> v;
+            v.load(src, p * 16, a.k, a.whole);
+            const uint32_t b = v.largest();
+            big = b > big ? b : big;
+        }
+        big = wave_max_bits(big);
+        if constexpr (WAVES > 1) {
+            if (lane == 0) bigs[wave] = big;
+            __syncthreads();
+            big = wave_max_bits(lane < WAVES ? bigs[lane] : 0);
+            __syncthreads();
+        }
+        const RowScale s(big);
+        uint8_t* to = a.w + code_at(a.l.blocks, row, 0);
+#pragma unroll
+        for (int h = 0; h < HELD; h++) {
+            const int64_t p = at + h * SPAN;
+            if (p < pieces) *reinterpret_cast<uint4*>(to + (p >> 2) * INT8_BLOCK + (p & 3) * 256) =
+                in ? held[h].codes(s.s, s.inv) : make_uint4(0, 0, 0, 0);
+        }
+        for (int64_t p = at + HELD * SPAN; p < pieces; p += SPAN) {
+            uint4 c = make_uint4(0, 0, 0, 0);
+            if (in) {
+                Values<TYPE> v;
+                v.load(src, p * 16, a.k, a.whole);
+                c = v.codes(s.s, s.inv);
+            }
+            *reinterpret_cast<uint4*>(to + (p >> 2) * INT8_BLOCK + (p & 3) * 256) = c;
+        }
+        if (at == 0) reinterpret_cast<float*>(a.w + a.l.scales)[row] = in ? s.stored : 0.f;
     }
 }
 
@@ -145,6 +267,16 @@ template <int N>
 __device__ __forceinline__ void landed_barrier() {
     __builtin_amdgcn_sched_barrier(0);
     __builtin_amdgcn_s_waitcnt(0x0070 | (N & 15) | ((N >> 4) << 14));
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+}
+
+// The wave's LDS accesses are done, then everyone's; its loads stay in flight.
+__device__ __forceinline__ void lds_barrier() {
+    __builtin_amdgcn_sched_barrier(0);
+    __builtin_amdgcn_s_waitcnt(0xC07F);
     asm volatile("" ::: "memory");
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
@@ -222,8 +354,7 @@ __device__ __forceinline__ int2 tile_of(int rows, int cols) {
 // operands each.
 template <int FR, int FT, int WR, int WT>
 __global__ void __launch_bounds__(64 * WR * WT) i8_tile_kernel(I8Args a, int32_t row_tiles, int32_t col_tiles) {
-    constexpr int AR = FR * WR, AT = FT * WT, WAVES = WR * WT, SA = AR / WAVES, SHARE = (AR + AT) / WAVES;
-    static_assert(AR % WAVES == 0 && AT % WAVES == 0, "whole blocks of each operand a wave");
+    constexpr int AR = FR * WR, AT = FT * WT, WAVES = WR * WT, SHARE = (AR + AT + WAVES - 1) / WAVES;
     constexpr int IMAGE = (AR + AT) * INT8_BLOCK;
     __shared__ i32x4 images[4 * IMAGE / 16];
     const int lane = static_cast<int>(threadIdx.x) & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -240,19 +371,21 @@ __global__ void __launch_bounds__(64 * WR * WT) i8_tile_kernel(I8Args a, int32_t
     const u32x4 xs = buffer_of(a.x + col0 * blocks * INT8_BLOCK, static_cast<uint32_t>(cols_here * blocks * INT8_BLOCK));
     typedef __attribute__((address_space(3))) i32x4* lds_ptr;
     const uint32_t lds = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((lds_ptr)images)), lane16 = 16u * lane;
-    // the wave's block i of an image, from its first stage on
-    uint32_t from[SHARE];
+    // the wave's blocks of an image (where they do not come out even, the last one
+    // twice: the waits count the same loads in every wave), from the first stage on
+    u32x4 source[SHARE];
+    uint32_t from[SHARE], to[SHARE];
 #pragma unroll
     for (int i = 0; i < SHARE; i++) {
-        const int tile = i < SA ? wave * SA + i : wave * (SHARE - SA) + i - SA;
-        const int last = static_cast<int>(i < SA ? rows_here : cols_here) - 1;
+        const int b = wave + i * WAVES < AR + AT ? wave + i * WAVES : AR + AT - 1;
+        const int last = static_cast<int>(b < AR ? rows_here : cols_here) - 1, tile = b < AR ? b : b - AR;
+        source[i] = b < AR ? ws : xs;
         from[i] = static_cast<uint32_t>(((tile < last ? tile : last) * blocks + first) * INT8_BLOCK);
+        to[i] = lds + b * INT8_BLOCK;
     }
     // block i of stage s (the last one again past the end) into image q
     const auto request = [&](int s, int q, int i) __attribute__((always_inline)) {
-        const int to = i < SA ? wave * SA + i : AR + wave * (SHARE - SA) + i - SA;
-        dma_block(i < SA ? ws : xs, lds + q * IMAGE + to * INT8_BLOCK, lane16,
-                  from[i] + static_cast<uint32_t>(s < count ? s : count - 1) * INT8_BLOCK);
+        dma_block(source[i], to[i] + q * IMAGE, lane16, from[i] + static_cast<uint32_t>(s < count ? s : count - 1) * INT8_BLOCK);
     };
     i32x4 acc[FR][FT], fr[2][FR], ft[2][FT];
 #pragma unroll
@@ -372,25 +505,186 @@ __global__ void __launch_bounds__(256) i8_join_kernel(I8Args a, int32_t chunks) 
     }
 }
 
+// ---- a few tokens -------------------------------------------------------------
+//
+// Up to 16 tokens are one operand's columns, and the weights one stream: a wave
+// takes every KS-th block of a row tile, KB by KB, sixteen of them under way, and
+// the KS waves of a workgroup add their sums through LDS.
+//
+// Where the tokens' values are few (x_type 0 to 2), every workgroup quantizes
+// them for itself while its first weights are under way, a piece of 16 values a
+// thread at a time, into the operand's order in LDS: a launch less.  Otherwise
+// they are packed, and a wave loads its operands beside the weights.
+constexpr int I8_BATCH = 8;  // blocks; two batches are under way
+
+struct I8Few {
+    I8Args g;
+    const void* raw;  // the tokens' values
+    int64_t ld, k;
+    bool whole;
+};
+
+template <int XT, int KS>
+__global__ void __launch_bounds__(64 * KS) i8_few_kernel(I8Few a) {
+    constexpr bool SELF = XT != I8_PACKED;
+    extern __shared__ i32x4 few_lds[];  // the waves' sums, then the tokens' codes
+    __shared__ uint32_t bigs[16];
+    const int lane = static_cast<int>(threadIdx.x) & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int m = static_cast<int>(a.g.m), blocks = static_cast<int>(a.g.wl.blocks);
+    const int mine = (blocks - wave + KS - 1) / KS;  // blocks of a tile
+    const int j = lane & 15, token = j < m ? j : m - 1;
+    const int64_t tile = blockIdx.x;
+    const i32x4* pw = reinterpret_cast<const i32x4*>(a.g.w) + tile * blocks * 64 + lane;
+    // block i of the wave's (past them the last one again)
+    const auto block = [&](int i) __attribute__((always_inline)) { return wave + (i < mine ? i : mine - 1) * KS; };
+    i32x4 w[2][I8_BATCH];
+    const auto load_w = [&](int q, int i0) __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = 0; i < I8_BATCH; i++) w[q][i] = __builtin_nontemporal_load(pw + block(i0 + i) * 64);
+    };
+    if (mine > 0) {
+        load_w(0, 0);
+        if (mine > I8_BATCH) load_w(1, I8_BATCH);
+    }
+    i32x4* codes = few_lds + KS * 64;
+    float sx = 0.f;
+    if constexpr (SELF) {
+        const int pieces = blocks * 4;
+        for (int t = 0; t < m; t++) {
+            const uint8_t* src = static_cast<const uint8_t*>(a.raw) + t * a.ld * (XT == ELEM_F32 ? 4 : 2);
+            Values<XT> first;
+            uint32_t big = 0;
+            const int at = static_cast<int>(threadIdx.x);
+            if (at < pieces) {
+                first.load(src, at * 16, a.k, a.whole);
+                big = first.largest();
+            }
+            for (int p = at + 64 * KS; p < pieces; p += 64 * KS) {
+                Values<XT> v;
+                v.load(src, p * 16, a.k, a.whole);
+                const uint32_t b = v.largest();
+                big = b > big ? b : big;
+            }
+            big = wave_max_bits(big);
+            if (lane == 0) bigs[wave] = big;
+            lds_barrier();
+            big = wave_max_bits(lane < KS ? bigs[lane] : 0);
+            const RowScale s(big);
+            sx = j == t ? s.stored : sx;
+            // place of piece p of token t: (block, k / 16 of it, token)
+            if (at < pieces) reinterpret_cast<uint4*>(codes)[at * m + t] = first.codes(s.s, s.inv);
+            for (int p = at + 64 * KS; p < pieces; p += 64 * KS) {
+                Values<XT> v;
+                v.load(src, p * 16, a.k, a.whole);
+                reinterpret_cast<uint4*>(codes)[p * m + t] = v.codes(s.s, s.inv);
+            }
+            lds_barrier();  // the codes, and bigs is free
+        }
+    } else {
+        sx = reinterpret_cast<const float*>(a.g.x + a.g.xl.scales)[token];
+    }
+    const i32x4* px = SELF ? codes + (lane >> 4) * m + token : reinterpret_cast<const i32x4*>(a.g.x) + (lane >> 4) * 16 + token;
+    i32x4 acc = {0, 0, 0, 0}, x[SELF ? 1 : 2][I8_BATCH];
+    const auto load_x = [&](int q, int i0) __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = 0; i < I8_BATCH; i++) x[q][i] = SELF ? px[block(i0 + i) * 4 * m] : px[block(i0 + i) * 64];
+    };
+    const auto batch = [&](auto parity, int i0) __attribute__((always_inline)) {
+        constexpr int q = decltype(parity)::value, qx = SELF ? 0 : q;
+        if constexpr (SELF) load_x(0, i0);
+        if (i0 + I8_BATCH <= mine) {
+#pragma unroll
+            for (int i = 0; i < I8_BATCH; i++) acc = mfma_i8(w[q][i], x[qx][i], acc);
+        } else {
+#pragma unroll
+            for (int i = 0; i < I8_BATCH; i++)
+                if (i0 + i < mine) acc = mfma_i8(w[q][i], x[qx][i], acc);
+        }
+        if (i0 + 2 * I8_BATCH < mine) {
+            load_w(q, i0 + 2 * I8_BATCH);
+            if constexpr (!SELF) load_x(qx, i0 + 2 * I8_BATCH);
+        }
+    };
+    if (mine > 0) {
+        if constexpr (!SELF) {
+            load_x(0, 0);
+            if (mine > I8_BATCH) load_x(SELF ? 0 : 1, I8_BATCH);
+        }
+        for (int i0 = 0; i0 < mine; i0 += 2 * I8_BATCH) {
+            batch(std::integral_constant<int, 0>{}, i0);
+            if (i0 + I8_BATCH < mine) batch(std::integral_constant<int, 1>{}, i0 + I8_BATCH);
+        }
+    }
+    if constexpr (KS > 1) {
+        few_lds[wave * 64 + lane] = acc;
+        __syncthreads();
+        if (wave > 0) return;
+#pragma unroll
+        for (int v = 1; v < KS; v++) acc += few_lds[v * 64 + lane];
+    }
+    const int64_t n = tile * 16 + 4 * (lane >> 4);
+    if (j < m && n < a.g.n)
+        i8_store4(a.g, j, n, acc, sx, *reinterpret_cast<const float4*>(a.g.w + a.g.wl.scales + 4 * n), i8_vec(a.g));
+}
+
 struct I8Plan {
+    bool few, self;  // i8_few_kernel, which quantizes the tokens itself
+    int ks;          // its waves a tile
     int shape;       // of the tiles
     int64_t chunks;  // of k
     int64_t chunk;   // blocks of k
     int64_t packed, workspace;
 };
 
-constexpr int I8_SHAPE_ROWS[] = {256, 128, 128, 256}, I8_SHAPE_COLS[] = {256, 128, 64, 256};
+// The tiles: rows, tokens, and of what a workgroup takes, in us: a stage, where
+// it has its CU to itself and where it shares it, and everything before and behind
+// the stages.  (4096 rows of k = 4096, us: 256 tokens in tiles of 128 x 64 15.7,
+// of 128 x 128 19.3; 1024 25.6 and 25.9; 4096 62.8 by 256 x 256, 79 by 128 x 128,
+// 93 by 128 x 64.  128 tokens by 128 x 32 12.6, by 128 x 64 14.2.)
+struct I8Shape {
+    int rows, cols;
+    float alone, shared, ends;
+};
+constexpr I8Shape I8_SHAPES[] = {{256, 256, 0.87f, 0.87f, 4.f}, {224, 256, 0.77f, 0.77f, 4.f}, {128, 128, 0.31f, 0.27f, 3.f},
+                                 {128, 64, 0.21f, 0.165f, 2.f}, {128, 32, 0.16f, 0.12f, 1.5f}};
+constexpr int I8_MAX_CHUNKS = 8;
+
+// The shape and the chunks of k that the above makes shortest: workgroups a CU
+// times what each takes, and with chunks the launch that adds them and its bytes.
+// (17 tokens of 4096 x 14336: whole 28 us, in eight chunks 18.8; 4096 tokens of
+// 14336 x 4096: four rounds of 256 rows 224 us, of 224 rows 217.)
+void i8_best_tiles(const Int8Layout& wl, int64_t m, int64_t cus, int* shape, int64_t* chunks) {
+    float best = INFINITY;
+    for (int s = 0; s < 5; s++) {
+        const I8Shape& t = I8_SHAPES[s];
+        const int64_t tiles = ((wl.tiles * 16 + t.rows - 1) / t.rows) * ((m + t.cols - 1) / t.cols);
+        for (int c = 1; c <= I8_MAX_CHUNKS && c <= wl.blocks; c++) {
+            const int64_t each = (tiles * c + cus - 1) / cus, stages = (wl.blocks + c - 1) / c;
+            float us = static_cast<float>(each) * (static_cast<float>(stages) * (each == 1 ? t.alone : t.shared) + t.ends);
+            if (c > 1) us += 2.5f + static_cast<float>(c) * static_cast<float>(m) * static_cast<float>(wl.tiles) * 16e-6f;
+            if (us < best) {
+                best = us;
+                *shape = s;
+                *chunks = c;
+            }
+        }
+    }
+}
 
 I8Plan i8_plan(const Int8Layout& wl, const Int8Layout& xl, int64_t m, bool packed) {
     I8Plan p{};
-    const auto tiles = [&](int s) {
-        return ((wl.tiles * 16 + I8_SHAPE_ROWS[s] - 1) / I8_SHAPE_ROWS[s]) * ((xl.tiles * 16 + I8_SHAPE_COLS[s] - 1) / I8_SHAPE_COLS[s]);
-    };
-    p.shape = tiles(0) >= 2 * num_cus() ? 0 : xl.tiles > 4 ? 1 : 2;
-    if (const char* e = getenv("I8_SHAPE")) p.shape = atoi(e);
-    p.chunks = 1;
-    while (p.chunks < 16 && tiles(p.shape) * p.chunks * 2 <= 2 * num_cus() && wl.blocks >= 16 * p.chunks) p.chunks *= 2;
-    if (const char* e = getenv("I8_CHUNKS")) p.chunks = atoi(e);
+    if (m <= 16) {
+        p.few = true;
+        // one token of 14336 x 4096: 13.4 us, so quantized first 16.1; two 16.9 and 16.6
+        p.self = !packed && m == 1;
+        // (us by two, four and eight waves a tile: 14336 x 4096 13.1, 13.4, 19.1; 4096 x 14336 19.9, 15.2, 14.2;
+        // 16384 x 1024 5.8, 8.1, 12.5; 1024 x 16384 18.3, 11.8, 10.5)
+        p.ks = wl.blocks < 32 ? 2 : wl.tiles < 2 * num_cus() && wl.blocks >= 64 ? 8 : 4;
+        p.packed = p.workspace = packed || p.self ? 0 : xl.total;
+        p.chunks = 1;
+        return p;
+    }
+    i8_best_tiles(wl, m, num_cus(), &p.shape, &p.chunks);
     p.chunk = (wl.blocks + p.chunks - 1) / p.chunks;
     p.chunks = (wl.blocks + p.chunk - 1) / p.chunk;
     p.packed = packed ? 0 : xl.total;
@@ -406,24 +700,52 @@ int i8_tile(const I8Args& a, const I8Plan& p, hipStream_t st) {
     return check_launch("vb_int8_gemm");
 }
 
+template <int XT>
+int i8_few(const I8Few& a, const I8Plan& p, hipStream_t st) {
+    const uint32_t grid = static_cast<uint32_t>(a.g.wl.tiles);
+    const uint32_t lds = static_cast<uint32_t>(p.ks * 1024 + (p.self ? a.g.m * a.g.wl.blocks * INT8_K : 0));
+    if (p.ks == 1) i8_few_kernel<XT, 1><<<grid, 64, lds, st>>>(a);
+    else if (p.ks == 2) i8_few_kernel<XT, 2><<<grid, 128, lds, st>>>(a);
+    else if (p.ks == 4) i8_few_kernel<XT, 4><<<grid, 256, lds, st>>>(a);
+    else i8_few_kernel<XT, 8><<<grid, 512, lds, st>>>(a);
+    return check_launch("vb_int8_gemm");
+}
+
 int i8_run(I8Args a, const I8Plan& p, hipStream_t st) {
     a.chunk = static_cast<int32_t>(p.chunk);
     if (p.chunks == 1) a.partial = nullptr;
     int rc = OK;
-    if (p.shape == 0) rc = i8_tile<8, 4, 2, 4>(a, p, st);
-    else if (p.shape == 1) rc = i8_tile<4, 4, 2, 2>(a, p, st);
-    else rc = i8_tile<4, 2, 2, 2>(a, p, st);
+    switch (p.shape) {
+        case 0: rc = i8_tile<8, 4, 2, 4>(a, p, st); break;
+        case 1: rc = i8_tile<7, 4, 2, 4>(a, p, st); break;
+        case 2: rc = i8_tile<4, 4, 2, 2>(a, p, st); break;
+        case 3: rc = i8_tile<4, 2, 2, 2>(a, p, st); break;
+        default: rc = i8_tile<2, 2, 4, 1>(a, p, st); break;
+    }
     if (rc != OK || p.chunks == 1) return rc;
     i8_join_kernel<<<i8_grid((a.m * a.wl.tiles * 4 + 255) / 256), 256, 0, st>>>(a, static_cast<int32_t>(p.chunks));
     return check_launch("vb_int8_gemm");
 }
 
-int i8_quantize(const I8Rows& a, int32_t type, hipStream_t st) {
-    const uint32_t grid = i8_grid(a.l.tiles * INT8_ROWS);
-    if (type == ELEM_F32) i8_quantize_kernel<ELEM_F32><<<grid, 256, 0, st>>>(a);
-    else if (type == ELEM_F16) i8_quantize_kernel<ELEM_F16><<<grid, 256, 0, st>>>(a);
-    else i8_quantize_kernel<ELEM_BF16><<<grid, 256, 0, st>>>(a);
+// Whether every row begins at a multiple of 16 bytes.
+bool whole_rows(const void* src, int32_t type, int64_t ld, int64_t rows) {
+    return reinterpret_cast<uintptr_t>(src) % 16 == 0 && (rows == 1 || ld * elem_bytes(type) % 16 == 0);
+}
+
+template <int TYPE>
+int i8_quantize_type(const I8Rows& a, hipStream_t st) {
+    // a workgroup a row until the tiles alone give every CU one
+    if (a.l.tiles < num_cus()) i8_quantize_kernel<TYPE, 16><<<i8_grid(a.l.tiles * INT8_ROWS), 1024, 0, st>>>(a);
+    else i8_quantize_kernel<TYPE, 1><<<i8_grid(a.l.tiles * 2), 512, 0, st>>>(a);
     return check_launch("vb_int8_quantize");
+}
+
+int i8_quantize(const void* src, int32_t type, int64_t ld, int64_t rows, int64_t k, uint8_t* w, const Int8Layout& l,
+                hipStream_t st) {
+    const I8Rows a{src, w, l, ld, rows, k, whole_rows(src, type, ld, rows)};
+    if (type == ELEM_F32) return i8_quantize_type<ELEM_F32>(a, st);
+    if (type == ELEM_F16) return i8_quantize_type<ELEM_F16>(a, st);
+    return i8_quantize_type<ELEM_BF16>(a, st);
 }
 
 int i8_layout_of(const char* what, int64_t rows, int64_t k, Int8Layout* l) {
@@ -469,7 +791,7 @@ int vb_int8_quantize(const void* src, int32_t type, int64_t ld, int64_t rows, in
                   static_cast<long long>(ld));
         return E_INVAL;
     }
-    return i8_quantize(I8Rows{src, static_cast<uint8_t*>(w), l, ld, rows, k}, type, as_stream(stream));
+    return i8_quantize(src, type, ld, rows, k, static_cast<uint8_t*>(w), l, as_stream(stream));
 }
 
 int vb_int8_dequant_rows(const void* w, float* out, int64_t rows, int64_t k, void* stream) {
@@ -516,10 +838,9 @@ int vb_int8_gemm(const void* w, int64_t rows, int64_t k, const void* x, int32_t 
     int8_layout(m, k, &a.xl);
     const I8Plan p = i8_plan(l, a.xl, m, x_type == I8_PACKED);
     a.x = static_cast<const uint8_t*>(x);
-    if (x_type != I8_PACKED) {
+    if (x_type != I8_PACKED && !p.self) {
         a.x = static_cast<const uint8_t*>(workspace);
-        if (const int rc = i8_quantize(I8Rows{x, static_cast<uint8_t*>(workspace), a.xl, x_ld, m, k}, x_type, as_stream(stream));
-            rc != OK)
+        if (const int rc = i8_quantize(x, x_type, x_ld, m, k, static_cast<uint8_t*>(workspace), a.xl, as_stream(stream)); rc != OK)
             return rc;
     }
     a.partial = reinterpret_cast<int32_t*>(static_cast<uint8_t*>(workspace) + p.packed);
@@ -528,7 +849,13 @@ int vb_int8_gemm(const void* w, int64_t rows, int64_t k, const void* x, int32_t 
     a.n = rows;
     a.m = m;
     a.out_type = y_type;
-    return i8_run(a, p, as_stream(stream));
+    if (!p.few) return i8_run(a, p, as_stream(stream));
+    I8Few f{a, x, x_ld, k, false};
+    if (!p.self) return i8_few<I8_PACKED>(f, p, as_stream(stream));
+    f.whole = whole_rows(x, x_type, x_ld, m);
+    if (x_type == ELEM_F32) return i8_few<ELEM_F32>(f, p, as_stream(stream));
+    if (x_type == ELEM_F16) return i8_few<ELEM_F16>(f, p, as_stream(stream));
+    return i8_few<ELEM_BF16>(f, p, as_stream(stream));
 }
 
 }  // extern "C"
