@@ -77,6 +77,42 @@ __device__ __forceinline__ int drafted_id(const VerifyArgs& a, int seq, int j) {
                               : static_cast<const int32_t*>(a.drafted)[p];
 }
 
+// VF_PIECE logits from an address of any whole element.
+template <int TYPE>
+struct Logits {
+    float v[VF_PIECE];
+    __device__ __forceinline__ void load(const void* z, int64_t i) {
+        if constexpr (TYPE == ELEM_F32) {
+            typedef float v4 __attribute__((ext_vector_type(4), aligned(4)));
+            const v4* p = reinterpret_cast<const v4*>(static_cast<const float*>(z) + i);
+            const v4 a = p[0], b = p[1];
+#pragma unroll
+            for (int j = 0; j < 4; j++) v[j] = a[j], v[4 + j] = b[j];
+        } else {
+            typedef uint32_t v4 __attribute__((ext_vector_type(4), aligned(2)));
+            const v4 a = *reinterpret_cast<const v4*>(static_cast<const uint16_t*>(z) + i);
+#pragma unroll
+            for (int j = 0; j < VF_PIECE; j++) {
+                const uint32_t h = a[j >> 1] >> 16 * (j & 1) & 0xffffu;
+                v[j] = TYPE == ELEM_BF16 ? __uint_as_float(h << 16)
+                                         : static_cast<float>(__builtin_bit_cast(_Float16, static_cast<uint16_t>(h)));
+            }
+        }
+    }
+    // the first n of them, -inf behind
+    __device__ __forceinline__ void load(const void* z, int64_t i, int n) {
+        if (n >= VF_PIECE) return load(z, i);
+#pragma unroll
+        for (int j = 0; j < VF_PIECE; j++) v[j] = j < n ? elem_ld(z, i + j, TYPE) : -INFINITY;
+    }
+    __device__ __forceinline__ float largest() const {
+        float m = v[0];
+#pragma unroll
+        for (int j = 1; j < VF_PIECE; j++) m = fmaxf(m, v[j]);
+        return m;
+    }
+};
+
 // 2^(c (z - m)); 0 for z = -inf (m finite).
 __device__ __forceinline__ double term(float z, double m, double c) {
     return exp2_64((static_cast<double>(z) - m) * c);
@@ -112,20 +148,32 @@ __global__ void __launch_bounds__(VF_THREADS) verify_stats_kernel(VerifyArgs a) 
         const int64_t at = of_target ? seq * a.target_seq + j * a.target_row : seq * a.draft_seq + j * a.draft_row;
         const double c = of_target ? a.c : a.cd;
         const int begin = slice * a.slice, end = a.vocab - begin < a.slice ? a.vocab : begin + a.slice;
-        float top = -INFINITY;
-        double sum = 0.0;
+        // The lane's sum is relative to the largest of its first logits: 64 bits have
+        // room for what is 2^900 times that, and only a logit past it (or the first
+        // one after nothing but -inf) moves the reference.
+        double ref = 0.0, sum = 0.0;
+        float top = -INFINITY, limit = -INFINITY;
         bool bad = false;
-        for (int i = begin + static_cast<int>(threadIdx.x); i < end; i += VF_THREADS) {
-            const float v = elem_ld(z, at + i, TYPE);
-            bad = bad || !(v < INFINITY);
-            if (v > top) {
-                sum = top > -INFINITY ? sum * term(top, v, c) : 0.0;
-                top = v;
+        for (int i = begin + static_cast<int>(threadIdx.x) * VF_PIECE; i < end; i += VF_THREADS * VF_PIECE) {
+            Logits<TYPE> l;
+            l.load(z, at + i, end - i);
+            const float most = l.largest();
+#pragma unroll
+            for (int j = 0; j < VF_PIECE; j++) bad = bad || !(l.v[j] < INFINITY);
+            if (most > limit) {
+                const double to = static_cast<double>(most);
+                sum = top > -INFINITY ? sum * exp2_64((ref - to) * c) : 0.0;
+                ref = to;
+                limit = fminf(static_cast<float>(to + 900.0 / c), 3.402823466e38f);
+                top = most;
             }
-            sum += v > -INFINITY ? term(v, top, c) : 0.0;
+            double part = 0.0;
+#pragma unroll
+            for (int j = 0; j < VF_PIECE; j++) part += exp2_64((static_cast<double>(l.v[j]) - ref) * c);
+            sum += top > -INFINITY ? part : 0.0;
         }
         const float all = wave_largest(top);
-        sum = wave_sum64(top > -INFINITY ? sum * term(top, all, c) : 0.0);
+        sum = wave_sum64(top > -INFINITY ? sum * exp2_64((ref - static_cast<double>(all)) * c) : 0.0);
         if (__any(bad)) sum = NAN;
         if (lane == 0) {
             tops[wave] = all;
@@ -167,17 +215,19 @@ struct Source {
     double pm, ps, qm, qs;  // their maxima and reciprocal sums
 };
 
-// Weight of id i, before the sum of them all divides it.  Of equal p and q the
-// roundings of two sums may leave some 2^-52 p, which is no weight.
+// max(p - q, 0).  Of equal p and q the roundings of two sums may leave some 2^-52
+// p, which is no weight.
+__device__ __forceinline__ double left_of(double p, double q) {
+    const double r = p - q;
+    return r > 0x1p-45 * p ? r : 0.0;
+}
+
+// Weight of id i, before the sum of them all divides it.  (A row of nothing but
+// -inf has the maximum 0 and the factor 0.)
 template <int TYPE>
 __device__ __forceinline__ double weight(const VerifyArgs& a, const Source& s, bool refused, int i) {
-    const float zp = elem_ld(a.target, s.p + i, TYPE);
-    double r = zp > -INFINITY ? term(zp, s.pm, a.c) * s.ps : 0.0;
-    if (refused && a.draft) {
-        const float zq = elem_ld(a.draft, s.q + i, TYPE);
-        const double q = zq > -INFINITY ? term(zq, s.qm, a.cd) * s.qs : 0.0;
-        r = r - q > 0x1p-45 * r ? r - q : 0.0;
-    }
+    const double r = term(elem_ld(a.target, s.p + i, TYPE), s.pm, a.c) * s.ps;
+    if (refused && a.draft) return left_of(r, term(elem_ld(a.draft, s.q + i, TYPE), s.qm, a.cd) * s.qs);
     return refused && i == s.without ? 0.0 : r;
 }
 
@@ -221,7 +271,7 @@ __device__ __forceinline__ Source decide(const VerifyArgs& a, int seq, int* verd
     if (s.refused && a.draft) {
         const double2 q = row_stats(a, seq, a.drafts + 1 + s.accepted, a.cd);
         s.q = seq * a.draft_seq + s.accepted * a.draft_row;
-        s.qm = q.x;
+        s.qm = q.x > -INFINITY ? q.x : 0.0;
         s.qs = q.y > 0.0 ? 1.0 / q.y : 0.0;
     }
     return s;
@@ -240,8 +290,18 @@ __global__ void __launch_bounds__(VF_THREADS) verify_rest_kernel(VerifyArgs a) {
         const int end = a.vocab - begin < a.rest_slice ? a.vocab : begin + a.rest_slice;
         double sum = 0.0;
         if (!s.bad)
-            for (int i = begin + static_cast<int>(threadIdx.x); i < end; i += VF_THREADS)
-                sum += weight<TYPE>(a, s, s.refused, i);
+            for (int i = begin + static_cast<int>(threadIdx.x) * VF_PIECE; i < end; i += VF_THREADS * VF_PIECE) {
+                Logits<TYPE> p, q;
+                p.load(a.target, s.p + i, end - i);
+                if (s.refused) q.load(a.draft, s.q + i, end - i);
+                double part = 0.0;
+#pragma unroll
+                for (int j = 0; j < VF_PIECE; j++) {
+                    const double r = term(p.v[j], s.pm, a.c) * s.ps;
+                    part += s.refused ? left_of(r, term(q.v[j], s.qm, a.cd) * s.qs) : r;
+                }
+                sum += part;
+            }
         sum = group_sum(sum, sums);
         if (threadIdx.x == 0) a.rest[item] = sum;
         __syncthreads();
