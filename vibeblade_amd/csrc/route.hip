@@ -99,7 +99,10 @@ __global__ void __launch_bounds__(64 * ROUTE_WAVES) route_kernel(RouteArgs a) {
         }
         // softmax: relative to the largest logit, the sum kept apart
         const auto score = [&](float x) __attribute__((always_inline)) {
-            if (a.sigmoid) return 1.0 / (1.0 + exp2_64(-static_cast<double>(x) * LOG2E));
+            if (a.sigmoid) {
+                const double e = exp2_64(-fabs(static_cast<double>(x)) * LOG2E);
+                return (x >= 0.f ? 1.0 : e) / (1.0 + e);
+            }
             return exp2_64((static_cast<double>(x) - static_cast<double>(top)) * LOG2E);
         };
         double s[V], sum = 1.0;

@@ -17,10 +17,13 @@
 //
 //   stats    (row, slice): the maximum and the sum of 2^(c (z - max)), c =
 //            log2(e) / T, of each slice of each row that a decision may need
-//   rest     (sequence, slice), with a drafter's logits: the sequence's
-//            decision from these, and the slice's sum of the weights of its token
-//   token    one workgroup a sequence: the decision, the slice that the random
-//            number falls into, then the place in it
+//   decide   (sequence), with a drafter's logits: what is accepted, and what the
+//            token is drawn from
+//   rest     (sequence, slice), with a drafter's logits: the slice's sum of the
+//            weights that the token is drawn by
+//   token    one workgroup a sequence: the slice that the random number falls
+//            into, then the place in it (without a drafter's logits the decision
+//            is made here, and the slices' sums are those of stats)
 //
 // A row with a NaN or +inf (target's or drafter's) ends the sequence at its
 // position: its token is -1, as it is where a mask leaves the target nothing.
@@ -41,6 +44,7 @@ constexpr int VF_PIECE = 8;          // logits of a load
 constexpr int VF_WIDE = 1024;        // threads of a sequence's last step
 constexpr double LOG2E = 1.4426950408889634;
 
+struct Source;
 struct VerifyArgs {
     const void* target;
     const void* draft;
@@ -51,6 +55,7 @@ struct VerifyArgs {
     int32_t* accepted;
     double2* stats;  // [sequence][row][slice]: maximum, sum
     double* rest;    // [sequence][slice]
+    Source* sources;  // [sequence]
     int64_t target_seq, target_row, draft_seq, draft_row, drafted_row, u_row;
     int32_t seqs, drafts, vocab, token_bytes, slices, slice, rests, rest_slice;
     double c, cd;  // log2(e) / T of the target and of the drafter
@@ -154,9 +159,13 @@ __global__ void __launch_bounds__(VF_THREADS) verify_stats_kernel(VerifyArgs a) 
         double ref = 0.0, sum = 0.0;
         float top = -INFINITY, limit = -INFINITY;
         bool bad = false;
-        for (int i = begin + static_cast<int>(threadIdx.x) * VF_PIECE; i < end; i += VF_THREADS * VF_PIECE) {
-            Logits<TYPE> l;
-            l.load(z, at + i, end - i);
+        Logits<TYPE> next;
+        const int i0 = begin + static_cast<int>(threadIdx.x) * VF_PIECE;
+        if (i0 < end) next.load(z, at + i0, end - i0);
+        for (int i = i0; i < end; i += VF_THREADS * VF_PIECE) {
+            const Logits<TYPE> l = next;
+            const int ahead = i + VF_THREADS * VF_PIECE;
+            if (ahead < end) next.load(z, at + ahead, end - ahead);
             const float most = l.largest();
 #pragma unroll
             for (int j = 0; j < VF_PIECE; j++) bad = bad || !(l.v[j] < INFINITY);
@@ -169,7 +178,7 @@ __global__ void __launch_bounds__(VF_THREADS) verify_stats_kernel(VerifyArgs a) 
             }
             double part = 0.0;
 #pragma unroll
-            for (int j = 0; j < VF_PIECE; j++) part += exp2_64((static_cast<double>(l.v[j]) - ref) * c);
+            for (int j = 0; j < VF_PIECE; j++) part += exp2_normal((static_cast<double>(l.v[j]) - ref) * c);
             sum += top > -INFINITY ? part : 0.0;
         }
         const float all = wave_largest(top);
@@ -212,7 +221,8 @@ struct Source {
     bool refused;  // from max(p - q, 0), else from p
     int without;   // q is 1 at this id (no drafter's logits), or -1
     int64_t p, q;  // rows: first logit
-    double pm, ps, qm, qs;  // their maxima and reciprocal sums
+    double pm, qm, ratio;  // their maxima; the sum of p's terms over that of q's (0: q has none)
+    double ps;             // the sum of p's terms
 };
 
 // max(p - q, 0).  Of equal p and q the roundings of two sums may leave some 2^-52
@@ -222,198 +232,218 @@ __device__ __forceinline__ double left_of(double p, double q) {
     return r > 0x1p-45 * p ? r : 0.0;
 }
 
-// Weight of id i, before the sum of them all divides it.  (A row of nothing but
-// -inf has the maximum 0 and the factor 0.)
+// Weight of id i, before the sum of them all divides it: p's term, less q's by
+// p's sum.  (A row of nothing but -inf has the maximum 0.)
 template <int TYPE>
-__device__ __forceinline__ double weight(const VerifyArgs& a, const Source& s, bool refused, int i) {
-    const double r = term(elem_ld(a.target, s.p + i, TYPE), s.pm, a.c) * s.ps;
-    if (refused && a.draft) return left_of(r, term(elem_ld(a.draft, s.q + i, TYPE), s.qm, a.cd) * s.qs);
+__device__ __forceinline__ double weight(const VerifyArgs& a, const Source& s, bool refused, int i, float zp, float zq) {
+    const double r = term(zp, s.pm, a.c);
+    if (refused && a.draft) return left_of(r, term(zq, s.qm, a.cd) * s.ratio);
     return refused && i == s.without ? 0.0 : r;
 }
 
-// The decision of a sequence, by a workgroup; verdicts: a place per draft.
+// Weights of ids i ... i + n - 1 (n up to VF_PIECE; 0 behind).
 template <int TYPE>
-__device__ __forceinline__ Source decide(const VerifyArgs& a, int seq, int* verdicts) {
+struct Weights {
+    double w[VF_PIECE], sum;
+    __device__ __forceinline__ Weights(const VerifyArgs& a, const Source& s, bool refused, int i, int n) {
+        Logits<TYPE> p, q;
+        if (n > 0) p.load(a.target, s.p + i, n);
+        if (n > 0 && refused && a.draft) q.load(a.draft, s.q + i, n);
+        sum = 0.0;
+#pragma unroll
+        for (int j = 0; j < VF_PIECE; j++) {
+            w[j] = n > 0 ? weight<TYPE>(a, s, refused, i + j, p.v[j], q.v[j]) : 0.0;
+            sum += w[j];
+        }
+    }
+};
+
+// The decision of a sequence, by a workgroup: a wave a position.
+struct Decision {
+    double2 p[VF_MAX_DRAFTS + 1], q[VF_MAX_DRAFTS + 1];  // rows' maxima and sums
+    int id[VF_MAX_DRAFTS + 1], verdict[VF_MAX_DRAFTS + 1];
+};
+template <int TYPE>
+__device__ __forceinline__ Source decide(const VerifyArgs& a, int seq, Decision& d) {
     const int wave = static_cast<int>(threadIdx.x) >> 6, waves = static_cast<int>(blockDim.x) >> 6;
+    const int lane = static_cast<int>(threadIdx.x) & 63;
     const int count = drafts_of(a, seq);
     // 0: accepted, 1: refused, 2: a row that holds NaN or +inf
     for (int j = wave; j <= count; j += waves) {
-        const double2 p = row_stats(a, seq, j, a.c);
-        int verdict = p.y != p.y ? 2 : 1;
+        int id = -1, verdict = 1;
+        float zp = -INFINITY, zq = -INFINITY, u = 0.f;
         if (j < count) {
-            const int d = drafted_id(a, seq, j);
-            const float zp = elem_ld(a.target, seq * a.target_seq + j * a.target_row + d, TYPE);
-            const double pd = zp > -INFINITY ? term(zp, p.x, a.c) : 0.0;
-            double qd = 1.0, qs = 1.0;
-            if (a.draft) {
-                const double2 q = row_stats(a, seq, a.drafts + 1 + j, a.cd);
-                const float zq = elem_ld(a.draft, seq * a.draft_seq + j * a.draft_row + d, TYPE);
-                qd = zq > -INFINITY ? term(zq, q.x, a.cd) : 0.0;
-                qs = q.y > 0.0 ? q.y : 1.0;
-                if (q.y != q.y) verdict = 2;
-            }
-            if (verdict == 1 && static_cast<double>(a.u[seq * a.u_row + j]) * qd * p.y < pd * qs) verdict = 0;
+            id = drafted_id(a, seq, j);
+            zp = elem_ld(a.target, seq * a.target_seq + j * a.target_row + id, TYPE);
+            if (a.draft) zq = elem_ld(a.draft, seq * a.draft_seq + j * a.draft_row + id, TYPE);
+            u = a.u[seq * a.u_row + j];
         }
-        verdicts[j] = verdict;
+        const double2 p = row_stats(a, seq, j, a.c);
+        double2 q = make_double2(0.0, 1.0);
+        double qd = 1.0;
+        if (j < count && a.draft) {
+            q = row_stats(a, seq, a.drafts + 1 + j, a.cd);
+            qd = zq > -INFINITY ? term(zq, q.x, a.cd) : 0.0;
+        }
+        const double pd = zp > -INFINITY ? term(zp, p.x, a.c) : 0.0;
+        if (p.y != p.y || q.y != q.y) verdict = 2;
+        else if (j < count && static_cast<double>(u) * qd * p.y < pd * (q.y > 0.0 ? q.y : 1.0)) verdict = 0;
+        if (lane == 0) {
+            d.p[j] = p;
+            d.q[j] = q;
+            d.id[j] = id;
+            d.verdict[j] = verdict;
+        }
     }
     __syncthreads();
     Source s{};
-    s.accepted = 0;
-    while (s.accepted < count && verdicts[s.accepted] == 0) s.accepted++;
-    s.bad = verdicts[s.accepted] == 2;
+    const uint64_t stops = __ballot(lane >= count || d.verdict[lane < count ? lane : 0] != 0);
+    s.accepted = __ffsll(static_cast<unsigned long long>(stops)) - 1;
+    const double2 p = d.p[s.accepted], q = d.q[s.accepted];
+    s.bad = d.verdict[s.accepted] == 2 || !(p.y > 0.0);  // (or nothing is left)
     s.refused = s.accepted < count;
-    s.without = s.refused && !a.draft ? drafted_id(a, seq, s.accepted) : -1;
-    const double2 p = row_stats(a, seq, s.accepted, a.c);
+    s.without = s.refused && !a.draft ? d.id[s.accepted] : -1;
     s.p = seq * a.target_seq + s.accepted * a.target_row;
     s.pm = p.x;
-    s.ps = p.y > 0.0 ? 1.0 / p.y : 0.0;
-    if (!(p.y > 0.0)) s.bad = true;  // nothing is left, or NaN
-    if (s.refused && a.draft) {
-        const double2 q = row_stats(a, seq, a.drafts + 1 + s.accepted, a.cd);
-        s.q = seq * a.draft_seq + s.accepted * a.draft_row;
-        s.qm = q.x > -INFINITY ? q.x : 0.0;
-        s.qs = q.y > 0.0 ? 1.0 / q.y : 0.0;
-    }
+    s.ps = p.y;
+    s.q = seq * a.draft_seq + s.accepted * a.draft_row;
+    s.qm = q.x > -INFINITY ? q.x : 0.0;
+    s.ratio = q.y > 0.0 ? p.y / q.y : 0.0;
     return s;
 }
 
 // ---- rest ---------------------------------------------------------------------
 
 template <int TYPE>
+__global__ void __launch_bounds__(VF_WIDE) verify_decide_kernel(VerifyArgs a) {
+    __shared__ Decision d;
+    for (int seq = static_cast<int>(blockIdx.x); seq < a.seqs; seq += static_cast<int>(gridDim.x)) {
+        const Source s = decide<TYPE>(a, seq, d);
+        if (threadIdx.x == 0) a.sources[seq] = s;
+        __syncthreads();
+    }
+}
+
+template <int TYPE>
 __global__ void __launch_bounds__(VF_THREADS) verify_rest_kernel(VerifyArgs a) {
-    __shared__ int verdicts[VF_MAX_DRAFTS + 1];
     __shared__ double sums[VF_THREADS / 64];
     for (int64_t item = blockIdx.x; item < static_cast<int64_t>(a.seqs) * a.rests; item += gridDim.x) {
         const int slice = static_cast<int>(item % a.rests), seq = static_cast<int>(item / a.rests);
-        const Source s = decide<TYPE>(a, seq, verdicts);
+        const Source s = a.sources[seq];
         const int begin = slice * a.rest_slice;
         const int end = a.vocab - begin < a.rest_slice ? a.vocab : begin + a.rest_slice;
         double sum = 0.0;
         if (!s.bad)
-            for (int i = begin + static_cast<int>(threadIdx.x) * VF_PIECE; i < end; i += VF_THREADS * VF_PIECE) {
-                Logits<TYPE> p, q;
-                p.load(a.target, s.p + i, end - i);
-                if (s.refused) q.load(a.draft, s.q + i, end - i);
-                double part = 0.0;
-#pragma unroll
-                for (int j = 0; j < VF_PIECE; j++) {
-                    const double r = term(p.v[j], s.pm, a.c) * s.ps;
-                    part += s.refused ? left_of(r, term(q.v[j], s.qm, a.cd) * s.qs) : r;
-                }
-                sum += part;
-            }
+            for (int i = begin + static_cast<int>(threadIdx.x) * VF_PIECE; i < end; i += VF_THREADS * VF_PIECE)
+                sum += Weights<TYPE>(a, s, s.refused, i, end - i).sum;
         sum = group_sum(sum, sums);
         if (threadIdx.x == 0) a.rest[item] = sum;
-        __syncthreads();
     }
 }
 
 // ---- token --------------------------------------------------------------------
 
+// The sum of the lanes up to each.
+__device__ __forceinline__ double lanes_up_to(double v) {
+    const int lane = static_cast<int>(threadIdx.x) & 63;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const double u = __shfl_up(v, o, 64);
+        v += lane >= o ? u : 0.0;
+    }
+    return v;
+}
+
+// Of the lanes' parts v, with `upto` their sums up to each: the first that ends
+// past the goal, or (by rounding, or at a random number of 1) the last that is
+// not 0; -1: all are 0.
+__device__ __forceinline__ int part_of(double v, double upto, double goal) {
+    const uint64_t some = __ballot(v > 0.0), past = __ballot(v > 0.0 && upto > goal);
+    return past ? __ffsll(static_cast<unsigned long long>(past)) - 1
+                : some ? 63 - __clzll(static_cast<long long>(some)) : -1;
+}
+
 // The first id of [begin, end) whose sum of weights, from `carry` on, exceeds
 // `goal`; the last id of a weight where rounding leaves none; -1 without weights.
-// By a workgroup of VF_WIDE threads.
+// By a workgroup of VF_WIDE threads, a piece a thread at a time.
 template <int TYPE>
 __device__ __forceinline__ int locate(const VerifyArgs& a, const Source& s, bool refused, int begin, int end, double carry,
                                       double goal, double* buf, int* found) {
     constexpr int WAVES = VF_WIDE / 64;
     const int lane = static_cast<int>(threadIdx.x) & 63, wave = static_cast<int>(threadIdx.x) >> 6;
-    const int share = ((end - begin + WAVES - 1) / WAVES + 63) / 64 * 64;
-    const int lo = begin + wave * share < end ? begin + wave * share : end, hi = lo + share < end ? lo + share : end;
-    double sum = 0.0;
-    for (int i = lo + lane; i < hi; i += 64) sum += weight<TYPE>(a, s, refused, i);
-    sum = wave_sum64(sum);
-    __syncthreads();
-    buf[wave] = sum;
-    if (threadIdx.x == 0) *found = -1;
-    __syncthreads();
-    // the wave whose share the goal falls into, or the last with a weight
-    int owner = -1;
-    double before = carry, at = carry;
-    for (int w = 0; w < WAVES; w++) {
-        if (buf[w] > 0.0) {
-            owner = w;
-            before = at;
-        }
-        at += buf[w];
-        if (at > goal && buf[w] > 0.0) break;
-    }
-    if (owner == wave) {
-        int last = -1;
-        for (int i0 = lo; i0 < hi; i0 += 64) {
-            const double w = i0 + lane < hi ? weight<TYPE>(a, s, refused, i0 + lane) : 0.0;
-            double c = w;
+    int last = -1;
+    for (int i0 = begin; i0 < end; i0 += VF_WIDE * VF_PIECE) {
+        const int i = i0 + static_cast<int>(threadIdx.x) * VF_PIECE;
+        const Weights<TYPE> w(a, s, refused, i, end - i);
+        const double upto = lanes_up_to(w.sum);
+        __syncthreads();  // (buf is free)
+        if (lane == 63) buf[wave] = upto;
+        if (threadIdx.x == 0) *found = -1;
+        __syncthreads();
+        const double mine = lane < WAVES ? buf[lane] : 0.0, waves = carry + lanes_up_to(mine);
+        const int owner = part_of(mine, waves, goal);
+        if (owner == wave) {
+            const double before = owner > 0 ? lane_value(waves, owner - 1) : carry;
+            const int who = part_of(w.sum, before + upto, goal);
+            if (lane == who) {
+                double at = before + upto - w.sum;
+                int id = -1;
 #pragma unroll
-            for (int o = 1; o < 64; o <<= 1) {
-                const double v = __shfl_up(c, o, 64);
-                if (lane >= o) c += v;
+                for (int j = 0; j < VF_PIECE; j++) {
+                    const bool open = id < 0 || !(at > goal);
+                    at += w.w[j];
+                    if (open && w.w[j] > 0.0) id = i + j;
+                }
+                *found = id;
             }
-            const uint64_t some = __ballot(w > 0.0), past = __ballot(w > 0.0 && before + c > goal);
-            if (past) {
-                last = i0 + __ffsll(static_cast<unsigned long long>(past)) - 1;
-                break;
-            }
-            if (some) last = i0 + 63 - __clzll(static_cast<long long>(some));
-            before += lane_value(c, 63);
         }
-        if (lane == 0) *found = last;
+        __syncthreads();
+        if (*found >= 0) last = *found;
+        carry = lane_value(waves, 63);
+        if (carry > goal && last >= 0) break;
     }
-    __syncthreads();
-    return *found;
+    return last;
 }
 
 template <int TYPE>
 __global__ void __launch_bounds__(VF_WIDE) verify_token_kernel(VerifyArgs a) {
-    __shared__ int verdicts[VF_MAX_DRAFTS + 1];
+    __shared__ Decision d;
     __shared__ double buf[VF_WIDE / 64];
-    __shared__ double parts[VF_MAX_SLICES];
     __shared__ int found;
     const int lane = static_cast<int>(threadIdx.x) & 63;
     const int rows = a.drafts + 1 + (a.draft ? a.drafts : 0);
     for (int seq = static_cast<int>(blockIdx.x); seq < a.seqs; seq += static_cast<int>(gridDim.x)) {
-        const Source s = decide<TYPE>(a, seq, verdicts);
+        const Source s = a.draft ? a.sources[seq] : decide<TYPE>(a, seq, d);
         const double u = static_cast<double>(a.u[seq * a.u_row + a.drafts]);
         int token = -1;
         if (!s.bad) {
-            // each slice's weights: summed by the pass before, or the target's own sums
+            // each slice's weights, one a lane: summed by the pass before, or the target's own sums
             const int slices = a.draft ? a.rests : a.slices, size = a.draft ? a.rest_slice : a.slice;
-            if (lane < slices && threadIdx.x < 64) {
-                double v;
+            double part = 0.0;
+            if (lane < slices) {
                 if (a.draft) {
-                    v = a.rest[static_cast<int64_t>(seq) * slices + lane];
+                    part = a.rest[static_cast<int64_t>(seq) * slices + lane];
                 } else {
                     const double2 p = a.stats[(static_cast<int64_t>(seq) * rows + s.accepted) * slices + lane];
-                    v = p.x > -INFINITY ? p.y * exp2_64((p.x - s.pm) * a.c) * s.ps : 0.0;
+                    part = p.x > -INFINITY ? p.y * exp2_64((p.x - s.pm) * a.c) : 0.0;
                 }
-                parts[lane] = v;
             }
-            __syncthreads();
             if (s.without >= 0) {  // the slice of the refused token, without it (the difference of sums would lose digits)
                 const int slice = s.without / size, begin = slice * size, end = a.vocab - begin < size ? a.vocab : begin + size;
                 double sum = 0.0;
-                for (int i = begin + static_cast<int>(threadIdx.x); i < end; i += VF_WIDE) sum += weight<TYPE>(a, s, true, i);
+                for (int i = begin + static_cast<int>(threadIdx.x) * VF_PIECE; i < end; i += VF_WIDE * VF_PIECE)
+                    sum += Weights<TYPE>(a, s, true, i, end - i).sum;
                 sum = group_sum(sum, buf);
-                if (threadIdx.x == 0) parts[slice] = sum;
-                __syncthreads();
+                part = lane == slice ? sum : part;
             }
-            double total = 0.0;
-            for (int i = 0; i < slices; i++) total += parts[i];
+            const double upto = lanes_up_to(part), total = lane_value(upto, 63);
             if (total > 0.0) {
                 const double goal = u * total;
-                int owner = -1;
-                double before = 0.0, at = 0.0;
-                for (int i = 0; i < slices; i++) {
-                    if (parts[i] > 0.0) {
-                        owner = i;
-                        before = at;
-                    }
-                    at += parts[i];
-                    if (at > goal && parts[i] > 0.0) break;
-                }
+                const int owner = part_of(part, upto, goal);
                 const int begin = owner * size, end = a.vocab - begin < size ? a.vocab : begin + size;
-                token = locate<TYPE>(a, s, s.refused, begin, end, before, goal, buf, &found);
-            } else {  // nothing is left of p behind q: from p itself (whose sum is 1)
-                token = locate<TYPE>(a, s, false, 0, a.vocab, 0.0, u, buf, &found);
+                token = locate<TYPE>(a, s, s.refused, begin, end, owner > 0 ? lane_value(upto, owner - 1) : 0.0, goal, buf, &found);
+            } else {  // nothing is left of p behind q: from p itself
+                token = locate<TYPE>(a, s, false, 0, a.vocab, 0.0, u * s.ps, buf, &found);
             }
         }
         for (int j = static_cast<int>(threadIdx.x); j <= a.drafts; j += VF_WIDE)
@@ -440,9 +470,9 @@ VerifyPlan verify_plan(int64_t seqs, int64_t drafts, int64_t vocab, bool draft) 
     };
     VerifyPlan p{};
     cut(rows, 8, &p.slices, &p.slice);
-    cut(seqs, 4, &p.rests, &p.rest_slice);
+    cut(seqs, 16, &p.rests, &p.rest_slice);
     if (!draft) p.rests = 0;
-    p.workspace = rows * p.slices * 16 + seqs * p.rests * 8;
+    p.workspace = rows * p.slices * 16 + (draft ? seqs * (p.rests * 8 + static_cast<int64_t>(sizeof(Source))) : 0);
     return p;
 }
 
@@ -453,6 +483,8 @@ int verify_launch(const VerifyArgs& a, hipStream_t st) {
                                 VF_THREADS, 0, st>>>(a);
     if (const int rc = check_launch("vb_verify_draft"); rc != OK) return rc;
     if (a.draft) {
+        verify_decide_kernel<TYPE><<<grid(a.seqs), VF_WIDE, 0, st>>>(a);
+        if (const int rc = check_launch("vb_verify_draft"); rc != OK) return rc;
         verify_rest_kernel<TYPE><<<grid(static_cast<int64_t>(a.seqs) * a.rests), VF_THREADS, 0, st>>>(a);
         if (const int rc = check_launch("vb_verify_draft"); rc != OK) return rc;
     }
@@ -529,6 +561,7 @@ int vb_verify_draft(const void* target, int32_t type, int64_t target_seq, int64_
     a.cd = LOG2E / static_cast<double>(draft_temperature);
     a.stats = static_cast<double2*>(workspace);
     a.rest = reinterpret_cast<double*>(a.stats + n_seqs * (n_drafts + 1 + (draft ? n_drafts : 0)) * p.slices);
+    a.sources = reinterpret_cast<Source*>(a.rest + n_seqs * p.rests);
     if (type == ELEM_F32) return verify_launch<ELEM_F32>(a, as_stream(stream));
     if (type == ELEM_F16) return verify_launch<ELEM_F16>(a, as_stream(stream));
     return verify_launch<ELEM_BF16>(a, as_stream(stream));

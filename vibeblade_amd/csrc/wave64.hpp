@@ -8,13 +8,16 @@
 
 namespace vb {
 
-// 2^x for x up to 1100 (above: infinity or 2^1100, below -1100: 0), relative
-// error below 2^-51: 2^n times the Chebyshev interpolation of 2^f, f = x - n
-// in [-1/2, 1/2], at eleven points, whose error is 2 (ln 2 / 4)^11 / 11! =
-// 2.2e-16.  NaN is not kept.
-__device__ __forceinline__ double exp2_64(double x) {
-    x = fmin(fmax(x, -1100.0), 1100.0);
-    const double n = __builtin_rint(x), f = x - n;
+// 2^x for x up to 1023, 2^-1021 for all x below, relative error below 2^-51: 2^n
+// times the Chebyshev interpolation of 2^f, f = x - n in [-1/2, 1/2], at eleven
+// points, whose error is 2 (ln 2 / 4)^11 / 11! = 2.2e-16.  The nearest integer n
+// is what x + 3 * 2^51 is rounded to and stands in that sum's low bits, and 2^n is
+// n added to the exponent: conversions and ldexp issue at a fraction of the rate
+// of sums and fmas.  NaN is not kept.
+constexpr double EXP2_LEAST = -1021.0;
+__device__ __forceinline__ double exp2_normal(double x) {
+    x = fmax(x, EXP2_LEAST);
+    const double shifted = x + 0x1.8p52, f = x - (shifted - 0x1.8p52);
     double p = 0x1.e6063f7217bc7p-28;
     p = __builtin_fma(p, f, 0x1.b675bca4eeebbp-24);
     p = __builtin_fma(p, f, 0x1.62bfd47773353p-20);
@@ -26,7 +29,13 @@ __device__ __forceinline__ double exp2_64(double x) {
     p = __builtin_fma(p, f, 0x1.ebfbdff82c598p-3);
     p = __builtin_fma(p, f, 0x1.62e42fefa3a19p-1);
     p = __builtin_fma(p, f, 1.0);
-    return __builtin_amdgcn_ldexp(p, static_cast<int>(n));
+    return __hiloint2double(__double2hiint(p) + (__double2loint(shifted) << 20), __double2loint(p));
+}
+
+// 2^x for x up to 1023, 0 below -1021.
+__device__ __forceinline__ double exp2_64(double x) {
+    const double p = exp2_normal(x);
+    return x < EXP2_LEAST ? 0.0 : p;
 }
 
 // v of the lane that CTRL names, of the rows of 16 lanes in ROWS; v itself in
