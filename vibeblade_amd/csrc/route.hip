@@ -77,6 +77,7 @@ __device__ __forceinline__ bool group_stays(const RouteArgs& a, T mine, int grou
 template <int TYPE, int V, typename T>
 __global__ void __launch_bounds__(64 * ROUTE_WAVES) route_kernel(RouteArgs a) {
     constexpr bool SCORED = sizeof(T) == 8;
+    const Exp2 exp2;
     const int lane = static_cast<int>(threadIdx.x) & 63;
     const int group = lane >> a.shift, first = (lane & ((1 << a.shift) - 1)) * V;
     const int here = group < a.groups && a.size > first ? (a.size - first < V ? a.size - first : V) : 0;
@@ -100,10 +101,10 @@ __global__ void __launch_bounds__(64 * ROUTE_WAVES) route_kernel(RouteArgs a) {
         // softmax: relative to the largest logit, the sum kept apart
         const auto score = [&](float x) __attribute__((always_inline)) {
             if (a.sigmoid) {
-                const double e = exp2_64(-fabs(static_cast<double>(x)) * LOG2E);
+                const double e = exp2(-fabs(static_cast<double>(x)) * LOG2E);
                 return (x >= 0.f ? 1.0 : e) / (1.0 + e);
             }
-            return exp2_64((static_cast<double>(x) - static_cast<double>(top)) * LOG2E);
+            return exp2((static_cast<double>(x) - static_cast<double>(top)) * LOG2E);
         };
         double s[V], sum = 1.0;
         if (SCORED || (!a.sigmoid && !a.renorm)) {

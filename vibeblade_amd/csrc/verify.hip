@@ -110,6 +110,29 @@ struct Logits {
 #pragma unroll
         for (int j = 0; j < VF_PIECE; j++) v[j] = j < n ? elem_ld(z, i + j, TYPE) : -INFINITY;
     }
+    // VF_PIECE of the logits [i, end) of a row at z[at], i the same in all of a
+    // workgroup, by lanes side by side: an instruction's 16 bytes a lane are one run.
+    __device__ __forceinline__ void spread(const void* z, int64_t at, int i, int end) {
+        if constexpr (TYPE == ELEM_F32) {
+            typedef float v4 __attribute__((ext_vector_type(4), aligned(4)));
+            const float* p = static_cast<const float*>(z) + at;
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                const int k = i + h * 4 * VF_THREADS + 4 * static_cast<int>(threadIdx.x);
+                if (k + 4 <= end) {
+                    const v4 a = __builtin_nontemporal_load(reinterpret_cast<const v4*>(p + k));
+#pragma unroll
+                    for (int j = 0; j < 4; j++) v[4 * h + j] = a[j];
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 4; j++) v[4 * h + j] = k + j < end ? p[k + j] : -INFINITY;
+                }
+            }
+        } else {
+            const int k = i + VF_PIECE * static_cast<int>(threadIdx.x);
+            load(z, at + k, end - k);
+        }
+    }
     __device__ __forceinline__ float largest() const {
         float m = v[0];
 #pragma unroll
@@ -119,8 +142,8 @@ struct Logits {
 };
 
 // 2^(c (z - m)); 0 for z = -inf (m finite).
-__device__ __forceinline__ double term(float z, double m, double c) {
-    return exp2_64((static_cast<double>(z) - m) * c);
+__device__ __forceinline__ double term(const Exp2& exp2, float z, double m, double c) {
+    return exp2((static_cast<double>(z) - m) * c);
 }
 
 // Sum over a workgroup of up to 16 waves, in every thread; buf: one place a wave.
@@ -138,6 +161,7 @@ __device__ __forceinline__ double group_sum(double v, double* buf) {
 
 template <int TYPE>
 __global__ void __launch_bounds__(VF_THREADS) verify_stats_kernel(VerifyArgs a) {
+    const Exp2 exp2;
     __shared__ float tops[VF_THREADS / 64];
     __shared__ double sums[VF_THREADS / 64];
     const int rows = a.drafts + 1 + (a.draft ? a.drafts : 0);
@@ -156,33 +180,50 @@ __global__ void __launch_bounds__(VF_THREADS) verify_stats_kernel(VerifyArgs a) 
         // The lane's sum is relative to the largest of its first logits: 64 bits have
         // room for what is 2^900 times that, and only a logit past it (or the first
         // one after nothing but -inf) moves the reference.
-        double ref = 0.0, sum = 0.0;
+        double ref = 0.0, at_ref = 0.0, sum = 0.0;  // at_ref: c ref, rounded; a term is 2^(c z - at_ref), one fma for the exponent
         float top = -INFINITY, limit = -INFINITY;
-        bool bad = false;
+        bool bad = false, far = false;  // far: rounding c ref may cost that much; a term is 2^(c (z - ref))
         Logits<TYPE> next;
-        const int i0 = begin + static_cast<int>(threadIdx.x) * VF_PIECE;
-        if (i0 < end) next.load(z, at + i0, end - i0);
-        for (int i = i0; i < end; i += VF_THREADS * VF_PIECE) {
+        next.spread(z, at, begin, end);
+        for (int i = begin; i < end; i += VF_THREADS * VF_PIECE) {
             const Logits<TYPE> l = next;
             const int ahead = i + VF_THREADS * VF_PIECE;
-            if (ahead < end) next.load(z, at + ahead, end - ahead);
+            if (ahead < end) next.spread(z, at, ahead, end);
             const float most = l.largest();
 #pragma unroll
             for (int j = 0; j < VF_PIECE; j++) bad = bad || !(l.v[j] < INFINITY);
             if (most > limit) {
                 const double to = static_cast<double>(most);
-                sum = top > -INFINITY ? sum * exp2_64((ref - to) * c) : 0.0;
+                sum = top > -INFINITY ? sum * exp2(far ? (ref - to) * c : __builtin_fma(-to, c, at_ref)) : 0.0;
                 ref = to;
+                at_ref = to * c;
+                if (!(fabs(at_ref) < 0x1p40)) {
+                    far = true;
+                    at_ref = 0.0;
+                } else {
+                    far = false;
+                }
                 limit = fminf(static_cast<float>(to + 900.0 / c), 3.402823466e38f);
                 top = most;
             }
             double part = 0.0;
+            if (!__any(far)) {
 #pragma unroll
-            for (int j = 0; j < VF_PIECE; j++) part += exp2_normal((static_cast<double>(l.v[j]) - ref) * c);
+                for (int j = 0; j < VF_PIECE; j++) part += exp2.quick(__builtin_fma(static_cast<double>(l.v[j]), c, -at_ref));
+            } else {
+#pragma unroll 1
+                for (int j = 0; j < VF_PIECE; j++) {
+                    float z_j = l.v[0];
+#pragma unroll
+                    for (int k = 1; k < VF_PIECE; k++) z_j = j == k ? l.v[k] : z_j;
+                    part += exp2.quick(far ? (static_cast<double>(z_j) - ref) * c : __builtin_fma(static_cast<double>(z_j), c, -at_ref));
+                }
+            }
             sum += top > -INFINITY ? part : 0.0;
         }
         const float all = wave_largest(top);
-        sum = wave_sum64(top > -INFINITY ? sum * exp2_64((ref - static_cast<double>(all)) * c) : 0.0);
+        sum = wave_sum64(top > -INFINITY ? sum * exp2(far ? (ref - static_cast<double>(all)) * c
+                                                          : __builtin_fma(-static_cast<double>(all), c, at_ref)) : 0.0);
         if (__any(bad)) sum = NAN;
         if (lane == 0) {
             tops[wave] = all;
@@ -194,7 +235,7 @@ __global__ void __launch_bounds__(VF_THREADS) verify_stats_kernel(VerifyArgs a) 
             for (int w = 1; w < VF_THREADS / 64; w++) m = fmaxf(m, tops[w]);
             double s = 0.0;
             for (int w = 0; w < VF_THREADS / 64; w++)
-                s += sums[w] != sums[w] ? NAN : tops[w] > -INFINITY ? sums[w] * term(tops[w], m, c) : 0.0;
+                s += sums[w] != sums[w] ? NAN : tops[w] > -INFINITY ? sums[w] * term(exp2, tops[w], m, c) : 0.0;
             a.stats[item] = make_double2(static_cast<double>(m), s);
         }
         __syncthreads();
@@ -204,13 +245,13 @@ __global__ void __launch_bounds__(VF_THREADS) verify_stats_kernel(VerifyArgs a) 
 // ---- the decision -------------------------------------------------------------
 
 // A row's maximum and sum from its slices, by a wave, in every lane.
-__device__ __forceinline__ double2 row_stats(const VerifyArgs& a, int seq, int row, double c) {
+__device__ __forceinline__ double2 row_stats(const Exp2& exp2, const VerifyArgs& a, int seq, int row, double c) {
     const int lane = static_cast<int>(threadIdx.x) & 63;
     const int rows = a.drafts + 1 + (a.draft ? a.drafts : 0);
     double2 v = make_double2(-INFINITY, 0.0);
     if (lane < a.slices) v = a.stats[(static_cast<int64_t>(seq) * rows + row) * a.slices + lane];
     const double m = wave_largest(v.x);
-    const double s = v.y != v.y ? NAN : v.x > -INFINITY ? v.y * exp2_64((v.x - m) * c) : 0.0;
+    const double s = v.y != v.y ? NAN : v.x > -INFINITY ? v.y * exp2((v.x - m) * c) : 0.0;
     return make_double2(m, wave_sum64(s));
 }
 
@@ -235,9 +276,9 @@ __device__ __forceinline__ double left_of(double p, double q) {
 // Weight of id i, before the sum of them all divides it: p's term, less q's by
 // p's sum.  (A row of nothing but -inf has the maximum 0.)
 template <int TYPE>
-__device__ __forceinline__ double weight(const VerifyArgs& a, const Source& s, bool refused, int i, float zp, float zq) {
-    const double r = term(zp, s.pm, a.c);
-    if (refused && a.draft) return left_of(r, term(zq, s.qm, a.cd) * s.ratio);
+__device__ __forceinline__ double weight(const Exp2& exp2, const VerifyArgs& a, const Source& s, bool refused, int i, float zp, float zq) {
+    const double r = term(exp2, zp, s.pm, a.c);
+    if (refused && a.draft) return left_of(r, term(exp2, zq, s.qm, a.cd) * s.ratio);
     return refused && i == s.without ? 0.0 : r;
 }
 
@@ -245,14 +286,14 @@ __device__ __forceinline__ double weight(const VerifyArgs& a, const Source& s, b
 template <int TYPE>
 struct Weights {
     double w[VF_PIECE], sum;
-    __device__ __forceinline__ Weights(const VerifyArgs& a, const Source& s, bool refused, int i, int n) {
+    __device__ __forceinline__ Weights(const Exp2& exp2, const VerifyArgs& a, const Source& s, bool refused, int i, int n) {
         Logits<TYPE> p, q;
         if (n > 0) p.load(a.target, s.p + i, n);
         if (n > 0 && refused && a.draft) q.load(a.draft, s.q + i, n);
         sum = 0.0;
 #pragma unroll
         for (int j = 0; j < VF_PIECE; j++) {
-            w[j] = n > 0 ? weight<TYPE>(a, s, refused, i + j, p.v[j], q.v[j]) : 0.0;
+            w[j] = n > 0 ? weight<TYPE>(exp2, a, s, refused, i + j, p.v[j], q.v[j]) : 0.0;
             sum += w[j];
         }
     }
@@ -264,7 +305,7 @@ struct Decision {
     int id[VF_MAX_DRAFTS + 1], verdict[VF_MAX_DRAFTS + 1];
 };
 template <int TYPE>
-__device__ __forceinline__ Source decide(const VerifyArgs& a, int seq, Decision& d) {
+__device__ __forceinline__ Source decide(const Exp2& exp2, const VerifyArgs& a, int seq, Decision& d) {
     const int wave = static_cast<int>(threadIdx.x) >> 6, waves = static_cast<int>(blockDim.x) >> 6;
     const int lane = static_cast<int>(threadIdx.x) & 63;
     const int count = drafts_of(a, seq);
@@ -278,14 +319,14 @@ __device__ __forceinline__ Source decide(const VerifyArgs& a, int seq, Decision&
             if (a.draft) zq = elem_ld(a.draft, seq * a.draft_seq + j * a.draft_row + id, TYPE);
             u = a.u[seq * a.u_row + j];
         }
-        const double2 p = row_stats(a, seq, j, a.c);
+        const double2 p = row_stats(exp2, a, seq, j, a.c);
         double2 q = make_double2(0.0, 1.0);
         double qd = 1.0;
         if (j < count && a.draft) {
-            q = row_stats(a, seq, a.drafts + 1 + j, a.cd);
-            qd = zq > -INFINITY ? term(zq, q.x, a.cd) : 0.0;
+            q = row_stats(exp2, a, seq, a.drafts + 1 + j, a.cd);
+            qd = zq > -INFINITY ? term(exp2, zq, q.x, a.cd) : 0.0;
         }
-        const double pd = zp > -INFINITY ? term(zp, p.x, a.c) : 0.0;
+        const double pd = zp > -INFINITY ? term(exp2, zp, p.x, a.c) : 0.0;
         if (p.y != p.y || q.y != q.y) verdict = 2;
         else if (j < count && static_cast<double>(u) * qd * p.y < pd * (q.y > 0.0 ? q.y : 1.0)) verdict = 0;
         if (lane == 0) {
@@ -316,9 +357,10 @@ __device__ __forceinline__ Source decide(const VerifyArgs& a, int seq, Decision&
 
 template <int TYPE>
 __global__ void __launch_bounds__(VF_WIDE) verify_decide_kernel(VerifyArgs a) {
+    const Exp2 exp2;
     __shared__ Decision d;
     for (int seq = static_cast<int>(blockIdx.x); seq < a.seqs; seq += static_cast<int>(gridDim.x)) {
-        const Source s = decide<TYPE>(a, seq, d);
+        const Source s = decide<TYPE>(exp2, a, seq, d);
         if (threadIdx.x == 0) a.sources[seq] = s;
         __syncthreads();
     }
@@ -326,6 +368,7 @@ __global__ void __launch_bounds__(VF_WIDE) verify_decide_kernel(VerifyArgs a) {
 
 template <int TYPE>
 __global__ void __launch_bounds__(VF_THREADS) verify_rest_kernel(VerifyArgs a) {
+    const Exp2 exp2;
     __shared__ double sums[VF_THREADS / 64];
     for (int64_t item = blockIdx.x; item < static_cast<int64_t>(a.seqs) * a.rests; item += gridDim.x) {
         const int slice = static_cast<int>(item % a.rests), seq = static_cast<int>(item / a.rests);
@@ -334,8 +377,13 @@ __global__ void __launch_bounds__(VF_THREADS) verify_rest_kernel(VerifyArgs a) {
         const int end = a.vocab - begin < a.rest_slice ? a.vocab : begin + a.rest_slice;
         double sum = 0.0;
         if (!s.bad)
-            for (int i = begin + static_cast<int>(threadIdx.x) * VF_PIECE; i < end; i += VF_THREADS * VF_PIECE)
-                sum += Weights<TYPE>(a, s, s.refused, i, end - i).sum;
+            for (int i = begin; i < end; i += VF_THREADS * VF_PIECE) {
+                Logits<TYPE> p, q;
+                p.spread(a.target, s.p, i, end);
+                if (s.refused) q.spread(a.draft, s.q, i, end);
+#pragma unroll
+                for (int j = 0; j < VF_PIECE; j++) sum += weight<TYPE>(exp2, a, s, s.refused, 0, p.v[j], q.v[j]);
+            }
         sum = group_sum(sum, sums);
         if (threadIdx.x == 0) a.rest[item] = sum;
     }
@@ -367,14 +415,14 @@ __device__ __forceinline__ int part_of(double v, double upto, double goal) {
 // `goal`; the last id of a weight where rounding leaves none; -1 without weights.
 // By a workgroup of VF_WIDE threads, a piece a thread at a time.
 template <int TYPE>
-__device__ __forceinline__ int locate(const VerifyArgs& a, const Source& s, bool refused, int begin, int end, double carry,
+__device__ __forceinline__ int locate(const Exp2& exp2, const VerifyArgs& a, const Source& s, bool refused, int begin, int end, double carry,
                                       double goal, double* buf, int* found) {
     constexpr int WAVES = VF_WIDE / 64;
     const int lane = static_cast<int>(threadIdx.x) & 63, wave = static_cast<int>(threadIdx.x) >> 6;
     int last = -1;
     for (int i0 = begin; i0 < end; i0 += VF_WIDE * VF_PIECE) {
         const int i = i0 + static_cast<int>(threadIdx.x) * VF_PIECE;
-        const Weights<TYPE> w(a, s, refused, i, end - i);
+        const Weights<TYPE> w(exp2, a, s, refused, i, end - i);
         const double upto = lanes_up_to(w.sum);
         __syncthreads();  // (buf is free)
         if (lane == 63) buf[wave] = upto;
@@ -407,13 +455,14 @@ __device__ __forceinline__ int locate(const VerifyArgs& a, const Source& s, bool
 
 template <int TYPE>
 __global__ void __launch_bounds__(VF_WIDE) verify_token_kernel(VerifyArgs a) {
+    const Exp2 exp2;
     __shared__ Decision d;
     __shared__ double buf[VF_WIDE / 64];
     __shared__ int found;
     const int lane = static_cast<int>(threadIdx.x) & 63;
     const int rows = a.drafts + 1 + (a.draft ? a.drafts : 0);
     for (int seq = static_cast<int>(blockIdx.x); seq < a.seqs; seq += static_cast<int>(gridDim.x)) {
-        const Source s = a.draft ? a.sources[seq] : decide<TYPE>(a, seq, d);
+        const Source s = a.draft ? a.sources[seq] : decide<TYPE>(exp2, a, seq, d);
         const double u = static_cast<double>(a.u[seq * a.u_row + a.drafts]);
         int token = -1;
         if (!s.bad) {
@@ -425,14 +474,14 @@ __global__ void __launch_bounds__(VF_WIDE) verify_token_kernel(VerifyArgs a) {
                     part = a.rest[static_cast<int64_t>(seq) * slices + lane];
                 } else {
                     const double2 p = a.stats[(static_cast<int64_t>(seq) * rows + s.accepted) * slices + lane];
-                    part = p.x > -INFINITY ? p.y * exp2_64((p.x - s.pm) * a.c) : 0.0;
+                    part = p.x > -INFINITY ? p.y * exp2((p.x - s.pm) * a.c) : 0.0;
                 }
             }
             if (s.without >= 0) {  // the slice of the refused token, without it (the difference of sums would lose digits)
                 const int slice = s.without / size, begin = slice * size, end = a.vocab - begin < size ? a.vocab : begin + size;
                 double sum = 0.0;
                 for (int i = begin + static_cast<int>(threadIdx.x) * VF_PIECE; i < end; i += VF_WIDE * VF_PIECE)
-                    sum += Weights<TYPE>(a, s, true, i, end - i).sum;
+                    sum += Weights<TYPE>(exp2, a, s, true, i, end - i).sum;
                 sum = group_sum(sum, buf);
                 part = lane == slice ? sum : part;
             }
@@ -441,9 +490,9 @@ __global__ void __launch_bounds__(VF_WIDE) verify_token_kernel(VerifyArgs a) {
                 const double goal = u * total;
                 const int owner = part_of(part, upto, goal);
                 const int begin = owner * size, end = a.vocab - begin < size ? a.vocab : begin + size;
-                token = locate<TYPE>(a, s, s.refused, begin, end, owner > 0 ? lane_value(upto, owner - 1) : 0.0, goal, buf, &found);
+                token = locate<TYPE>(exp2, a, s, s.refused, begin, end, owner > 0 ? lane_value(upto, owner - 1) : 0.0, goal, buf, &found);
             } else {  // nothing is left of p behind q: from p itself
-                token = locate<TYPE>(a, s, false, 0, a.vocab, 0.0, u * s.ps, buf, &found);
+                token = locate<TYPE>(exp2, a, s, false, 0, a.vocab, 0.0, u * s.ps, buf, &found);
             }
         }
         for (int j = static_cast<int>(threadIdx.x); j <= a.drafts; j += VF_WIDE)
@@ -462,7 +511,7 @@ VerifyPlan verify_plan(int64_t seqs, int64_t drafts, int64_t vocab, bool draft) 
     const int64_t rows = seqs * (drafts + 1 + (draft ? drafts : 0));
     const auto cut = [&](int64_t n, int64_t groups, int64_t* slices, int64_t* slice) {
         const int64_t most = (vocab + VF_THREADS * VF_PIECE - 1) / (VF_THREADS * VF_PIECE);
-        int64_t want = (groups * num_cus() + n - 1) / (n > 0 ? n : 1);
+        int64_t want = groups * num_cus() / (n > 0 ? n : 1);
         want = want < 1 ? 1 : want < VF_MAX_SLICES ? want : VF_MAX_SLICES;
         want = want < most ? want : most;
         *slice = ((vocab + want - 1) / want + VF_PIECE - 1) / VF_PIECE * VF_PIECE;
