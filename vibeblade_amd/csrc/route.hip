@@ -44,20 +44,42 @@ struct RouteArgs {
     float scale;
 };
 
+// v of the lane 1 << s away within the eight, from DPP where there is one.
+template <typename T>
+__device__ __forceinline__ T lane_across(T v, int s) {
+    switch (s) {
+        case 0: return dpp_or_self<0xB1>(v);   // quad_perm [1,0,3,2]
+        case 1: return dpp_or_self<0x4E>(v);   // quad_perm [2,3,0,1]
+        case 2: return dpp_or_self<0x141>(v);  // row_half_mirror: quads are alike by now
+        case 3: return dpp_or_self<0x140>(v);  // row_mirror: so are eights
+        default: return __shfl_xor(v, 1 << s, 64);
+    }
+}
+
+__device__ __forceinline__ float smaller(float a, float b) { return fminf(a, b); }
+__device__ __forceinline__ double smaller(double a, double b) { return fmin(a, b); }
+
 // The sum of the two largest (a >= b) of a group's 1 << shift lanes, in each of
 // them.  -inf: none; one alone counts for itself.
-__device__ __forceinline__ double group_top2(double a, double b, int shift) {
-    for (int s = 0; s < shift; s++) {
-        const double oa = __shfl_xor(a, 1 << s, 64), ob = __shfl_xor(b, 1 << s, 64);
-        b = fmax(fmin(a, oa), fmax(b, ob));
-        a = fmax(a, oa);
+template <typename T>
+__device__ __forceinline__ T group_top2(T a, T b, int shift) {
+#pragma unroll
+    for (int s = 0; s < 6; s++) {
+        if (s >= shift) break;
+        const T oa = lane_across(a, s), ob = lane_across(b, s);
+        b = larger(smaller(a, oa), larger(b, ob));
+        a = larger(a, oa);
     }
-    return a + (b > -INFINITY ? b : 0.0);
+    return a + (b > -INFINITY ? b : T(0));
 }
 
 template <typename T>
 __device__ __forceinline__ T group_largest(T v, int shift) {
-    for (int s = 0; s < shift; s++) v = larger(v, __shfl_xor(v, 1 << s, 64));
+#pragma unroll
+    for (int s = 0; s < 6; s++) {
+        if (s >= shift) break;
+        v = larger(v, lane_across(v, s));
+    }
     return v;
 }
 
@@ -72,16 +94,82 @@ __device__ __forceinline__ bool group_stays(const RouteArgs& a, T mine, int grou
     return before < a.kept;
 }
 
-// T: what the choice is held in, float where it is the logit itself and double
-// where it is a score with a bias, or groups go by sums of scores.
-template <int TYPE, int V, typename T>
+// What the lanes take in the rounds: lane r the r-th expert and its logit.
+struct Taken {
+    int id = -1;
+    float z = -INFINITY;
+};
+
+// `rounds` rounds over the choices c (of which the first a.topk count); the
+// smallest difference of one round's choice to the next.
+template <int V, typename T>
+__device__ __forceinline__ T take(const RouteArgs& a, T (&c)[V], const float (&z)[V], int base, int rounds, Taken& out) {
+    const int lane = static_cast<int>(threadIdx.x) & 63;
+    T gap = INFINITY, last = INFINITY;
+    for (int r = 0; r < rounds; r++) {
+        T most = c[0];
+#pragma unroll
+        for (int v = 1; v < V; v++) most = larger(most, c[v]);
+        const T best = wave_largest(most);
+        if (best == -INFINITY) break;  // no expert is left
+        gap = smaller(gap, last - best);
+        last = best;
+        const int owner = __ffsll(static_cast<unsigned long long>(__ballot(most == best))) - 1;
+        int at = 0;
+        float zat = z[0];
+#pragma unroll
+        for (int v = V - 1; v >= 0; v--) {
+            at = c[v] == best ? v : at;
+            zat = c[v] == best ? z[v] : zat;
+        }
+        if (lane == owner) {
+#pragma unroll
+            for (int v = 0; v < V; v++) c[v] = v == at ? -INFINITY : c[v];
+        }
+        const int chosen = __builtin_amdgcn_readlane(base + at, owner);
+        const float chosen_z = lane_value(zat, owner);
+        if (lane == r && r < a.topk) {
+            out.id = chosen;
+            out.z = chosen_z;
+        }
+    }
+    return gap;
+}
+
+// What groups go by, in every lane of each: the largest of the choices c, or the
+// sum of the two largest values.
+template <int V, typename T>
+__device__ __forceinline__ T group_score(const RouteArgs& a, const T (&c)[V], const T (&value)[V]) {
+    if (a.top2) {
+        T x = -INFINITY, y = -INFINITY;
+#pragma unroll
+        for (int v = 0; v < V; v++) {
+            y = larger(y, smaller(x, value[v]));
+            x = larger(x, value[v]);
+        }
+        return group_top2(x, y, a.shift);
+    }
+    T most = c[0];
+#pragma unroll
+    for (int v = 1; v < V; v++) most = larger(most, c[v]);
+    return group_largest(most, a.shift);
+}
+
+// SCORED: choices are scores with a bias, or groups go by sums of scores.  These
+// are first taken in fp32, which is enough where no two that are compared lie
+// within its error (`sure`; of scores of 256 experts two do in one token of
+// several hundred), and in 64 bits where they do.  Choices that are logits are
+// exact in fp32.
+template <int TYPE, int V, bool SCORED>
 __global__ void __launch_bounds__(64 * ROUTE_WAVES) route_kernel(RouteArgs a) {
-    constexpr bool SCORED = sizeof(T) == 8;
     const Exp2 exp2;
     const int lane = static_cast<int>(threadIdx.x) & 63;
     const int group = lane >> a.shift, first = (lane & ((1 << a.shift) - 1)) * V;
     const int here = group < a.groups && a.size > first ? (a.size - first < V ? a.size - first : V) : 0;
     const int base = group * a.size + first;
+    float b[V];
+#pragma unroll
+    for (int v = 0; v < V; v++) b[v] = SCORED && a.bias && v < here ? a.bias[base + v] : 0.f;
     for (int64_t token = static_cast<int64_t>(blockIdx.x) * ROUTE_WAVES + (threadIdx.x >> 6); token < a.tokens;
          token += static_cast<int64_t>(gridDim.x) * ROUTE_WAVES) {
         float z[V];
@@ -106,91 +194,85 @@ __global__ void __launch_bounds__(64 * ROUTE_WAVES) route_kernel(RouteArgs a) {
             }
             return exp2((static_cast<double>(x) - static_cast<double>(top)) * LOG2E);
         };
-        double s[V], sum = 1.0;
-        if (SCORED || (!a.sigmoid && !a.renorm)) {
+        double sum = 1.0;
+        const auto total = [&]() __attribute__((always_inline)) {
             double part = 0.0;
 #pragma unroll
-            for (int v = 0; v < V; v++) {
-                s[v] = z[v] > -INFINITY ? score(z[v]) : 0.0;
-                part += s[v];
-            }
-            if (!a.sigmoid) sum = wave_sum64(part);
-        }
-        T c[V];
+            for (int v = 0; v < V; v++) part += z[v] > -INFINITY ? score(z[v]) : 0.0;
+            return wave_sum64(part);
+        };
+        Taken taken;
         if constexpr (SCORED) {
-            double value[V];
+            float c[V], value[V], most = 0.f, sum32 = 1.f;
+            if (!a.sigmoid) {
+                float part = 0.f;
+#pragma unroll
+                for (int v = 0; v < V; v++) {
+                    value[v] = __builtin_amdgcn_exp2f((z[v] - top) * static_cast<float>(LOG2E));
+                    part += z[v] > -INFINITY ? value[v] : 0.f;
+                }
+                sum32 = __builtin_amdgcn_rcpf(wave_sum_dpp(part));
+            }
 #pragma unroll
             for (int v = 0; v < V; v++) {
-                const float b = a.bias && v < here ? a.bias[base + v] : 0.f;
-                value[v] = z[v] > -INFINITY ? (a.sigmoid ? s[v] : s[v] / sum) + static_cast<double>(b) : -INFINITY;
+                const float s = a.sigmoid ? __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-z[v] * static_cast<float>(LOG2E)))
+                                          : value[v] * sum32;
+                value[v] = z[v] > -INFINITY ? s + b[v] : -INFINITY;
                 bad = bad || value[v] != value[v];
-                c[v] = a.bias ? value[v] : static_cast<double>(z[v]);
+                c[v] = a.bias ? value[v] : z[v];
+                most = fabsf(value[v]) < INFINITY ? fmaxf(most, fabsf(value[v])) : most;
             }
+            // Two choices' difference: scores are at most 1 and less than 2e-6 off (an
+            // exponent's rounding costs at most x e^-x half steps, a sum of 512 terms 22 of
+            // them), the sum with a bias half a step of itself.
+            const float off = 4e-6f + 0x1p-22f * wave_largest(most);
+            bool sure = true;
             if (a.kept < a.groups) {
-                T mine;
-                if (a.top2) {
-                    double x = -INFINITY, y = -INFINITY;
-#pragma unroll
-                    for (int v = 0; v < V; v++) {
-                        y = fmax(y, fmin(x, value[v]));
-                        x = fmax(x, value[v]);
-                    }
-                    mine = group_top2(x, y, a.shift);
-                } else {
-                    mine = c[0];
-#pragma unroll
-                    for (int v = 1; v < V; v++) mine = larger(mine, c[v]);
-                    mine = group_largest(mine, a.shift);
-                }
+                const float mine = group_score<V, float>(a, c, value);
                 const bool stays = group_stays(a, mine, group);
+                // the least group that stays, and the best of those that do not; logits are exact
+                const float in = -wave_largest(stays ? -mine : -INFINITY), out = wave_largest(stays || group >= a.groups ? -INFINITY : mine);
+                sure = !(in - out <= (a.top2 ? 2.f * off : a.bias ? off : -1.f));
 #pragma unroll
                 for (int v = 0; v < V; v++) c[v] = stays ? c[v] : -INFINITY;
             }
+            const float gap = take<V, float>(a, c, z, base, a.bias ? a.topk + 1 : a.topk, taken);
+            if (a.bias) sure = sure && gap > off;
+            if (__any(bad || !sure)) {
+                taken = Taken{};
+                double c[V], value[V];
+                if (!a.sigmoid) sum = total();
+#pragma unroll
+                for (int v = 0; v < V; v++) {
+                    value[v] = z[v] > -INFINITY ? score(z[v]) / sum + static_cast<double>(b[v]) : -INFINITY;
+                    bad = bad || value[v] != value[v];
+                    c[v] = a.bias ? value[v] : static_cast<double>(z[v]);
+                }
+                if (a.kept < a.groups) {
+                    const bool stays = group_stays(a, group_score<V, double>(a, c, value), group);
+#pragma unroll
+                    for (int v = 0; v < V; v++) c[v] = stays ? c[v] : -INFINITY;
+                }
+                if (!__any(bad)) take<V, double>(a, c, z, base, a.topk, taken);
+            }
         } else {
+            float c[V];
 #pragma unroll
             for (int v = 0; v < V; v++) c[v] = z[v];
             if (a.kept < a.groups) {
-                T mine = c[0];
-#pragma unroll
-                for (int v = 1; v < V; v++) mine = larger(mine, c[v]);
-                const bool stays = group_stays(a, group_largest(mine, a.shift), group);
+                const bool stays = group_stays(a, group_score<V, float>(a, c, c), group);
 #pragma unroll
                 for (int v = 0; v < V; v++) c[v] = stays ? c[v] : -INFINITY;
             }
+            if (!__any(bad)) take<V, float>(a, c, z, base, a.topk, taken);
         }
-        int id = -1;
-        float mine_z = -INFINITY;
         const bool none = __any(bad);
-        if (!none) {
-            for (int r = 0; r < a.topk; r++) {
-                T most = c[0];
-#pragma unroll
-                for (int v = 1; v < V; v++) most = larger(most, c[v]);
-                const T best = wave_largest(most);
-                if (best == -INFINITY) break;  // no expert is left
-                const int owner = __ffsll(static_cast<unsigned long long>(__ballot(most == best))) - 1;
-                int at = 0;
-                float zat = z[0];
-#pragma unroll
-                for (int v = V - 1; v >= 0; v--) {
-                    at = c[v] == best ? v : at;
-                    zat = c[v] == best ? z[v] : zat;
-                }
-#pragma unroll
-                for (int v = 0; v < V; v++) c[v] = lane == owner && v == at ? -INFINITY : c[v];
-                const int chosen = __builtin_amdgcn_readlane(base + at, owner);
-                const float chosen_z = lane_value(zat, owner);
-                if (lane == r) {
-                    id = chosen;
-                    mine_z = chosen_z;
-                }
-            }
-        }
-        double w = id >= 0 ? score(mine_z) : 0.0;
+        double w = !none && taken.id >= 0 ? score(taken.z) : 0.0;
         if (a.renorm) sum = wave_sum64(w);
+        else if (!a.sigmoid) sum = total();
         w = w > 0.0 ? w / sum : 0.0;  // (all chosen scores 0: weights 0)
         if (lane < a.topk) {
-            a.ids[token * a.topk + lane] = id;
+            a.ids[token * a.topk + lane] = none ? -1 : taken.id;
             a.w[token * a.topk + lane] = none ? NAN : static_cast<float>(static_cast<double>(a.scale) * w);
         }
     }
@@ -200,8 +282,8 @@ template <int TYPE, int V>
 int route_launch(const RouteArgs& a, hipStream_t st) {
     const int64_t want = (a.tokens + ROUTE_WAVES - 1) / ROUTE_WAVES;
     const uint32_t grid = static_cast<uint32_t>(want < (1 << 20) ? want : 1 << 20);
-    if (a.bias || (a.top2 && a.kept < a.groups)) route_kernel<TYPE, V, double><<<grid, 64 * ROUTE_WAVES, 0, st>>>(a);
-    else route_kernel<TYPE, V, float><<<grid, 64 * ROUTE_WAVES, 0, st>>>(a);
+    if (a.bias || (a.top2 && a.kept < a.groups)) route_kernel<TYPE, V, true><<<grid, 64 * ROUTE_WAVES, 0, st>>>(a);
+    else route_kernel<TYPE, V, false><<<grid, 64 * ROUTE_WAVES, 0, st>>>(a);
     return check_launch("vb_route_experts");
 }
 
