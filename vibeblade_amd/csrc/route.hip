@@ -94,16 +94,85 @@ __device__ __forceinline__ bool group_stays(const RouteArgs& a, T mine, int grou
     return before < a.kept;
 }
 
-// What the lanes take in the rounds: lane r the r-th expert and its logit.
+// What the lanes take in the rounds: lane r the r-th expert.
 struct Taken {
     int id = -1;
-    float z = -INFINITY;
 };
+
+// The order of floats as that of unsigned numbers (-0 is 0), and back.
+__device__ __forceinline__ uint32_t order_bits(float v) {
+    const uint32_t u = __float_as_uint(v + 0.f);
+    return u ^ (static_cast<uint32_t>(static_cast<int32_t>(u) >> 31) | 0x80000000u);
+}
+__device__ __forceinline__ float order_value(uint32_t o) { return __uint_as_float(o & 0x80000000u ? o ^ 0x80000000u : ~o); }
+constexpr uint32_t ORDER_NONE = 0x007fffffu;  // of -inf
+
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint32_t dpp_max_u(uint32_t v) {
+    const uint32_t u = __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xF, false);
+    return u > v ? u : v;
+}
+__device__ __forceinline__ uint32_t wave_largest_u(uint32_t v) {
+    v = dpp_max_u<0xB1, 0xF>(v);
+    v = dpp_max_u<0x4E, 0xF>(v);
+    v = dpp_max_u<0x141, 0xF>(v);
+    v = dpp_max_u<0x140, 0xF>(v);
+    v = dpp_max_u<0x142, 0xA>(v);
+    v = dpp_max_u<0x143, 0xC>(v);
+    return __builtin_amdgcn_readlane(v, 63);
+}
+
+// The lane's choices in descending order, equal ones by the lower place.
+template <int V>
+struct Sorted {
+    uint32_t key[V];
+    int at[V];
+    __device__ __forceinline__ explicit Sorted(const float (&c)[V]) {
+#pragma unroll
+        for (int v = 0; v < V; v++) key[v] = order_bits(c[v]), at[v] = v;
+#pragma unroll
+        for (int n = V - 1; n > 0; n--)  // neighbours only: equal ones keep their order
+#pragma unroll
+            for (int v = 0; v < n; v++) {
+                const bool swap = key[v + 1] > key[v];
+                const uint32_t k = swap ? key[v] : key[v + 1];
+                const int i = swap ? at[v] : at[v + 1];
+                key[v] = swap ? key[v + 1] : key[v];
+                at[v] = swap ? at[v + 1] : at[v];
+                key[v + 1] = k;
+                at[v + 1] = i;
+            }
+    }
+};
+
+// As `take` below, from sorted choices: a round's is the largest of the lanes'
+// first ones, and the lane that gave it moves up its others.
+template <int V>
+__device__ __forceinline__ float take_sorted(const RouteArgs& a, Sorted<V>& c, int base, int rounds, Taken& out) {
+    const int lane = static_cast<int>(threadIdx.x) & 63;
+    float gap = INFINITY, last = INFINITY;
+    for (int r = 0; r < rounds; r++) {
+        const uint32_t best = wave_largest_u(c.key[0]);
+        if (best <= ORDER_NONE) break;  // no expert is left
+        const float value = order_value(best);
+        gap = fminf(gap, last - value);
+        last = value;
+        const int owner = __ffsll(static_cast<unsigned long long>(__ballot(c.key[0] == best))) - 1;
+        const int chosen = __builtin_amdgcn_readlane(base + c.at[0], owner);
+        out.id = lane == r && r < a.topk ? chosen : out.id;
+        if (lane == owner) {
+#pragma unroll
+            for (int v = 0; v + 1 < V; v++) c.key[v] = c.key[v + 1], c.at[v] = c.at[v + 1];
+            c.key[V - 1] = 0;
+        }
+    }
+    return gap;
+}
 
 // `rounds` rounds over the choices c (of which the first a.topk count); the
 // smallest difference of one round's choice to the next.
 template <int V, typename T>
-__device__ __forceinline__ T take(const RouteArgs& a, T (&c)[V], const float (&z)[V], int base, int rounds, Taken& out) {
+__device__ __forceinline__ T take(const RouteArgs& a, T (&c)[V], int base, int rounds, Taken& out) {
     const int lane = static_cast<int>(threadIdx.x) & 63;
     T gap = INFINITY, last = INFINITY;
     for (int r = 0; r < rounds; r++) {
@@ -116,24 +185,27 @@ __device__ __forceinline__ T take(const RouteArgs& a, T (&c)[V], const float (&z
         last = best;
         const int owner = __ffsll(static_cast<unsigned long long>(__ballot(most == best))) - 1;
         int at = 0;
-        float zat = z[0];
 #pragma unroll
-        for (int v = V - 1; v >= 0; v--) {
-            at = c[v] == best ? v : at;
-            zat = c[v] == best ? z[v] : zat;
-        }
+        for (int v = V - 1; v >= 0; v--) at = c[v] == best ? v : at;
         if (lane == owner) {
 #pragma unroll
             for (int v = 0; v < V; v++) c[v] = v == at ? -INFINITY : c[v];
         }
         const int chosen = __builtin_amdgcn_readlane(base + at, owner);
-        const float chosen_z = lane_value(zat, owner);
-        if (lane == r && r < a.topk) {
-            out.id = chosen;
-            out.z = chosen_z;
-        }
+        out.id = lane == r && r < a.topk ? chosen : out.id;
     }
     return gap;
+}
+
+// Choices in fp32: sorted where a lane has few.
+template <int V>
+__device__ __forceinline__ float take_fp32(const RouteArgs& a, float (&c)[V], int base, int rounds, Taken& out) {
+    if constexpr (V <= 4) {
+        Sorted<V> s(c);
+        return take_sorted<V>(a, s, base, rounds, out);
+    } else {
+        return take<V, float>(a, c, base, rounds, out);
+    }
 }
 
 // What groups go by, in every lane of each: the largest of the choices c, or the
@@ -170,6 +242,16 @@ __global__ void __launch_bounds__(64 * ROUTE_WAVES) route_kernel(RouteArgs a) {
     float b[V];
 #pragma unroll
     for (int v = 0; v < V; v++) b[v] = SCORED && a.bias && v < here ? a.bias[base + v] : 0.f;
+    // Two choices' difference: scores are at most 1 and less than 2e-6 off (an
+    // exponent's rounding costs at most x e^-x half steps, a sum of 512 terms 22 of
+    // them), the sum with a bias half a step of itself.
+    float off = 0.f;
+    if constexpr (SCORED) {
+        float most = 0.f;
+#pragma unroll
+        for (int v = 0; v < V; v++) most = fabsf(b[v]) < INFINITY ? fmaxf(most, fabsf(b[v])) : most;
+        off = 4e-6f + 0x1p-22f * (1.f + wave_largest(most));
+    }
     for (int64_t token = static_cast<int64_t>(blockIdx.x) * ROUTE_WAVES + (threadIdx.x >> 6); token < a.tokens;
          token += static_cast<int64_t>(gridDim.x) * ROUTE_WAVES) {
         float z[V];
@@ -203,7 +285,7 @@ __global__ void __launch_bounds__(64 * ROUTE_WAVES) route_kernel(RouteArgs a) {
         };
         Taken taken;
         if constexpr (SCORED) {
-            float c[V], value[V], most = 0.f, sum32 = 1.f;
+            float c[V], value[V], sum32 = 1.f;
             if (!a.sigmoid) {
                 float part = 0.f;
 #pragma unroll
@@ -220,12 +302,7 @@ __global__ void __launch_bounds__(64 * ROUTE_WAVES) route_kernel(RouteArgs a) {
                 value[v] = z[v] > -INFINITY ? s + b[v] : -INFINITY;
                 bad = bad || value[v] != value[v];
                 c[v] = a.bias ? value[v] : z[v];
-                most = fabsf(value[v]) < INFINITY ? fmaxf(most, fabsf(value[v])) : most;
             }
-            // Two choices' difference: scores are at most 1 and less than 2e-6 off (an
-            // exponent's rounding costs at most x e^-x half steps, a sum of 512 terms 22 of
-            // them), the sum with a bias half a step of itself.
-            const float off = 4e-6f + 0x1p-22f * wave_largest(most);
             bool sure = true;
             if (a.kept < a.groups) {
                 const float mine = group_score<V, float>(a, c, value);
@@ -236,7 +313,7 @@ __global__ void __launch_bounds__(64 * ROUTE_WAVES) route_kernel(RouteArgs a) {
 #pragma unroll
                 for (int v = 0; v < V; v++) c[v] = stays ? c[v] : -INFINITY;
             }
-            const float gap = take<V, float>(a, c, z, base, a.bias ? a.topk + 1 : a.topk, taken);
+            const float gap = take_fp32<V>(a, c, base, a.bias ? a.topk + 1 : a.topk, taken);
             if (a.bias) sure = sure && gap > off;
             if (__any(bad || !sure)) {
                 taken = Taken{};
@@ -253,7 +330,7 @@ __global__ void __launch_bounds__(64 * ROUTE_WAVES) route_kernel(RouteArgs a) {
 #pragma unroll
                     for (int v = 0; v < V; v++) c[v] = stays ? c[v] : -INFINITY;
                 }
-                if (!__any(bad)) take<V, double>(a, c, z, base, a.topk, taken);
+                if (!__any(bad)) take<V, double>(a, c, base, a.topk, taken);
             }
         } else {
             float c[V];
@@ -264,10 +341,10 @@ __global__ void __launch_bounds__(64 * ROUTE_WAVES) route_kernel(RouteArgs a) {
 #pragma unroll
                 for (int v = 0; v < V; v++) c[v] = stays ? c[v] : -INFINITY;
             }
-            if (!__any(bad)) take<V, float>(a, c, z, base, a.topk, taken);
+            if (!__any(bad)) take_fp32<V>(a, c, base, a.topk, taken);
         }
         const bool none = __any(bad);
-        double w = !none && taken.id >= 0 ? score(taken.z) : 0.0;
+        double w = !none && taken.id >= 0 ? score(elem_ld(a.z, token * a.ld + taken.id, TYPE)) : 0.0;
         if (a.renorm) sum = wave_sum64(w);
         else if (!a.sigmoid) sum = total();
         w = w > 0.0 ? w / sum : 0.0;  // (all chosen scores 0: weights 0)
