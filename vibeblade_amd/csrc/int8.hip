@@ -43,43 +43,44 @@ __device__ __forceinline__ int code_of(float v, float s, float inv) {
     return off ? c + (r > 0.f ? 1 : -1) : c;
 }
 
-// 16 consecutive values of a row, from k0 on (0 past the row's end).
+// 16 consecutive values of a row, from k0 on (0 past the row's end), as they lie
+// in memory: a thread holds several such pieces.
 template <int TYPE>
 struct Values {
-    float v[16];
+    static constexpr int WORDS = TYPE == ELEM_F32 ? 16 : 8;
+    uint32_t raw[WORDS];
     // whole: rows begin at multiples of 16 bytes
     __device__ __forceinline__ void load(const void* row, int64_t k0, int64_t k, bool whole) {
         if (whole && k0 + 16 <= k) {
-            if constexpr (TYPE == ELEM_F32) {
+            const uint4* p = reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(row) + k0 * (TYPE == ELEM_F32 ? 4 : 2));
 #pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    const float4 f = reinterpret_cast<const float4*>(static_cast<const float*>(row) + k0)[i];
-                    v[4 * i] = f.x, v[4 * i + 1] = f.y, v[4 * i + 2] = f.z, v[4 * i + 3] = f.w;
-                }
-            } else {
-#pragma unroll
-                for (int i = 0; i < 2; i++) {
-                    const uint4 q = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(row) + k0)[i];
-                    const uint32_t u[4] = {q.x, q.y, q.z, q.w};
-#pragma unroll
-                    for (int j = 0; j < 8; j++) {
-                        const uint32_t h = u[j >> 1] >> 16 * (j & 1) & 0xffffu;
-                        v[8 * i + j] = TYPE == ELEM_BF16 ? __uint_as_float(h << 16)
-                                                         : static_cast<float>(__builtin_bit_cast(_Float16, static_cast<uint16_t>(h)));
-                    }
-                }
+            for (int i = 0; i < WORDS / 4; i++) {
+                const uint4 q = p[i];
+                raw[4 * i] = q.x, raw[4 * i + 1] = q.y, raw[4 * i + 2] = q.z, raw[4 * i + 3] = q.w;
             }
+        } else if constexpr (TYPE == ELEM_F32) {
+#pragma unroll
+            for (int i = 0; i < 16; i++) raw[i] = k0 + i < k ? static_cast<const uint32_t*>(row)[k0 + i] : 0u;
         } else {
 #pragma unroll
-            for (int i = 0; i < 16; i++) v[i] = k0 + i < k ? elem_ld(row, k0 + i, TYPE) : 0.f;
+            for (int i = 0; i < 8; i++) {
+                const uint32_t lo = k0 + 2 * i < k ? static_cast<const uint16_t*>(row)[k0 + 2 * i] : 0u;
+                const uint32_t hi = k0 + 2 * i + 1 < k ? static_cast<const uint16_t*>(row)[k0 + 2 * i + 1] : 0u;
+                raw[i] = lo | hi << 16;
+            }
         }
+    }
+    __device__ __forceinline__ float value(int i) const {
+        if constexpr (TYPE == ELEM_F32) return __uint_as_float(raw[i]);
+        else if constexpr (TYPE == ELEM_BF16) return __uint_as_float(i & 1 ? raw[i >> 1] & 0xffff0000u : raw[i >> 1] << 16);
+        else return static_cast<float>(__builtin_bit_cast(_Float16, static_cast<uint16_t>(raw[i >> 1] >> 16 * (i & 1))));
     }
     // the largest magnitude as bits: infinities and NaN from 0x7f800000 on
     __device__ __forceinline__ uint32_t largest() const {
         uint32_t b = 0;
 #pragma unroll
         for (int i = 0; i < 16; i++) {
-            const uint32_t m = __float_as_uint(v[i]) & 0x7fffffffu;
+            const uint32_t m = __float_as_uint(value(i)) & 0x7fffffffu;
             b = m > b ? m : b;
         }
         return b;
@@ -93,13 +94,13 @@ struct Values {
         float most = 0.f;
 #pragma unroll
         for (int i = 0; i < 16; i++) {
-            const float q = __builtin_fmaf(v[i], inv, 12582912.f);
+            const float v = value(i), q = __builtin_fmaf(v, inv, 12582912.f);
             t[i] = __float_as_uint(q);
-            most = fmaxf(most, fabsf(__builtin_fmaf(12582912.f - q, s, v[i])));
+            most = fmaxf(most, fabsf(__builtin_fmaf(12582912.f - q, s, v)));
         }
         if (!(most + most < s)) {
 #pragma unroll
-            for (int i = 0; i < 16; i++) t[i] = static_cast<uint32_t>(code_of(v[i], s, inv));
+            for (int i = 0; i < 16; i++) t[i] = static_cast<uint32_t>(code_of(value(i), s, inv));
         }
 #pragma unroll
         for (int i = 0; i < 4; i++) {
@@ -464,25 +465,23 @@ __global__ void __launch_bounds__(64 * WR * WT) i8_tile_kernel(I8Args a, int32_t
         }
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         __builtin_amdgcn_wave_barrier();
-        const int pieces = FR * size;  // of 16 bytes, of a token
-        for (int i = lane; i < 16 * pieces; i += 64) {
-            const int row = i / pieces, piece = i % pieces;
-            const int64_t n = n0 + piece * 16 / size;
-            if (t0 + row >= a.m || n >= width) continue;
-            const uint4 v = *reinterpret_cast<const uint4*>(mine + row * pitch + piece * 16);
-            uint8_t* to = y + ((t0 + row) * width + n) * size;
-            if (vec) {
-                *reinterpret_cast<uint4*>(to) = v;
-            } else {
-                const uint32_t u[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-                for (int j = 0; j < 8; j++) {
-                    if (size == 2) {
-                        if (n + j < width) reinterpret_cast<uint16_t*>(to)[j] = static_cast<uint16_t>(u[j >> 1] >> 16 * (j & 1));
-                    } else if (j < 4 && n + j < width) {
-                        reinterpret_cast<uint32_t*>(to)[j] = u[j];
-                    }
-                }
+        if (vec) {
+            const int pieces = FR * size;  // of 16 bytes, of a token
+            for (int i = lane; i < 16 * pieces; i += 64) {
+                const int row = i / pieces, piece = i % pieces;
+                const int64_t n = n0 + piece * 16 / size;
+                if (t0 + row >= a.m || n >= width) continue;
+                *reinterpret_cast<uint4*>(y + ((t0 + row) * width + n) * size) =
+                    *reinterpret_cast<const uint4*>(mine + row * pitch + piece * 16);
+            }
+        } else {  // value by value, a run of them an instruction
+            for (int i = lane; i < 16 * 16 * FR; i += 64) {
+                const int row = i / (16 * FR), n = i % (16 * FR);
+                if (t0 + row >= a.m || n0 + n >= width) continue;
+                uint8_t* to = y + ((t0 + row) * width + n0 + n) * size;
+                const uint8_t* from = mine + row * pitch + n * size;
+                if (size == 4) *reinterpret_cast<uint32_t*>(to) = *reinterpret_cast<const uint32_t*>(from);
+                else *reinterpret_cast<uint16_t*>(to) = *reinterpret_cast<const uint16_t*>(from);
             }
         }
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
@@ -490,18 +489,32 @@ __global__ void __launch_bounds__(64 * WR * WT) i8_tile_kernel(I8Args a, int32_t
     }
 }
 
-// The chunks' sums of four neighbouring rows and a token a thread.
+// The chunks' sums of four neighbouring rows and a token a thread; where rows of y
+// do not take whole stores, of one row, so that a wave's are a run (203 tokens of
+// 5121 rows in two chunks: 6.2 us by fours).
 __global__ void __launch_bounds__(256) i8_join_kernel(I8Args a, int32_t chunks) {
-    const int64_t fours = a.wl.tiles * 4, all = a.m * fours;
-    const bool vec = i8_vec(a);
-    for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < all; i += static_cast<int64_t>(gridDim.x) * 256) {
-        const int64_t t = i / fours, n = i % fours * 4;
-        if (n >= a.n) continue;
-        const i32x4* p = reinterpret_cast<const i32x4*>(a.partial) + i;
-        i32x4 sum = p[0];
-        for (int c = 1; c < chunks; c++) sum += p[c * all];
-        i8_store4(a, t, n, sum, reinterpret_cast<const float*>(a.x + a.xl.scales)[t],
-                  *reinterpret_cast<const float4*>(a.w + a.wl.scales + 4 * n), vec);
+    const int64_t fours = a.wl.tiles * 4, all = a.m * fours, stride = static_cast<int64_t>(gridDim.x) * 256;
+    if (i8_vec(a)) {
+        for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < all; i += stride) {
+            const int64_t t = i / fours, n = i % fours * 4;
+            if (n >= a.n) continue;
+            const i32x4* p = reinterpret_cast<const i32x4*>(a.partial) + i;
+            i32x4 sum = p[0];
+            for (int c = 1; c < chunks; c++) sum += p[c * all];
+            i8_store4(a, t, n, sum, reinterpret_cast<const float*>(a.x + a.xl.scales)[t],
+                      *reinterpret_cast<const float4*>(a.w + a.wl.scales + 4 * n), true);
+        }
+    } else {
+        for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < 4 * all; i += stride) {
+            const int64_t t = i / (4 * fours), n = i % (4 * fours);
+            if (n >= a.n) continue;
+            int sum = a.partial[i];
+            for (int c = 1; c < chunks; c++) sum += a.partial[i + c * 4 * all];
+            float v = static_cast<float>(sum) * reinterpret_cast<const float*>(a.x + a.xl.scales)[t] *
+                      reinterpret_cast<const float*>(a.w + a.wl.scales)[n];
+            if (a.bias) v += a.bias[n];
+            elem_st(a.y, t * a.n + n, a.out_type, v);
+        }
     }
 }
 
@@ -723,7 +736,7 @@ int i8_run(I8Args a, const I8Plan& p, hipStream_t st) {
         default: rc = i8_tile<2, 2, 4, 1>(a, p, st); break;
     }
     if (rc != OK || p.chunks == 1) return rc;
-    i8_join_kernel<<<i8_grid((a.m * a.wl.tiles * 4 + 255) / 256), 256, 0, st>>>(a, static_cast<int32_t>(p.chunks));
+    i8_join_kernel<<<i8_grid((a.m * a.wl.tiles * ((a.n & 3) == 0 ? 4 : 16) + 255) / 256), 256, 0, st>>>(a, static_cast<int32_t>(p.chunks));
     return check_launch("vb_int8_gemm");
 }
 
