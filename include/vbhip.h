@@ -487,8 +487,9 @@ int vb_route_experts(const void* logits, int32_t type, int64_t ld, int64_t n_tok
 /* ---- products in 8-bit integers ----------------------------------------------------
  * A matrix of codes q[r, k] (8 bits, signed) and a scale s[r] per row: weights
  * (rows = output channels) and activations (rows = tokens) alike, in one packed
- * layout of vb_int8_bytes(rows, k) bytes (16-byte aligned; k at most 131071, so
- * that sums of products stay within 32 bits; -1 for other shapes).
+ * layout of vb_int8_bytes(rows, k) bytes (16-byte aligned; at most 2^26 rows, k
+ * at most 131071, so that sums of products stay within 32 bits; -1 for other
+ * shapes).
  *
  * vb_int8_pack lays out codes (row stride ld) and fp32 scales that a program
  * has.  vb_int8_quantize makes them of src (row stride ld, element type as
@@ -503,7 +504,8 @@ int vb_int8_dequant_rows(const void* w, float* out, int64_t rows, int64_t k, voi
  * the m tokens of x, y of the element type y_type.  x_type 0 to 2: x has row
  * stride x_ld and is quantized in the call, as vb_int8_quantize does; 3: x is
  * packed (m rows of k).  Sums are exact; they are converted to fp32 once,
- * multiplied by s_x, then by s_w, and the result is rounded to y_type.  A NaN or
+ * multiplied by s_x, then by s_w, and the result is rounded to y_type: finite
+ * while their product with s_x is below 2^128.  A NaN or
  * an infinity of x makes its own token's results NaN.  y overlaps no operand.
  * workspace: at least vb_int8_workspace(...) bytes (asked on the device of the
  * call), 16-byte aligned, free again when the call's work is done. */

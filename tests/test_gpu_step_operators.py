@@ -525,6 +525,52 @@ def test_int8_refusals():
         quantize_tokens(torch.ones(1, K_MAX + 1, device="cuda"))
 
 
+@pytest.mark.parametrize("dtype", [F32, F16])
+def test_int8_one_token_of_the_longest_k(dtype):
+    """Its codes fill most of a workgroup's shared memory."""
+    x = normal(3, 1, K_MAX).to(dtype)
+    qw = torch.randint(-128, 128, (40, K_MAX), generator=torch.Generator().manual_seed(4), dtype=torch.int8)
+    sw = 0.001 * (0.5 + uniform(5, 40))
+    y = int8_gemm(Int8QTensor.from_int8(qw.cuda(), sw.cuda()), x.cuda())
+    sx = scales64(x)
+    close(y, *product64(codes64(x, sx), sx, qw, sw, None, F32))
+
+
+def test_int8_weights_past_4_gb():
+    n, k = 33000, K_MAX  # 4.3 GB of codes
+    g = torch.Generator(device="cuda").manual_seed(1)
+    qw = torch.cat([torch.randint(-128, 128, (3000, k), generator=g, dtype=torch.int8, device="cuda") for _ in range(11)])
+    w = Int8QTensor.from_int8(qw, torch.ones(n, device="cuda"))
+    some = torch.tensor([0, 16383, 16384, 32767, 32768, 32999])
+    for m in (1, 20, 200):
+        x = torch.randint(-128, 128, (m, k), generator=g, dtype=torch.int8, device="cuda")
+        y = int8_gemm(w, Int8QTensor.from_int8(x, torch.ones(m, device="cuda")))
+        want = x.cpu().double() @ qw[some.cuda()].cpu().double().T
+        assert torch.equal(y[:, some.cuda()].cpu(), want.float())
+
+
+def test_rows_far_apart():
+    """Rows whose offsets pass 32 bits."""
+    room = torch.empty((1 << 32) + 40000, dtype=F16, device="cuda")
+    step = (1 << 31) + 24
+    z = normal(1, 2, 3000).to(F16)
+    far = room.as_strided((2, 3000), (step, 1), 8)
+    far.copy_(z)
+    ids, w = route_experts(far[:, :200], 5)
+    assert torch.equal(ids.cpu(), route64(z[:, :200], 5)[0])
+    weights = Int8QTensor.quantize(normal(2, 50, 3000).cuda())
+    assert torch.equal(int8_gemm(weights, far), int8_gemm(weights, z.cuda()))
+    u, drafted = uniform(3, 2, 2), torch.randint(0, 3000, (2, 1), generator=torch.Generator().manual_seed(4))
+    target, draft = normal(5, 2, 2, 3000).to(F16), normal(6, 2, 1, 3000).to(F16)
+    t = room.as_strided((2, 2, 3000), (step, 9000, 1), 4096)
+    d = room.as_strided((2, 1, 3000), (step, 1, 1), 24576)
+    t.copy_(target)
+    d.copy_(draft)
+    for dz, given in ((None, None), (draft, d)):
+        got, want = verify_draft(t, drafted.cuda(), u.cuda(), given), verify64(target, drafted, u, dz)
+        assert torch.equal(got[0].cpu(), want[0]) and torch.equal(got[1].cpu(), want[1])
+
+
 def test_int8_backend_matmul():
     w = Int8QTensor.quantize(normal(1, 48, 96).cuda())
     a = normal(2, 5, 96)

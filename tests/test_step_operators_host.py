@@ -50,7 +50,8 @@ def test_int8_bytes(lib):
     assert lib.vb_int8_bytes(17, 65) == 4 * 1024 + 128
     assert lib.vb_int8_bytes(128256, 16384) == 128256 * 16384 + 4 * 128256
     assert lib.vb_int8_bytes(16, K_MAX) == 2048 * 1024 + 64
-    for bad in ((0, 64), (16, 0), (-1, 64), (1 << 31, 64), (16, K_MAX + 1)):
+    assert lib.vb_int8_bytes(1 << 26, 64) == (1 << 26) * 68
+    for bad in ((0, 64), (16, 0), (-1, 64), (1 << 31, 64), ((1 << 26) + 1, 64), (16, K_MAX + 1)):
         assert lib.vb_int8_bytes(*bad) == -1
 
 
@@ -60,7 +61,7 @@ def gemm_args(**kw):
 
 
 @pytest.mark.parametrize("bad", [dict(w=None), dict(x=None), dict(y=None), dict(w=PTR + 8), dict(x_type=3, x=PTR + 4),
-                                 dict(x_type=4), dict(x_type=-1), dict(y_type=3), dict(x_ld=-1), dict(m=-1), dict(m=1 << 31),
+                                 dict(x_type=4), dict(x_type=-1), dict(y_type=3), dict(x_ld=-1), dict(m=-1), dict(m=1 << 31), dict(m=1 << 26, rows=1 << 20, x_type=3),
                                  dict(rows=0), dict(k=0), dict(k=K_MAX + 1)])
 def test_int8_gemm_refuses(lib, bad):
     assert lib.vb_int8_gemm(*gemm_args(**bad)) == INVAL

@@ -767,6 +767,11 @@ I8Plan i8_plan(const Int8Layout& wl, const Int8Layout& xl, int64_t m, bool packe
 template <int FR, int FT, int WR, int WT>
 int i8_tile(const I8Args& a, const I8Plan& p, hipStream_t st) {
     const int64_t rows = (a.wl.tiles + FR * WR - 1) / (FR * WR), cols = (a.xl.tiles + FT * WT - 1) / (FT * WT);
+    if (rows * cols * p.chunks * 64 * WR * WT >= int64_t(1) << 32) {  // threads of a launch
+        set_error("vb_int8_gemm: %lld x %lld outputs are too many for a launch", static_cast<long long>(a.m),
+                  static_cast<long long>(a.n));
+        return E_INVAL;
+    }
     const dim3 grid(static_cast<uint32_t>((rows * cols + I8_DIES - 1) / I8_DIES * I8_DIES), static_cast<uint32_t>(p.chunks));
     i8_tile_kernel<FR, FT, WR, WT><<<grid, 64 * WR * WT, 0, st>>>(a, static_cast<int32_t>(rows), static_cast<int32_t>(cols));
     return check_launch("vb_int8_gemm");
@@ -823,8 +828,8 @@ int i8_quantize(const void* src, int32_t type, int64_t ld, int64_t rows, int64_t
 
 int i8_layout_of(const char* what, int64_t rows, int64_t k, Int8Layout* l) {
     if (!int8_layout(rows, k, l)) {
-        set_error("%s: no layout for %lld x %lld (k at most %lld)", what, static_cast<long long>(rows),
-                  static_cast<long long>(k), static_cast<long long>(INT8_MAX_K));
+        set_error("%s: no layout for %lld x %lld (at most %lld rows, k at most %lld)", what, static_cast<long long>(rows),
+                  static_cast<long long>(k), static_cast<long long>(INT8_MAX_ROWS), static_cast<long long>(INT8_MAX_K));
         return E_INVAL;
     }
     return OK;
@@ -880,7 +885,7 @@ int vb_int8_dequant_rows(const void* w, float* out, int64_t rows, int64_t k, voi
 
 int64_t vb_int8_workspace(int64_t m, int64_t rows, int64_t k, int32_t x_type) {
     Int8Layout wl, xl;
-    if (m < 0 || m > 0x7fffffff - 255 || (x_type != I8_PACKED && !elem_type(x_type)) || !int8_layout(rows, k, &wl)) return -1;
+    if (m < 0 || m > INT8_MAX_ROWS || (x_type != I8_PACKED && !elem_type(x_type)) || !int8_layout(rows, k, &wl)) return -1;
     if (m == 0) return 0;
     return int8_layout(m, k, &xl) ? i8_plan(wl, xl, m, x_type == I8_PACKED).workspace : -1;
 }

@@ -25,9 +25,12 @@ struct Int8Layout {
     int64_t scales, total;  // byte offset of the scales, bytes
 };
 
+// rows that a workgroup of 512 threads a tile can be launched for
+constexpr int64_t INT8_MAX_ROWS = 1 << 26;
+
 // false for shapes that there is no layout for
 inline bool int8_layout(int64_t rows, int64_t k, Int8Layout* out) {
-    if (rows <= 0 || k <= 0 || rows > 0x7fffffff - 255 || k > INT8_MAX_K) return false;
+    if (rows <= 0 || k <= 0 || rows > INT8_MAX_ROWS || k > INT8_MAX_K) return false;
     out->tiles = (rows + INT8_ROWS - 1) / INT8_ROWS;
     out->blocks = (k + INT8_K - 1) / INT8_K;
     out->scales = out->tiles * out->blocks * INT8_BLOCK;
