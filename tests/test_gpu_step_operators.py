@@ -875,6 +875,50 @@ def test_captured_verify_steps_replay():
             assert torch.equal(a.nan_to_num(7.0), b.nan_to_num(7.0))
 
 
+def test_captured_calls_of_every_route_replay():
+    """Tiles whole and in chunks, the stream of few tokens, residuals, many experts: replayed on new inputs with eager
+    work between, against eager calls."""
+    w = Int8QTensor.quantize(normal(1, 700, 3000).cuda())
+    small = Int8QTensor.quantize(normal(2, 96, 300).cuda())
+    experts = make_experts(70, 256, 256)
+
+    def calls(s):
+        out = [int8_gemm(w, s["x"][:m]) for m in (1, 9, 40, 300)] + [int8_gemm(small, s["x"][:130, :300], out_dtype=BF16)]
+        routing = route_experts(s["z"], 9, scores="sigmoid", bias=s["bias"], groups=7, groups_kept=4, group_score="top2")
+        out += [*routing, moe_grouped_ffn(*experts, s["t"], routing=routing)[0]]
+        out += verify_draft(s["target"], s["drafted"], s["u"], draft=s["draft"], lengths=s["lengths"])
+        return out
+
+    def fill(s, seed):
+        for i, name in enumerate(("x", "z", "bias", "t", "target", "draft")):
+            s[name].copy_(normal(seed + i, *s[name].shape))
+        s["u"].copy_(uniform(seed + 9, *s["u"].shape))
+        s["drafted"].copy_(s["draft"].argmax(2))
+
+    s = {"x": torch.empty(300, 3000, device="cuda"), "z": torch.empty(12, 70, device="cuda"), "bias": torch.empty(70, device="cuda"),
+         "t": torch.empty(12, 256, device="cuda"), "target": torch.empty(5, 4, 9001, device="cuda"),
+         "draft": torch.empty(5, 3, 9001, device="cuda"), "u": torch.empty(5, 4, device="cuda"),
+         "drafted": torch.empty(5, 3, dtype=torch.int64, device="cuda"),
+         "lengths": torch.tensor([3, 0, 2, 3, 1], dtype=torch.int32, device="cuda")}
+    fill(s, 100)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        calls(s)
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out = calls(s)
+    for turn in range(4):
+        fill(s, 200 + 20 * turn)
+        g.replay()
+        want = calls(s)
+        torch.cuda.synchronize()
+        for a, b in zip(out, want):
+            assert torch.equal(a, b)
+
+
 def test_calls_on_two_streams_at_once():
     w = step_weights()
     jobs = [[normal(90 + i, 5, 256).cuda(), torch.randint(0, 1024, (4,)).cuda(), uniform(95 + i, 5).cuda()] for i in range(2)]

@@ -25,8 +25,8 @@
 //            into, then the place in it (without a drafter's logits the decision
 //            is made here, and the slices' sums are those of stats)
 //
-// The terms' 64-bit arithmetic (fifteen instructions of it a logit, which issue
-// at about half fp32's rate) and the memory bound many rows about alike (64
+// The terms' arithmetic (23 instructions a logit, fifteen of them 64-bit) and the
+// memory bound many rows about alike (64
 // sequences of 4 drafts over 128256 fp32 ids: stats 61 us, 4.8 TB/s; without the
 // terms it takes 52, without the loads 54), the residual by its two terms a logit
 // (19 us for 64 rows and rows of drafts); few rows wait for launches and for one
