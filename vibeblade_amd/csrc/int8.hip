@@ -56,14 +56,15 @@ template <int TYPE>
 struct Values {
     static constexpr int WORDS = TYPE == ELEM_F32 ? 16 : 8;
     uint32_t raw[WORDS];
-    // whole: rows begin at multiples of 16 bytes
-    __device__ __forceinline__ void load(const void* row, int64_t k0, int64_t k, bool whole) {
-        if (whole && k0 + 16 <= k) {
-            const uint4* p = reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(row) + k0 * (TYPE == ELEM_F32 ? 4 : 2));
+    __device__ __forceinline__ void load(const void* row, int64_t k0, int64_t k) {
+        if (k0 + 16 <= k) {  // (rows begin at any element; a load of 16 bytes does not mind)
+            typedef uint32_t v4 __attribute__((ext_vector_type(4), aligned(2)));
+            const v4* p = reinterpret_cast<const v4*>(static_cast<const uint8_t*>(row) + k0 * (TYPE == ELEM_F32 ? 4 : 2));
 #pragma unroll
             for (int i = 0; i < WORDS / 4; i++) {
-                const uint4 q = p[i];
-                raw[4 * i] = q.x, raw[4 * i + 1] = q.y, raw[4 * i + 2] = q.z, raw[4 * i + 3] = q.w;
+                const v4 q = p[i];
+#pragma unroll
+                for (int j = 0; j < 4; j++) raw[4 * i + j] = q[j];
             }
         } else if constexpr (TYPE == ELEM_F32) {
 #pragma unroll
@@ -152,7 +153,6 @@ struct I8Rows {
     uint8_t* w;
     Int8Layout l;
     int64_t ld, rows, k;
-    bool whole;  // rows of src begin at multiples of 16 bytes
 };
 
 // A row by a workgroup, which few rows need; a thread's first HELD pieces of 16
@@ -174,14 +174,14 @@ __global__ void __launch_bounds__(64 * WAVES) i8_quantize_rows_kernel(I8Rows a) 
         for (int h = 0; h < HELD; h++) {
             const int64_t p = at + h * SPAN;
             if (in && p < pieces) {
-                held[h].load(src, p * 16, a.k, a.whole);
+                held[h].load(src, p * 16, a.k);
                 const uint32_t b = held[h].largest();
                 big = b > big ? b : big;
             }
         }
         for (int64_t p = at + HELD * SPAN; in && p < pieces; p += SPAN) {
             Values<TYPE> v;
-            v.load(src, p * 16, a.k, a.whole);
+            v.load(src, p * 16, a.k);
             const uint32_t b = v.largest();
             big = b > big ? b : big;
         }
@@ -202,7 +202,7 @@ __global__ void __launch_bounds__(64 * WAVES) i8_quantize_rows_kernel(I8Rows a) 
             uint4 c = make_uint4(0, 0, 0, 0);
             if (in) {
                 Values<TYPE> v;
-                v.load(src, p * 16, a.k, a.whole);
+                v.load(src, p * 16, a.k);
                 c = v.codes(s.s, s.inv);
             }
             *reinterpret_cast<uint4*>(to + (p >> 2) * INT8_BLOCK + (p & 3) * 256) = c;
@@ -217,7 +217,7 @@ __global__ void __launch_bounds__(64 * WAVES) i8_quantize_rows_kernel(I8Rows a) 
 template <int TYPE>
 __global__ void __launch_bounds__(1024) i8_quantize_tiles_kernel(I8Rows a) {
     __shared__ uint32_t bigs[16][16];
-    constexpr int WAVES = 16, HELD = 4;
+    constexpr int WAVES = 16, HELD = TYPE == ELEM_F32 ? 3 : 4;  // (four of fp32 spill)
     const int lane = static_cast<int>(threadIdx.x) & 63, wave = static_cast<int>(threadIdx.x) >> 6;
     const int j = lane & 15, k16 = 16 * (lane >> 4);
     for (int64_t tile = blockIdx.x; tile < a.l.tiles; tile += gridDim.x) {
@@ -229,7 +229,7 @@ __global__ void __launch_bounds__(1024) i8_quantize_tiles_kernel(I8Rows a) {
 #pragma unroll
         for (int h = 0; h < HELD; h++) {
             const int64_t b = wave + h * WAVES;
-            if (in && b < a.l.blocks) held[h].load(src, b * INT8_K + k16, a.k, a.whole);
+            if (in && b < a.l.blocks) held[h].load(src, b * INT8_K + k16, a.k);
         }
 #pragma unroll
         for (int h = 0; h < HELD; h++) {
@@ -240,7 +240,7 @@ __global__ void __launch_bounds__(1024) i8_quantize_tiles_kernel(I8Rows a) {
         }
         for (int64_t b = wave + HELD * WAVES; in && b < a.l.blocks; b += WAVES) {
             Values<TYPE> v;
-            v.load(src, b * INT8_K + k16, a.k, a.whole);
+            v.load(src, b * INT8_K + k16, a.k);
             const uint32_t most = v.largest();
             big = most > big ? most : big;
         }
@@ -265,7 +265,7 @@ __global__ void __launch_bounds__(1024) i8_quantize_tiles_kernel(I8Rows a) {
             uint4 c = make_uint4(0, 0, 0, 0);
             if (in) {
                 Values<TYPE> v;
-                v.load(src, b * INT8_K + k16, a.k, a.whole);
+                v.load(src, b * INT8_K + k16, a.k);
                 c = v.codes(s.s, s.inv);
             }
             to[b * 64] = c;
@@ -512,7 +512,9 @@ __global__ void __launch_bounds__(64 * WR * WT) i8_tile_kernel(I8Args a, int32_t
     const int64_t n0 = (row0 + wr * FR) * 16, width = a.partial ? a.wl.tiles * 16 : a.n;
     uint8_t* const y = a.partial ? reinterpret_cast<uint8_t*>(a.partial) + static_cast<int64_t>(blockIdx.y) * a.m * width * 4
                                  : static_cast<uint8_t*>(a.y);
-    const bool vec = (width * size & 15) == 0 && (reinterpret_cast<uintptr_t>(y) & 15) == 0;
+    // the bytes that every run of a token's results begins at a multiple of
+    const uint32_t apart = static_cast<uint32_t>(width * size) | static_cast<uint32_t>(reinterpret_cast<uintptr_t>(y)) | 16u;
+    const int unit = static_cast<int>(apart & (0u - apart));
 #pragma unroll
     for (int t = 0; t < FT; t++) {
         const int64_t t0 = (col0 + wt * FT + t) * 16;
@@ -535,25 +537,19 @@ __global__ void __launch_bounds__(64 * WR * WT) i8_tile_kernel(I8Args a, int32_t
         }
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         __builtin_amdgcn_wave_barrier();
-        if (vec) {
-            const int pieces = FR * size;  // of 16 bytes, of a token
+        const auto out = [&](auto piece) __attribute__((always_inline)) {
+            using P = decltype(piece);
+            const int each = static_cast<int>(sizeof(P)) / size, pieces = 16 * FR / each;  // values of a piece, pieces of a token
             for (int i = lane; i < 16 * pieces; i += 64) {
-                const int row = i / pieces, piece = i % pieces;
-                const int64_t n = n0 + piece * 16 / size;
-                if (t0 + row >= a.m || n >= width) continue;
-                *reinterpret_cast<uint4*>(y + ((t0 + row) * width + n) * size) =
-                    *reinterpret_cast<const uint4*>(mine + row * pitch + piece * 16);
-            }
-        } else {  // value by value, a run of them an instruction
-            for (int i = lane; i < 16 * 16 * FR; i += 64) {
-                const int row = i / (16 * FR), n = i % (16 * FR);
+                const int row = i / pieces, n = i % pieces * each;
                 if (t0 + row >= a.m || n0 + n >= width) continue;
-                uint8_t* to = y + ((t0 + row) * width + n0 + n) * size;
-                const uint8_t* from = mine + row * pitch + n * size;
-                if (size == 4) *reinterpret_cast<uint32_t*>(to) = *reinterpret_cast<const uint32_t*>(from);
-                else *reinterpret_cast<uint16_t*>(to) = *reinterpret_cast<const uint16_t*>(from);
+                *reinterpret_cast<P*>(y + ((t0 + row) * width + n0 + n) * size) = *reinterpret_cast<const P*>(mine + row * pitch + n * size);
             }
-        }
+        };
+        if (unit == 16) out(uint4{});
+        else if (unit == 8) out(uint2{});
+        else if (unit == 4) out(uint32_t{});
+        else out(uint16_t{});
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         __builtin_amdgcn_wave_barrier();
     }
@@ -604,7 +600,6 @@ struct I8Few {
     I8Args g;
     const void* raw;  // the tokens' values
     int64_t ld, k;
-    bool whole;
 };
 
 template <int XT, int KS>
@@ -639,12 +634,12 @@ __global__ void __launch_bounds__(64 * KS) i8_few_kernel(I8Few a) {
             uint32_t big = 0;
             const int at = static_cast<int>(threadIdx.x);
             if (at < pieces) {
-                first.load(src, at * 16, a.k, a.whole);
+                first.load(src, at * 16, a.k);
                 big = first.largest();
             }
             for (int p = at + 64 * KS; p < pieces; p += 64 * KS) {
                 Values<XT> v;
-                v.load(src, p * 16, a.k, a.whole);
+                v.load(src, p * 16, a.k);
                 const uint32_t b = v.largest();
                 big = b > big ? b : big;
             }
@@ -658,7 +653,7 @@ __global__ void __launch_bounds__(64 * KS) i8_few_kernel(I8Few a) {
             if (at < pieces) reinterpret_cast<uint4*>(codes)[at * m + t] = first.codes(s.s, s.inv);
             for (int p = at + 64 * KS; p < pieces; p += 64 * KS) {
                 Values<XT> v;
-                v.load(src, p * 16, a.k, a.whole);
+                v.load(src, p * 16, a.k);
                 reinterpret_cast<uint4*>(codes)[p * m + t] = v.codes(s.s, s.inv);
             }
             lds_barrier();  // the codes, and bigs is free
@@ -698,13 +693,11 @@ __global__ void __launch_bounds__(64 * KS) i8_few_kernel(I8Few a) {
             if (i0 + I8_BATCH < mine) batch(std::integral_constant<int, 1>{}, i0 + I8_BATCH);
         }
     }
-    if constexpr (KS > 1) {
-        few_lds[wave * 64 + lane] = acc;
-        __syncthreads();
-        if (wave > 0) return;
+    few_lds[wave * 64 + lane] = acc;
+    __syncthreads();
+    if (wave > 0) return;
 #pragma unroll
-        for (int v = 1; v < KS; v++) acc += few_lds[v * 64 + lane];
-    }
+    for (int v = 1; v < KS; v++) acc += few_lds[v * 64 + lane];
     const int64_t n = tile * 16 + 4 * (lane >> 4);
     if (j < m && n < a.g.n)
         i8_store4(a.g, j, n, acc, sx, *reinterpret_cast<const float4*>(a.g.w + a.g.wl.scales + 4 * n), i8_vec(a.g));
@@ -792,8 +785,7 @@ template <int XT>
 int i8_few(const I8Few& a, const I8Plan& p, hipStream_t st) {
     const uint32_t grid = static_cast<uint32_t>(a.g.wl.tiles);
     const uint32_t lds = static_cast<uint32_t>(p.ks * 1024 + (p.self ? a.g.m * a.g.wl.blocks * INT8_K : 0));
-    if (p.ks == 1) i8_few_kernel<XT, 1><<<grid, 64, lds, st>>>(a);
-    else if (p.ks == 2) i8_few_kernel<XT, 2><<<grid, 128, lds, st>>>(a);
+    if (p.ks == 2) i8_few_kernel<XT, 2><<<grid, 128, lds, st>>>(a);
     else if (p.ks == 4) i8_few_kernel<XT, 4><<<grid, 256, lds, st>>>(a);
     else i8_few_kernel<XT, 8><<<grid, 512, lds, st>>>(a);
     return check_launch("vb_int8_gemm");
@@ -815,11 +807,6 @@ int i8_run(I8Args a, const I8Plan& p, hipStream_t st) {
     return check_launch("vb_int8_gemm");
 }
 
-// Whether every row begins at a multiple of 16 bytes.
-bool whole_rows(const void* src, int32_t type, int64_t ld, int64_t rows) {
-    return reinterpret_cast<uintptr_t>(src) % 16 == 0 && (rows == 1 || ld * elem_bytes(type) % 16 == 0);
-}
-
 template <int TYPE>
 int i8_quantize_type(const I8Rows& a, hipStream_t st) {
     // a workgroup a row, of four waves where those hold it, until tiles alone give half of the CUs one
@@ -831,7 +818,7 @@ int i8_quantize_type(const I8Rows& a, hipStream_t st) {
 
 int i8_quantize(const void* src, int32_t type, int64_t ld, int64_t rows, int64_t k, uint8_t* w, const Int8Layout& l,
                 hipStream_t st) {
-    const I8Rows a{src, w, l, ld, rows, k, whole_rows(src, type, ld, rows)};
+    const I8Rows a{src, w, l, ld, rows, k};
     if (type == ELEM_F32) return i8_quantize_type<ELEM_F32>(a, st);
     if (type == ELEM_F16) return i8_quantize_type<ELEM_F16>(a, st);
     return i8_quantize_type<ELEM_BF16>(a, st);
@@ -939,9 +926,8 @@ int vb_int8_gemm(const void* w, int64_t rows, int64_t k, const void* x, int32_t 
     a.m = m;
     a.out_type = y_type;
     if (!p.few) return i8_run(a, p, as_stream(stream));
-    I8Few f{a, x, x_ld, k, false};
+    const I8Few f{a, x, x_ld, k};
     if (!p.self) return i8_few<I8_PACKED>(f, p, as_stream(stream));
-    f.whole = whole_rows(x, x_type, x_ld, m);
     if (x_type == ELEM_F32) return i8_few<ELEM_F32>(f, p, as_stream(stream));
     if (x_type == ELEM_F16) return i8_few<ELEM_F16>(f, p, as_stream(stream));
     return i8_few<ELEM_BF16>(f, p, as_stream(stream));
