@@ -590,16 +590,16 @@ __global__ void __launch_bounds__(256) i8_join_kernel(I8Args a, int32_t chunks) 
 // takes every KS-th block of a row tile, KB by KB, sixteen of them under way, and
 // the KS waves of a workgroup add their sums through LDS.
 //
-// Where the tokens' values are few (x_type 0 to 2), every workgroup quantizes
-// them for itself while its first weights are under way, a piece of 16 values a
-// thread at a time, into the operand's order in LDS: a launch less.  Otherwise
-// they are packed, and a wave loads its operands beside the weights.
+// One token's values (x_type 0 to 2) every workgroup quantizes for itself while
+// its first weights are under way, a piece of 16 a thread at a time, into the
+// operand's order in LDS: a launch less.  Otherwise the tokens are packed, and a
+// wave loads its operands beside the weights.
 constexpr int I8_BATCH = 8;  // blocks; two batches are under way
 
 struct I8Few {
     I8Args g;
-    const void* raw;  // the tokens' values
-    int64_t ld, k;
+    const void* raw;  // one token's values
+    int64_t k;
 };
 
 template <int XT, int KS>
@@ -627,45 +627,40 @@ __global__ void __launch_bounds__(64 * KS) i8_few_kernel(I8Few a) {
     i32x4* codes = few_lds + KS * 64;
     float sx = 0.f;
     if constexpr (SELF) {
-        const int pieces = blocks * 4;
-        for (int t = 0; t < m; t++) {
-            const uint8_t* src = static_cast<const uint8_t*>(a.raw) + t * a.ld * (XT == ELEM_F32 ? 4 : 2);
-            Values<XT> first;
-            uint32_t big = 0;
-            const int at = static_cast<int>(threadIdx.x);
-            if (at < pieces) {
-                first.load(src, at * 16, a.k);
-                big = first.largest();
-            }
-            for (int p = at + 64 * KS; p < pieces; p += 64 * KS) {
-                Values<XT> v;
-                v.load(src, p * 16, a.k);
-                const uint32_t b = v.largest();
-                big = b > big ? b : big;
-            }
-            big = wave_max_bits(big);
-            if (lane == 0) bigs[wave] = big;
-            lds_barrier();
-            big = wave_max_bits(lane < KS ? bigs[lane] : 0);
-            const RowScale s(big);
-            sx = j == t ? s.stored : sx;
-            // place of piece p of token t: (block, k / 16 of it, token)
-            if (at < pieces) reinterpret_cast<uint4*>(codes)[at * m + t] = first.codes(s.s, s.inv);
-            for (int p = at + 64 * KS; p < pieces; p += 64 * KS) {
-                Values<XT> v;
-                v.load(src, p * 16, a.k);
-                reinterpret_cast<uint4*>(codes)[p * m + t] = v.codes(s.s, s.inv);
-            }
-            lds_barrier();  // the codes, and bigs is free
+        const int pieces = blocks * 4, at = static_cast<int>(threadIdx.x);
+        Values<XT> first;
+        uint32_t big = 0;
+        if (at < pieces) {
+            first.load(a.raw, at * 16, a.k);
+            big = first.largest();
         }
+        for (int p = at + 64 * KS; p < pieces; p += 64 * KS) {
+            Values<XT> v;
+            v.load(a.raw, p * 16, a.k);
+            const uint32_t b = v.largest();
+            big = b > big ? b : big;
+        }
+        big = wave_max_bits(big);
+        if (lane == 0) bigs[wave] = big;
+        lds_barrier();
+        big = wave_max_bits(lane < KS ? bigs[lane] : 0);
+        const RowScale s(big);
+        sx = s.stored;
+        if (at < pieces) reinterpret_cast<uint4*>(codes)[at] = first.codes(s.s, s.inv);
+        for (int p = at + 64 * KS; p < pieces; p += 64 * KS) {
+            Values<XT> v;
+            v.load(a.raw, p * 16, a.k);
+            reinterpret_cast<uint4*>(codes)[p] = v.codes(s.s, s.inv);
+        }
+        lds_barrier();
     } else {
         sx = reinterpret_cast<const float*>(a.g.x + a.g.xl.scales)[token];
     }
-    const i32x4* px = SELF ? codes + (lane >> 4) * m + token : reinterpret_cast<const i32x4*>(a.g.x) + (lane >> 4) * 16 + token;
+    const i32x4* px = SELF ? codes + (lane >> 4) : reinterpret_cast<const i32x4*>(a.g.x) + (lane >> 4) * 16 + token;
     i32x4 acc = {0, 0, 0, 0}, x[SELF ? 1 : 2][I8_BATCH];
     const auto load_x = [&](int q, int i0) __attribute__((always_inline)) {
 #pragma unroll
-        for (int i = 0; i < I8_BATCH; i++) x[q][i] = SELF ? px[block(i0 + i) * 4 * m] : px[block(i0 + i) * 64];
+        for (int i = 0; i < I8_BATCH; i++) x[q][i] = px[block(i0 + i) * (SELF ? 4 : 64)];
     };
     const auto batch = [&](auto parity, int i0) __attribute__((always_inline)) {
         constexpr int q = decltype(parity)::value, qx = SELF ? 0 : q;
@@ -704,7 +699,7 @@ __global__ void __launch_bounds__(64 * KS) i8_few_kernel(I8Few a) {
 }
 
 struct I8Plan {
-    bool few, self;  // i8_few_kernel, which quantizes the tokens itself
+    bool few, self;  // i8_few_kernel, which quantizes the token itself
     int ks;          // its waves a tile
     int shape;       // of the tiles
     int64_t chunks;  // of k
@@ -784,7 +779,7 @@ int i8_tile(const I8Args& a, const I8Plan& p, hipStream_t st) {
 template <int XT>
 int i8_few(const I8Few& a, const I8Plan& p, hipStream_t st) {
     const uint32_t grid = static_cast<uint32_t>(a.g.wl.tiles);
-    const uint32_t lds = static_cast<uint32_t>(p.ks * 1024 + (p.self ? a.g.m * a.g.wl.blocks * INT8_K : 0));
+    const uint32_t lds = static_cast<uint32_t>(p.ks * 1024 + (p.self ? a.g.wl.blocks * INT8_K : 0));
     if (p.ks == 2) i8_few_kernel<XT, 2><<<grid, 128, lds, st>>>(a);
     else if (p.ks == 4) i8_few_kernel<XT, 4><<<grid, 256, lds, st>>>(a);
     else i8_few_kernel<XT, 8><<<grid, 512, lds, st>>>(a);
@@ -926,7 +921,7 @@ int vb_int8_gemm(const void* w, int64_t rows, int64_t k, const void* x, int32_t 
     a.m = m;
     a.out_type = y_type;
     if (!p.few) return i8_run(a, p, as_stream(stream));
-    const I8Few f{a, x, x_ld, k};
+    const I8Few f{a, x, k};
     if (!p.self) return i8_few<I8_PACKED>(f, p, as_stream(stream));
     if (x_type == ELEM_F32) return i8_few<ELEM_F32>(f, p, as_stream(stream));
     if (x_type == ELEM_F16) return i8_few<ELEM_F16>(f, p, as_stream(stream));
