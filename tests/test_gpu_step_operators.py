@@ -803,6 +803,64 @@ def test_verify_draft_refusals():
         verify_draft(torch.zeros(1, 65, 4, device="cuda"), torch.zeros(1, 64, dtype=torch.int32, device="cuda"), torch.zeros(1, 65, device="cuda"))
 
 
+# Rows of several pieces a slice (a workgroup takes 2048 logits at a time, 576 rows of 20011 make slices of 6672, 320
+# rows of 3336): what the sums are relative to begins with a slice's first logits.
+
+def leading(seqs, k, vocab, lead, temperature, seed):
+    """Three ids a row, behind the first 2048, `lead` powers of two over all others."""
+    step = temperature * math.log(2)
+    target = normal(seed, seqs, k + 1, vocab, scale=0.5 * temperature)
+    ids = 2048 + torch.stack([torch.randperm(1200, generator=torch.Generator().manual_seed(seed + 7 + i))[:3]
+                              for i in range(seqs * (k + 1))]).view(seqs, k + 1, 3)
+    dz = target[:, :k].clone()
+    top = lead * step + 0.7 * temperature * normal(seed + 1, seqs, k + 1, 3)
+    target.scatter_(2, ids, top)
+    dz.scatter_(2, ids[:, :k], top[:, :k] + 0.4 * temperature * normal(seed + 2, seqs, k, 3))
+    which = torch.randint(0, 3, (seqs, k, 1), generator=torch.Generator().manual_seed(seed + 3))
+    return target, ids[:, :k].gather(2, which)[..., 0], uniform(seed + 4, seqs, k + 1), dz
+
+
+@pytest.mark.parametrize("temperature", [1.0, 0.05, 0.02, 0.01])
+@pytest.mark.parametrize("lead", [40, 61, 130, 300, 520, 700, 890, 910, 2000])
+def test_verify_draft_leads_behind_the_first_logits(lead, temperature):
+    target, drafted, u, dz = leading(64, 4, 20011, lead, temperature, lead)
+    _, accepted = check_verify(target, drafted, u, dz, temperature=temperature)
+    assert set(accepted.tolist()) >= {0, 4}
+    check_verify(target, drafted, u, None, temperature=temperature)
+
+
+@pytest.mark.parametrize("temperature", [0.05, 0.03, 0.025, 0.02, 0.015, 0.01])
+@pytest.mark.parametrize("vocab", [20011, 32003])
+def test_verify_draft_nearly_greedy_batches(temperature, vocab):
+    """Likely ids anywhere in rows of ordinary spread."""
+    target, _, u, dz = make_drafts(64, 4, vocab, seed=37, agree=0.01)
+    ids = torch.randint(0, vocab, (64, 5, 2), generator=torch.Generator().manual_seed(38))
+    top = 20.0 + temperature * normal(39, 64, 5, 2)
+    target.scatter_(2, ids, top)
+    dz.scatter_(2, ids[:, :4], top[:, :4] + 0.3 * temperature * normal(40, 64, 4, 2))
+    check_verify(target, ids[:, :4, 0], u, dz, temperature=temperature)
+    check_verify(target, ids[:, :4, 0], u, None, temperature=temperature)
+
+
+@pytest.mark.parametrize("rise", [7, 59, 61, 100, 450, 899, 901, 3000])
+def test_verify_draft_rows_that_rise(rise):
+    """A whole row a slice (2100 rows), each piece of 2048 `rise` powers of two over the one before, or under it."""
+    target, drafted, u, dz = make_drafts(300, 3, 9001, seed=41, agree=0.3)
+    for sign in (1, -1):
+        up = (sign * rise * math.log(2) * (torch.arange(9001) // 2048)).float()
+        at = torch.arange(9001) >= 8192 if sign > 0 else torch.arange(9001) < 2048
+        d = torch.where(at, dz, -INF).argmax(2)
+        check_verify(target + up, d, u, dz + up)
+
+
+@pytest.mark.parametrize("temperature,scale", [(1e-30, 1.0), (1e-12, 1.0), (1e-6, 1.0), (1.0, 1e13), (1.0, 1e37), (1e30, 1.0), (1e4, 1e3)])
+def test_verify_draft_extremes_of_long_slices(temperature, scale):
+    target, drafted, u, dz = make_drafts(64, 4, 20011, seed=43, agree=0.2)
+    drafted[::2] = target[::2, :4].argmax(2)
+    check_verify(target * scale, drafted, u, dz * scale, temperature=temperature)
+    check_verify(target * scale, drafted, u, None, temperature=temperature)
+
+
 # ---- together, on streams and in graphs ---------------------------------------------------
 
 def step_weights():

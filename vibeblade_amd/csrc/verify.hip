@@ -187,7 +187,9 @@ __global__ void __launch_bounds__(VF_THREADS) verify_stats_kernel(VerifyArgs a) 
         const int begin = slice * a.slice, end = a.vocab - begin < a.slice ? a.vocab : begin + a.slice;
         // The lane's sum is relative to the largest of its first logits: 64 bits have
         // room for what is 2^900 times that, and only a logit past it (or the first
-        // one after nothing but -inf) moves the reference.
+        // one after nothing but -inf) moves the reference.  What is stored is relative
+        // to the slice's largest logit: terms of a row by its maximum are at most 1 and
+        // its sum at most the vocabulary, so products of the two stay finite.
         double ref = 0.0, at_ref = 0.0, sum = 0.0;  // at_ref: c ref, rounded; a term is 2^(c z - at_ref), one fma for the exponent
         float top = -INFINITY, limit = -INFINITY;
         bool bad = false, far = false;  // far: rounding c ref may cost that much; a term is 2^(c (z - ref))
@@ -202,7 +204,7 @@ __global__ void __launch_bounds__(VF_THREADS) verify_stats_kernel(VerifyArgs a) 
             for (int j = 0; j < VF_PIECE; j++) bad = bad || !(l.v[j] < INFINITY);
             if (most > limit) {
                 const double to = static_cast<double>(most);
-                sum = top > -INFINITY ? sum * exp2(far ? (ref - to) * c : __builtin_fma(-to, c, at_ref)) : 0.0;
+                sum = limit > -INFINITY ? sum * exp2(far ? (ref - to) * c : __builtin_fma(-to, c, at_ref)) : 0.0;
                 ref = to;
                 at_ref = to * c;
                 if (!(fabs(at_ref) < 0x1p40)) {
@@ -212,8 +214,8 @@ __global__ void __launch_bounds__(VF_THREADS) verify_stats_kernel(VerifyArgs a) 
                     far = false;
                 }
                 limit = fminf(static_cast<float>(to + 900.0 / c), 3.402823466e38f);
-                top = most;
             }
+            top = fmaxf(top, most);
             double part = 0.0;
             if (!__any(far)) {
 #pragma unroll
