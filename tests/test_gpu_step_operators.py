@@ -861,6 +861,19 @@ def test_verify_draft_extremes_of_long_slices(temperature, scale):
     check_verify(target * scale, drafted, u, None, temperature=temperature)
 
 
+@pytest.mark.parametrize("logit,temperature", [(12.0, 1e-9), (8.0, 1e-9), (-9.0, 1.1e-9), (12.0, 1.2e-8), (3.0, 2e-10)])
+def test_verify_draft_neighbours_at_a_low_temperature(logit, temperature):
+    """One logit the next float over all others, hundreds of powers of two above them."""
+    row = torch.full((20011,), logit)
+    row[5000] = torch.nextafter(row[0], torch.tensor(INF))
+    u = uniform(45, 300, 2)
+    drafted = torch.full((300, 1), 5000)
+    target = row.cuda().expand(300, 2, 20011)
+    for dz in (None, target[:, :1]):
+        tokens, accepted = verify_draft(target, drafted.cuda(), u.cuda(), dz, temperature=temperature)
+        assert (tokens.cpu() == 5000).all() and (accepted.cpu() == 1).all()
+
+
 # ---- together, on streams and in graphs ---------------------------------------------------
 
 def step_weights():

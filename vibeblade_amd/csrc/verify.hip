@@ -185,11 +185,13 @@ __global__ void __launch_bounds__(VF_THREADS) verify_stats_kernel(VerifyArgs a) 
         const int64_t at = of_target ? seq * a.target_seq + j * a.target_row : seq * a.draft_seq + j * a.draft_row;
         const double c = of_target ? a.c : a.cd;
         const int begin = slice * a.slice, end = a.vocab - begin < a.slice ? a.vocab : begin + a.slice;
-        // The lane's sum is relative to the largest of its first logits: 64 bits have
-        // room for what is 2^900 times that, and only a logit past it (or the first
-        // one after nothing but -inf) moves the reference.  What is stored is relative
-        // to the slice's largest logit: terms of a row by its maximum are at most 1 and
-        // its sum at most the vocabulary, so products of the two stay finite.
+        // The lane's sum is relative to the largest of its first logits: only a logit
+        // that is 2^450 times that (or the first one after nothing but -inf) moves the
+        // reference.  fp32 rounds the border up by half a step at most, and by no more
+        // than the 450: exponents stay below 901 (from 1024 on there is no 2^x), and a
+        // term of up to 2^450 is good to 2^-45, the fma's rounding.  What is stored is
+        // relative to the slice's largest logit: terms of a row by its maximum are at
+        // most 1 and its sum at most the vocabulary, so products of the two stay finite.
         double ref = 0.0, at_ref = 0.0, sum = 0.0;  // at_ref: c ref, rounded; a term is 2^(c z - at_ref), one fma for the exponent
         float top = -INFINITY, limit = -INFINITY;
         bool bad = false, far = false;  // far: rounding c ref may cost that much; a term is 2^(c (z - ref))
@@ -213,7 +215,7 @@ __global__ void __launch_bounds__(VF_THREADS) verify_stats_kernel(VerifyArgs a) 
                 } else {
                     far = false;
                 }
-                limit = fminf(static_cast<float>(to + 900.0 / c), 3.402823466e38f);
+                limit = fminf(static_cast<float>(to + 450.0 / c), 3.402823466e38f);
             }
             top = fmaxf(top, most);
             double part = 0.0;
