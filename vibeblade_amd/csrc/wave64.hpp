@@ -15,20 +15,15 @@ namespace vb {
 constexpr double EXP2_LEAST = -1021.0;
 struct Exp2 {
     double c10, c9, c8, c7, c6, c5, c4, c3, c2, c1;
-    double q8, q7, q6, q5, q4, q3, q2, q1, q0;
     // In scalar registers, and the compiler does not know them: a fma takes one of
-    // them as it is, where a known constant is first moved to vector registers (26
-    // instructions a logit in the draft verification, so 21).  Their number counts:
-    // 24 M wave instructions, two thirds of them 64-bit, took 61 us without a load,
-    // 6 cycles each.
+    // them as it is, where a known constant is first moved to vector registers (five
+    // instructions more a logit in the draft verification, whose 64-bit terms bound
+    // it as much as memory does).
     __device__ __forceinline__ Exp2()
         : c10(0x1.e6063f7217bc7p-28), c9(0x1.b675bca4eeebbp-24), c8(0x1.62bfd47773353p-20), c7(0x1.ffcb54062e698p-17),
           c6(0x1.430913096fd9fp-13), c5(0x1.5d87fe9d7a584p-10), c4(0x1.3b2ab6fba1ddap-7), c3(0x1.c6b08d703ce49p-5),
-          c2(0x1.ebfbdff82c598p-3), c1(0x1.62e42fefa3a19p-1),
-          q8(0x1.63d136366db24p-20), q7(0x1.00dc4a532fb8ep-16), q6(0x1.4308ac85aa947p-13),
-          q5(0x1.5d8745a728441p-10), q4(0x1.3b2ab7181b755p-7), q3(0x1.c6b08dd6fd234p-5), q2(0x1.ebfbdff823cedp-3), q1(0x1.62e42fef84cf0p-1), q0(0x1.0000000000000p+0) {
+          c2(0x1.ebfbdff82c598p-3), c1(0x1.62e42fefa3a19p-1) {
         asm("" : "+s"(c10), "+s"(c9), "+s"(c8), "+s"(c7), "+s"(c6), "+s"(c5), "+s"(c4), "+s"(c3), "+s"(c2), "+s"(c1));
-        asm("" : "+s"(q8), "+s"(q7), "+s"(q6), "+s"(q5), "+s"(q4), "+s"(q3), "+s"(q2), "+s"(q1), "+s"(q0));
     }
     __device__ __forceinline__ double normal(double x) const {
         x = fmax(x, EXP2_LEAST);
@@ -43,20 +38,6 @@ struct Exp2 {
         p = __builtin_fma(p, f, c2);
         p = __builtin_fma(p, f, c1);
         p = __builtin_fma(p, f, 1.0);
-        return __hiloint2double(__double2hiint(p) + (__double2loint(shifted) << 20), __double2loint(p));
-    }
-    // The same from nine points, relative error 1.1e-12, for terms of long sums.
-    __device__ __forceinline__ double quick(double x) const {
-        x = fmax(x, EXP2_LEAST);
-        const double shifted = x + 0x1.8p52, f = x - (shifted - 0x1.8p52);
-        double p = __builtin_fma(q8, f, q7);
-        p = __builtin_fma(p, f, q6);
-        p = __builtin_fma(p, f, q5);
-        p = __builtin_fma(p, f, q4);
-        p = __builtin_fma(p, f, q3);
-        p = __builtin_fma(p, f, q2);
-        p = __builtin_fma(p, f, q1);
-        p = __builtin_fma(p, f, q0);
         return __hiloint2double(__double2hiint(p) + (__double2loint(shifted) << 20), __double2loint(p));
     }
     // 2^x for x up to 1023, 0 below -1021.
