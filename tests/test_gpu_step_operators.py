@@ -177,6 +177,18 @@ def test_route_experts_nan_and_infinities(scores, bias):
         check_route(z, 5, bias=b, scores=scores)
 
 
+@pytest.mark.parametrize("scores", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("sign", [1.0, -1.0])
+def test_route_experts_group_sums_past_fp32(scores, sign):
+    """Two biases whose sum is no fp32 number: groups are told apart in 64 bits all the same."""
+    z = normal(27, 20, 12)
+    b = torch.tensor([3.0, 2.9, 0.0, 0.0, 3.3, 3.2, 0.0, 0.0, 3.1, 3.0, 0.0, 0.0]) * 1e38
+    if sign < 0:
+        b = -torch.tensor([3.3, 3.2, 3.35, 3.25, 3.0, 2.9, 3.1, 3.05, 3.2, 3.1, 3.3, 3.15]) * 1e38
+    for kept, topk in ((1, 1), (1, 2), (2, 3)):
+        check_route(z, topk, bias=b, scores=scores, groups=3, groups_kept=kept, group_score="top2")
+
+
 def test_route_experts_scores_closer_than_fp32_are_told_apart():
     # sigmoid(z) + b of neighbours differ by 2^-30 or less: equal in fp32
     z = torch.zeros(64, 128)

@@ -252,13 +252,15 @@ __global__ void __launch_bounds__(64 * ROUTE_WAVES) route_kernel(RouteArgs a) {
     for (int v = 0; v < V; v++) b[v] = SCORED && a.bias && v < here ? a.bias[base + v] : 0.f;
     // Two choices' difference: scores are at most 1 and less than 2e-6 off (an
     // exponent's rounding costs at most x e^-x half steps, a sum of 512 terms 22 of
-    // them), the sum with a bias half a step of itself.
+    // them), the sum with a bias half a step of itself.  The sum of two past 2^126
+    // may be no fp32 number, and an infinity is equal to any other: never sure.
     float off = 0.f;
     if constexpr (SCORED) {
         float most = 0.f;
 #pragma unroll
         for (int v = 0; v < V; v++) most = fabsf(b[v]) < INFINITY ? fmaxf(most, fabsf(b[v])) : most;
-        off = 4e-6f + 0x1p-22f * (1.f + wave_largest(most));
+        most = wave_largest(most);
+        off = most < 0x1p126f ? 4e-6f + 0x1p-22f * (1.f + most) : INFINITY;
     }
     for (int64_t token = static_cast<int64_t>(blockIdx.x) * ROUTE_WAVES + (threadIdx.x >> 6); token < a.tokens;
          token += static_cast<int64_t>(gridDim.x) * ROUTE_WAVES) {
