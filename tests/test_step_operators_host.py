@@ -5,9 +5,10 @@ import pytest
 import torch
 
 from vibeblade_amd import _lib
+from vibeblade_amd.group4 import GroupQTensor
 from vibeblade_amd.int8 import K_MAX, Int8QTensor, int8_gemm, quantize_tokens
 from vibeblade_amd.moe import ExpertRouter
-from vibeblade_amd.tensor import EXPERTS_MAX, moe_grouped_ffn, route_experts, verify_draft
+from vibeblade_amd.tensor import EXPERTS_MAX, QTensor, moe_grouped_ffn, route_experts, verify_draft
 
 OK, INVAL, UNSUPPORTED = 0, -1, -2
 PTR = 0x1000  # never dereferenced: the calls below are refused or empty
@@ -165,6 +166,17 @@ def test_host_tensors_are_refused():
         Int8QTensor(torch.zeros(1088, dtype=torch.uint8), 16, 64)
     with pytest.raises(ValueError, match="cuda"):
         verify_draft(torch.zeros(1, 2, 8), torch.zeros(1, 1, dtype=torch.int32), torch.zeros(1, 2))
+
+
+@pytest.mark.parametrize("kind", [QTensor, GroupQTensor])
+def test_int8_gemm_takes_its_own_weights_alone(kind):
+    """Other weights have rows, k and a pointer too, to fewer bytes than the kernels read."""
+    w = object.__new__(kind)
+    w.data, w.rows, w.k, w.qtype = torch.zeros(32, 144, dtype=torch.uint8), 32, 256, 12
+    with pytest.raises(ValueError, match="W must be an Int8QTensor"):
+        int8_gemm(w, torch.zeros(1, 256))
+    with pytest.raises(ValueError, match="W must be an Int8QTensor"):
+        int8_gemm(torch.zeros(32, 256), torch.zeros(1, 256))
 
 
 def test_router_options_are_named():

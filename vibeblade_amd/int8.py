@@ -125,6 +125,8 @@ def int8_gemm(w: Int8QTensor, x, bias: torch.Tensor | None = None, out: torch.Te
     ``out_dtype`` (or ``out``: contiguous, apart from the operands).  Sums of products are exact; they are rounded
     to fp32, scaled, and the result is rounded once to its type.  A NaN or an infinity makes its own token's results
     NaN."""
+    if not isinstance(w, Int8QTensor):  # (other weights hold fewer bytes than the products read)
+        raise ValueError(f"int8_gemm: W must be an Int8QTensor, got {type(w).__name__}")
     packed = isinstance(x, Int8QTensor)
     dev = x.device if packed else _gpu_tensor(x, "int8_gemm: x")
     if dev != w.device:
