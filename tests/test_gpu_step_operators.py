@@ -537,6 +537,21 @@ def test_int8_refusals():
         quantize_tokens(torch.ones(1, K_MAX + 1, device="cuda"))
 
 
+@pytest.mark.parametrize("m", [2, 5, 30])
+def test_int8_out_of_another_shape_is_refused(m):
+    w = Int8QTensor.quantize(normal(1, 24, 128).cuda())
+    x = normal(2, m, 128).cuda()
+    for out in (torch.full((24, m), 7.0, device="cuda"), torch.full((m * 24,), 7.0, device="cuda"),
+                torch.full((m, 4, 6), 7.0, device="cuda"), torch.full((1, m, 24), 7.0, device="cuda")):
+        with pytest.raises(ValueError, match="out must be"):
+            int8_gemm(w, x, out=out)
+        assert (out == 7).all()
+    with pytest.raises(ValueError, match="out must be"):
+        int8_gemm(w, x[0], out=torch.empty(1, 24, device="cuda"))
+    out = torch.empty(24, device="cuda")
+    assert torch.equal(int8_gemm(w, x[0], out=out), int8_gemm(w, x)[0])
+
+
 @pytest.mark.parametrize("dtype", [F32, F16])
 def test_int8_one_token_of_the_longest_k(dtype):
     """Its codes fill most of a workgroup's shared memory."""

@@ -122,9 +122,9 @@ def int8_gemm(w: Int8QTensor, x, bias: torch.Tensor | None = None, out: torch.Te
 
     x: float32 / float16 / bfloat16 on w's device, rows of any stride, quantized in the call as ``quantize_tokens``
     does; or its result, which several products may share.  bias: (rows,) float32.  The result is float32, or of
-    ``out_dtype`` (or ``out``: contiguous, apart from the operands).  Sums of products are exact; they are rounded
-    to fp32, scaled, and the result is rounded once to its type.  A NaN or an infinity makes its own token's results
-    NaN."""
+    ``out_dtype`` (or ``out``: contiguous, of the result's shape, apart from the operands).  Sums of products are
+    exact; they are rounded to fp32, scaled, and the result is rounded once to its type.  A NaN or an infinity makes
+    its own token's results NaN."""
     if not isinstance(w, Int8QTensor):  # (other weights hold fewer bytes than the products read)
         raise ValueError(f"int8_gemm: W must be an Int8QTensor, got {type(w).__name__}")
     packed = isinstance(x, Int8QTensor)
@@ -152,7 +152,7 @@ def int8_gemm(w: Int8QTensor, x, bias: torch.Tensor | None = None, out: torch.Te
         y_type = _elem(out, "int8_gemm: out_dtype")
     else:
         if not isinstance(out, torch.Tensor) or out.device != dev or not out.is_contiguous() \
-                or out.numel() != m * w.rows or out.dtype not in _ELEM or out_dtype not in (None, out.dtype):
+                or tuple(out.shape) != shape or out.dtype not in _ELEM or out_dtype not in (None, out.dtype):
             raise ValueError(f"int8_gemm: out must be a contiguous {shape} tensor on {dev}"
                              f"{'' if out_dtype is None else f' of {out_dtype}'}")
         y_type = _ELEM[out.dtype]
