@@ -1,6 +1,7 @@
 """Refusals and host-side rules of expert routing, 8-bit integer products and
 draft verification.  CPU only: every call here is turned down before a launch,
 or touches no device at all."""
+import numpy as np
 import pytest
 import torch
 
@@ -8,6 +9,7 @@ from vibeblade_amd import _lib
 from vibeblade_amd.group4 import GroupQTensor
 from vibeblade_amd.int8 import K_MAX, Int8QTensor, int8_gemm, quantize_tokens
 from vibeblade_amd.moe import ExpertRouter
+from vibeblade_amd.moe_profiler import HotColdMap
 from vibeblade_amd.tensor import EXPERTS_MAX, QTensor, moe_grouped_ffn, route_experts, verify_draft
 
 OK, INVAL, UNSUPPORTED = 0, -1, -2
@@ -188,3 +190,10 @@ def test_router_options_are_named():
     assert ExpertRouter(w, 2).options == {}
     assert EXPERTS_MAX == 512
     assert callable(moe_grouped_ffn) and callable(int8_gemm)
+
+
+def test_hit_rate_passes_over_ids_of_no_expert():
+    m = HotColdMap({0: [0, 1]}, {0: [2, 3]}, 1, 4)
+    assert m.hit_rate(0, np.array([[0, -1], [2, -1], [1, 0]])) == 0.75  # as the executor counts the same routing
+    assert m.hit_rate(0, np.array([[-1, -1]])) == 0.0
+    assert m.hit_rate(0, np.array([0, 2])) == 0.5

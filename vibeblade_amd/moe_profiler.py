@@ -44,8 +44,10 @@ class HotColdMap:
 
     def hit_rate(self, layer_idx: int, expert_indices) -> float:
         """Share of the routed expert ids (any shape) that are hot in this layer;
-        0 when nothing was routed."""
+        0 when nothing was routed.  Negative ids name no expert (a router with a
+        mask leaves them) and do not count."""
         routed = np.asarray(expert_indices).reshape(-1).astype(np.int64)
+        routed = routed[routed >= 0]
         if routed.size == 0:
             return 0.0
         hot = np.fromiter((int(e) for e in self.hot_experts.get(layer_idx, ())), dtype=np.int64)
