@@ -8,7 +8,7 @@ import torch
 from vibeblade_amd import _lib
 from vibeblade_amd.group4 import GroupQTensor
 from vibeblade_amd.int8 import K_MAX, Int8QTensor, int8_gemm, quantize_tokens
-from vibeblade_amd.moe import ExpertRouter
+from vibeblade_amd.moe import ExpertRouter, MoEExpertSet
 from vibeblade_amd.moe_profiler import HotColdMap
 from vibeblade_amd.tensor import EXPERTS_MAX, QTensor, moe_grouped_ffn, route_experts, verify_draft
 
@@ -197,3 +197,16 @@ def test_hit_rate_passes_over_ids_of_no_expert():
     assert m.hit_rate(0, np.array([[0, -1], [2, -1], [1, 0]])) == 0.75  # as the executor counts the same routing
     assert m.hit_rate(0, np.array([[-1, -1]])) == 0.0
     assert m.hit_rate(0, np.array([0, 2])) == 0.5
+
+
+def test_experts_batch_refuses_ids_of_no_expert():
+    """-1 is no expert in a routing, not the last one."""
+    rng = np.random.RandomState(0)
+    gate, up, down = (rng.randn(4, *s).astype(np.float32) for s in ((6, 8), (6, 8), (8, 6)))
+    experts = MoEExpertSet(gate, up, down)
+    for bad in ([1, -1], np.array([[0, 3], [-1, 2]])):
+        with pytest.raises(IndexError, match="no expert"):
+            experts.get_experts_batch(bad)
+    for ids in ([1, 3, 1], np.array([], dtype=np.int64)):
+        for got, want in zip(experts.get_experts_batch(ids), (gate, up, down)):
+            assert np.array_equal(got, np.transpose(want[np.asarray(ids)], (0, 2, 1)))

@@ -240,6 +240,8 @@ class MoEExpertSet:
         if self._q:
             raise TypeError("get_experts_batch returns dense arrays; not available for quantized experts")
         idx = np.asarray(indices)
+        if (idx < 0).any():
+            raise IndexError("get_experts_batch: a negative id names no expert (a router with a mask leaves -1)")
         return (np.transpose(self.gate[idx], (0, 2, 1)), np.transpose(self.up[idx], (0, 2, 1)),
                 np.transpose(self.down[idx], (0, 2, 1)))
 
