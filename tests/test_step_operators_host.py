@@ -156,6 +156,13 @@ def test_routed_experts_refuse_types_and_small_workspaces(lib):
     assert lib.vb_moe_grouped_ffn_routed(*routed_args(n_tokens=0, idx=None, weights=None, x=None, y=None)) == OK
 
 
+def test_routed_experts_of_no_tokens_with_more_choices_than_experts(lib):
+    """A call's experts may be fewer than a token's choices: so without tokens too."""
+    assert lib.vb_moe_grouped_ffn_routed(*routed_args(n_exp=1, n_tokens=0, idx=None, weights=None, x=None, y=None)) == OK
+    assert lib.vb_moe_grouped_ffn_routed(*routed_args(n_exp=1, n_tokens=0)) == OK
+    assert lib.vb_moe_grouped_ffn_routed(*routed_args(n_exp=1)) == -4  # past the arguments' checks: no workspace
+
+
 def test_host_tensors_are_refused():
     z = torch.zeros(2, 8)
     with pytest.raises(ValueError, match="cuda"):

@@ -588,11 +588,11 @@ bool moe_quant_type(int32_t t) {
 
 namespace {
 int moe_grouped_ffn(const void* const* wg, const void* const* wu, const void* const* wd, int32_t n_exp, const float* x,
-                    int32_t n_tokens, const float* router_logits, const GivenRouting& given, int32_t topk, float* y,
-                    int32_t* out_idx, float* out_w, int64_t h, int64_t i, int32_t gate_up_type, int32_t down_type,
-                    void* workspace, size_t workspace_bytes, void* stream) {
+                    int32_t n_tokens, const float* router_logits, bool routed, const GivenRouting& given, int32_t topk,
+                    float* y, int32_t* out_idx, float* out_w, int64_t h, int64_t i, int32_t gate_up_type,
+                    int32_t down_type, void* workspace, size_t workspace_bytes, void* stream) {
     hipStream_t st = as_stream(stream);
-    if (n_exp <= 0 || n_exp > MOE_MAX_EXPERTS || topk <= 0 || topk > MOE_MAX_TOPK || (topk > n_exp && !given.idx) ||
+    if (n_exp <= 0 || n_exp > MOE_MAX_EXPERTS || topk <= 0 || topk > MOE_MAX_TOPK || (topk > n_exp && !routed) ||
         n_tokens < 0 || static_cast<int64_t>(n_tokens) * topk > MOE_MAX_SLOTS || h <= 0 || i <= 0 || !wg ||
         !wu || !wd || (n_tokens > 0 && (!x || !(router_logits || (given.idx && given.w)) || !y))) {
         set_error("vb_moe_grouped_ffn: bad arguments (n_exp<=%d, topk<=%d, tokens*topk<=%d)", MOE_MAX_EXPERTS,
@@ -726,8 +726,8 @@ extern "C" int vb_moe_grouped_ffn_types(const void* const* wg, const void* const
                                         int32_t topk, float* y, int32_t* out_idx, float* out_w, int64_t h, int64_t i,
                                         int32_t gate_up_type, int32_t down_type, void* workspace,
                                         size_t workspace_bytes, void* stream) {
-    return moe_grouped_ffn(wg, wu, wd, n_exp, x, n_tokens, router_logits, GivenRouting{}, topk, y, out_idx, out_w, h, i,
-                           gate_up_type, down_type, workspace, workspace_bytes, stream);
+    return moe_grouped_ffn(wg, wu, wd, n_exp, x, n_tokens, router_logits, false, GivenRouting{}, topk, y, out_idx, out_w,
+                           h, i, gate_up_type, down_type, workspace, workspace_bytes, stream);
 }
 
 extern "C" int vb_moe_grouped_ffn_routed(const void* const* wg, const void* const* wu, const void* const* wd,
@@ -739,8 +739,9 @@ extern "C" int vb_moe_grouped_ffn_routed(const void* const* wg, const void* cons
         set_error("vb_moe_grouped_ffn_routed: null routing, its row stride below topk, or a negative first expert");
         return E_INVAL;
     }
-    return moe_grouped_ffn(wg, wu, wd, n_exp, x, n_tokens, nullptr, GivenRouting{idx, weights, routing_ld, first_expert},
-                           topk, y, nullptr, nullptr, h, i, gate_up_type, down_type, workspace, workspace_bytes, stream);
+    return moe_grouped_ffn(wg, wu, wd, n_exp, x, n_tokens, nullptr, true,
+                           GivenRouting{idx, weights, routing_ld, first_expert}, topk, y, nullptr, nullptr, h, i,
+                           gate_up_type, down_type, workspace, workspace_bytes, stream);
 }
 
 extern "C" int vb_moe_grouped_ffn(const void* const* wg, const void* const* wu, const void* const* wd,
