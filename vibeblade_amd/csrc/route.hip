@@ -259,8 +259,7 @@ __global__ void __launch_bounds__(64 * ROUTE_WAVES) route_kernel(RouteArgs a) {
         float most = 0.f;
 #pragma unroll
         for (int v = 0; v < V; v++) most = fabsf(b[v]) < INFINITY ? fmaxf(most, fabsf(b[v])) : most;
-        most = wave_largest(most);
-        off = most < 0x1p126f ? 4e-6f + 0x1p-22f * (1.f + most) : INFINITY;
+        off = __builtin_fmaf(4.f * wave_largest(most), 0x1p-24f, 4e-6f + 0x1p-22f);  // (4 * 2^126 is infinite)
     }
     for (int64_t token = static_cast<int64_t>(blockIdx.x) * ROUTE_WAVES + (threadIdx.x >> 6); token < a.tokens;
          token += static_cast<int64_t>(gridDim.x) * ROUTE_WAVES) {
