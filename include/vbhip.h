@@ -476,7 +476,8 @@ int vb_group4_gemv(const void* w, int64_t rows, int64_t k, int32_t group, int32_
  *       stay) of their experts by c, in descending order, equal ones (and
  *       equal groups) by the lower id;
  *   out_w[t, j] = scale * s of it, over the sum of the chosen s with renorm.
- * Scores, choices and sums are 64 bits.  An expert whose logit or bias is -inf
+ * Scores, choices and sums are 64 bits (a softmax score below 2^-1021 of the
+ * token's largest counts as 0), the scale fp32.  An expert whose logit or bias is -inf
  * is never chosen; where too few are left the id is -1, the weight 0.  A token
  * with a NaN logit or choice, or +inf under softmax, has ids -1 and weights
  * NaN.  (vb_moe_route keeps the reference's routing, whose logits are clamped.) */
@@ -528,9 +529,10 @@ int vb_int8_gemm(const void* w, int64_t rows, int64_t k, const void* x, int32_t 
  *       outside the vocabulary ends them too.
  *   tokens[s, 0..n_drafts]: the accepted ids, the next token, then -1.
  *   accepted[s]: their number.
- * Sums are 64 bits.  A row that holds NaN or +inf, or a target row of nothing but
- * -inf, ends its sequence with the token -1; rows behind the first refused
- * draft are without effect.  drafted: ids of token_bytes (4 or 8), row stride
+ * Exponentials (to 2^-51, 0 below 2^-1021 of the row's largest) and sums are 64
+ * bits, the temperatures fp32.  A row that holds NaN or +inf, or a target row of
+ * nothing but -inf, ends its sequence with the token -1; rows behind the first
+ * refused draft are without effect.  drafted: ids of token_bytes (4 or 8), row stride
  * drafted_row; outputs contiguous.  workspace: at least
  * vb_verify_draft_workspace(...) bytes (asked on the device of the call),
  * 16-byte aligned, free again when the call's work is done. */

@@ -723,7 +723,11 @@ constexpr int I8_MAX_CHUNKS = 8;
 // The shape and the chunks of k that the above makes shortest: workgroups a CU
 // times what each takes, and with chunks the launch that adds them and its bytes.
 // (17 tokens of 4096 x 14336: whole 28 us, in eight chunks 18.8; 4096 tokens of
-// 14336 x 4096: four rounds of 256 rows 224 us, of 224 rows 217.)
+// 14336 x 4096: four rounds of 256 rows 224 us, of 224 rows 217.)  It ranks shapes
+// and is no forecast: there is no term for the memory, which bounds tens to hundreds
+// of tokens.  Modelled, measured: 4096 tokens of 14336 x 4096 213, 214; of 4096 x
+// 14336 199, 175; 203 of 5121 x 4100 9.8 and 5.6 to add the chunks, 15.1 and 5.5; 64
+// of 14336 x 4096 12, 20.5 of which quantizing is about 3.
 void i8_best_tiles(const Int8Layout& wl, int64_t m, int64_t cus, int* shape, int64_t* chunks) {
     float best = INFINITY;
     for (int s = 0; s < 5; s++) {

@@ -12,10 +12,9 @@
 // sequence's last random number: the tokens are distributed as the target's own.
 //
 // Exponentials and sums are 64 bits, those of whole slices and those within them
-// by the same 2^x (nine points of it in place of eleven, an error of 1.1e-12, took
-// 4 of 90 us off 64 sequences of 128256 ids).  A token is an id, found by comparing
-// a random number with a sum over a vocabulary; in fp32 the order of the additions
-// would decide about one in a hundred of them.
+// by the same 2^x of eleven points (nine have an error of 1.1e-12).  A token is an
+// id, found by comparing a random number with a sum over a vocabulary; in fp32 the
+// order of the additions would decide about one in a hundred of them.
 //
 //   stats    (row, slice): the maximum and the sum of 2^(c (z - max)), c =
 //            log2(e) / T, of each slice of each row that a decision may need
@@ -27,10 +26,10 @@
 //            into, then the place in it (without a drafter's logits the decision
 //            is made here, and the slices' sums are those of stats)
 //
-// The terms' arithmetic (23 instructions a logit, fifteen of them 64-bit) and the
-// memory bound many rows about alike (64
-// sequences of 4 drafts over 128256 fp32 ids: stats 61 us, 4.8 TB/s; without the
-// terms it takes 52, without the loads 54), the residual by its two terms a logit
+// The terms' arithmetic (25 instructions a logit, seventeen of them 64-bit) bounds
+// many rows before the memory does (64 sequences of 4 drafts over 128256 fp32 ids:
+// stats 66 us, 4.5 TB/s; without the terms it takes 52, without the loads 61; nine
+// points of 2^x take 61), the residual by its two terms a logit
 // (19 us for 64 rows and rows of drafts); few rows wait for launches and for one
 // workgroup's chain of loads, sums over waves and barriers (one sequence 4.8 + 8
 // us, eight of 32003 ids 7.5 + 3.5 + 4.6 + 6.6).
@@ -521,10 +520,10 @@ struct VerifyPlan {
     int64_t slices, slice, rests, rest_slice, workspace;
 };
 
-// Slices of a row: for the sums of rows at most eight workgroups a CU, as many as
-// are resident (more and fewer are no faster: 64 sequences 61 us with three slices
-// a row, 63 with four), for the residual sixteen (22 us with four, 18 with
-// sixteen), and whole pieces of a workgroup.
+// Slices of a row: for the sums of rows at most eight workgroups a CU, about as many
+// as are resident (64 sequences have three slices a row; four were 2 us slower), for
+// the residual sixteen (22 us with four, 18 with sixteen), and whole pieces of a
+// workgroup.
 VerifyPlan verify_plan(int64_t seqs, int64_t drafts, int64_t vocab, bool draft) {
     const int64_t rows = seqs * (drafts + 1 + (draft ? drafts : 0));
     const auto cut = [&](int64_t n, int64_t groups, int64_t* slices, int64_t* slice) {
