@@ -32,7 +32,7 @@
 // points of 2^x take 61), the residual by its two terms a logit
 // (19 us for 64 rows and rows of drafts); few rows wait for launches and for one
 // workgroup's chain of loads, sums over waves and barriers (one sequence 4.8 + 8
-// us, eight of 32003 ids 7.5 + 3.5 + 4.6 + 6.6).
+// us, eight of 32003 ids 7.2 + 3.1 + 4.7 + 6.6).
 //
 // A row with a NaN or +inf (target's or drafter's) ends the sequence at its
 // position: its token is -1, as it is where a mask leaves the target nothing.

@@ -630,9 +630,9 @@ def route_experts(logits: torch.Tensor, topk: int, *, scores: str = "softmax", b
         weight = scale * s, over the sum of the chosen s with ``renorm``
 
     Scores are compared in 64 bits (a softmax score below 2^-1021 of the token's largest counts as 0); ``scale`` is
-    rounded to float32.  A logit or bias of -inf keeps an expert from being chosen: where too few are
-    left the index is -1 and the weight 0.  A token with a NaN (or, under softmax, +inf) has indices -1 and weights
-    NaN.  ``moe_grouped_ffn(..., routing=(indices, weights))`` runs the experts; ``moe_route`` keeps the reference's
+    rounded to float32.  A logit or bias of -inf keeps an expert from being chosen: where too few are left the index
+    is -1 and the weight 0.  A token with a NaN (or, under softmax, +inf) has indices -1 and weights NaN.
+    ``moe_grouped_ffn(..., routing=(indices, weights))`` runs the experts; ``moe_route`` keeps the reference's
     routing, which clamps the logits to +-50."""
     dev = _gpu_tensor(logits, "route_experts: logits")
     if logits.dim() != 2 or not 0 < logits.shape[1] <= EXPERTS_MAX:
@@ -681,9 +681,9 @@ def verify_draft(target: torch.Tensor, drafted: torch.Tensor, uniforms: torch.Te
         the first id whose sum of weights exceeds the last random number times the sum of all
 
     so that the tokens are distributed as the target's own.  Exponentials and sums are 64 bits, the temperatures (1e-30
-    to 1e30) are rounded to float32; a difference p - q below 2^-45 p counts as 0.  ``lengths`` (seqs,) int32: how many drafts of each
-    sequence count (an id outside the vocabulary ends them too).  Logits of -inf are never drawn.  A row with a NaN or
-    +inf, or a target row of -inf only, ends its sequence with the token -1."""
+    to 1e30) are rounded to float32; a difference p - q below 2^-45 p counts as 0.  ``lengths`` (seqs,) int32: how many
+    drafts of each sequence count (an id outside the vocabulary ends them too).  Logits of -inf are never drawn.  A row
+    with a NaN or +inf, or a target row of -inf only, ends its sequence with the token -1."""
     dev = _gpu_tensor(target, "verify_draft: target")
     if target.dim() != 3 or target.shape[1] == 0 or target.shape[2] == 0:
         raise ValueError(f"verify_draft: target must be (seqs, k + 1, vocab), got {tuple(target.shape)}")
